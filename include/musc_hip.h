@@ -187,6 +187,7 @@ int musc_msm_pools_scores_f32(const float* z, int pools, int n, int p, int c, in
 /* ------------------------------------------------------------------------ */
 #define MUSC_DTYPE_F32 0
 #define MUSC_DTYPE_F16 1
+#define MUSC_DTYPE_BF16 2  /* musc_rmsnorm_rows*, musc_rotary, musc_masked_attention only */
 
 /* Output layouts of musc_lnamd_f32 (R radii, L layers, B images, P patches). */
 #define MUSC_LAYOUT_RBPLC 0  /* out[r][b][p][l][c]: one (B,P,L,C) block per radius,
@@ -371,6 +372,52 @@ int musc_attention_weights_strided(const void* q, const void* k, int dtype, int 
 int musc_layernorm_rows(const void* x, const void* residual, void* sum_out,
                         const float* weight, const float* bias, int dtype, int rows, int width,
                         float eps, void* y, hipStream_t stream);
+
+/* Root-mean-square norm of the rows of (rows, width) x, row strides in elements (the last
+ * dimension contiguous), dtype MUSC_DTYPE_F32, _F16 or _BF16, fp32 statistics:
+ *   s = x + residual rounded to the dtype, written to the contiguous sum_out (residual == NULL:
+ *       s = x, sum_out unused);
+ *   y = s * weight / sqrt(mean(s^2) + eps), rounded once to the contiguous y.
+ * weight: width values of weight_dtype (the dtype or MUSC_DTYPE_F32), or NULL for 1.
+ * sum_out may alias x or residual (and y may alias x without a residual) where that has the
+ * same layout.  The sum of squares is fp32: rows whose squares overflow it give y = 0.
+ * width <= 32768 (16-bit) or 16384 (fp32), MUSC_ERR_UNSUPPORTED beyond; any alignment of the
+ * elements (16-byte vectors are used where every row allows them). */
+int musc_rmsnorm_rows(const void* x, long long x_stride, const void* residual, long long residual_stride,
+                      void* sum_out, const void* weight, int weight_dtype, int dtype, int rows, int width,
+                      float eps, void* y, hipStream_t stream);
+
+#define MUSC_FP8_E4M3 0  /* OCP E4M3, largest number 448 */
+#define MUSC_FP8_E5M2 1  /* OCP E5M2, largest number 57344 */
+/* The same with y in 8 bits: contiguous (rows, width) bytes y of the format and fp32 scales,
+ * y * scale being the norm's value.  group == 0: one scale per row, scales (rows,); group 32,
+ * 64, 128 or 256 (width a multiple of it): one for each group columns, scales (rows, width /
+ * group).  scale = max|y| / largest number (1 for a group of zeros, never below the smallest
+ * normal fp32 number); a NaN in a row makes its scales and 8-bit values NaN. */
+int musc_rmsnorm_rows_8bit(const void* x, long long x_stride, const void* residual, long long residual_stride,
+                           void* sum_out, const void* weight, int weight_dtype, int dtype, int rows, int width,
+                           float eps, int format, int group, void* y, float* scales, hipStream_t stream);
+
+/* Rotary positions with several axes.  For every token (b, t) and pair i < pairs, with
+ * turns = positions[b * pos_sb + t * axes + axis[i]] * frequency[i] in float64, the channels
+ * (a, b) = (i, pairs + i), or (2 i, 2 i + 1) with adjacent != 0, of every head become
+ * (a cos - b sin, b cos + a sin) of 2 pi turns (inverse != 0: of -2 pi turns), in fp32, rounded
+ * once to the dtype (MUSC_DTYPE_F32, _F16, _BF16); channels from 2 * pairs on are copied.
+ *   q, k      heads of d channels at b * sb + t * st + h * sh (elements, >= 0), written at
+ *             b * ob + t * ot + h * oh of q_out, k_out; k_heads == 0: q alone.  An output may
+ *             be its input with the same strides (in place); otherwise they may not overlap.
+ *   positions (batch, t, axes) float32, or int32 with int_positions != 0; pos_sb == 0 shares
+ *             one (t, axes) table between the batch.
+ *   frequency (pairs,) float64 on the device, turns per unit of position; axis (pairs,) int32 on
+ *             the device, each in [0, axes).
+ * pairs <= 256, d <= 512, q_heads + k_heads <= 1024 (MUSC_ERR_UNSUPPORTED beyond). */
+int musc_rotary(const void* q, int q_heads, long long q_sb, long long q_st, long long q_sh,
+                void* q_out, long long qo_sb, long long qo_st, long long qo_sh,
+                const void* k, int k_heads, long long k_sb, long long k_st, long long k_sh,
+                void* k_out, long long ko_sb, long long ko_st, long long ko_sh,
+                int dtype, int batch, int t, int d, const void* positions, int int_positions,
+                long long pos_sb, int axes, const double* frequency, const int* axis, int pairs,
+                int adjacent, int inverse, hipStream_t stream);
 
 #define MUSC_ACT_QUICK_GELU 0  /* x * sigmoid(1.702 x), transformer.py:32-35 (fp16: the
                                   three torch ops' roundings: 1.702 x, sigmoid, product) */

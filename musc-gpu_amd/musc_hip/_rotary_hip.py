@@ -1,0 +1,109 @@
+"""Rotary positions with several axes (time, height, width) on MI355X (libmusc_hip musc_rotary).
+
+For encoders of images and video of any size, whose blocks turn q and k by the token's place
+instead of adding a position embedding of one grid (the reference's encoder has only the
+latter, models/backbone/open_clip/transformer.py:391-398).  q and k are read in place from a
+packed projection; all heads of a token share its angles, whose whole turns are taken off in
+float64.
+"""
+from __future__ import annotations
+
+import math
+
+import torch
+
+from . import _runtime as rt
+
+_STORAGE = {torch.float32: rt.DTYPE_F32, torch.float16: rt.DTYPE_F16, torch.bfloat16: rt.DTYPE_BF16}
+
+
+class RotaryAxes:
+    """Which pairs of a head's channels turn with which axis, and how fast.
+
+    sections: pairs of each axis, in order (e.g. (0, 16, 16) for 64 channels turned by rows and
+    columns of (time, height, width) positions); their sum R may leave channels from 2 R on as
+    they are.  Pair i of n in its axis's section turns base ** -(i / n) radians per unit of
+    position; with `shared`, pair i of all R turns base ** -(i / R).  Pairs are channels
+    (i, R + i), or (2 i, 2 i + 1) with `adjacent`.  Kept by the caller and used by any call with
+    the same head width."""
+
+    def __init__(self, head_dim: int, sections, base: float = 10000.0, shared: bool = False, adjacent: bool = False,
+                 device='cuda'):
+        sections = [int(n) for n in sections]
+        pairs = sum(sections)
+        if not sections or min(sections) < 0 or pairs < 1 or 2 * pairs > head_dim:
+            raise ValueError('sections must be pair counts, at least one pair and at most head_dim channels in all')
+        if not (base > 0 and math.isfinite(base)):
+            raise ValueError('base must be a positive number')
+        axis, turns = [], []
+        for a, n in enumerate(sections):
+            for i in range(n):
+                exponent = len(axis) / pairs if shared else i / n
+                turns.append(float(base) ** -exponent / (2 * math.pi))
+                axis.append(a)
+        self.head_dim, self.pairs, self.axes, self.adjacent = int(head_dim), pairs, len(sections), bool(adjacent)
+        self.frequency = torch.tensor(turns, dtype=torch.float64, device=device)
+        self.axis = torch.tensor(axis, dtype=torch.int32, device=device)
+
+
+def _head_rows(x, name, like, axes):
+    rt.require_device_tensor(x, name)
+    if x.dim() != 4 or x.shape[-1] != axes.head_dim or x.dtype not in _STORAGE:
+        raise ValueError(f'{name} must be a (B, T, heads, {axes.head_dim}) float32, float16 or bfloat16 tensor')
+    if like is not None and (x.shape[:2] != like.shape[:2] or x.dtype != like.dtype or x.device != like.device):
+        raise ValueError(f'{name} must match q in batch, tokens, dtype and device')
+    return x if x.stride(-1) == 1 else x.contiguous()
+
+
+def _strides(x):
+    """Strides of batch, token and head in elements; a dimension of one element has none."""
+    return [st if n > 1 else 0 for n, st in zip(x.shape[:3], x.stride()[:3])]
+
+
+def _output(out, x, name):
+    if out is None:
+        return torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    rt.require_device_tensor(out, name)
+    if out.shape != x.shape or out.dtype != x.dtype or out.device != x.device or out.stride(-1) != 1:
+        raise ValueError(f'{name} must match its input in shape, dtype and device, its last dimension contiguous')
+    if 0 in [st for n, st in zip(out.shape, out.stride()) if n > 1]:
+        raise ValueError(f'{name} has elements that share memory')
+    return out
+
+
+def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, axes: RotaryAxes, inverse: bool = False,
+           out=None):
+    """(q, k) turned by their tokens' positions, or q alone where k is None.
+
+    q (B, T, heads, D), k (B, T, kv_heads, D), any strides with a contiguous last dimension;
+    positions (T, axes) or (B, T, axes), float32 or int32.  inverse turns back (the transpose).
+    out: the tensors to write, (q_out, k_out) or q_out; they may be q and k themselves, and may
+    not overlap them otherwise.  No backward pass."""
+    q2 = _head_rows(q, 'q', None, axes)
+    k2 = None if k is None else _head_rows(k, 'k', q, axes)
+    rt.require_no_gradient(q, k)
+    b, t, h, d = q2.shape
+    rt.require_device_tensor(positions, 'positions')
+    if positions.dtype not in (torch.float32, torch.int32) or positions.device != q.device or positions.shape not in (
+            (t, axes.axes), (b, t, axes.axes)):
+        raise ValueError(f"positions must be float32 or int32 of shape (T, {axes.axes}) or (B, T, {axes.axes}) on q's device")
+    if axes.frequency.device != q.device:
+        raise ValueError("axes must be on q's device")
+    positions = positions.contiguous()
+    outs = out if k is not None else (out, None)
+    if k is not None and out is not None and len(out) != 2:
+        raise ValueError('out must be (q_out, k_out)')
+    with torch.cuda.device(q.device):
+        qo = _output(outs[0] if outs is not None else None, q2, 'q_out')
+        ko = None if k2 is None else _output(outs[1] if outs is not None else None, k2, 'k_out')
+        if b and t and h:
+            if k2 is None or not k2.shape[2]:
+                k_args = (None, 0, 0, 0, 0, None, 0, 0, 0)
+            else:
+                k_args = (k2.data_ptr(), k2.shape[2], *_strides(k2), ko.data_ptr(), *_strides(ko))
+            rt.check(rt.library().musc_rotary(
+                q2.data_ptr(), h, *_strides(q2), qo.data_ptr(), *_strides(qo), *k_args, _STORAGE[q.dtype], b, t, d,
+                positions.data_ptr(), int(positions.dtype == torch.int32), 0 if positions.dim() == 2 else t * axes.axes,
+                axes.axes, axes.frequency.data_ptr(), axes.axis.data_ptr(), axes.pairs, int(axes.adjacent), int(inverse),
+                rt.stream(q.device)), 'musc_rotary')
+    return qo if k is None else (qo, ko)

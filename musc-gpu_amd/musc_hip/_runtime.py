@@ -31,6 +31,9 @@ MUSC_ERR_SCRATCH_LIMIT = 1004
 
 DTYPE_F32 = 0
 DTYPE_F16 = 1
+DTYPE_BF16 = 2
+FP8_E4M3 = 0
+FP8_E5M2 = 1
 ACT_QUICK_GELU = 0
 ACT_GELU = 1
 LAYOUT_RBPLC = 0
@@ -75,6 +78,10 @@ SIGNATURES = {
     'musc_attention_fwd_strided': (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _ll, _ll, _ll, _ll, _ll, _ll, _f, _vp]),
     'musc_attention_weights_strided': (_i, [_vp, _vp, _i, _i, _i, _i, _i, _ll, _ll, _ll, _f, _vp, _vp, _sz, _vp]),
     'musc_layernorm_rows': (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _f, _vp, _vp]),
+    'musc_rmsnorm_rows': (_i, [_vp, _ll, _vp, _ll, _vp, _vp, _i, _i, _i, _i, _f, _vp, _vp]),
+    'musc_rmsnorm_rows_8bit': (_i, [_vp, _ll, _vp, _ll, _vp, _vp, _i, _i, _i, _i, _f, _i, _i, _vp, _vp, _vp]),
+    'musc_rotary': (_i, [_vp, _i, _ll, _ll, _ll, _vp, _ll, _ll, _ll, _vp, _i, _ll, _ll, _ll, _vp, _ll, _ll, _ll,
+                         _i, _i, _i, _i, _vp, _i, _ll, _i, _vp, _vp, _i, _i, _i, _vp]),
     'musc_activation': (_i, [_vp, _vp, _i, _i, _ll, _vp]),
     'musc_calibrate_mfma_f32': (_i, [_vp, _i, _i, ctypes.POINTER(ctypes.c_double), _vp]),
     'musc_calibrate_mfma_f16': (_i, [_vp, _i, _i, ctypes.POINTER(ctypes.c_double), _vp]),
@@ -185,6 +192,12 @@ def require_device_tensor(t: torch.Tensor, name: str) -> None:
         raise ValueError(f'{name} must be a GPU tensor')
     if torch.version.hip is None:
         raise RuntimeError('musc_hip requires a ROCm build of PyTorch')
+
+
+def require_no_gradient(*tensors) -> None:
+    """Operators without a backward pass refuse inputs that ask for one."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise ValueError('this operator has no backward pass: call it under torch.no_grad() or detach its inputs')
 
 
 def workspace(nbytes: int, device: torch.device) -> torch.Tensor:
