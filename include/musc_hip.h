@@ -373,6 +373,48 @@ int musc_layernorm_rows(const void* x, const void* residual, void* sum_out,
                         const float* weight, const float* bias, int dtype, int rows, int width,
                         float eps, void* y, hipStream_t stream);
 
+/* Attention over the keys that a query may see (packed images, padded batches, prefixes,
+ * frames), with an optional cap on the scores and an optional bias by distance:
+ *   score(i, j) = c(scale q_i . k_j) - sum_a slopes[head][a] |q_position[i][a] - k_position[j][a]|
+ *   c(s) = cap tanh(s / cap) for cap > 0, else s
+ *   seen(i, j) = document(i) == document(j), both >= 0, and order(j) <= order(i)
+ *   out_i = softmax over the seen keys of score(i, .) times V; zeros where none is seen.
+ * fp32 scores, softmax statistics and accumulation; the probabilities are rounded to 16-bit
+ * types for their product with V.  What unseen keys hold (infinities and NaN among it) has no
+ * effect.  No other call's result depends on it, and nothing is kept between calls. */
+typedef struct musc_masked_attention {
+  const void *q, *k, *v;  /* heads of d channels at b * sb + token * st + head * sh (elements) */
+  void* out;
+  long long q_sb, q_st, q_sh, k_sb, k_st, k_sh, v_sb, v_st, v_sh, o_sb, o_st, o_sh;
+  int dtype;              /* MUSC_DTYPE_F32, _F16 or _BF16 */
+  int batch, q_len, k_len;
+  int heads, kv_heads;    /* query head h reads key head h / (heads / kv_heads) */
+  int d;                  /* multiple of 16 bytes, at most 128 channels */
+  float scale, cap;       /* cap 0: none */
+  /* documents (and orders): int32, token t of batch entry b at b * tokens_sb + t; tokens_sb 0
+   * shares one row between the batch.  Both sides' documents or neither (every key is seen);
+   * both orders or neither. */
+  const int *q_documents, *q_order, *k_documents, *k_order;
+  long long q_tokens_sb, k_tokens_sb;
+  const int* k_summary;   /* musc_token_summary of the keys, with documents; 16-byte aligned */
+  long long k_summary_sb; /* in groups of 32 keys: ceil(k_len / 32), or 0 with one shared row */
+  /* positions: float32 (tokens, axes) rows, likewise; slopes (heads, axes) float32 */
+  const float *q_positions, *k_positions;
+  long long q_positions_sb, k_positions_sb;
+  const float* slopes;
+  int axes;               /* 0: no bias; at most 3 */
+} musc_masked_attention;
+
+/* Summary of (batch, t) documents and orders (NULL: none): four int32 per group of 32 keys,
+ * (batch, ceil(t / 32), 4).  Made again when a document or order changes. */
+int musc_token_summary(const int* documents, const int* order, int batch, int t, int* summary, hipStream_t stream);
+/* Few rows are split over their keys and joined through a workspace (16-byte aligned; 0 bytes
+ * where nothing is split).  Every row of q, k, v and out starts on 16 bytes; 64 rows of K and V
+ * span less than 2 GiB (MUSC_ERR_UNSUPPORTED). */
+int musc_masked_attention_workspace_bytes(const musc_masked_attention* call, size_t* out);
+int musc_masked_attention_fwd(const musc_masked_attention* call, void* workspace, size_t workspace_bytes,
+                              hipStream_t stream);
+
 /* Root-mean-square norm of the rows of (rows, width) x, row strides in elements (the last
  * dimension contiguous), dtype MUSC_DTYPE_F32, _F16 or _BF16, fp32 statistics:
  *   s = x + residual rounded to the dtype, written to the contiguous sum_out (residual == NULL:

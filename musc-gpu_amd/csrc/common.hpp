@@ -59,6 +59,15 @@ inline void launch_fill_u32(uint32_t* dst, size_t count, uint32_t value, hipStre
   hipLaunchKernelGGL(fill_u32_kernel<0>, dim3((unsigned)blocks), dim3(256), 0, s, dst, count, value);
 }
 
+// Grid of `blocks` workgroups over two dimensions (one holds fewer than 2^32 threads); the
+// kernel's workgroup number is linear_block(), and numbers past `blocks` have no work.
+inline dim3 linear_grid(long long blocks) {
+  constexpr long long kRow = 1 << 20;
+  if (blocks <= kRow) return dim3((unsigned)blocks);
+  return dim3((unsigned)kRow, (unsigned)((blocks + kRow - 1) / kRow));
+}
+__device__ inline long long linear_block() { return (long long)blockIdx.y * gridDim.x + blockIdx.x; }
+
 inline int check_launch() {
   hipError_t e = hipGetLastError();
   return e == hipSuccess ? MUSC_OK : static_cast<int>(e);

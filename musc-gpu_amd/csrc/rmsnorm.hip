@@ -87,7 +87,7 @@ __global__ __launch_bounds__(kTpr < 256 ? 256 : kTpr) void rmsnorm_kernel(const 
   __shared__ float shared[kTpr / kWave];
   constexpr int kRows = kTpr < 256 ? 256 / kTpr : 1;
   const int t = threadIdx.x % kTpr;
-  const long long row = (long long)blockIdx.x * kRows + threadIdx.x / kTpr;
+  const long long row = linear_block() * kRows + threadIdx.x / kTpr;
   if (row >= a.rows) return;  // whole waves, and whole workgroups where kTpr > kWave
   const int width = a.width;
   float v[kC][N], w[kC][N];
@@ -212,7 +212,7 @@ int launch(const Args& a, bool vec, hipStream_t stream) {
   const int vectors = (a.width + N - 1) / N;
 #define MUSC_RMS(TPR, C, VEC)                                                                                       \
   hipLaunchKernelGGL((rmsnorm_kernel<kDtype, kEight, TPR, C, VEC>),                                                 \
-                     dim3((unsigned)((a.rows + (TPR < 256 ? 256 / TPR : 1) - 1) / (TPR < 256 ? 256 / TPR : 1))),    \
+                     linear_grid(((long long)a.rows + (TPR < 256 ? 256 / TPR : 1) - 1) / (TPR < 256 ? 256 / TPR : 1)), \
                      dim3(TPR < 256 ? 256 : TPR), 0, stream, a)
 #define MUSC_RMS_C(TPR)                                                                                             \
   if (!vec) MUSC_RMS(TPR, 4, false);                                                                                \

@@ -54,7 +54,8 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(const Args a) {
   __shared__ float2 table[kTable];
   __shared__ long long at_b[kMaxTokens];
   __shared__ int at_t[kMaxTokens];
-  const long long first = (long long)blockIdx.x * a.tokens, total = (long long)a.batch * a.t;
+  const long long first = linear_block() * a.tokens, total = (long long)a.batch * a.t;
+  if (first >= total) return;
   const int here = (int)min((long long)a.tokens, total - first);
   const int pairs = a.pairs;
   for (int e = threadIdx.x; e < here * pairs; e += kThreads) {
@@ -133,13 +134,13 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(const Args a) {
 }
 
 template <int kDtype>
-void launch(const Args& a, bool adjacent, bool vec, unsigned grid, hipStream_t stream) {
+void launch(const Args& a, bool adjacent, bool vec, dim3 grid, hipStream_t stream) {
   if (adjacent) {
-    if (vec) hipLaunchKernelGGL((rotary_kernel<kDtype, true, true>), dim3(grid), dim3(kThreads), 0, stream, a);
-    else hipLaunchKernelGGL((rotary_kernel<kDtype, true, false>), dim3(grid), dim3(kThreads), 0, stream, a);
+    if (vec) hipLaunchKernelGGL((rotary_kernel<kDtype, true, true>), grid, dim3(kThreads), 0, stream, a);
+    else hipLaunchKernelGGL((rotary_kernel<kDtype, true, false>), grid, dim3(kThreads), 0, stream, a);
   } else {
-    if (vec) hipLaunchKernelGGL((rotary_kernel<kDtype, false, true>), dim3(grid), dim3(kThreads), 0, stream, a);
-    else hipLaunchKernelGGL((rotary_kernel<kDtype, false, false>), dim3(grid), dim3(kThreads), 0, stream, a);
+    if (vec) hipLaunchKernelGGL((rotary_kernel<kDtype, false, true>), grid, dim3(kThreads), 0, stream, a);
+    else hipLaunchKernelGGL((rotary_kernel<kDtype, false, false>), grid, dim3(kThreads), 0, stream, a);
   }
 }
 
@@ -199,7 +200,7 @@ extern "C" int musc_rotary(const void* q, int q_heads, long long q_sb, long long
   const long long per_token = heads * a.items, divisor = heads > a.items ? heads : a.items;
   while (tokens > 1 && tokens * per_token * divisor > 0xffffffffLL) --tokens;
   a.tokens = tokens;
-  const unsigned grid = (unsigned)((total + tokens - 1) / tokens);
+  const dim3 grid = linear_grid((total + tokens - 1) / tokens);
   if (dtype == MUSC_DTYPE_F32) launch<MUSC_DTYPE_F32>(a, adjacent, vec, grid, stream);
   else if (dtype == MUSC_DTYPE_F16) launch<MUSC_DTYPE_F16>(a, adjacent, vec, grid, stream);
   else launch<MUSC_DTYPE_BF16>(a, adjacent, vec, grid, stream);

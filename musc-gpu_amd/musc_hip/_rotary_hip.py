@@ -55,22 +55,6 @@ def _head_rows(x, name, like, axes):
     return x if x.stride(-1) == 1 else x.contiguous()
 
 
-def _strides(x):
-    """Strides of batch, token and head in elements; a dimension of one element has none."""
-    return [st if n > 1 else 0 for n, st in zip(x.shape[:3], x.stride()[:3])]
-
-
-def _output(out, x, name):
-    if out is None:
-        return torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    rt.require_device_tensor(out, name)
-    if out.shape != x.shape or out.dtype != x.dtype or out.device != x.device or out.stride(-1) != 1:
-        raise ValueError(f'{name} must match its input in shape, dtype and device, its last dimension contiguous')
-    if 0 in [st for n, st in zip(out.shape, out.stride()) if n > 1]:
-        raise ValueError(f'{name} has elements that share memory')
-    return out
-
-
 def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, axes: RotaryAxes, inverse: bool = False,
            out=None):
     """(q, k) turned by their tokens' positions, or q alone where k is None.
@@ -94,15 +78,15 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, axe
     if k is not None and out is not None and len(out) != 2:
         raise ValueError('out must be (q_out, k_out)')
     with torch.cuda.device(q.device):
-        qo = _output(outs[0] if outs is not None else None, q2, 'q_out')
-        ko = None if k2 is None else _output(outs[1] if outs is not None else None, k2, 'k_out')
+        qo = rt.output_like(outs[0] if outs is not None else None, q2, 'q_out')
+        ko = None if k2 is None else rt.output_like(outs[1] if outs is not None else None, k2, 'k_out')
         if b and t and h:
             if k2 is None or not k2.shape[2]:
                 k_args = (None, 0, 0, 0, 0, None, 0, 0, 0)
             else:
-                k_args = (k2.data_ptr(), k2.shape[2], *_strides(k2), ko.data_ptr(), *_strides(ko))
+                k_args = (k2.data_ptr(), k2.shape[2], *rt.token_strides(k2), ko.data_ptr(), *rt.token_strides(ko))
             rt.check(rt.library().musc_rotary(
-                q2.data_ptr(), h, *_strides(q2), qo.data_ptr(), *_strides(qo), *k_args, _STORAGE[q.dtype], b, t, d,
+                q2.data_ptr(), h, *rt.token_strides(q2), qo.data_ptr(), *rt.token_strides(qo), *k_args, _STORAGE[q.dtype], b, t, d,
                 positions.data_ptr(), int(positions.dtype == torch.int32), 0 if positions.dim() == 2 else t * axes.axes,
                 axes.axes, axes.frequency.data_ptr(), axes.axis.data_ptr(), axes.pairs, int(axes.adjacent), int(inverse),
                 rt.stream(q.device)), 'musc_rotary')

@@ -44,6 +44,20 @@ LNAMD_RAW_SUMS = 4
 MSM_NORMALIZE_ROWS = 1
 MSM_ENGINES = {'fp32': 0, 'split16': 1}
 
+class MaskedAttention(ctypes.Structure):
+    """musc_masked_attention of include/musc_hip.h, field by field."""
+    _fields_ = (
+        [(n, ctypes.c_void_p) for n in ('q', 'k', 'v', 'out')]
+        + [(f'{x}_{s}', ctypes.c_longlong) for x in 'qkvo' for s in ('sb', 'st', 'sh')]
+        + [(n, ctypes.c_int) for n in ('dtype', 'batch', 'q_len', 'k_len', 'heads', 'kv_heads', 'd')]
+        + [('scale', ctypes.c_float), ('cap', ctypes.c_float)]
+        + [(n, ctypes.c_void_p) for n in ('q_documents', 'q_order', 'k_documents', 'k_order')]
+        + [('q_tokens_sb', ctypes.c_longlong), ('k_tokens_sb', ctypes.c_longlong), ('k_summary', ctypes.c_void_p),
+           ('k_summary_sb', ctypes.c_longlong), ('q_positions', ctypes.c_void_p), ('k_positions', ctypes.c_void_p),
+           ('q_positions_sb', ctypes.c_longlong), ('k_positions_sb', ctypes.c_longlong), ('slopes', ctypes.c_void_p),
+           ('axes', ctypes.c_int)])
+
+
 # Every symbol include/musc_hip.h declares, with its ctypes signature.
 _vp, _i, _f, _sz, _ll = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_size_t, ctypes.c_longlong
 SIGNATURES = {
@@ -78,6 +92,9 @@ SIGNATURES = {
     'musc_attention_fwd_strided': (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _ll, _ll, _ll, _ll, _ll, _ll, _f, _vp]),
     'musc_attention_weights_strided': (_i, [_vp, _vp, _i, _i, _i, _i, _i, _ll, _ll, _ll, _f, _vp, _vp, _sz, _vp]),
     'musc_layernorm_rows': (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _f, _vp, _vp]),
+    'musc_token_summary': (_i, [_vp, _vp, _i, _i, _vp, _vp]),
+    'musc_masked_attention_workspace_bytes': (_i, [ctypes.POINTER(MaskedAttention), ctypes.POINTER(_sz)]),
+    'musc_masked_attention_fwd': (_i, [ctypes.POINTER(MaskedAttention), _vp, _sz, _vp]),
     'musc_rmsnorm_rows': (_i, [_vp, _ll, _vp, _ll, _vp, _vp, _i, _i, _i, _i, _f, _vp, _vp]),
     'musc_rmsnorm_rows_8bit': (_i, [_vp, _ll, _vp, _ll, _vp, _vp, _i, _i, _i, _i, _f, _i, _i, _vp, _vp, _vp]),
     'musc_rotary': (_i, [_vp, _i, _ll, _ll, _ll, _vp, _ll, _ll, _ll, _vp, _i, _ll, _ll, _ll, _vp, _ll, _ll, _ll,
@@ -198,6 +215,24 @@ def require_no_gradient(*tensors) -> None:
     """Operators without a backward pass refuse inputs that ask for one."""
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise ValueError('this operator has no backward pass: call it under torch.no_grad() or detach its inputs')
+
+
+def token_strides(x: torch.Tensor) -> list[int]:
+    """Batch, token and head strides of a (B, T, heads, D) tensor in elements; a dimension of
+    one element has none."""
+    return [st if n > 1 else 0 for n, st in zip(x.shape[:3], x.stride()[:3])]
+
+
+def output_like(out: torch.Tensor | None, x: torch.Tensor, name: str) -> torch.Tensor:
+    """A new contiguous tensor like x, or the caller's `out` if it can be written as one."""
+    if out is None:
+        return torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    require_device_tensor(out, name)
+    if out.shape != x.shape or out.dtype != x.dtype or out.device != x.device or out.stride(-1) != 1:
+        raise ValueError(f'{name} must match its input in shape, dtype and device, its last dimension contiguous')
+    if 0 in [st for n, st in zip(out.shape, out.stride()) if n > 1]:
+        raise ValueError(f'{name} has elements that share memory')
+    return out
 
 
 def workspace(nbytes: int, device: torch.device) -> torch.Tensor:

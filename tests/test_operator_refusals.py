@@ -62,3 +62,58 @@ def rotary_args(**kw):
     (dict(d=512, pairs=256, t=0), OK), (dict(batch=0), OK)])
 def test_rotary(lib, change, code):
     assert lib.musc_rotary(*rotary_args(**change)) == code
+
+
+def attention_call(**kw):
+    from musc_hip import _runtime as rt
+    c = rt.MaskedAttention()
+    for x in 'qkv':
+        setattr(c, x, 4096)
+        for s, n in (('sb', 64 * 64 * 2), ('st', 128), ('sh', 64)):
+            setattr(c, f'{x}_{s}', n)
+    c.out, c.o_sb, c.o_st, c.o_sh = 4096, 64 * 64 * 2, 128, 64
+    c.dtype, c.batch, c.q_len, c.k_len, c.heads, c.kv_heads, c.d, c.scale = 1, 2, 64, 64, 2, 2, 64, 0.125
+    for name, value in kw.items():
+        setattr(c, name, value)
+    return c
+
+
+@pytest.mark.parametrize('change,code', [
+    (dict(q=0), INVALID), (dict(out=0), INVALID), (dict(dtype=3), INVALID), (dict(batch=0), INVALID),
+    (dict(q_len=0), INVALID), (dict(k_len=0), INVALID), (dict(heads=3), INVALID), (dict(kv_heads=0), INVALID),
+    (dict(d=136), UNSUPPORTED), (dict(d=60), UNSUPPORTED), (dict(dtype=0, d=66), UNSUPPORTED), (dict(q=4104), INVALID),
+    (dict(k_st=130), INVALID), (dict(v_sh=-64), INVALID), (dict(o_st=4), INVALID), (dict(k_st=1 << 28), UNSUPPORTED),
+    (dict(cap=-1.0), INVALID), (dict(cap=float('nan')), INVALID), (dict(scale=float('inf')), INVALID),
+    (dict(q_documents=4096), INVALID), (dict(q_documents=4096, k_documents=4096), INVALID),
+    (dict(q_documents=4096, k_documents=4096, k_summary=4100), INVALID),
+    (dict(q_order=4096, k_order=4096), INVALID), (dict(q_documents=4098, k_documents=4096, k_summary=4096), INVALID),
+    (dict(q_documents=4096, k_documents=4096, k_summary=4096, q_order=4096), INVALID),
+    (dict(axes=4), UNSUPPORTED), (dict(axes=1), INVALID), (dict(axes=1, q_positions=4096, k_positions=4096), INVALID),
+    (dict(q_tokens_sb=-1), INVALID), (dict(batch=1 << 20, kv_heads=2, q_len=1 << 20), UNSUPPORTED)])
+def test_masked_attention(lib, change, code):
+    need = ctypes.c_size_t()
+    call = attention_call(**change)
+    assert lib.musc_masked_attention_workspace_bytes(call, ctypes.byref(need)) == code
+    assert lib.musc_masked_attention_fwd(call, None, ctypes.c_size_t(0), None) == code
+
+
+def test_masked_attention_workspace(lib):
+    need = ctypes.c_size_t(1)
+    assert lib.musc_masked_attention_workspace_bytes(None, ctypes.byref(need)) == INVALID
+    assert lib.musc_masked_attention_workspace_bytes(attention_call(), None) == INVALID
+    # a full grid is not split; one row over many keys is, and refuses to run without its parts
+    assert lib.musc_masked_attention_workspace_bytes(attention_call(batch=64, q_len=1024), ctypes.byref(need)) == OK
+    assert need.value == 0
+    one = attention_call(q_len=1, k_len=4096)
+    assert lib.musc_masked_attention_workspace_bytes(one, ctypes.byref(need)) == OK and need.value > 0
+    assert lib.musc_masked_attention_fwd(one, None, need, None) == WORKSPACE
+    assert lib.musc_masked_attention_fwd(one, P, ctypes.c_size_t(need.value - 1), None) == WORKSPACE
+    assert lib.musc_masked_attention_fwd(one, ctypes.c_void_p(4100), need, None) == WORKSPACE
+
+
+@pytest.mark.parametrize('args,code', [
+    ((None, None, 1, 64, P, None), INVALID), ((P, None, 1, 64, None, None), INVALID), ((P, P, -1, 64, P, None), INVALID),
+    ((ctypes.c_void_p(4098), None, 1, 64, P, None), INVALID), ((P, None, 1, 64, ctypes.c_void_p(4104), None), INVALID),
+    ((P, None, 0, 64, P, None), OK), ((P, None, 1 << 16, 1 << 16, P, None), UNSUPPORTED)])
+def test_token_summary(lib, args, code):
+    assert lib.musc_token_summary(*args) == code
