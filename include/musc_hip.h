@@ -390,7 +390,7 @@ typedef struct musc_masked_attention {
   int batch, q_len, k_len;
   int heads, kv_heads;    /* query head h reads key head h / (heads / kv_heads) */
   int d;                  /* multiple of 16 bytes, at most 128 channels */
-  float scale, cap;       /* cap 0: none */
+  float scale, cap;       /* cap 0: none; other magnitudes of both within 2^-60 .. 2^60 */
   /* documents (and orders): int32, token t of batch entry b at b * tokens_sb + t; tokens_sb 0
    * shares one row between the batch.  Both sides' documents or neither (every key is seen);
    * both orders or neither. */

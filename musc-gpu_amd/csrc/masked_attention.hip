@@ -22,15 +22,19 @@
 #include <hip/hip_bf16.h>
 #include <hip/hip_fp16.h>
 
+#include <type_traits>
+
 #include "common.hpp"
 
 namespace musc {
 namespace mattn {
 
 typedef float floatx16 __attribute__((ext_vector_type(16)));
+typedef float float2v __attribute__((ext_vector_type(2)));
+typedef int int4v __attribute__((ext_vector_type(4)));
 typedef short short4v __attribute__((ext_vector_type(4)));
-typedef _Float16 half8 __attribute__((ext_vector_type(8)));
-typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
+typedef short short8v __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(3))) void lds_void;
 
 constexpr int kBufferFlags = 0x00020000;   // buffer resource word 3 for raw byte-addressed loads
 constexpr int kNowhere = 0x7fffff00;       // a byte offset past every extent: such loads give zeros
@@ -50,7 +54,8 @@ struct Type<MUSC_DTYPE_F32> {
 template <>
 struct Type<MUSC_DTYPE_F16> {
   typedef _Float16 T;
-  typedef half8 Vec;
+  typedef T Vec __attribute__((ext_vector_type(8)));
+  typedef T Two __attribute__((ext_vector_type(2)));
   static constexpr int kTile = 64;
   // probabilities are formed 2^7 times as large, at most 2^15 with the slack: entries down to
   // 2^-21 of the largest stay normal fp16 numbers
@@ -58,17 +63,33 @@ struct Type<MUSC_DTYPE_F16> {
   static __device__ __forceinline__ floatx16 mfma(Vec a, Vec b, floatx16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
   }
+  static __device__ __forceinline__ float add_both(Two p, float sum) {
+    return __builtin_amdgcn_fdot2(p, Two{(T)1.f, (T)1.f}, sum, false);
+  }
 };
 template <>
 struct Type<MUSC_DTYPE_BF16> {
   typedef __bf16 T;
-  typedef bf8 Vec;
+  typedef T Vec __attribute__((ext_vector_type(8)));
+  typedef T Two __attribute__((ext_vector_type(2)));
   static constexpr int kTile = 64;
   static constexpr float kShift = 0.f;
   static __device__ __forceinline__ floatx16 mfma(Vec a, Vec b, floatx16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
   }
+  static __device__ __forceinline__ float add_both(Two p, float sum) {
+    return __builtin_amdgcn_fdot2_f32_bf16(p, Two{(T)1.f, (T)1.f}, sum, false);
+  }
 };
+
+// Staged rows of K and V: 128, 256 or 512 bytes, their 16-byte chunks permuted by the row so
+// that the lanes one LDS read serves together touch different banks: 16 neighbouring rows of
+// one chunk (K's operands) take 16 places of a 256-byte window, and so do 4 neighbouring rows
+// of 4 chunks (V's transposing reads).  Chunk c of row r is at place c ^ swizzle(r).
+template <int kPitch>
+__device__ __forceinline__ constexpr int swizzle(int r) {
+  return kPitch == 128 ? (((r >> 1) & 1) << 2) | ((r >> 2) & 3) : ((r & 3) << 2) | ((r >> 2) & 3);
+}
 
 struct Args {
   musc_masked_attention c;
@@ -127,50 +148,63 @@ __global__ __launch_bounds__(256) void token_summary_kernel(const int* __restric
   if (threadIdx.x % kSummaryKeys == 0) summary[g] = s;
 }
 
-// tanh for 16-bit operands: 1 - 2 / (1 + e^2x), absolute error a few 2^-24
-__device__ __forceinline__ float tanh_fast(float x) {
-  return fmaf(-2.f, __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(2.f * kLog2e * x)), 1.f);
+// Loads straight from memory into LDS, lane l's 16 (or 4) bytes to `to` + 16 l (or 4 l), `to`
+// uniform.  From inline assembly, as the compiler, which cannot tell the two buffers apart,
+// would wait for them before reading the other one; the loop waits for them itself.
+__device__ __forceinline__ void load_to_lds_16(uint32_t to, int offset, int4v from) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+               :: "s"(to), "v"(offset), "s"(from) : "memory", "m0");
+}
+__device__ __forceinline__ void load_to_lds_4(const void* place, int offset, int4v from) {
+  const uint32_t to = __builtin_amdgcn_readfirstlane((uint32_t)(size_t)(lds_void*)place);
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
+               :: "s"(to), "v"(offset), "s"(from) : "memory", "m0");
+}
+__device__ __forceinline__ int4v resource(const void* base, long long bytes) {
+  const unsigned long long at = reinterpret_cast<unsigned long long>(base);
+  return int4v{__builtin_amdgcn_readfirstlane((int)(uint32_t)at), __builtin_amdgcn_readfirstlane((int)(uint32_t)(at >> 32)),
+               __builtin_amdgcn_readfirstlane((int)bytes), kBufferFlags};
 }
 
 // kWaves waves of 32 rows each; kD: head width rounded up to 64, 96 or 128.
 template <int kDtype, int kD, int kWaves>
-__global__ __launch_bounds__(kWaves * kWave) void masked_attention_kernel(const Args a) {
+__global__ __launch_bounds__(kWaves * kWave, kWaves > 1 ? 2 : 1) void masked_attention_kernel(const Args a) {
   using Ty = Type<kDtype>;
   typedef typename Ty::T T;
   constexpr bool k16 = kDtype != MUSC_DTYPE_F32;
   constexpr int kTile = Ty::kTile, kSub = kTile / 32;
-  constexpr int kPer = 16 / (int)sizeof(T);            // elements of a 16-byte vector
-  constexpr int kPitch = kD + kPer;                    // elements of a staged row
-  constexpr int kBuffers = kWaves > 1 ? 2 : 1;         // one wave reads a tile before it stores the next
-  constexpr int kThreads = kWaves * kWave;
-  constexpr int kChunks = kTile * (kD / kPer) / kThreads;  // vectors of K (and of V) a thread stages
-  static_assert(kTile * (kD / kPer) % kThreads == 0, "whole vectors per thread");
+  constexpr int kPer = 16 / (int)sizeof(T);                 // elements of a 16-byte chunk
+  constexpr int kPitch = (kD <= 64 ? 64 : 128) * (int)sizeof(T);
+  constexpr int kPlaces = kPitch / 16;                      // chunks of a staged row
+  constexpr int kPart = kTile * kPitch;                     // bytes of a staged K or V tile
+  constexpr int kLoads = kPart / 1024 / kWaves;             // loads of K (and of V) per wave
+  static_assert(kLoads * kWaves * 1024 == kPart, "whole loads per wave");
   constexpr int kO = kD / 32;
-  __shared__ __attribute__((aligned(16))) T Ks[kBuffers][kTile * kPitch];
-  __shared__ __attribute__((aligned(16))) T Vs[kBuffers][kTile * kPitch];
-  __shared__ __attribute__((aligned(16))) int docs_s[kBuffers][kTile], ords_s[kBuffers][kTile];
+  __shared__ __attribute__((aligned(1024))) char staged[2][2 * kPart];
+  __shared__ __attribute__((aligned(16))) int docs_s[2][64], ords_s[2][64];
+  __shared__ float pos_s[2][64 * kMaxAxes];
   __shared__ Range ranges[kWaves];
 
   const musc_masked_attention& c = a.c;
   const long long unit = xcd_logical_id(blockIdx.x, gridDim.x);
   if (unit >= a.units) return;
   const int split = (int)(unit % a.splits);
-  const int row_tile = (int)(unit / a.splits % a.row_tiles);
+  // later rows first: with an order they see more keys, and the longest work should not start last
+  const int row_tile = a.row_tiles - 1 - (int)(unit / a.splits % a.row_tiles);
   const long long bh = unit / a.splits / a.row_tiles;
   const int b = (int)(bh / c.kv_heads), kvh = (int)(bh % c.kv_heads);
-  const int tid = threadIdx.x, wave = tid / kWave, lane = tid % kWave;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid % kWave;
   const int lq = lane & 31, lh = lane >> 5;
   const int row = (row_tile * kWaves + wave) * 32 + lq;
   const bool inside = row < a.rows;
   const int token = inside ? row / a.group : 0;
   const int head = kvh * a.group + (inside ? row % a.group : 0);
-  const int d = c.d, k_len = c.k_len;
+  const int d = c.d, k_len = c.k_len, axes = c.axes;
 
   // this row's document and order; rows outside the tensor and padding have none
-  int qdoc = -2, qord = 0;
+  int qdoc = -1, qord = 0;
   if (inside) {
     qdoc = c.q_documents ? c.q_documents[b * c.q_tokens_sb + token] : 0;
-    if (qdoc < 0) qdoc = -2;
     if (c.q_order) qord = c.q_order[b * c.q_tokens_sb + token];
   }
   const bool live = qdoc >= 0;
@@ -192,125 +226,149 @@ __global__ __launch_bounds__(kWaves * kWave) void masked_attention_kernel(const 
     }
   }
 
-  // Q fragments, zeros past d
+  // keys of calls without documents or orders have 0
+  if (tid < 64) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) docs_s[i][tid] = 0, ords_s[i][tid] = 0;
+  }
+  __syncthreads();
+
+  // Q fragments, zeros past d.  Scores stay "raw" until the exponential: score in log2 units =
+  // raw * to_log2 (+ a constant that cancels), to_log2 > 0:
+  //   no cap   raw = +- q . k (Q negated for a negative scale), to_log2 = |scale| log2 e
+  //   cap      raw = -1 / (1 + e^2x), x = scale q . k / cap, as cap tanh x = cap (1 + 2 raw);
+  //            fp32: raw = tanh x
+  const bool capped = c.cap > 0.f;
+  const float scale = c.scale == 0.f ? 1.f : c.scale;
+  const float to_log2 = (capped ? (k16 ? 2.f * c.cap : c.cap) : fabsf(scale)) * kLog2e;
+  const float by_cap = capped ? scale / c.cap * (k16 ? 2.f * kLog2e : 1.f) : 0.f;
+  const bool negate = !capped && scale < 0.f;
   const T* qrow = static_cast<const T*>(c.q) + b * c.q_sb + (long long)token * c.q_st + head * c.q_sh;
-  constexpr int kQ = k16 ? kD / 16 : kD / 8;
+  constexpr int kQ = kD / (2 * kPer);
   typedef T TVec __attribute__((ext_vector_type(kPer)));
   TVec qf[kQ];
 #pragma unroll
   for (int m = 0; m < kQ; ++m) {
-    const int at = (k16 ? 16 * m + 8 * lh : 8 * m + 4 * lh);
+    const int at = (2 * m + lh) * kPer;
     TVec x = {};
-    if (live && at < d) x = *reinterpret_cast<const TVec*>(qrow + at);
-    qf[m] = x;
+    if (live && at < d && c.scale != 0.f) x = *reinterpret_cast<const TVec*>(qrow + at);
+    qf[m] = negate ? -x : x;
   }
-  const int axes = c.axes;
-  float qpos[kMaxAxes], slope[kMaxAxes];  // the B operand of the distances: 1 and -position
+  float qpos[kMaxAxes], slope[kMaxAxes];  // the B operand of the distances: 1 and -position; raw slopes
 #pragma unroll
   for (int x = 0; x < kMaxAxes; ++x) {
     qpos[x] = 0.f, slope[x] = 0.f;
     if (x < axes) {
       const float p = c.q_positions[b * c.q_positions_sb + (long long)token * axes + x];
       qpos[x] = lh == 0 ? 1.f : -p;
-      slope[x] = c.slopes[head * axes + x] * kLog2e;
+      slope[x] = c.slopes[head * axes + x] * kLog2e / to_log2;
     }
   }
-  const float scale_log2 = c.scale * kLog2e;
-  const float cap_log2 = c.cap * kLog2e, scale_by_cap = c.cap > 0.f ? c.scale / c.cap : 0.f;
 
   // tiles of this split
   const int lo = (int)((long long)a.key_tiles * split / a.splits);
   const int hi = (int)((long long)a.key_tiles * (split + 1) / a.splits);
 
-  // K and V rows of a tile through buffer resources that end with the last key
-  const T* kbase = static_cast<const T*>(c.k) + b * c.k_sb + (long long)kvh * c.k_sh;
-  const T* vbase = static_cast<const T*>(c.v) + b * c.v_sb + (long long)kvh * c.v_sh;
-  TVec kreg[kChunks], vreg[kChunks];
-  int dreg = 0, oreg = 0;
-  float kpos[kMaxAxes][kSub], kpos_next[kMaxAxes][kSub];
-  auto load_tile = [&](int tile) {
+  // Staging: load i of a tile fills 1024 bytes, whole rows; wave w issues loads w, w + kWaves, ..
+  const char* kbase = reinterpret_cast<const char*>(static_cast<const T*>(c.k) + b * c.k_sb + (long long)kvh * c.k_sh);
+  const char* vbase = reinterpret_cast<const char*>(static_cast<const T*>(c.v) + b * c.v_sb + (long long)kvh * c.v_sh);
+  const long long k_row = c.k_st * (long long)sizeof(T), v_row = c.v_st * (long long)sizeof(T);
+  const uint32_t staged_at = (uint32_t)(size_t)(lds_void*)&staged[0][0];
+  auto load_tile = [&](int tile, int buf) __attribute__((always_inline)) {
     const int first = tile * kTile, rem = min(k_len - first, kTile);
-    const auto rk = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(kbase + (long long)first * c.k_st), (short)0,
-                                                      (int)(((rem - 1) * c.k_st + d) * (int)sizeof(T)), kBufferFlags);
-    const auto rv = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(vbase + (long long)first * c.v_st), (short)0,
-                                                      (int)(((rem - 1) * c.v_st + d) * (int)sizeof(T)), kBufferFlags);
+    const int4v rk = resource(kbase + first * k_row, (rem - 1) * k_row + d * (int)sizeof(T));
+    const int4v rv = resource(vbase + first * v_row, (rem - 1) * v_row + d * (int)sizeof(T));
 #pragma unroll
-    for (int i = 0; i < kChunks; ++i) {
-      const int e = i * kThreads + tid, key = e / (kD / kPer), at = e % (kD / kPer) * kPer;
-      const int ko = at < d ? (int)((key * c.k_st + at) * (int)sizeof(T)) : kNowhere;
-      const int vo = at < d ? (int)((key * c.v_st + at) * (int)sizeof(T)) : kNowhere;
-      kreg[i] = __builtin_bit_cast(TVec, __builtin_amdgcn_raw_buffer_load_b128(rk, ko, 0, 0));
-      vreg[i] = __builtin_bit_cast(TVec, __builtin_amdgcn_raw_buffer_load_b128(rv, vo, 0, 0));
+    for (int j = 0; j < kLoads; ++j) {
+      const int i = wave + kWaves * j;
+      const int r = i * (64 / kPlaces) + lane / kPlaces, chunk = (lane % kPlaces) ^ swizzle<kPitch>(r);
+      const bool there = chunk * kPer < d;
+      const uint32_t to = __builtin_amdgcn_readfirstlane(staged_at + buf * 2 * kPart + i * 1024);
+      load_to_lds_16(to, there ? (int)(r * k_row) + chunk * 16 : kNowhere, rk);
+      load_to_lds_16(to + kPart, there ? (int)(r * v_row) + chunk * 16 : kNowhere, rv);
     }
-    if (tid < kTile) {
-      const int key = first + tid;
-      dreg = key < k_len ? 0 : -1, oreg = 0;
-      if (key < k_len && c.k_documents) dreg = max(c.k_documents[b * c.k_tokens_sb + key], -1);
-      if (key < k_len && c.k_order) oreg = c.k_order[b * c.k_tokens_sb + key];
+    if (wave == kWaves - 1) {
+      if (c.k_documents)
+        load_to_lds_4(&docs_s[buf][0], lane * 4,
+                      resource(c.k_documents + b * c.k_tokens_sb + first, rem * 4));
+      if (c.k_order)
+        load_to_lds_4(&ords_s[buf][0], lane * 4,
+                      resource(c.k_order + b * c.k_tokens_sb + first, rem * 4));
+      if (axes) {
+        const int4v rp = resource(c.k_positions + b * c.k_positions_sb + (long long)first * axes, rem * axes * 4);
+#pragma unroll
+        for (int x = 0; x < kMaxAxes; ++x)
+          if (x < axes) load_to_lds_4(&pos_s[buf][64 * x], (64 * x + lane) * 4, rp);
+      }
     }
-#pragma unroll
-    for (int x = 0; x < kMaxAxes; ++x)
-      if (x < axes)
-#pragma unroll
-        for (int s = 0; s < kSub; ++s) {
-          const int key = min(first + 32 * s + lq, k_len - 1);
-          kpos_next[x][s] = c.k_positions[b * c.k_positions_sb + (long long)key * axes + x];
-        }
-  };
-  auto store_tile = [&](int buf) {
-#pragma unroll
-    for (int i = 0; i < kChunks; ++i) {
-      const int e = i * kThreads + tid, key = e / (kD / kPer), at = e % (kD / kPer) * kPer;
-      *reinterpret_cast<TVec*>(&Ks[buf][key * kPitch + at]) = kreg[i];
-      *reinterpret_cast<TVec*>(&Vs[buf][key * kPitch + at]) = vreg[i];
-    }
-    if (tid < kTile) docs_s[buf][tid] = dreg, ords_s[buf][tid] = oreg;
-#pragma unroll
-    for (int x = 0; x < kMaxAxes; ++x)
-#pragma unroll
-      for (int s = 0; s < kSub; ++s) kpos[x][s] = kpos_next[x][s];
   };
 
   floatx16 o[kO];
-  float m_run, l_run;
+  float m_run, l_run;  // running maximum (raw) and sum of this half's keys
+  float base;          // exponent of a score: raw * to_log2 + base
   bool mixed_seen;
 
   // one staged tile; whole: every row sees every key.  careful: in a mixed tile, products
   // of keys that a row does not see are left out one by one (their V may be infinite or NaN)
-  auto attend = [&](int buf, bool whole, bool careful) {
+  auto attend = [&](int buf, int tile, bool whole, auto careful_c) __attribute__((always_inline)) {
+    constexpr bool careful = decltype(careful_c)::value;
+    const char* ks = staged[buf];
+    const char* vs = staged[buf] + kPart;
     floatx16 s[kSub];
+    TVec kf[kSub][kQ];
 #pragma unroll
-    for (int u = 0; u < kSub; ++u) {
+    for (int u = 0; u < kSub; ++u)
+#pragma unroll
+      for (int m = 0; m < kQ; ++m)
+        kf[u][m] = *reinterpret_cast<const TVec*>(ks + (32 * u + lq) * kPitch + ((2 * m + lh) ^ swizzle<kPitch>(lq)) * 16);
+    __builtin_amdgcn_sched_barrier(0);  // all reads in flight before the first product waits
+#pragma unroll
+    for (int u = 0; u < kSub; ++u)
 #pragma unroll
       for (int v = 0; v < 16; ++v) s[u][v] = 0.f;
-      const T* krow = &Ks[buf][(32 * u + lq) * kPitch];
-      if constexpr (k16) {
 #pragma unroll
-        for (int m = 0; m < kQ; ++m)
-          s[u] = Ty::mfma(*reinterpret_cast<const TVec*>(krow + 16 * m + 8 * lh), qf[m], s[u]);
-      } else {
+    for (int m = 0; m < kQ; ++m)
 #pragma unroll
-        for (int m = 0; m < kQ; ++m) {
-          const TVec x = *reinterpret_cast<const TVec*>(krow + 8 * m + 4 * lh);
+      for (int u = 0; u < kSub; ++u) {
+        if constexpr (k16) {
+          s[u] = Ty::mfma(kf[u][m], qf[m], s[u]);
+        } else {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) s[u] = __builtin_amdgcn_mfma_f32_32x32x2f32(x[j], qf[m][j], s[u], 0, 0, 0);
+          for (int j = 0; j < 4; ++j) s[u] = __builtin_amdgcn_mfma_f32_32x32x2f32(kf[u][m][j], qf[m][j], s[u], 0, 0, 0);
         }
       }
+    // V^T fragments by transposing LDS reads, in flight during the softmax: within a group of 16
+    // lanes, lane i's element j is element i % 4 of the 8 bytes that lane 4 j + i / 4 addressed,
+    // so with V row-major the lane that addresses V[key0 + r / 4][d0 + 4 (r % 4) ..] (r its place
+    // in the group) hands element j of lane i the value V[key0 + j][d0 + i]: the A operand's row
+    // d0 + i, k = j
+    short8v vf[k16 && !careful ? 2 * kSub : 1][k16 && !careful ? kO : 1];
+    auto read_v = [&](int mm, int x) {
+      auto tr = [&](int upper) {
+        const int r = 16 * mm + 8 * upper + 4 * lh + ((lq & 15) >> 2);
+        const int chunk = 4 * x + 2 * (lq >> 4) + ((lq & 3) >> 1);
+        typedef __attribute__((address_space(3))) short4v lds_short4v;
+        return __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (lds_short4v*)(vs + r * kPitch + (chunk ^ swizzle<kPitch>(r)) * 16 + 8 * (lq & 1)));
+      };
+      const short4v f0 = tr(0), f1 = tr(1);
+      return short8v{f0[0], f0[1], f0[2], f0[3], f1[0], f1[1], f1[2], f1[3]};
+    };
+    if constexpr (k16 && !careful) {
+#pragma unroll
+      for (int mm = 0; mm < 2 * kSub; ++mm)
+#pragma unroll
+        for (int x = 0; x < kO; ++x) vf[mm][x] = read_v(mm, x);
+      __builtin_amdgcn_sched_barrier(0);
     }
-    // scores in log2 units
-    if (cap_log2 > 0.f) {
+    if (capped) {
 #pragma unroll
       for (int u = 0; u < kSub; ++u)
 #pragma unroll
         for (int v = 0; v < 16; ++v) {
-          const float x = s[u][v] * scale_by_cap;
-          s[u][v] = cap_log2 * (k16 ? tanh_fast(x) : tanhf(x));
+          const float x = s[u][v] * by_cap;
+          s[u][v] = k16 ? __builtin_amdgcn_rcpf(-1.f - __builtin_amdgcn_exp2f(x)) : tanhf(x);
         }
-    } else {
-#pragma unroll
-      for (int u = 0; u < kSub; ++u)
-#pragma unroll
-        for (int v = 0; v < 16; ++v) s[u][v] *= scale_log2;
     }
     // distances from the matrix cores: position(j) * 1 + 1 * -position(i), exact in fp32
 #pragma unroll
@@ -321,7 +379,8 @@ __global__ __launch_bounds__(kWaves * kWave) void masked_attention_kernel(const 
           floatx16 apart;
 #pragma unroll
           for (int v = 0; v < 16; ++v) apart[v] = 0.f;
-          apart = __builtin_amdgcn_mfma_f32_32x32x2f32(lh == 0 ? kpos[x][u] : 1.f, qpos[x], apart, 0, 0, 0);
+          const float kp = pos_s[buf][(32 * u + lq) * axes + x];
+          apart = __builtin_amdgcn_mfma_f32_32x32x2f32(lh == 0 ? kp : 1.f, qpos[x], apart, 0, 0, 0);
 #pragma unroll
           for (int v = 0; v < 16; ++v) s[u][v] = fmaf(-slope[x], fabsf(apart[v]), s[u][v]);
         }
@@ -329,19 +388,19 @@ __global__ __launch_bounds__(kWaves * kWave) void masked_attention_kernel(const 
     uint32_t seen = 0xffffffffu;
     if (!whole) {
       mixed_seen = true;
-      seen = 0;
+      const int rem = k_len - tile * kTile;
 #pragma unroll
       for (int u = 0; u < kSub; ++u)
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-          const int4 kd = *reinterpret_cast<const int4*>(&docs_s[buf][32 * u + 8 * g + 4 * lh]);
-          const int4 ko = *reinterpret_cast<const int4*>(&ords_s[buf][32 * u + 8 * g + 4 * lh]);
-          const bool see[4] = {kd.x == qdoc && ko.x <= qord, kd.y == qdoc && ko.y <= qord,
-                               kd.z == qdoc && ko.z <= qord, kd.w == qdoc && ko.w <= qord};
+          const int key = 32 * u + 8 * g + 4 * lh;
+          const int4v kd = *reinterpret_cast<const int4v*>(&docs_s[buf][key]);
+          const int4v ko = *reinterpret_cast<const int4v*>(&ords_s[buf][key]);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            if (!see[i]) s[u][4 * g + i] = -INFINITY;
-            if (see[i]) seen |= 1u << (16 * u + 4 * g + i);
+            const bool see = kd[i] == qdoc && ko[i] <= qord && key + i < rem;
+            s[u][4 * g + i] = see ? s[u][4 * g + i] : -INFINITY;
+            if (careful && !see) seen &= ~(1u << (16 * u + 4 * g + i));
           }
         }
     }
@@ -351,86 +410,89 @@ __global__ __launch_bounds__(kWaves * kWave) void masked_attention_kernel(const 
 #pragma unroll
       for (int v = 0; v < 16; ++v) top = __builtin_elementwise_maximum(top, s[u][v]);
     top = halves_max(top);
-    if (!__all(top <= m_run + kLazyLog2)) {
+    if (!__all((top - m_run) * to_log2 <= kLazyLog2)) {  // false at first, and for NaN
       const float m_new = fmaxf(m_run, top);
-      const float alpha = __builtin_amdgcn_exp2f(m_run - (m_new == -INFINITY ? 0.f : m_new));  // 0 at first
+      const float alpha = m_run == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m_run - m_new) * to_log2);
       l_run *= alpha;
 #pragma unroll
       for (int x = 0; x < kO; ++x)
 #pragma unroll
         for (int v = 0; v < 16; ++v) o[x][v] *= alpha;
       m_run = m_new;
+      base = Ty::kShift - (m_run == -INFINITY ? 0.f : m_run * to_log2);
     }
-    const float base = (m_run == -INFINITY ? 0.f : m_run) - Ty::kShift;  // nothing seen yet: e^-inf = 0
-    float sum = 0.f;
 #pragma unroll
     for (int u = 0; u < kSub; ++u)
 #pragma unroll
-      for (int v = 0; v < 16; ++v) {
-        s[u][v] = __builtin_amdgcn_exp2f(s[u][v] - base);
-        sum += s[u][v];
-      }
-    l_run += sum;  // this half's keys
+      for (int v = 0; v < 16; ++v) s[u][v] = __builtin_amdgcn_exp2f(fmaf(s[u][v], to_log2, base));
+    TVec p[2 * kSub];
+    if constexpr (k16) {
+#pragma unroll
+      for (int mm = 0; mm < 2 * kSub; ++mm)
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) {
+          const float2v f = {s[mm >> 1][8 * (mm & 1) + j], s[mm >> 1][8 * (mm & 1) + j + 1]};
+          const auto two = __builtin_convertvector(f, typename Ty::Two);
+          p[mm][j] = two[0], p[mm][j + 1] = two[1];
+          l_run = Ty::add_both(two, l_run);  // the sum of what the product uses
+        }
+    } else {
+#pragma unroll
+      for (int u = 0; u < kSub; ++u)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) l_run += s[u][v];
+    }
     if (careful && !whole) {
+#pragma unroll 1
       for (int key = 0; key < kTile; ++key) {
         const int u0 = key >> 5, v0 = ((key & 31) >> 3) * 4 + (key & 3), from = lq + 32 * ((key >> 2) & 1);
-        float p = 0.f;
+        float pr = 0.f;
 #pragma unroll
         for (int u = 0; u < kSub; ++u)
 #pragma unroll
           for (int v = 0; v < 16; ++v)
-            if (u == u0 && v == v0) p = s[u][v];
-        p = __shfl(p, from, kWave);
+            if (u == u0 && v == v0) pr = (float)(T)s[u][v];
+        pr = __shfl(pr, from, kWave);
         const bool see = (__shfl(seen, from, kWave) >> (16 * u0 + v0)) & 1;
-        const T* vrow = &Vs[buf][key * kPitch];
 #pragma unroll
         for (int x = 0; x < kO; ++x)
 #pragma unroll
           for (int v = 0; v < 16; ++v) {
-            const float value = (float)vrow[32 * x + 8 * (v >> 2) + 4 * lh + (v & 3)];
-            if (see) o[x][v] = fmaf(p, value, o[x][v]);
+            if (v % 4 == 0) __builtin_amdgcn_sched_barrier(0);  // few values at a time
+            const int at = 32 * x + 8 * (v >> 2) + 4 * lh + (v & 3);
+            const T value = *reinterpret_cast<const T*>(vs + key * kPitch + ((at / kPer) ^ swizzle<kPitch>(key)) * 16 +
+                                                        at % kPer * (int)sizeof(T));
+            if (see) o[x][v] = fmaf(pr, (float)value, o[x][v]);
           }
       }
       return;
     }
     if constexpr (k16) {
-      // V^T fragments by transposing LDS reads: within a group of 16 lanes, lane i's element j
-      // is element i % 4 of the 8 bytes that lane 4 j + i / 4 addressed, so with V row-major the
-      // lane that addresses V[key0 + r / 4][d0 + 4 (r % 4) ..] (r its place in the group) hands
-      // element j of lane i the value V[key0 + j][d0 + i]: the A operand's row d0 + i, k = j
-      const T* vb = &Vs[buf][(4 * lh + ((lq & 15) >> 2)) * kPitch + 16 * (lq >> 4) + 4 * (lq & 3)];
-      auto tr = [&](int off) {
-        typedef __attribute__((address_space(3))) short4v lds_short4v;
-        return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4v*)(vb + off));
-      };
 #pragma unroll
-      for (int mm = 0; mm < 2 * kSub; ++mm) {
-        TVec p;
+      for (int mm = 0; mm < 2 * kSub; ++mm)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) p[j] = (T)s[mm >> 1][8 * (mm & 1) + j];
-#pragma unroll
-        for (int x = 0; x < kO; ++x) {
-          const short4v f0 = tr(16 * mm * kPitch + 32 * x), f1 = tr((16 * mm + 8) * kPitch + 32 * x);
-          typedef short short8v __attribute__((ext_vector_type(8)));
-          const short8v f = {f0[0], f0[1], f0[2], f0[3], f1[0], f1[1], f1[2], f1[3]};
-          o[x] = Ty::mfma(__builtin_bit_cast(TVec, f), p, o[x]);
-        }
-      }
+        for (int x = 0; x < kO; ++x)
+          o[x] = Ty::mfma(__builtin_bit_cast(TVec, careful ? read_v(mm, x) : vf[careful ? 0 : mm][careful ? 0 : x]), p[mm], o[x]);
     } else {
       // step e takes keys 8 (e / 4) + 4 lh + e % 4: register e of s
 #pragma unroll
-      for (int e = 0; e < 16; ++e)
+      for (int u = 0; u < kSub; ++u)
 #pragma unroll
-        for (int x = 0; x < kO; ++x)
-          o[x] = __builtin_amdgcn_mfma_f32_32x32x2f32(Vs[buf][(8 * (e >> 2) + 4 * lh + (e & 3)) * kPitch + 32 * x + lq],
-                                                      s[0][e], o[x], 0, 0, 0);
+        for (int e = 0; e < 16; ++e)
+#pragma unroll
+          for (int x = 0; x < kO; ++x) {
+            const int r = 32 * u + 8 * (e >> 2) + 4 * lh + (e & 3);
+            const float f = *reinterpret_cast<const float*>(vs + r * kPitch + ((8 * x + (lq >> 2)) ^ swizzle<kPitch>(r)) * 16 +
+                                                            4 * (lq & 3));
+            o[x] = __builtin_amdgcn_mfma_f32_32x32x2f32(f, s[u][e], o[x], 0, 0, 0);
+          }
     }
   };
 
   // the tiles of this split that some row of the workgroup may see, 64 sorted at a time
   int chunk = 0;
   unsigned long long todo = 0, any_word = 0, whole_word = 0;
-  auto sort_tiles = [&]() {
+  auto sort_tiles = [&]() __attribute__((always_inline)) {
     const int t = chunk * 64 + lane;
     int4 k = make_int4(0, 0, 0, 0);
     const bool here = t >= lo && t < hi;
@@ -454,7 +516,7 @@ __global__ __launch_bounds__(kWaves * kWave) void masked_attention_kernel(const 
     int tile;
     bool any, whole;
   };
-  auto next_tile = [&]() -> Next {
+  auto next_tile = [&]() __attribute__((always_inline)) -> Next {
     while (todo == 0) {
       ++chunk;
       if ((long long)chunk * 64 >= hi) return Next{-1, false, false};
@@ -465,38 +527,38 @@ __global__ __launch_bounds__(kWaves * kWave) void masked_attention_kernel(const 
     return Next{chunk * 64 + bit, (bool)((any_word >> bit) & 1), (bool)((whole_word >> bit) & 1)};
   };
 
-  for (int pass = 0;; ++pass) {
+  auto walk = [&](auto careful_c) __attribute__((always_inline)) {
 #pragma unroll
     for (int x = 0; x < kO; ++x)
 #pragma unroll
       for (int v = 0; v < 16; ++v) o[x][v] = 0.f;
-    m_run = -INFINITY, l_run = 0.f, mixed_seen = false;
+    m_run = -INFINITY, l_run = 0.f, base = Ty::kShift, mixed_seen = false;
     chunk = lo / 64 - 1;
     todo = 0;
     Next now = next_tile();
-    if (now.tile >= 0) load_tile(now.tile);
+    if (now.tile >= 0) load_tile(now.tile, 0);
     int buf = 0;
     while (now.tile >= 0) {
-      store_tile(buf);
       const Next then = next_tile();
-      if (then.tile >= 0) load_tile(then.tile);
-      __syncthreads();  // a buffer is written again only past the next tile's barrier
-      if (now.any) attend(buf, now.whole, pass > 0);
-      if constexpr (kBuffers == 1) __syncthreads();
-      else buf ^= 1;
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's share of tile `now` is in LDS
+      __syncthreads();  // everyone's is, and everyone is done with the other buffer
+      if (then.tile >= 0) load_tile(then.tile, buf ^ 1);
+      if (now.any) attend(buf, now.tile, now.whole, careful_c);
+      buf ^= 1;
       now = then;
     }
-    if (pass > 0) break;
-    // 0 * V of an unseen key is NaN where V is not finite: then all over again, with care
-    bool bad = false;
-    if (mixed_seen && live) {
+  };
+  walk(std::integral_constant<bool, false>{});
+  // 0 * V of an unseen key is NaN where V is not finite: then all over again, with care
+  bool bad = false;
+  if (mixed_seen && live) {
 #pragma unroll
-      for (int x = 0; x < kO; ++x)
+    for (int x = 0; x < kO; ++x)
 #pragma unroll
-        for (int v = 0; v < 16; ++v) bad |= !(fabsf(o[x][v]) < INFINITY);
-    }
-    if (!__syncthreads_or(bad)) break;
+      for (int v = 0; v < 16; ++v) bad |= !(fabsf(o[x][v]) < INFINITY);
   }
+  // also the barrier before the buffers are filled again
+  if (__syncthreads_or(bad)) walk(std::integral_constant<bool, true>{});
 
   l_run = halves_sum(l_run);
   if (!inside) return;
@@ -519,7 +581,7 @@ __global__ __launch_bounds__(kWaves * kWave) void masked_attention_kernel(const 
   } else {
     const long long part = (bh * a.rows + row) * a.splits + split;
     if (lh == 0) {
-      a.part_ml[2 * part] = live ? m_run : -INFINITY;
+      a.part_ml[2 * part] = live ? m_run * to_log2 : -INFINITY;
       a.part_ml[2 * part + 1] = live ? l_run : 0.f;
     }
     float* prow = a.part_o + part * d;
@@ -534,41 +596,56 @@ __global__ __launch_bounds__(kWaves * kWave) void masked_attention_kernel(const 
   }
 }
 
-// Joins the splits of a row, in their order: one wave per row, two channels per lane.
+// Joins the splits of a row, in their order: four waves per row, each every fourth split with two
+// channels per lane, then the four in order.
+constexpr int kMaxSplits = 256;
 template <int kDtype>
-__global__ __launch_bounds__(256) void join_kernel(const Args a, long long total_rows) {
+__global__ __launch_bounds__(256) void join_kernel(const Args a) {
   typedef typename Type<kDtype>::T T;
+  __shared__ float weight[kMaxSplits], tops[4], sums[4];
+  __shared__ float2 parts[4][kWave];
   const musc_masked_attention& c = a.c;
-  const long long r = (long long)blockIdx.x * 4 + threadIdx.x / kWave;
-  if (r >= total_rows) return;
-  const int lane = threadIdx.x % kWave;
+  const long long r = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
+  const int splits = a.splits;
+  // the largest of the maxima, each split's factor and the sum; a part without keys has sum 0
+  // (one whose scores are NaN has its sum NaN)
+  const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + r * splits;
+  const float2 mine = tid < splits ? ml[tid] : make_float2(-INFINITY, 0.f);
+  const float top_here = wave_max(mine.x);
+  if (lane == 0) tops[wave] = top_here;
+  __syncthreads();
+  const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+  const float w = mine.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(mine.x - top);
+  if (tid < splits) weight[tid] = w;
+  const float sum_here = wave_sum(mine.y == 0.f ? 0.f : w * mine.y);
+  if (lane == 0) sums[wave] = sum_here;
+  __syncthreads();
+  const float sum = sums[0] + sums[1] + sums[2] + sums[3];
+  const bool ok = 2 * lane < c.d;
+  const float* at = a.part_o + r * splits * c.d + (ok ? 2 * lane : 0);
+  float2 y = make_float2(0.f, 0.f);
+#pragma unroll 4
+  for (int s = wave; s < splits; s += 4) {
+    const float2 p = *reinterpret_cast<const float2*>(at + (long long)s * c.d);
+    const float f = weight[s];
+    if (f != 0.f) y.x = fmaf(f, p.x, y.x), y.y = fmaf(f, p.y, y.y);
+  }
+  parts[wave][lane] = y;
+  __syncthreads();
+  if (wave != 0 || !ok) return;
+#pragma unroll
+  for (int i = 1; i < 4; ++i) y.x += parts[i][lane].x, y.y += parts[i][lane].y;
+  const float inv = 1.f / sum;
   const long long bh = r / a.rows;
   const int row = (int)(r % a.rows), token = row / a.group;
   const int head = (int)(bh % c.kv_heads) * a.group + row % a.group;
-  const float* ml = a.part_ml + 2 * r * a.splits;
-  float top = -INFINITY;
-  for (int s = 0; s < a.splits; ++s) top = fmaxf(top, ml[2 * s]);
-  float sum = 0.f, y0 = 0.f, y1 = 0.f;
-  const bool ok = 2 * lane < c.d;
-  for (int s = 0; s < a.splits; ++s) {
-    const float m = ml[2 * s];
-    if (ml[2 * s + 1] == 0.f) continue;  // nothing seen (a part whose scores are NaN has its sum NaN)
-    const float w = __builtin_amdgcn_exp2f(m - top);
-    sum = fmaf(w, ml[2 * s + 1], sum);
-    if (ok) {
-      const float2 p = *reinterpret_cast<const float2*>(a.part_o + (r * a.splits + s) * c.d + 2 * lane);
-      y0 = fmaf(w, p.x, y0);
-      y1 = fmaf(w, p.y, y1);
-    }
-  }
-  if (!ok) return;
-  const float inv = 1.f / sum;
   typedef T Two __attribute__((ext_vector_type(2)));
-  Two y;
-  y[0] = sum == 0.f ? (T)0.f : (T)(y0 * inv);
-  y[1] = sum == 0.f ? (T)0.f : (T)(y1 * inv);
+  Two out;
+  out[0] = sum == 0.f ? (T)0.f : (T)(y.x * inv);
+  out[1] = sum == 0.f ? (T)0.f : (T)(y.y * inv);
   T* orow = static_cast<T*>(c.out) + (bh / c.kv_heads) * c.o_sb + (long long)token * c.o_st + head * c.o_sh;
-  *reinterpret_cast<Two*>(orow + 2 * lane) = y;
+  *reinterpret_cast<Two*>(orow + 2 * lane) = out;
 }
 
 // Shape of the launch: rows per workgroup, tiles and splits.
@@ -588,7 +665,7 @@ int plan(const musc_masked_attention& c, Args& a, int& waves) {
   const long long want = waves == 1 ? 2048 : 512;
   if (whole < want / 2) splits = (want + whole - 1) / whole;
   if (splits > a.key_tiles) splits = a.key_tiles;
-  if (splits > 256) splits = 256;
+  if (splits > kMaxSplits) splits = kMaxSplits;
   a.splits = splits < 1 ? 1 : (int)splits;
   a.units = whole * a.splits;
   if (a.units >= (0x100000000LL >> 8)) return MUSC_ERR_UNSUPPORTED;  // 256 threads each in one grid dimension
@@ -611,7 +688,10 @@ int check(const musc_masked_attention* c) {
   if (c->dtype != MUSC_DTYPE_F32 && c->dtype != MUSC_DTYPE_F16 && c->dtype != MUSC_DTYPE_BF16) return MUSC_ERR_INVALID_ARG;
   if (c->batch < 1 || c->q_len < 1 || c->k_len < 1 || c->heads < 1 || c->kv_heads < 1 || c->heads % c->kv_heads)
     return MUSC_ERR_INVALID_ARG;
-  if (!(c->cap >= 0.f) || c->cap > 3e38f || !(fabsf(c->scale) <= 3e38f)) return MUSC_ERR_INVALID_ARG;
+  // scores, slopes and the cap are taken relative to one another
+  const float least = 0x1p-60f, most = 0x1p60f;
+  if (!(c->cap >= 0.f) || (c->cap > 0.f && !(c->cap >= least && c->cap <= most))) return MUSC_ERR_INVALID_ARG;
+  if (!(fabsf(c->scale) <= most) || (c->scale != 0.f && fabsf(c->scale) < least)) return MUSC_ERR_INVALID_ARG;
   const int per = c->dtype == MUSC_DTYPE_F32 ? 4 : 8, size = 16 / per;
   if (c->d < 1 || c->d > 128 || c->d % per) return MUSC_ERR_UNSUPPORTED;
   if (!aligned(c->q, c->q_sb, c->q_st, c->q_sh, per) || !aligned(c->k, c->k_sb, c->k_st, c->k_sh, per) ||
@@ -650,7 +730,7 @@ void launch(const Args& a, int waves, hipStream_t stream) {
   else launch<kDtype, 128>(a, waves, stream);
   if (a.splits > 1) {
     const long long rows = (long long)a.c.batch * a.c.kv_heads * a.rows;
-    hipLaunchKernelGGL((join_kernel<kDtype>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream, a, rows);
+    hipLaunchKernelGGL((join_kernel<kDtype>), dim3((unsigned)rows), dim3(256), 0, stream, a);
   }
 }
 
