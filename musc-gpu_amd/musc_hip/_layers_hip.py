@@ -65,6 +65,8 @@ _FP8 = {torch.float8_e4m3fn: rt.FP8_E4M3, torch.float8_e5m2: rt.FP8_E5M2}
 
 def _rows(x: torch.Tensor, width: int):
     """(tensor, row stride) of x as rows of `width`; rows that no one stride reaches are copied."""
+    if x.is_contiguous():
+        return x, width
     if x.dim() == 2 and x.stride(1) == 1 and x.stride(0) >= width:
         return x, x.stride(0)
     return x.contiguous(), width
@@ -72,37 +74,43 @@ def _rows(x: torch.Tensor, width: int):
 
 def _rms(x, weight, eps, residual, dtype, group):
     rt.require_device_tensor(x, 'x')
-    if x.dtype not in _STORAGE or x.dim() < 1 or x.shape[-1] < 1:
+    if rt.elsewhere(x):
+        with torch.cuda.device(x.device):
+            return _rms(x, weight, eps, residual, dtype, group)
+    storage, index = _STORAGE.get(x.dtype), x.get_device()
+    if storage is None or x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError('x must be a float32, float16 or bfloat16 tensor with at least one column')
     rt.require_no_gradient(x, weight, residual)
     width = x.shape[-1]
     rows = x.numel() // width
+    w_ptr, w_dtype = None, rt.DTYPE_F32
     if weight is not None:
         rt.require_device_tensor(weight, 'weight')
-        if weight.device != x.device or weight.numel() != width or weight.dtype not in (x.dtype, torch.float32):
+        if weight.get_device() != index or weight.numel() != width or weight.dtype not in (x.dtype, torch.float32):
             raise ValueError("weight must be on x's device, one value per column, in x's dtype or float32")
         weight = weight.contiguous()
+        w_ptr, w_dtype = weight.data_ptr(), _STORAGE[weight.dtype]
     x2, x_stride = _rows(x, width)
-    r2, r_stride = None, 0
+    s, r_ptr, r_stride, s_ptr = None, None, 0, None
     if residual is not None:
         rt.require_device_tensor(residual, 'residual')
-        if residual.shape != x.shape or residual.dtype != x.dtype or residual.device != x.device:
+        if residual.shape != x.shape or residual.dtype != x.dtype or residual.get_device() != index:
             raise ValueError('residual must match x in shape, dtype and device')
         r2, r_stride = _rows(residual, width)
-    w_ptr, w_dtype = (None, rt.DTYPE_F32) if weight is None else (weight.data_ptr(), _STORAGE[weight.dtype])
-    with torch.cuda.device(x.device):
-        s = torch.empty(x.shape, dtype=x.dtype, device=x.device) if r2 is not None else None
-        y = torch.empty(x.shape, dtype=x.dtype if dtype is None else dtype, device=x.device)
-        head = (x2.data_ptr(), x_stride, None if r2 is None else r2.data_ptr(), r_stride,
-                None if s is None else s.data_ptr(), w_ptr, w_dtype, _STORAGE[x.dtype], rows, width, float(eps))
-        if dtype is None:
-            if rows:
-                rt.check(rt.library().musc_rmsnorm_rows(*head, y.data_ptr(), rt.stream(x.device)), 'musc_rmsnorm_rows')
-            return y if s is None else (s, y)
-        scales = torch.empty((*x.shape[:-1], width // group if group else 1), dtype=torch.float32, device=x.device)
+        s = torch.empty_like(x, memory_format=torch.contiguous_format)
+        r_ptr, s_ptr = r2.data_ptr(), s.data_ptr()
+    y = torch.empty_like(x, dtype=dtype, memory_format=torch.contiguous_format)
+    if dtype is None:
         if rows:
-            rt.check(rt.library().musc_rmsnorm_rows_8bit(*head, _FP8[dtype], group, y.data_ptr(), scales.data_ptr(),
-                                                         rt.stream(x.device)), 'musc_rmsnorm_rows_8bit')
+            rt.check(rt.library().musc_rmsnorm_rows(x2.data_ptr(), x_stride, r_ptr, r_stride, s_ptr, w_ptr, w_dtype, storage,
+                                                    rows, width, eps, y.data_ptr(), rt.current_stream(index)),
+                     'musc_rmsnorm_rows')
+        return y if s is None else (s, y)
+    scales = torch.empty((*x.shape[:-1], width // group if group else 1), dtype=torch.float32, device=x.device)
+    if rows:
+        rt.check(rt.library().musc_rmsnorm_rows_8bit(x2.data_ptr(), x_stride, r_ptr, r_stride, s_ptr, w_ptr, w_dtype, storage,
+                                                     rows, width, eps, _FP8[dtype], group, y.data_ptr(), scales.data_ptr(),
+                                                     rt.current_stream(index)), 'musc_rmsnorm_rows_8bit')
     return (y, scales) if s is None else (s, y, scales)
 
 

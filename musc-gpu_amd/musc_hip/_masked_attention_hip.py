@@ -70,30 +70,26 @@ class Tokens:
                 docs.data_ptr(), None if self.order is None else self.order.data_ptr(), self.summary.shape[0],
                 docs.shape[-1], self.summary.data_ptr(), rt.stream(docs.device)), 'musc_token_summary')
 
-    def rows(self, name: str, x: torch.Tensor, batch: int, tokens: int, device) -> int:
-        """Batch stride of one of the tensors, 0 where the batch shares one row."""
-        token_dim = 1 if x.is_floating_point() else 0
-        dims = x.dim() - token_dim
-        if x.shape[dims - 1] != tokens or (dims == 2 and x.shape[0] not in (1, batch)) or x.device != device:
-            raise ValueError(f'{name} has {tuple(x.shape)}: {tokens} tokens of {batch} batch entries (or 1) on {device} needed')
-        return 0 if dims == 1 or x.shape[0] == 1 else x.stride(0)
+
+def _batch_stride(name: str, x: torch.Tensor, leading, batch: int, tokens: int, index: int) -> int:
+    """Batch stride of documents or positions, `leading` their (T,) or (B, T); 0 where the batch
+    shares one row."""
+    if leading[-1] == tokens and x.get_device() == index:
+        if len(leading) == 1 or leading[0] == 1:
+            return 0
+        if leading[0] == batch:
+            return x.stride(0)
+    raise ValueError(f'{name} has {tuple(x.shape)}: {tokens} tokens of {batch} batch entries (or 1) on device {index} needed')
 
 
 _EVERY = Tokens()
 
 
-def _heads(x, name, like):
-    rt.require_device_tensor(x, name)
-    if x.dim() != 4 or x.dtype not in _STORAGE:
-        raise ValueError(f'{name} must be a (B, T, heads, D) float32, float16 or bfloat16 tensor')
-    if like is not None and (x.dtype != like.dtype or x.device != like.device or x.shape[0] != like.shape[0]
-                             or x.shape[3] != like.shape[3]):
-        raise ValueError(f'{name} must match q in batch, head width, dtype and device')
-    per = 16 // x.element_size()
-    if x.stride(3) == 1 and x.data_ptr() % 16 == 0:
-        strides = rt.token_strides(x)
-        if not any(s % per for s in strides):
-            return x, strides
+def _heads(x, per):
+    """x, copied where its rows do not start on 16 bytes (per elements), and its strides."""
+    strides = rt.token_strides(x)
+    if x.stride(3) == 1 and not x.data_ptr() % 16 and not (strides[0] | strides[1] | strides[2]) % per:
+        return x, strides
     x = x.contiguous()
     return x, rt.token_strides(x)
 
@@ -111,65 +107,76 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: f
     all lets every query see every key.  A query that sees no key gets zeros.
     cap > 0: scores become cap tanh(score / cap) before the bias.  slopes: float32 (heads, axes),
     needs positions on both sides.  No backward pass."""
+    for name, x in (('q', q), ('k', k), ('v', v)):
+        rt.require_device_tensor(x, name)
+        if x.dim() != 4:
+            raise ValueError(f'{name} must be a (B, T, heads, D) tensor')
+    if rt.elsewhere(q):
+        with torch.cuda.device(q.device):
+            return masked_attention(q, k, v, scale, keys, queries, cap, slopes, out)
     rt.require_no_gradient(q, k, v, slopes)
-    q, qs = _heads(q, 'q', None)
-    k, ks = _heads(k, 'k', q)
-    v, vs = _heads(v, 'v', q)
+    dtype, index = q.dtype, q.get_device()
+    if dtype not in _STORAGE:
+        raise ValueError('q must be float32, float16 or bfloat16')
     b, tq, h, d = q.shape
-    tk, hk = k.shape[1:3]
+    kb, tk, hk, kd = k.shape
+    if kb != b or kd != d or k.dtype != dtype or v.dtype != dtype or k.get_device() != index or v.get_device() != index:
+        raise ValueError('k and v must match q in batch, head width, dtype and device')
     if v.shape != k.shape:
         raise ValueError('v must match k in shape')
     if hk < 1 or h % hk:
         raise ValueError('heads of q must be a multiple of the heads of k')
     per = 16 // q.element_size()
     if d < per or d > 128 or d % per:
-        raise ValueError(f'head width {d}: multiples of {per} up to 128 are supported for {q.dtype}')
+        raise ValueError(f'head width {d}: multiples of {per} up to 128 are supported for {dtype}')
+    q, qs = _heads(q, per)
+    k, ks = _heads(k, per)
+    v, vs = _heads(v, per)
     keys = _EVERY if keys is None else keys
     queries = keys if queries is None else queries
-    device = q.device
-    if (keys.documents is None) != (queries.documents is None) or (keys.order is None) != (queries.order is None):
+    kdocs, qdocs, kord, qord = keys.documents, queries.documents, keys.order, queries.order
+    if (kdocs is None) != (qdocs is None) or (kord is None) != (qord is None):
         raise ValueError('keys and queries must both have documents, and both an order, or neither')
-    docs, orders, q_sb, k_sb, sum_sb = (None, None), (None, None), 0, 0, 0
-    summary = None
-    if keys.documents is not None:
+    q_sb = k_sb = sum_sb = qd_ptr = kd_ptr = qo_ptr = ko_ptr = sum_ptr = 0
+    if kdocs is not None:
         if keys.summary is None:
             raise ValueError('keys were made with queries_only')
-        q_sb = queries.rows('queries.documents', queries.documents, b, tq, device)
-        k_sb = keys.rows('keys.documents', keys.documents, b, tk, device)
-        docs = queries.documents.data_ptr(), keys.documents.data_ptr()
-        if keys.order is not None:
-            orders = queries.order.data_ptr(), keys.order.data_ptr()
-        summary, sum_sb = keys.summary.data_ptr(), (keys.summary.shape[1] if k_sb else 0)
-    axes, pos, qp_sb, kp_sb, slope_ptr = 0, (None, None), 0, 0, None
+        q_sb = _batch_stride('queries.documents', qdocs, qdocs.shape, b, tq, index)
+        k_sb = _batch_stride('keys.documents', kdocs, kdocs.shape, b, tk, index)
+        qd_ptr, kd_ptr, sum_ptr = qdocs.data_ptr(), kdocs.data_ptr(), keys.summary.data_ptr()
+        sum_sb = keys.summary.shape[1] if k_sb else 0
+        if kord is not None:
+            qo_ptr, ko_ptr = qord.data_ptr(), kord.data_ptr()
+    axes = qp_ptr = kp_ptr = qp_sb = kp_sb = slope_ptr = 0
     if slopes is not None:
-        if keys.positions is None or queries.positions is None:
+        kpos, qpos = keys.positions, queries.positions
+        if kpos is None or qpos is None:
             raise ValueError('slopes need positions of keys and queries')
-        axes = keys.positions.shape[-1]
+        axes = kpos.shape[-1]
         rt.require_device_tensor(slopes, 'slopes')
-        if (slopes.dtype != torch.float32 or slopes.shape not in ((h, axes), (h,) if axes == 1 else (h, axes))
-                or queries.positions.shape[-1] != axes or slopes.device != device):
+        if (slopes.dtype != torch.float32 or slopes.get_device() != index or qpos.shape[-1] != axes
+                or not (slopes.shape == (h, axes) or (axes == 1 and slopes.shape == (h,)))):
             raise ValueError(f"slopes must be float32 ({h}, {axes}) on q's device, positions of both sides have as many axes")
         slopes = slopes.contiguous()
-        qp_sb = queries.rows('queries.positions', queries.positions, b, tq, device)
-        kp_sb = keys.rows('keys.positions', keys.positions, b, tk, device)
-        pos, slope_ptr = (queries.positions.data_ptr(), keys.positions.data_ptr()), slopes.data_ptr()
-    with torch.cuda.device(device):
-        o = rt.output_like(out, q, 'out')
-        os_ = rt.token_strides(o)
-        if o.data_ptr() % 16 or any(s % per for s in os_):
-            raise ValueError('rows of out must start on 16 bytes')
-        if not (b and tq and h):
-            return o
-        if not tk:
-            return o.zero_()
-        call = rt.MaskedAttention(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), *qs, *ks, *vs, *os_,
-                                  _STORAGE[q.dtype], b, tq, tk, h, hk, d, float(scale), float(cap), docs[0], orders[0],
-                                  docs[1], orders[1], q_sb, k_sb, summary, sum_sb, pos[0], pos[1], qp_sb, kp_sb,
-                                  slope_ptr, axes)
-        lib, need = rt.library(), ctypes.c_size_t()
-        rt.check(lib.musc_masked_attention_workspace_bytes(call, ctypes.byref(need)),
-                 'musc_masked_attention_workspace_bytes')
-        ws = torch.empty(need.value, dtype=torch.uint8, device=device) if need.value else None
-        rt.check(lib.musc_masked_attention_fwd(call, None if ws is None else ws.data_ptr(), need.value,
-                                               rt.stream(device)), 'musc_masked_attention_fwd')
+        qp_sb = _batch_stride('queries.positions', qpos, qpos.shape[:-1], b, tq, index)
+        kp_sb = _batch_stride('keys.positions', kpos, kpos.shape[:-1], b, tk, index)
+        qp_ptr, kp_ptr, slope_ptr = qpos.data_ptr(), kpos.data_ptr(), slopes.data_ptr()
+    o = rt.output_like(out, q, 'out')
+    os_ = rt.token_strides(o)
+    if o.data_ptr() % 16 or (os_[0] | os_[1] | os_[2]) % per:
+        raise ValueError('rows of out must start on 16 bytes')
+    if not (b and tq and h):
+        return o
+    if not tk:
+        return o.zero_()
+    call = rt.PACK_MASKED_ATTENTION.pack(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), *qs, *ks, *vs, *os_, _STORAGE[dtype], b, tq, tk, h, hk, d,
+        scale, cap, qd_ptr, qo_ptr, kd_ptr, ko_ptr, q_sb, k_sb, sum_ptr, sum_sb, qp_ptr, kp_ptr, qp_sb, kp_sb, slope_ptr,
+        axes)
+    lib, need, ws = rt.library(), ctypes.c_size_t(), None
+    rt.check(lib.musc_masked_attention_workspace_bytes(call, ctypes.byref(need)), 'musc_masked_attention_workspace_bytes')
+    if need.value:
+        ws = torch.empty(need.value, dtype=torch.uint8, device=q.device)
+    rt.check(lib.musc_masked_attention_fwd(call, None if ws is None else ws.data_ptr(), need.value,
+                                           rt.current_stream(index)), 'musc_masked_attention_fwd')
     return o

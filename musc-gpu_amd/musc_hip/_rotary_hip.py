@@ -46,12 +46,10 @@ class RotaryAxes:
         self.axis = torch.tensor(axis, dtype=torch.int32, device=device)
 
 
-def _head_rows(x, name, like, axes):
+def _head_rows(x, name, axes):
     rt.require_device_tensor(x, name)
     if x.dim() != 4 or x.shape[-1] != axes.head_dim or x.dtype not in _STORAGE:
         raise ValueError(f'{name} must be a (B, T, heads, {axes.head_dim}) float32, float16 or bfloat16 tensor')
-    if like is not None and (x.shape[:2] != like.shape[:2] or x.dtype != like.dtype or x.device != like.device):
-        raise ValueError(f'{name} must match q in batch, tokens, dtype and device')
     return x if x.stride(-1) == 1 else x.contiguous()
 
 
@@ -63,31 +61,38 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, axe
     positions (T, axes) or (B, T, axes), float32 or int32.  inverse turns back (the transpose).
     out: the tensors to write, (q_out, k_out) or q_out; they may be q and k themselves, and may
     not overlap them otherwise.  No backward pass."""
-    q2 = _head_rows(q, 'q', None, axes)
-    k2 = None if k is None else _head_rows(k, 'k', q, axes)
+    q2 = _head_rows(q, 'q', axes)
+    if rt.elsewhere(q):
+        with torch.cuda.device(q.device):
+            return rotary(q, k, positions, axes, inverse, out)
     rt.require_no_gradient(q, k)
+    index = q.get_device()
     b, t, h, d = q2.shape
+    k2, ko, k_args = None, None, (None, 0, 0, 0, 0, None, 0, 0, 0)
+    if k is not None:
+        k2 = _head_rows(k, 'k', axes)
+        if k2.shape[0] != b or k2.shape[1] != t or k2.dtype != q2.dtype or k2.get_device() != index:
+            raise ValueError('k must match q in batch, tokens, dtype and device')
+        if out is not None and len(out) != 2:
+            raise ValueError('out must be (q_out, k_out)')
     rt.require_device_tensor(positions, 'positions')
-    if positions.dtype not in (torch.float32, torch.int32) or positions.device != q.device or positions.shape not in (
-            (t, axes.axes), (b, t, axes.axes)):
+    shape = positions.shape
+    if (positions.dtype not in (torch.float32, torch.int32) or positions.get_device() != index
+            or (shape != (b, t, axes.axes) and shape != (t, axes.axes))):
         raise ValueError(f"positions must be float32 or int32 of shape (T, {axes.axes}) or (B, T, {axes.axes}) on q's device")
-    if axes.frequency.device != q.device:
+    if axes.frequency.get_device() != index:
         raise ValueError("axes must be on q's device")
     positions = positions.contiguous()
-    outs = out if k is not None else (out, None)
-    if k is not None and out is not None and len(out) != 2:
-        raise ValueError('out must be (q_out, k_out)')
-    with torch.cuda.device(q.device):
-        qo = rt.output_like(outs[0] if outs is not None else None, q2, 'q_out')
-        ko = None if k2 is None else rt.output_like(outs[1] if outs is not None else None, k2, 'k_out')
-        if b and t and h:
-            if k2 is None or not k2.shape[2]:
-                k_args = (None, 0, 0, 0, 0, None, 0, 0, 0)
-            else:
-                k_args = (k2.data_ptr(), k2.shape[2], *rt.token_strides(k2), ko.data_ptr(), *rt.token_strides(ko))
-            rt.check(rt.library().musc_rotary(
-                q2.data_ptr(), h, *rt.token_strides(q2), qo.data_ptr(), *rt.token_strides(qo), *k_args, _STORAGE[q.dtype], b, t, d,
-                positions.data_ptr(), int(positions.dtype == torch.int32), 0 if positions.dim() == 2 else t * axes.axes,
-                axes.axes, axes.frequency.data_ptr(), axes.axis.data_ptr(), axes.pairs, int(axes.adjacent), int(inverse),
-                rt.stream(q.device)), 'musc_rotary')
+    if k2 is not None:
+        ko = rt.output_like(out[1] if out is not None else None, k2, 'k_out')
+        if k2.shape[2]:
+            k_args = (k2.data_ptr(), k2.shape[2], *rt.token_strides(k2), ko.data_ptr(), *rt.token_strides(ko))
+        out = out[0] if out is not None else None
+    qo = rt.output_like(out, q2, 'q_out')
+    if b and t and h:
+        rt.check(rt.library().musc_rotary(
+            q2.data_ptr(), h, *rt.token_strides(q2), qo.data_ptr(), *rt.token_strides(qo), *k_args, _STORAGE[q2.dtype], b, t,
+            d, positions.data_ptr(), positions.dtype == torch.int32, 0 if len(shape) == 2 else t * axes.axes, axes.axes,
+            axes.frequency.data_ptr(), axes.axis.data_ptr(), axes.pairs, axes.adjacent, inverse,
+            rt.current_stream(index)), 'musc_rotary')
     return qo if k is None else (qo, ko)

@@ -92,7 +92,7 @@ def attention_call(**kw):
     (dict(q_tokens_sb=-1), INVALID), (dict(batch=1 << 20, kv_heads=2, q_len=1 << 20), UNSUPPORTED)])
 def test_masked_attention(lib, change, code):
     need = ctypes.c_size_t()
-    call = attention_call(**change)
+    call = ctypes.byref(attention_call(**change))
     assert lib.musc_masked_attention_workspace_bytes(call, ctypes.byref(need)) == code
     assert lib.musc_masked_attention_fwd(call, None, ctypes.c_size_t(0), None) == code
 
@@ -100,15 +100,22 @@ def test_masked_attention(lib, change, code):
 def test_masked_attention_workspace(lib):
     need = ctypes.c_size_t(1)
     assert lib.musc_masked_attention_workspace_bytes(None, ctypes.byref(need)) == INVALID
-    assert lib.musc_masked_attention_workspace_bytes(attention_call(), None) == INVALID
+    assert lib.musc_masked_attention_workspace_bytes(ctypes.byref(attention_call()), None) == INVALID
     # a full grid is not split; one row over many keys is, and refuses to run without its parts
-    assert lib.musc_masked_attention_workspace_bytes(attention_call(batch=64, q_len=1024), ctypes.byref(need)) == OK
+    assert lib.musc_masked_attention_workspace_bytes(ctypes.byref(attention_call(batch=64, q_len=1024)), ctypes.byref(need)) == OK
     assert need.value == 0
-    one = attention_call(q_len=1, k_len=4096)
+    one = ctypes.byref(attention_call(q_len=1, k_len=4096))
     assert lib.musc_masked_attention_workspace_bytes(one, ctypes.byref(need)) == OK and need.value > 0
     assert lib.musc_masked_attention_fwd(one, None, need, None) == WORKSPACE
     assert lib.musc_masked_attention_fwd(one, P, ctypes.c_size_t(need.value - 1), None) == WORKSPACE
     assert lib.musc_masked_attention_fwd(one, ctypes.c_void_p(4100), need, None) == WORKSPACE
+
+
+def test_packed_call_is_the_structure(lib):
+    from musc_hip import _runtime as rt
+    values = list(range(1, 24)) + [0.5, 2.0] + list(range(26, 40))
+    packed = rt.MaskedAttention.from_buffer_copy(rt.PACK_MASKED_ATTENTION.pack(*values))
+    assert [getattr(packed, name) for name, _ in rt.MaskedAttention._fields_] == values
 
 
 @pytest.mark.parametrize('args,code', [
