@@ -82,6 +82,12 @@ struct Type<MUSC_DTYPE_BF16> {
   }
 };
 
+// Keys of a tile: workgroups of one wave take 32, so that four of them fit a CU's LDS.
+template <int kDtype, int kWaves>
+constexpr int tile_keys() {
+  return kWaves == 1 ? 32 : Type<kDtype>::kTile;
+}
+
 // Staged rows of K and V: 128, 256 or 512 bytes, their 16-byte chunks permuted by the row so
 // that the lanes one LDS read serves together touch different banks: 16 neighbouring rows of
 // one chunk (K's operands) take 16 places of a 256-byte window, and so do 4 neighbouring rows
@@ -172,7 +178,7 @@ __global__ __launch_bounds__(kWaves * kWave, kWaves > 1 ? 2 : 1) void masked_att
   using Ty = Type<kDtype>;
   typedef typename Ty::T T;
   constexpr bool k16 = kDtype != MUSC_DTYPE_F32;
-  constexpr int kTile = Ty::kTile, kSub = kTile / 32;
+  constexpr int kTile = tile_keys<kDtype, kWaves>(), kSub = kTile / 32;
   constexpr int kPer = 16 / (int)sizeof(T);                 // elements of a 16-byte chunk
   constexpr int kPitch = (kD <= 64 ? 64 : 128) * (int)sizeof(T);
   constexpr int kPlaces = kPitch / 16;                      // chunks of a staged row
@@ -188,11 +194,13 @@ __global__ __launch_bounds__(kWaves * kWave, kWaves > 1 ? 2 : 1) void masked_att
   const musc_masked_attention& c = a.c;
   const long long unit = xcd_logical_id(blockIdx.x, gridDim.x);
   if (unit >= a.units) return;
-  const int split = (int)(unit % a.splits);
+  // uniform numbers in scalar registers (the divisions leave them in vector ones)
+  const auto uniform = [](long long x) { return __builtin_amdgcn_readfirstlane((int)x); };
+  const int split = uniform(unit % a.splits);
   // later rows first: with an order they see more keys, and the longest work should not start last
-  const int row_tile = a.row_tiles - 1 - (int)(unit / a.splits % a.row_tiles);
-  const long long bh = unit / a.splits / a.row_tiles;
-  const int b = (int)(bh / c.kv_heads), kvh = (int)(bh % c.kv_heads);
+  const int row_tile = a.row_tiles - 1 - uniform(unit / a.splits % a.row_tiles);
+  const int bh = uniform(unit / a.splits / a.row_tiles);
+  const int b = uniform(bh / c.kv_heads), kvh = bh - b * c.kv_heads;
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid % kWave;
   const int lq = lane & 31, lh = lane >> 5;
   const int row = (row_tile * kWaves + wave) * 32 + lq;
@@ -266,22 +274,31 @@ __global__ __launch_bounds__(kWaves * kWave, kWaves > 1 ? 2 : 1) void masked_att
   }
 
   // tiles of this split
-  const int lo = (int)((long long)a.key_tiles * split / a.splits);
-  const int hi = (int)((long long)a.key_tiles * (split + 1) / a.splits);
+  const int lo = uniform((long long)a.key_tiles * split / a.splits);
+  const int hi = uniform((long long)a.key_tiles * (split + 1) / a.splits);
 
   // Staging: load i of a tile fills 1024 bytes, whole rows; wave w issues loads w, w + kWaves, ..
+  // Each goes through a resource of its own rows that ends with the last key, so a lane's offset
+  // is the same in all of them (but for the permutation, where that changes with i); a wave that
+  // issues all of them itself has the registers for their offsets in one resource.
   const char* kbase = reinterpret_cast<const char*>(static_cast<const T*>(c.k) + b * c.k_sb + (long long)kvh * c.k_sh);
   const char* vbase = reinterpret_cast<const char*>(static_cast<const T*>(c.v) + b * c.v_sb + (long long)kvh * c.v_sh);
   const long long k_row = c.k_st * (long long)sizeof(T), v_row = c.v_st * (long long)sizeof(T);
   const uint32_t staged_at = (uint32_t)(size_t)(lds_void*)&staged[0][0];
+  constexpr int kRows = 64 / kPlaces;  // rows of a load
   auto load_tile = [&](int tile, int buf) __attribute__((always_inline)) {
     const int first = tile * kTile, rem = min(k_len - first, kTile);
-    const int4v rk = resource(kbase + first * k_row, (rem - 1) * k_row + d * (int)sizeof(T));
-    const int4v rv = resource(vbase + first * v_row, (rem - 1) * v_row + d * (int)sizeof(T));
+    int4v rk = resource(kbase + first * k_row, (rem - 1) * k_row + d * (int)sizeof(T));
+    int4v rv = resource(vbase + first * v_row, (rem - 1) * v_row + d * (int)sizeof(T));
 #pragma unroll
     for (int j = 0; j < kLoads; ++j) {
-      const int i = wave + kWaves * j;
-      const int r = i * (64 / kPlaces) + lane / kPlaces, chunk = (lane % kPlaces) ^ swizzle<kPitch>(r);
+      const int i = wave + kWaves * j, rows = rem - i * kRows;
+      if constexpr (kWaves > 1) {
+        const long long key = first + i * kRows;
+        rk = resource(kbase + key * k_row, rows > 0 ? (rows - 1) * k_row + d * (int)sizeof(T) : 0);
+        rv = resource(vbase + key * v_row, rows > 0 ? (rows - 1) * v_row + d * (int)sizeof(T) : 0);
+      }
+      const int r = lane / kPlaces + (kWaves > 1 ? 0 : i * kRows), chunk = (lane % kPlaces) ^ swizzle<kPitch>(i * kRows + lane / kPlaces);
       const bool there = chunk * kPer < d;
       const uint32_t to = __builtin_amdgcn_readfirstlane(staged_at + buf * 2 * kPart + i * 1024);
       load_to_lds_16(to, there ? (int)(r * k_row) + chunk * 16 : kNowhere, rk);
@@ -312,15 +329,26 @@ __global__ __launch_bounds__(kWaves * kWave, kWaves > 1 ? 2 : 1) void masked_att
   // of keys that a row does not see are left out one by one (their V may be infinite or NaN)
   auto attend = [&](int buf, int tile, bool whole, auto careful_c) __attribute__((always_inline)) {
     constexpr bool careful = decltype(careful_c)::value;
-    const char* ks = staged[buf];
-    const char* vs = staged[buf] + kPart;
+    // Byte places of this lane's operands: row lq (K) or the row and chunk of its V operand, in
+    // chunk order from the permutation's exclusive or, which all further chunks keep.  Formed
+    // anew for each tile, as keeping all of them would take the registers of the operands.
+    int k_at = buf * 2 * kPart + lq * kPitch + ((lh ^ swizzle<kPitch>(lq)) << 4);
+    int v_at = buf * 2 * kPart + kPart;
+    if constexpr (k16) {
+      const int r = 4 * lh + ((lq & 15) >> 2);
+      v_at += r * kPitch + (((2 * (lq >> 4) + ((lq & 3) >> 1)) ^ swizzle<kPitch>(r)) << 4) + 8 * (lq & 1);
+    } else {
+      v_at += 4 * lh * kPitch + (((lq >> 2) ^ lh) << 4) + 4 * (lq & 3);
+    }
+    asm volatile("" : "+v"(k_at), "+v"(v_at));
+    const char* all = &staged[0][0];
     floatx16 s[kSub];
     TVec kf[kSub][kQ];
 #pragma unroll
     for (int u = 0; u < kSub; ++u)
 #pragma unroll
       for (int m = 0; m < kQ; ++m)
-        kf[u][m] = *reinterpret_cast<const TVec*>(ks + (32 * u + lq) * kPitch + ((2 * m + lh) ^ swizzle<kPitch>(lq)) * 16);
+        kf[u][m] = *reinterpret_cast<const TVec*>(all + (k_at ^ (m << 5)) + 32 * u * kPitch);
     __builtin_amdgcn_sched_barrier(0);  // all reads in flight before the first product waits
 #pragma unroll
     for (int u = 0; u < kSub; ++u)
@@ -344,12 +372,11 @@ __global__ __launch_bounds__(kWaves * kWave, kWaves > 1 ? 2 : 1) void masked_att
     // d0 + i, k = j
     short8v vf[k16 && !careful ? 2 * kSub : 1][k16 && !careful ? kO : 1];
     auto read_v = [&](int mm, int x) {
+      // key0 = 16 mm + 4 lh (+ 8: the permutation's bit 1), d0 = 32 x + 16 (lq / 16)
       auto tr = [&](int upper) {
-        const int r = 16 * mm + 8 * upper + 4 * lh + ((lq & 15) >> 2);
-        const int chunk = 4 * x + 2 * (lq >> 4) + ((lq & 3) >> 1);
         typedef __attribute__((address_space(3))) short4v lds_short4v;
         return __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (lds_short4v*)(vs + r * kPitch + (chunk ^ swizzle<kPitch>(r)) * 16 + 8 * (lq & 1)));
+            (lds_short4v*)(all + (v_at ^ (x << 6) ^ (upper << 5)) + (16 * mm + 8 * upper) * kPitch));
       };
       const short4v f0 = tr(0), f1 = tr(1);
       return short8v{f0[0], f0[1], f0[2], f0[3], f1[0], f1[1], f1[2], f1[3]};
@@ -460,7 +487,7 @@ __global__ __launch_bounds__(kWaves * kWave, kWaves > 1 ? 2 : 1) void masked_att
           for (int v = 0; v < 16; ++v) {
             if (v % 4 == 0) __builtin_amdgcn_sched_barrier(0);  // few values at a time
             const int at = 32 * x + 8 * (v >> 2) + 4 * lh + (v & 3);
-            const T value = *reinterpret_cast<const T*>(vs + key * kPitch + ((at / kPer) ^ swizzle<kPitch>(key)) * 16 +
+            const T value = *reinterpret_cast<const T*>(staged[buf] + kPart + key * kPitch + ((at / kPer) ^ swizzle<kPitch>(key)) * 16 +
                                                         at % kPer * (int)sizeof(T));
             if (see) o[x][v] = fmaf(pr, (float)value, o[x][v]);
           }
@@ -481,9 +508,9 @@ __global__ __launch_bounds__(kWaves * kWave, kWaves > 1 ? 2 : 1) void masked_att
         for (int e = 0; e < 16; ++e)
 #pragma unroll
           for (int x = 0; x < kO; ++x) {
-            const int r = 32 * u + 8 * (e >> 2) + 4 * lh + (e & 3);
-            const float f = *reinterpret_cast<const float*>(vs + r * kPitch + ((8 * x + (lq >> 2)) ^ swizzle<kPitch>(r)) * 16 +
-                                                            4 * (lq & 3));
+            const float f = *reinterpret_cast<const float*>(
+                all + (v_at ^ (x << 7) ^ ((e & 3) << 6) ^ (((e >> 2) & 1) << 5)) +
+                (32 * u + 8 * (e >> 2) + (e & 3)) * kPitch);
             o[x] = __builtin_amdgcn_mfma_f32_32x32x2f32(f, s[u][e], o[x], 0, 0, 0);
           }
     }
@@ -579,7 +606,7 @@ __global__ __launch_bounds__(kWaves * kWave, kWaves > 1 ? 2 : 1) void masked_att
         if (at < d) *reinterpret_cast<Four*>(orow + at) = y;
       }
   } else {
-    const long long part = (bh * a.rows + row) * a.splits + split;
+    const long long part = ((long long)bh * a.rows + row) * a.splits + split;
     if (lh == 0) {
       a.part_ml[2 * part] = live ? m_run * to_log2 : -INFINITY;
       a.part_ml[2 * part + 1] = live ? l_run : 0.f;
@@ -650,13 +677,13 @@ __global__ __launch_bounds__(256) void join_kernel(const Args a) {
 
 // Shape of the launch: rows per workgroup, tiles and splits.
 int plan(const musc_masked_attention& c, Args& a, int& waves) {
-  const int tile = c.dtype == MUSC_DTYPE_F32 ? 32 : 64;
   a.c = c;
   a.group = c.heads / c.kv_heads;
   const long long rows = (long long)c.q_len * a.group;
   if (rows > 0x7fffff00LL || c.k_len > 0x7fffff00) return MUSC_ERR_UNSUPPORTED;
   a.rows = (int)rows;
   waves = rows <= 32 ? 1 : 4;
+  const int tile = waves == 1 || c.dtype == MUSC_DTYPE_F32 ? 32 : 64;
   a.row_tiles = (int)((rows + 32 * waves - 1) / (32 * waves));
   a.key_tiles = (c.k_len + tile - 1) / tile;
   a.summaries = (c.k_len + kSummaryKeys - 1) / kSummaryKeys;
