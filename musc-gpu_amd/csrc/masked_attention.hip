@@ -42,6 +42,7 @@ constexpr float kLazyLog2 = 8.f;           // the running maximum moves once a t
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kSummaryKeys = 32;
 constexpr int kMaxAxes = 3;
+constexpr int kRowTile = 128;  // rows of a workgroup of four waves
 
 template <int kDtype>
 struct Type;
@@ -99,7 +100,7 @@ __device__ __forceinline__ constexpr int swizzle(int r) {
 
 struct Args {
   musc_masked_attention c;
-  int group, rows, row_tiles, key_tiles, splits, summaries;
+  int group, rows, row_tiles, key_tiles, splits, summaries, heads_at_once;
   long long units;
   float* part_ml;  // (units in (b, kv head), rows, split) x (maximum, sum)
   float* part_o;   // the same x d
@@ -154,6 +155,53 @@ __global__ __launch_bounds__(256) void token_summary_kernel(const int* __restric
   if (threadIdx.x % kSummaryKeys == 0) summary[g] = s;
 }
 
+// Self-attention's row tiles for 1, 2, 4 and 8 query heads per key head, one after the other:
+// (batch, 2, row_tiles) int32 each.
+struct Schedule {
+  int batch, t, groups;
+  int tiles[4];      // row tiles
+  long long first[5];  // (batch entry, row tile) pairs before this number of heads
+  __device__ __forceinline__ int which(long long i) const { return (i >= first[1]) + (i >= first[2]) + (i >= first[3]); }
+};
+
+// Work of each row tile: the groups of 32 keys that its rows may see.  One wave per tile.
+__global__ __launch_bounds__(kWave) void row_work_kernel(const int* __restrict__ documents, const int* __restrict__ order,
+                                                         const int4* __restrict__ summary, const Schedule s,
+                                                         int* __restrict__ out) {
+  const int w = s.which(blockIdx.x), lane = threadIdx.x;
+  const int i = (int)(blockIdx.x - s.first[w]), b = i / s.tiles[w], tile = i % s.tiles[w];
+  const int first = tile * (kRowTile >> w), last = min(first + (kRowTile >> w), s.t) - 1;
+  Range r = {0x7fffffff, -1, 0x7fffffff, (int)0x80000000};
+  for (int k = first + lane; k <= last; k += kWave) {
+    const int doc = documents[(long long)b * s.t + k], ord = order ? order[(long long)b * s.t + k] : 0;
+    if (doc < 0) continue;
+    r = Range{min(r.dmin, doc), max(r.dmax, doc), min(r.omin, ord), max(r.omax, ord)};
+  }
+  r = Range{wave_min_int(r.dmin), wave_max_int(r.dmax), wave_min_int(r.omin), wave_max_int(r.omax)};
+  int count = 0;
+  for (int g = lane; g < s.groups; g += kWave) {
+    const int4 k = summary[(long long)b * s.groups + g];
+    count += k.y >= 0 && k.x <= r.dmax && k.y >= r.dmin && k.z <= r.omax;
+  }
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) count += __shfl_xor(count, off, kWave);
+  if (lane == 0) out[2 * s.first[w] + (2LL * b + 1) * s.tiles[w] + tile] = count;
+}
+
+// The row tiles by their work, most first (later ones first where it is the same).
+__global__ __launch_bounds__(256) void row_order_kernel(const Schedule s, int* __restrict__ out) {
+  const long long at = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (at >= s.first[4]) return;
+  const int w = s.which(at), n = s.tiles[w];
+  const int i = (int)(at - s.first[w]), b = i / n, tile = i % n;
+  int* mine = out + 2 * s.first[w] + 2LL * b * n;
+  const int* work = mine + n;
+  const int here = work[tile];
+  int rank = 0;
+  for (int j = 0; j < n; ++j) rank += work[j] > here || (work[j] == here && j > tile);
+  mine[rank] = tile;
+}
+
 // Loads straight from memory into LDS, lane l's 16 (or 4) bytes to `to` + 16 l (or 4 l), `to`
 // uniform.  From inline assembly, as the compiler, which cannot tell the two buffers apart,
 // would wait for them before reading the other one; the loop waits for them itself.
@@ -174,7 +222,7 @@ __device__ __forceinline__ int4v resource(const void* base, long long bytes) {
 
 // kWaves waves of 32 rows each; kD: head width rounded up to 64, 96 or 128.
 template <int kDtype, int kD, int kWaves>
-__global__ __launch_bounds__(kWaves * kWave, kWaves > 1 ? 2 : 1) void masked_attention_kernel(const Args a) {
+__global__ __launch_bounds__(kWaves * kWave, kWaves == 1 ? 1 : kD == 64 && kDtype != MUSC_DTYPE_F32 ? 3 : 2) void masked_attention_kernel(const Args a) {
   using Ty = Type<kDtype>;
   typedef typename Ty::T T;
   constexpr bool k16 = kDtype != MUSC_DTYPE_F32;
@@ -192,15 +240,29 @@ __global__ __launch_bounds__(kWaves * kWave, kWaves > 1 ? 2 : 1) void masked_att
   __shared__ Range ranges[kWaves];
 
   const musc_masked_attention& c = a.c;
-  const long long unit = xcd_logical_id(blockIdx.x, gridDim.x);
-  if (unit >= a.units) return;
   // uniform numbers in scalar registers (the divisions leave them in vector ones)
   const auto uniform = [](long long x) { return __builtin_amdgcn_readfirstlane((int)x); };
-  const int split = uniform(unit % a.splits);
-  // later rows first: with an order they see more keys, and the longest work should not start last
-  const int row_tile = a.row_tiles - 1 - uniform(unit / a.splits % a.row_tiles);
-  const int bh = uniform(unit / a.splits / a.row_tiles);
+  int split, row_tile, bh;
+  if (a.heads_at_once) {
+    // one XCD works on heads_at_once heads together, row tile by row tile (the longest first)
+    const int per_xcd = c.batch * c.kv_heads / kXcds, local = blockIdx.x / kXcds;
+    const int of_group = a.heads_at_once * a.row_tiles * a.splits, first = uniform(local / of_group) * a.heads_at_once;
+    const int at_once = min(a.heads_at_once, per_xcd - first), in_group = uniform(local % of_group);
+    split = uniform(in_group % a.splits);
+    bh = blockIdx.x % kXcds * per_xcd + first + uniform(in_group / a.splits % at_once);
+    row_tile = uniform(in_group / a.splits / at_once);
+  } else {
+    const long long unit = xcd_logical_id(blockIdx.x, gridDim.x);
+    if (unit >= a.units) return;
+    split = uniform(unit % a.splits);
+    row_tile = uniform(unit / a.splits % a.row_tiles);
+    bh = uniform(unit / a.splits / a.row_tiles);
+  }
   const int b = uniform(bh / c.kv_heads), kvh = bh - b * c.kv_heads;
+  // by the caller's order, or later rows first: with an order of tokens they see more keys, and
+  // the longest work should not start last
+  row_tile = kWaves > 1 && c.row_order ? uniform(c.row_order[b * c.row_order_sb + row_tile]) : a.row_tiles - 1 - row_tile;
+  row_tile = min(max(row_tile, 0), a.row_tiles - 1);
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid % kWave;
   const int lq = lane & 31, lh = lane >> 5;
   const int row = (row_tile * kWaves + wave) * 32 + lq;
@@ -695,6 +757,15 @@ int plan(const musc_masked_attention& c, Args& a, int& waves) {
   if (splits > kMaxSplits) splits = kMaxSplits;
   a.splits = splits < 1 ? 1 : (int)splits;
   a.units = whole * a.splits;
+  // Heads that an XCD (32 CUs, 2 or 3 workgroups each) works on together: enough for two rounds of
+  // workgroups, so that short work fills the gaps of long work, and no more, as they share its L2.
+  // 0: the heads do not divide over the XCDs.
+  const long long heads = (long long)c.batch * c.kv_heads;
+  a.heads_at_once = 0;
+  if (heads % kXcds == 0) {
+    const long long enough = (128 + a.row_tiles - 1) / a.row_tiles, per_xcd = heads / kXcds;
+    a.heads_at_once = (int)(enough < per_xcd ? enough : per_xcd);
+  }
   if (a.units >= (0x100000000LL >> 8)) return MUSC_ERR_UNSUPPORTED;  // 256 threads each in one grid dimension
   return MUSC_OK;
 }
@@ -734,9 +805,10 @@ int check(const musc_masked_attention* c) {
   const uintptr_t words = reinterpret_cast<uintptr_t>(c->q_documents) | reinterpret_cast<uintptr_t>(c->k_documents) |
                           reinterpret_cast<uintptr_t>(c->q_order) | reinterpret_cast<uintptr_t>(c->k_order) |
                           reinterpret_cast<uintptr_t>(c->q_positions) | reinterpret_cast<uintptr_t>(c->k_positions) |
-                          reinterpret_cast<uintptr_t>(c->slopes);
+                          reinterpret_cast<uintptr_t>(c->slopes) | reinterpret_cast<uintptr_t>(c->row_order);
   if ((words & 3) || (reinterpret_cast<uintptr_t>(c->k_summary) & 15)) return MUSC_ERR_INVALID_ARG;
-  if ((c->q_tokens_sb | c->k_tokens_sb | c->q_positions_sb | c->k_positions_sb | c->k_summary_sb) < 0)
+  if ((c->q_tokens_sb | c->k_tokens_sb | c->q_positions_sb | c->k_positions_sb | c->k_summary_sb |
+       c->row_order_sb) < 0)
     return MUSC_ERR_INVALID_ARG;
   return MUSC_OK;
 }
@@ -778,6 +850,27 @@ extern "C" int musc_token_summary(const int* documents, const int* order, int ba
   if (blocks >= (0x100000000LL >> 8)) return MUSC_ERR_UNSUPPORTED;
   hipLaunchKernelGGL(mattn::token_summary_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, documents, order, batch,
                      t, groups, reinterpret_cast<int4*>(summary));
+  return check_launch();
+}
+
+extern "C" int musc_token_schedule(const int* documents, const int* order, const int* summary, int batch, int t,
+                                   int* row_order, hipStream_t stream) {
+  if (!documents || !summary || !row_order || batch < 0 || t < 0) return MUSC_ERR_INVALID_ARG;
+  if (((reinterpret_cast<uintptr_t>(documents) | reinterpret_cast<uintptr_t>(order) |
+        reinterpret_cast<uintptr_t>(row_order)) & 3) || (reinterpret_cast<uintptr_t>(summary) & 15))
+    return MUSC_ERR_INVALID_ARG;
+  if (t > MUSC_SCHEDULE_MAX_TOKENS) return MUSC_ERR_UNSUPPORTED;
+  if (batch == 0 || t == 0) return MUSC_OK;
+  mattn::Schedule s{batch, t, (t + mattn::kSummaryKeys - 1) / mattn::kSummaryKeys, {}, {}};
+  for (int w = 0; w < 4; ++w) {
+    s.tiles[w] = (t + (mattn::kRowTile >> w) - 1) / (mattn::kRowTile >> w);
+    s.first[w + 1] = s.first[w] + (long long)batch * s.tiles[w];
+  }
+  if (s.first[4] >= (0x100000000LL >> 8)) return MUSC_ERR_UNSUPPORTED;
+  hipLaunchKernelGGL(mattn::row_work_kernel, dim3((unsigned)s.first[4]), dim3(kWave), 0, stream, documents, order,
+                     reinterpret_cast<const int4*>(summary), s, row_order);
+  hipLaunchKernelGGL(mattn::row_order_kernel, dim3((unsigned)((s.first[4] + 255) / 256)), dim3(256), 0, stream, s,
+                     row_order);
   return check_launch();
 }
 

@@ -17,6 +17,9 @@ from . import _runtime as rt
 
 _STORAGE = {torch.float32: rt.DTYPE_F32, torch.float16: rt.DTYPE_F16, torch.bfloat16: rt.DTYPE_BF16}
 SUMMARY_KEYS = 32
+ROW_TILE = 128
+SCHEDULE_GROUPS = (1, 2, 4, 8)
+SCHEDULE_MAX_TOKENS = 65536
 
 
 class Tokens:
@@ -32,7 +35,9 @@ class Tokens:
     positions  float32 (T, axes) or (B, T, axes), up to 3 axes, for the bias by distance.
 
     The tensors are kept, not copied.  As keys they are also summarised (32 at a time) when the
-    object is made; call refresh() after changing them in place.  queries_only leaves that out."""
+    object is made, on the current stream, and the groups of rows of self-attention over them put
+    in the order of their work; call refresh() after changing them in place.  queries_only leaves
+    that out."""
 
     def __init__(self, documents=None, order=None, positions=None, queries_only: bool = False):
         for name, x, dtype in (('documents', documents, torch.int32), ('order', order, torch.int32),
@@ -55,9 +60,17 @@ class Tokens:
                                           or positions.device != documents.device):
                 raise ValueError('positions must have the tokens of documents')
         self.documents, self.order, self.positions, self.summary = documents, order, positions, None
+        self._row_order = None
         if documents is not None and not queries_only:
             b, t = documents.shape if documents.dim() == 2 else (1, documents.shape[0])
             self.summary = torch.empty((b, -(-t // SUMMARY_KEYS), 4), dtype=torch.int32, device=documents.device)
+            if 0 < t <= SCHEDULE_MAX_TOKENS:
+                # one after the other for 1, 2, 4 and 8 query heads per key head
+                tiles = [-(-t * group // ROW_TILE) for group in SCHEDULE_GROUPS]
+                self._row_order = torch.empty((b * 2 * sum(tiles),), dtype=torch.int32, device=documents.device)
+                starts = [b * 2 * sum(tiles[:i]) for i in range(len(tiles))]
+                self._row_order_at = {g: (self._row_order.data_ptr() + 4 * at, 2 * n)
+                                      for g, at, n in zip(SCHEDULE_GROUPS, starts, tiles)}
             self.refresh()
 
     def refresh(self) -> None:
@@ -69,6 +82,11 @@ class Tokens:
             rt.check(rt.library().musc_token_summary(
                 docs.data_ptr(), None if self.order is None else self.order.data_ptr(), self.summary.shape[0],
                 docs.shape[-1], self.summary.data_ptr(), rt.stream(docs.device)), 'musc_token_summary')
+            if self._row_order is not None:
+                rt.check(rt.library().musc_token_schedule(
+                    docs.data_ptr(), None if self.order is None else self.order.data_ptr(), self.summary.data_ptr(),
+                    self.summary.shape[0], docs.shape[-1], self._row_order.data_ptr(), rt.stream(docs.device)),
+                    'musc_token_schedule')
 
 
 def _batch_stride(name: str, x: torch.Tensor, leading, batch: int, tokens: int, index: int) -> int:
@@ -169,10 +187,14 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: f
         return o
     if not tk:
         return o.zero_()
+    order_ptr = order_sb = 0
+    if queries is keys and kdocs is not None and keys._row_order is not None:
+        order_ptr, order_sb = keys._row_order_at.get(h // hk, (0, 0))
+        order_sb = order_sb if k_sb else 0
     call = rt.PACK_MASKED_ATTENTION.pack(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), *qs, *ks, *vs, *os_, _STORAGE[dtype], b, tq, tk, h, hk, d,
         scale, cap, qd_ptr, qo_ptr, kd_ptr, ko_ptr, q_sb, k_sb, sum_ptr, sum_sb, qp_ptr, kp_ptr, qp_sb, kp_sb, slope_ptr,
-        axes)
+        axes, order_ptr, order_sb)
     lib, need, ws = rt.library(), ctypes.c_size_t(), None
     rt.check(lib.musc_masked_attention_workspace_bytes(call, ctypes.byref(need)), 'musc_masked_attention_workspace_bytes')
     if need.value:

@@ -56,11 +56,11 @@ class MaskedAttention(ctypes.Structure):
         + [('q_tokens_sb', ctypes.c_longlong), ('k_tokens_sb', ctypes.c_longlong), ('k_summary', ctypes.c_void_p),
            ('k_summary_sb', ctypes.c_longlong), ('q_positions', ctypes.c_void_p), ('k_positions', ctypes.c_void_p),
            ('q_positions_sb', ctypes.c_longlong), ('k_positions_sb', ctypes.c_longlong), ('slopes', ctypes.c_void_p),
-           ('axes', ctypes.c_int)])
+           ('axes', ctypes.c_int), ('row_order', ctypes.c_void_p), ('row_order_sb', ctypes.c_longlong)])
 
 
 # The same as bytes: packing 45 fields at once takes 4 us less than setting them one by one
-PACK_MASKED_ATTENTION = struct.Struct('@4P12q7i2f4P2qPq2P2qPi4x')
+PACK_MASKED_ATTENTION = struct.Struct('@4P12q7i2f4P2qPq2P2qPiPq')
 assert PACK_MASKED_ATTENTION.size == ctypes.sizeof(MaskedAttention)
 
 
@@ -99,6 +99,7 @@ SIGNATURES = {
     'musc_attention_weights_strided': (_i, [_vp, _vp, _i, _i, _i, _i, _i, _ll, _ll, _ll, _f, _vp, _vp, _sz, _vp]),
     'musc_layernorm_rows': (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _f, _vp, _vp]),
     'musc_token_summary': (_i, [_vp, _vp, _i, _i, _vp, _vp]),
+    'musc_token_schedule': (_i, [_vp, _vp, _vp, _i, _i, _vp, _vp]),
     'musc_masked_attention_workspace_bytes': (_i, [_vp, ctypes.POINTER(_sz)]),
     'musc_masked_attention_fwd': (_i, [_vp, _vp, _sz, _vp]),
     'musc_rmsnorm_rows': (_i, [_vp, _ll, _vp, _ll, _vp, _vp, _i, _i, _i, _i, _f, _vp, _vp]),

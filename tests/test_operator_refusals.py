@@ -89,7 +89,7 @@ def attention_call(**kw):
     (dict(q_order=4096, k_order=4096), INVALID), (dict(q_documents=4098, k_documents=4096, k_summary=4096), INVALID),
     (dict(q_documents=4096, k_documents=4096, k_summary=4096, q_order=4096), INVALID),
     (dict(axes=4), UNSUPPORTED), (dict(axes=1), INVALID), (dict(axes=1, q_positions=4096, k_positions=4096), INVALID),
-    (dict(q_tokens_sb=-1), INVALID), (dict(batch=1 << 20, kv_heads=2, q_len=1 << 20), UNSUPPORTED)])
+    (dict(q_tokens_sb=-1), INVALID), (dict(row_order=4098), INVALID), (dict(row_order_sb=-1), INVALID), (dict(batch=1 << 20, kv_heads=2, q_len=1 << 20), UNSUPPORTED)])
 def test_masked_attention(lib, change, code):
     need = ctypes.c_size_t()
     call = ctypes.byref(attention_call(**change))
@@ -113,7 +113,7 @@ def test_masked_attention_workspace(lib):
 
 def test_packed_call_is_the_structure(lib):
     from musc_hip import _runtime as rt
-    values = list(range(1, 24)) + [0.5, 2.0] + list(range(26, 40))
+    values = list(range(1, 24)) + [0.5, 2.0] + list(range(26, 42))
     packed = rt.MaskedAttention.from_buffer_copy(rt.PACK_MASKED_ATTENTION.pack(*values))
     assert [getattr(packed, name) for name, _ in rt.MaskedAttention._fields_] == values
 
@@ -124,3 +124,14 @@ def test_packed_call_is_the_structure(lib):
     ((P, None, 0, 64, P, None), OK), ((P, None, 1 << 16, 1 << 16, P, None), UNSUPPORTED)])
 def test_token_summary(lib, args, code):
     assert lib.musc_token_summary(*args) == code
+
+
+@pytest.mark.parametrize('change,code', [
+    (dict(documents=None), INVALID), (dict(summary=None), INVALID), (dict(rows=None), INVALID),
+    (dict(batch=-1), INVALID), (dict(t=-1), INVALID), (dict(summary=ctypes.c_void_p(4104)), INVALID),
+    (dict(order=ctypes.c_void_p(4098)), INVALID), (dict(batch=0), OK), (dict(t=0), OK),
+    (dict(batch=1 << 12, t=1 << 16), UNSUPPORTED), (dict(t=65537), UNSUPPORTED)])
+def test_token_schedule(lib, change, code):
+    a = dict(documents=P, order=None, summary=P, batch=1, t=64, rows=P, stream=None)
+    a.update(change)
+    assert lib.musc_token_schedule(*a.values()) == code
