@@ -202,12 +202,21 @@ __global__ __launch_bounds__(256) void row_order_kernel(const Schedule s, int* _
   mine[rank] = tile;
 }
 
-// Loads straight from memory into LDS, lane l's 16 (or 4) bytes to `to` + 16 l (or 4 l), `to`
-// uniform.  From inline assembly, as the compiler, which cannot tell the two buffers apart,
+template <int kN, int kI = 0, typename F>
+__device__ __forceinline__ void unroll(F f) {
+  if constexpr (kI < kN) {
+    f(std::integral_constant<int, kI>{});
+    unroll<kN, kI + 1>(f);
+  }
+}
+
+// Loads straight from memory into LDS, lane l's 16 (or 4) bytes to `to` (+ kTo) + 16 l (or
+// 4 l), `to` uniform.  From inline assembly, as the compiler, which cannot tell the two buffers apart,
 // would wait for them before reading the other one; the loop waits for them itself.
-__device__ __forceinline__ void load_to_lds_16(uint32_t to, int offset, int4v from) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
-               :: "s"(to), "v"(offset), "s"(from) : "memory", "m0");
+template <int kTo>
+__device__ __forceinline__ void load_to_lds_16(uint32_t to, int offset, int4v from, int from_offset) {
+  asm volatile("s_add_u32 m0, %0, %4\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+               :: "s"(to), "v"(offset), "s"(from), "s"(from_offset), "i"(kTo) : "memory", "m0", "scc");
 }
 __device__ __forceinline__ void load_to_lds_4(const void* place, int offset, int4v from) {
   const uint32_t to = __builtin_amdgcn_readfirstlane((uint32_t)(size_t)(lds_void*)place);
@@ -340,31 +349,42 @@ __global__ __launch_bounds__(kWaves * kWave, kWaves == 1 ? 1 : kD == 64 && kDtyp
   const int hi = uniform((long long)a.key_tiles * (split + 1) / a.splits);
 
   // Staging: load i of a tile fills 1024 bytes, whole rows; wave w issues loads w, w + kWaves, ..
-  // Each goes through a resource of its own rows that ends with the last key, so a lane's offset
-  // is the same in all of them (but for the permutation, where that changes with i); a wave that
-  // issues all of them itself has the registers for their offsets in one resource.
+  // The loads of a whole tile share a resource based at the wave's first row, and a scalar offset
+  // leads to the rows of each; in the last, partial tile each has a resource of its own that ends
+  // with the last key.  Lanes of channels past d load from nowhere.
   const char* kbase = reinterpret_cast<const char*>(static_cast<const T*>(c.k) + b * c.k_sb + (long long)kvh * c.k_sh);
   const char* vbase = reinterpret_cast<const char*>(static_cast<const T*>(c.v) + b * c.v_sb + (long long)kvh * c.v_sh);
-  const long long k_row = c.k_st * (long long)sizeof(T), v_row = c.v_st * (long long)sizeof(T);
-  const uint32_t staged_at = (uint32_t)(size_t)(lds_void*)&staged[0][0];
+  const uint32_t k_row = (uint32_t)(c.k_st * (long long)sizeof(T)), v_row = (uint32_t)(c.v_st * (long long)sizeof(T));
+  const uint32_t staged_at = (uint32_t)(size_t)(lds_void*)&staged[0][0] + wave * 1024;
   constexpr int kRows = 64 / kPlaces;  // rows of a load
+  const int row_bytes = d * (int)sizeof(T);
   auto load_tile = [&](int tile, int buf) __attribute__((always_inline)) {
-    const int first = tile * kTile, rem = min(k_len - first, kTile);
-    int4v rk = resource(kbase + first * k_row, (rem - 1) * k_row + d * (int)sizeof(T));
-    int4v rv = resource(vbase + first * v_row, (rem - 1) * v_row + d * (int)sizeof(T));
-#pragma unroll
-    for (int j = 0; j < kLoads; ++j) {
-      const int i = wave + kWaves * j, rows = rem - i * kRows;
-      if constexpr (kWaves > 1) {
-        const long long key = first + i * kRows;
-        rk = resource(kbase + key * k_row, rows > 0 ? (rows - 1) * k_row + d * (int)sizeof(T) : 0);
-        rv = resource(vbase + key * v_row, rows > 0 ? (rows - 1) * v_row + d * (int)sizeof(T) : 0);
-      }
-      const int r = lane / kPlaces + (kWaves > 1 ? 0 : i * kRows), chunk = (lane % kPlaces) ^ swizzle<kPitch>(i * kRows + lane / kPlaces);
-      const bool there = chunk * kPer < d;
-      const uint32_t to = __builtin_amdgcn_readfirstlane(staged_at + buf * 2 * kPart + i * 1024);
-      load_to_lds_16(to, there ? (int)(r * k_row) + chunk * 16 : kNowhere, rk);
-      load_to_lds_16(to + kPart, there ? (int)(r * v_row) + chunk * 16 : kNowhere, rv);
+    const int first = tile * kTile, rem = min(k_len - first, kTile), mine = wave * kRows;
+    const uint32_t to = __builtin_amdgcn_readfirstlane(staged_at + buf * 2 * kPart);
+    const char* kt = kbase + (unsigned long long)(uint32_t)(first + mine) * k_row;
+    const char* vt = vbase + (unsigned long long)(uint32_t)(first + mine) * v_row;
+    auto lane_offset = [&](int j, uint32_t row) {
+      const int r = lane / kPlaces, chunk = (lane % kPlaces) ^ swizzle<kPitch>((wave + kWaves * j) * kRows + r);
+      return chunk * kPer < d ? (int)(r * row) + chunk * 16 : kNowhere;
+    };
+    if (rem == kTile) {
+      const int4v rk = resource(kt, (long long)(kTile - mine - 1) * k_row + row_bytes);
+      const int4v rv = resource(vt, (long long)(kTile - mine - 1) * v_row + row_bytes);
+      unroll<kLoads>([&](auto jc) {
+        constexpr int j = decltype(jc)::value;
+        load_to_lds_16<j * kWaves * 1024>(to, lane_offset(j, k_row), rk, (int)(j * kWaves * kRows * k_row));
+        load_to_lds_16<j * kWaves * 1024 + kPart>(to, lane_offset(j, v_row), rv, (int)(j * kWaves * kRows * v_row));
+      });
+    } else {
+      unroll<kLoads>([&](auto jc) {
+        constexpr int j = decltype(jc)::value;
+        const int rows = rem - mine - j * kWaves * kRows;
+        const unsigned long long at = j * kWaves * kRows;
+        load_to_lds_16<j * kWaves * 1024>(
+            to, lane_offset(j, k_row), resource(kt + at * k_row, rows > 0 ? (long long)(rows - 1) * k_row + row_bytes : 0), 0);
+        load_to_lds_16<j * kWaves * 1024 + kPart>(
+            to, lane_offset(j, v_row), resource(vt + at * v_row, rows > 0 ? (long long)(rows - 1) * v_row + row_bytes : 0), 0);
+      });
     }
     if (wave == kWaves - 1) {
       if (c.k_documents)
