@@ -114,16 +114,22 @@ __device__ __forceinline__ float halves_sum(float v) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
+// Minimum over the wave by lane-crossing moves (no LDS): lanes get their neighbours 1, 2, 4, 8 to
+// the left within rows of 16, then the rows' last lanes go on to the next rows; lane 63 has it.
+template <int kMove, int kRows>
+__device__ __forceinline__ int min_with(int v) {
+  return min(v, __builtin_amdgcn_update_dpp(0x7fffffff, v, kMove, kRows, 0xf, false));
+}
 __device__ __forceinline__ int wave_min_int(int v) {
-#pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) v = min(v, __shfl_xor(v, off, kWave));
-  return __builtin_amdgcn_readfirstlane(v);
+  v = min_with<0x111, 0xf>(v);
+  v = min_with<0x112, 0xf>(v);
+  v = min_with<0x114, 0xf>(v);
+  v = min_with<0x118, 0xf>(v);
+  v = min_with<0x142, 0xa>(v);
+  v = min_with<0x143, 0xc>(v);
+  return __builtin_amdgcn_readlane(v, 63);
 }
-__device__ __forceinline__ int wave_max_int(int v) {
-#pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) v = max(v, __shfl_xor(v, off, kWave));
-  return __builtin_amdgcn_readfirstlane(v);
-}
+__device__ __forceinline__ int wave_max_int(int v) { return ~wave_min_int(~v); }
 
 // The documents and orders of a set of rows: what a tile is compared with.
 struct Range {
@@ -251,42 +257,83 @@ __global__ __launch_bounds__(kWaves * kWave, kWaves == 1 ? 1 : kD == 64 && kDtyp
   const musc_masked_attention& c = a.c;
   // uniform numbers in scalar registers (the divisions leave them in vector ones)
   const auto uniform = [](long long x) { return __builtin_amdgcn_readfirstlane((int)x); };
-  int split, row_tile, bh;
+  uint32_t split, row_tile, bh;
   if (a.heads_at_once) {
     // one XCD works on heads_at_once heads together, row tile by row tile (the longest first)
-    const int per_xcd = c.batch * c.kv_heads / kXcds, local = blockIdx.x / kXcds;
-    const int of_group = a.heads_at_once * a.row_tiles * a.splits, first = uniform(local / of_group) * a.heads_at_once;
-    const int at_once = min(a.heads_at_once, per_xcd - first), in_group = uniform(local % of_group);
-    split = uniform(in_group % a.splits);
-    bh = blockIdx.x % kXcds * per_xcd + first + uniform(in_group / a.splits % at_once);
-    row_tile = uniform(in_group / a.splits / at_once);
+    const uint32_t per_xcd = (uint32_t)(c.batch * c.kv_heads) / kXcds, local = blockIdx.x / kXcds;
+    const uint32_t of_group = (uint32_t)(a.heads_at_once * a.row_tiles * a.splits);
+    const uint32_t group = uniform(local / of_group), in_group = local - group * of_group;
+    const uint32_t first = group * a.heads_at_once, at_once = min((uint32_t)a.heads_at_once, per_xcd - first);
+    const uint32_t rest = uniform(in_group / a.splits);
+    split = in_group - rest * a.splits;
+    row_tile = uniform(rest / at_once);
+    bh = blockIdx.x % kXcds * per_xcd + first + (rest - row_tile * at_once);
   } else {
-    const long long unit = xcd_logical_id(blockIdx.x, gridDim.x);
-    if (unit >= a.units) return;
-    split = uniform(unit % a.splits);
-    row_tile = uniform(unit / a.splits % a.row_tiles);
-    bh = uniform(unit / a.splits / a.row_tiles);
+    const uint32_t unit = (blockIdx.x % kXcds) * (gridDim.x / kXcds) + blockIdx.x / kXcds;
+    if (unit >= (uint32_t)a.units) return;
+    const uint32_t rest = uniform(unit / a.splits);
+    split = unit - rest * a.splits;
+    bh = uniform(rest / a.row_tiles);
+    row_tile = rest - bh * a.row_tiles;
   }
   const int b = uniform(bh / c.kv_heads), kvh = bh - b * c.kv_heads;
-  // by the caller's order, or later rows first: with an order of tokens they see more keys, and
-  // the longest work should not start last
-  row_tile = kWaves > 1 && c.row_order ? uniform(c.row_order[b * c.row_order_sb + row_tile]) : a.row_tiles - 1 - row_tile;
-  row_tile = min(max(row_tile, 0), a.row_tiles - 1);
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid % kWave;
   const int lq = lane & 31, lh = lane >> 5;
-  const int row = (row_tile * kWaves + wave) * 32 + lq;
+
+  // tiles of this split, 64 sorted at a time by the keys' summary; the first 64 are asked for now
+  const int lo = uniform((long long)a.key_tiles * split / a.splits);
+  const int hi = uniform((long long)a.key_tiles * (split + 1) / a.splits);
+  const int4* summary = c.k_summary ? reinterpret_cast<const int4*>(c.k_summary) + b * c.k_summary_sb : nullptr;
+  auto summary_of = [&](int t) __attribute__((always_inline)) {
+    int4 k = make_int4(0, 0, 0, 0);
+    if (summary && t >= lo && t < hi) {
+      k = summary[(long long)t * kSub];
+      if (kSub > 1 && t * kSub + 1 < a.summaries) {
+        const int4 n = summary[(long long)t * kSub + 1];
+        k = make_int4(min(k.x, n.x), max(k.y, n.y), min(k.z, n.z), max(k.w, n.w));
+      }
+    }
+    return k;
+  };
+  const int4 first_summary = summary_of(lo / 64 * 64 + lane);
+
+  // by the caller's order, or later rows first: with an order of tokens they see more keys, and
+  // the longest work should not start last
+  int tile_of_rows = a.row_tiles - 1 - (int)row_tile;
+  if (kWaves > 1 && c.row_order) tile_of_rows = uniform(c.row_order[b * c.row_order_sb + row_tile]);
+  tile_of_rows = min(max(tile_of_rows, 0), a.row_tiles - 1);
+  const int row = (tile_of_rows * kWaves + wave) * 32 + lq;
   const bool inside = row < a.rows;
-  const int token = inside ? row / a.group : 0;
-  const int head = kvh * a.group + (inside ? row % a.group : 0);
+  const int token = inside ? (int)((uint32_t)row / (uint32_t)a.group) : 0;
+  const int head = kvh * a.group + (inside ? row - token * a.group : 0);
   const int d = c.d, k_len = c.k_len, axes = c.axes;
 
-  // this row's document and order; rows outside the tensor and padding have none
-  int qdoc = -1, qord = 0;
-  if (inside) {
-    qdoc = c.q_documents ? c.q_documents[b * c.q_tokens_sb + token] : 0;
-    if (c.q_order) qord = c.q_order[b * c.q_tokens_sb + token];
+  // this row's document and order (rows outside the tensor read token 0's), its Q and positions,
+  // all asked for before any is used
+  int qdoc = 0, qord = 0;
+  if (c.q_documents) qdoc = c.q_documents[b * c.q_tokens_sb + token];
+  if (c.q_order) qord = c.q_order[b * c.q_tokens_sb + token];
+  const T* qrow = static_cast<const T*>(c.q) + b * c.q_sb + (long long)token * c.q_st + head * c.q_sh;
+  constexpr int kQ = kD / (2 * kPer);
+  typedef T TVec __attribute__((ext_vector_type(kPer)));
+  TVec qf[kQ];
+#pragma unroll
+  for (int m = 0; m < kQ; ++m) {
+    const int at = (2 * m + lh) * kPer;
+    qf[m] = TVec{};
+    if (at < d) qf[m] = *reinterpret_cast<const TVec*>(qrow + at);
   }
-  const bool live = qdoc >= 0;
+  float qpos[kMaxAxes], slope[kMaxAxes];
+#pragma unroll
+  for (int x = 0; x < kMaxAxes; ++x) {
+    qpos[x] = 0.f, slope[x] = 0.f;
+    if (x < axes) {
+      qpos[x] = c.q_positions[b * c.q_positions_sb + (long long)token * axes + x];
+      slope[x] = c.slopes[head * axes + x];
+    }
+  }
+
+  const bool live = inside && qdoc >= 0;
   Range mine, all_rows;
   mine.dmin = wave_min_int(live ? qdoc : 0x7fffffff);
   mine.dmax = wave_max_int(live ? qdoc : -1);
@@ -295,7 +342,14 @@ __global__ __launch_bounds__(kWaves * kWave, kWaves == 1 ? 1 : kD == 64 && kDtyp
   all_rows = mine;
   if constexpr (kWaves > 1) {
     if (lane == 0) ranges[wave] = mine;
-    __syncthreads();
+  }
+  // keys of calls without documents or orders have 0
+  if (tid < 64) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) docs_s[i][tid] = 0, ords_s[i][tid] = 0;
+  }
+  __syncthreads();
+  if constexpr (kWaves > 1) {
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
       all_rows.dmin = min(all_rows.dmin, ranges[w].dmin);
@@ -305,14 +359,7 @@ __global__ __launch_bounds__(kWaves * kWave, kWaves == 1 ? 1 : kD == 64 && kDtyp
     }
   }
 
-  // keys of calls without documents or orders have 0
-  if (tid < 64) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) docs_s[i][tid] = 0, ords_s[i][tid] = 0;
-  }
-  __syncthreads();
-
-  // Q fragments, zeros past d.  Scores stay "raw" until the exponential: score in log2 units =
+  // Scores stay "raw" until the exponential: score in log2 units =
   // raw * to_log2 (+ a constant that cancels), to_log2 > 0:
   //   no cap   raw = +- q . k (Q negated for a negative scale), to_log2 = |scale| log2 e
   //   cap      raw = -1 / (1 + e^2x), x = scale q . k / cap, as cap tanh x = cap (1 + 2 raw);
@@ -322,31 +369,17 @@ __global__ __launch_bounds__(kWaves * kWave, kWaves == 1 ? 1 : kD == 64 && kDtyp
   const float to_log2 = (capped ? (k16 ? 2.f * c.cap : c.cap) : fabsf(scale)) * kLog2e;
   const float by_cap = capped ? scale / c.cap * (k16 ? 2.f * kLog2e : 1.f) : 0.f;
   const bool negate = !capped && scale < 0.f;
-  const T* qrow = static_cast<const T*>(c.q) + b * c.q_sb + (long long)token * c.q_st + head * c.q_sh;
-  constexpr int kQ = kD / (2 * kPer);
-  typedef T TVec __attribute__((ext_vector_type(kPer)));
-  TVec qf[kQ];
 #pragma unroll
   for (int m = 0; m < kQ; ++m) {
-    const int at = (2 * m + lh) * kPer;
-    TVec x = {};
-    if (live && at < d && c.scale != 0.f) x = *reinterpret_cast<const TVec*>(qrow + at);
-    qf[m] = negate ? -x : x;
+    if (negate) qf[m] = -qf[m];
+    if (c.scale == 0.f) qf[m] = TVec{};
   }
-  float qpos[kMaxAxes], slope[kMaxAxes];  // the B operand of the distances: 1 and -position; raw slopes
+  // the B operand of the distances: 1 and -position; slopes in raw units
 #pragma unroll
   for (int x = 0; x < kMaxAxes; ++x) {
-    qpos[x] = 0.f, slope[x] = 0.f;
-    if (x < axes) {
-      const float p = c.q_positions[b * c.q_positions_sb + (long long)token * axes + x];
-      qpos[x] = lh == 0 ? 1.f : -p;
-      slope[x] = c.slopes[head * axes + x] * kLog2e / to_log2;
-    }
+    qpos[x] = x < axes ? (lh == 0 ? 1.f : -qpos[x]) : 0.f;
+    slope[x] = slope[x] * kLog2e / to_log2;
   }
-
-  // tiles of this split
-  const int lo = uniform((long long)a.key_tiles * split / a.splits);
-  const int hi = uniform((long long)a.key_tiles * (split + 1) / a.splits);
 
   // Staging: load i of a tile fills 1024 bytes, whole rows; wave w issues loads w, w + kWaves, ..
   // The loads of a whole tile share a resource based at the wave's first row, and a scalar offset
@@ -598,21 +631,12 @@ __global__ __launch_bounds__(kWaves * kWave, kWaves == 1 ? 1 : kD == 64 && kDtyp
     }
   };
 
-  // the tiles of this split that some row of the workgroup may see, 64 sorted at a time
+  // the tiles that some row of the workgroup may see
   int chunk = 0;
   unsigned long long todo = 0, any_word = 0, whole_word = 0;
-  auto sort_tiles = [&]() __attribute__((always_inline)) {
+  auto sort_tiles = [&](const int4 k) __attribute__((always_inline)) {
     const int t = chunk * 64 + lane;
-    int4 k = make_int4(0, 0, 0, 0);
     const bool here = t >= lo && t < hi;
-    if (here && c.k_summary) {
-      const int4* sum = reinterpret_cast<const int4*>(c.k_summary) + b * c.k_summary_sb + (long long)t * kSub;
-      k = sum[0];
-      if (kSub > 1 && t * kSub + 1 < a.summaries) {
-        const int4 n = sum[1];
-        k = make_int4(min(k.x, n.x), max(k.y, n.y), min(k.z, n.z), max(k.w, n.w));
-      }
-    }
     auto may_see = [&](const Range& r) {
       return here && k.y >= 0 && k.x <= r.dmax && k.y >= r.dmin && k.z <= r.omax;
     };
@@ -628,8 +652,8 @@ __global__ __launch_bounds__(kWaves * kWave, kWaves == 1 ? 1 : kD == 64 && kDtyp
   auto next_tile = [&]() __attribute__((always_inline)) -> Next {
     while (todo == 0) {
       ++chunk;
-      if ((long long)chunk * 64 >= hi) return Next{-1, false, false};
-      sort_tiles();
+      if (chunk * 64 >= hi) return Next{-1, false, false};
+      sort_tiles(summary_of(chunk * 64 + lane));
     }
     const int bit = __builtin_ctzll(todo);
     todo &= todo - 1;
@@ -642,8 +666,8 @@ __global__ __launch_bounds__(kWaves * kWave, kWaves == 1 ? 1 : kD == 64 && kDtyp
 #pragma unroll
       for (int v = 0; v < 16; ++v) o[x][v] = 0.f;
     m_run = -INFINITY, l_run = 0.f, base = Ty::kShift, mixed_seen = false;
-    chunk = lo / 64 - 1;
-    todo = 0;
+    chunk = lo / 64;
+    sort_tiles(decltype(careful_c)::value ? summary_of(lo / 64 * 64 + lane) : first_summary);
     Next now = next_tile();
     if (now.tile >= 0) load_tile(now.tile, 0);
     int buf = 0;
