@@ -1,140 +1,9 @@
-// Softmax attention over the keys that a query may see, for packed images, padded batches,
-// prefixes and frames, with an optional cap on the scores and an optional bias by distance:
-//
-//   score(i, j) = c(scale q_i . k_j) - sum_a slope[head, a] |p_a(i) - p_a(j)|
-//   c(s)        = cap tanh(s / cap), or s
-//   seen(i, j)  = document(i) == document(j) >= 0 and order(j) <= order(i)
-//   out_i       = sum_seen e^(score - max) v_j / sum_seen e^(score - max); zeros if none is seen
-//
-// One pass over the keys with the running maximum and sum of the softmax.  As in the
-// unmasked kernels a wave forms S^T = K Q^T, so that a lane owns one query row and its
-// maximum, sum and probabilities stay in its registers; O^T += V^T P^T follows with P in
-// place.  A row is a (token, head of the group) pair: the heads that share a key head are
-// neighbouring rows, so K and V are read once for all of them.
-//
-// Keys come in tiles of kTile.  A small summary of the keys (per 32 of them the range of
-// documents and orders, made once per batch) sorts a tile, for the rows of a wave, into unseen
-// (skipped without reading K or V), seen whole (no mask is evaluated) and mixed (each score is
-// tested).  64 tiles are sorted at a time, one per lane.
-//
-// Few rows (a new token, a pooling latent): the keys are split over workgroups of one wave
-// that write (maximum, sum, output) parts, and a second kernel joins them in a fixed order.
-#include <hip/hip_bf16.h>
-#include <hip/hip_fp16.h>
-
-#include <type_traits>
-
-#include "common.hpp"
+// Masked attention's C entry points: the keys' summary, the order of self-attention's row
+// tiles, and the launch of masked_attention_kernel.hpp's kernels.
+#include "masked_attention.hpp"
 
 namespace musc {
 namespace mattn {
-
-typedef float floatx16 __attribute__((ext_vector_type(16)));
-typedef float float2v __attribute__((ext_vector_type(2)));
-typedef int int4v __attribute__((ext_vector_type(4)));
-typedef short short4v __attribute__((ext_vector_type(4)));
-typedef short short8v __attribute__((ext_vector_type(8)));
-typedef __attribute__((address_space(3))) void lds_void;
-
-constexpr int kBufferFlags = 0x00020000;   // buffer resource word 3 for raw byte-addressed loads
-constexpr int kNowhere = 0x7fffff00;       // a byte offset past every extent: such loads give zeros
-constexpr float kLazyLog2 = 8.f;           // the running maximum moves once a tile exceeds it by this
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kSummaryKeys = 32;
-constexpr int kMaxAxes = 3;
-constexpr int kRowTile = 128;  // rows of a workgroup of four waves
-
-template <int kDtype>
-struct Type;
-template <>
-struct Type<MUSC_DTYPE_F32> {
-  typedef float T;
-  static constexpr int kTile = 32;
-  static constexpr float kShift = 0.f;
-};
-template <>
-struct Type<MUSC_DTYPE_F16> {
-  typedef _Float16 T;
-  typedef T Vec __attribute__((ext_vector_type(8)));
-  typedef T Two __attribute__((ext_vector_type(2)));
-  static constexpr int kTile = 64;
-  // probabilities are formed 2^7 times as large, at most 2^15 with the slack: entries down to
-  // 2^-21 of the largest stay normal fp16 numbers
-  static constexpr float kShift = 7.f;
-  static __device__ __forceinline__ floatx16 mfma(Vec a, Vec b, floatx16 c) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
-  }
-  static __device__ __forceinline__ float add_both(Two p, float sum) {
-    return __builtin_amdgcn_fdot2(p, Two{(T)1.f, (T)1.f}, sum, false);
-  }
-};
-template <>
-struct Type<MUSC_DTYPE_BF16> {
-  typedef __bf16 T;
-  typedef T Vec __attribute__((ext_vector_type(8)));
-  typedef T Two __attribute__((ext_vector_type(2)));
-  static constexpr int kTile = 64;
-  static constexpr float kShift = 0.f;
-  static __device__ __forceinline__ floatx16 mfma(Vec a, Vec b, floatx16 c) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
-  }
-  static __device__ __forceinline__ float add_both(Two p, float sum) {
-    return __builtin_amdgcn_fdot2_f32_bf16(p, Two{(T)1.f, (T)1.f}, sum, false);
-  }
-};
-
-// Keys of a tile: workgroups of one wave take 32, so that four of them fit a CU's LDS.
-template <int kDtype, int kWaves>
-constexpr int tile_keys() {
-  return kWaves == 1 ? 32 : Type<kDtype>::kTile;
-}
-
-// Staged rows of K and V: 128, 256 or 512 bytes, their 16-byte chunks permuted by the row so
-// that the lanes one LDS read serves together touch different banks: 16 neighbouring rows of
-// one chunk (K's operands) take 16 places of a 256-byte window, and so do 4 neighbouring rows
-// of 4 chunks (V's transposing reads).  Chunk c of row r is at place c ^ swizzle(r).
-template <int kPitch>
-__device__ __forceinline__ constexpr int swizzle(int r) {
-  return kPitch == 128 ? (((r >> 1) & 1) << 2) | ((r >> 2) & 3) : ((r & 3) << 2) | ((r >> 2) & 3);
-}
-
-struct Args {
-  musc_masked_attention c;
-  int group, rows, row_tiles, key_tiles, splits, summaries, heads_at_once;
-  long long units;
-  float* part_ml;  // (units in (b, kv head), rows, split) x (maximum, sum)
-  float* part_o;   // the same x d
-};
-
-__device__ __forceinline__ float halves_max(float v) {
-  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return __builtin_elementwise_maximum(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-__device__ __forceinline__ float halves_sum(float v) {
-  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
-}
-// Minimum over the wave by lane-crossing moves (no LDS): lanes get their neighbours 1, 2, 4, 8 to
-// the left within rows of 16, then the rows' last lanes go on to the next rows; lane 63 has it.
-template <int kMove, int kRows>
-__device__ __forceinline__ int min_with(int v) {
-  return min(v, __builtin_amdgcn_update_dpp(0x7fffffff, v, kMove, kRows, 0xf, false));
-}
-__device__ __forceinline__ int wave_min_int(int v) {
-  v = min_with<0x111, 0xf>(v);
-  v = min_with<0x112, 0xf>(v);
-  v = min_with<0x114, 0xf>(v);
-  v = min_with<0x118, 0xf>(v);
-  v = min_with<0x142, 0xa>(v);
-  v = min_with<0x143, 0xc>(v);
-  return __builtin_amdgcn_readlane(v, 63);
-}
-__device__ __forceinline__ int wave_max_int(int v) { return ~wave_min_int(~v); }
-
-// The documents and orders of a set of rows: what a tile is compared with.
-struct Range {
-  int dmin, dmax, omin, omax;
-};
 
 // Per 32 keys: smallest and largest document (negative ones count as -1), smallest and largest
 // order of the keys that have a document.  One wave handles two groups of 32.
@@ -206,579 +75,6 @@ __global__ __launch_bounds__(256) void row_order_kernel(const Schedule s, int* _
   int rank = 0;
   for (int j = 0; j < n; ++j) rank += work[j] > here || (work[j] == here && j > tile);
   mine[rank] = tile;
-}
-
-template <int kN, int kI = 0, typename F>
-__device__ __forceinline__ void unroll(F f) {
-  if constexpr (kI < kN) {
-    f(std::integral_constant<int, kI>{});
-    unroll<kN, kI + 1>(f);
-  }
-}
-
-// Loads straight from memory into LDS, lane l's 16 (or 4) bytes to `to` (+ kTo) + 16 l (or
-// 4 l), `to` uniform.  From inline assembly, as the compiler, which cannot tell the two buffers apart,
-// would wait for them before reading the other one; the loop waits for them itself.
-template <int kTo>
-__device__ __forceinline__ void load_to_lds_16(uint32_t to, int offset, int4v from, int from_offset) {
-  asm volatile("s_add_u32 m0, %0, %4\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
-               :: "s"(to), "v"(offset), "s"(from), "s"(from_offset), "i"(kTo) : "memory", "m0", "scc");
-}
-__device__ __forceinline__ void load_to_lds_4(const void* place, int offset, int4v from) {
-  const uint32_t to = __builtin_amdgcn_readfirstlane((uint32_t)(size_t)(lds_void*)place);
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
-               :: "s"(to), "v"(offset), "s"(from) : "memory", "m0");
-}
-__device__ __forceinline__ int4v resource(const void* base, long long bytes) {
-  const unsigned long long at = reinterpret_cast<unsigned long long>(base);
-  return int4v{__builtin_amdgcn_readfirstlane((int)(uint32_t)at), __builtin_amdgcn_readfirstlane((int)(uint32_t)(at >> 32)),
-               __builtin_amdgcn_readfirstlane((int)bytes), kBufferFlags};
-}
-
-// kWaves waves of 32 rows each; kD: head width rounded up to 64, 96 or 128.
-template <int kDtype, int kD, int kWaves>
-__global__ __launch_bounds__(kWaves * kWave, kWaves == 1 ? 1 : kD == 64 && kDtype != MUSC_DTYPE_F32 ? 3 : 2) void masked_attention_kernel(const Args a) {
-  using Ty = Type<kDtype>;
-  typedef typename Ty::T T;
-  constexpr bool k16 = kDtype != MUSC_DTYPE_F32;
-  constexpr int kTile = tile_keys<kDtype, kWaves>(), kSub = kTile / 32;
-  constexpr int kPer = 16 / (int)sizeof(T);                 // elements of a 16-byte chunk
-  constexpr int kPitch = (kD <= 64 ? 64 : 128) * (int)sizeof(T);
-  constexpr int kPlaces = kPitch / 16;                      // chunks of a staged row
-  constexpr int kPart = kTile * kPitch;                     // bytes of a staged K or V tile
-  constexpr int kLoads = kPart / 1024 / kWaves;             // loads of K (and of V) per wave
-  static_assert(kLoads * kWaves * 1024 == kPart, "whole loads per wave");
-  constexpr int kO = kD / 32;
-  __shared__ __attribute__((aligned(1024))) char staged[2][2 * kPart];
-  __shared__ __attribute__((aligned(16))) int docs_s[2][64], ords_s[2][64];
-  __shared__ float pos_s[2][64 * kMaxAxes];
-  __shared__ Range ranges[kWaves];
-
-  const musc_masked_attention& c = a.c;
-  // uniform numbers in scalar registers (the divisions leave them in vector ones)
-  const auto uniform = [](long long x) { return __builtin_amdgcn_readfirstlane((int)x); };
-  uint32_t split, row_tile, bh;
-  if (a.heads_at_once) {
-    // one XCD works on heads_at_once heads together, row tile by row tile (the longest first)
-    const uint32_t per_xcd = (uint32_t)(c.batch * c.kv_heads) / kXcds, local = blockIdx.x / kXcds;
-    const uint32_t of_group = (uint32_t)(a.heads_at_once * a.row_tiles * a.splits);
-    const uint32_t group = uniform(local / of_group), in_group = local - group * of_group;
-    const uint32_t first = group * a.heads_at_once, at_once = min((uint32_t)a.heads_at_once, per_xcd - first);
-    const uint32_t rest = uniform(in_group / a.splits);
-    split = in_group - rest * a.splits;
-    row_tile = uniform(rest / at_once);
-    bh = blockIdx.x % kXcds * per_xcd + first + (rest - row_tile * at_once);
-  } else {
-    const uint32_t unit = (blockIdx.x % kXcds) * (gridDim.x / kXcds) + blockIdx.x / kXcds;
-    if (unit >= (uint32_t)a.units) return;
-    const uint32_t rest = uniform(unit / a.splits);
-    split = unit - rest * a.splits;
-    bh = uniform(rest / a.row_tiles);
-    row_tile = rest - bh * a.row_tiles;
-  }
-  const int b = uniform(bh / c.kv_heads), kvh = bh - b * c.kv_heads;
-  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid % kWave;
-  const int lq = lane & 31, lh = lane >> 5;
-
-  // tiles of this split, 64 sorted at a time by the keys' summary; the first 64 are asked for now
-  const int lo = uniform((long long)a.key_tiles * split / a.splits);
-  const int hi = uniform((long long)a.key_tiles * (split + 1) / a.splits);
-  const int4* summary = c.k_summary ? reinterpret_cast<const int4*>(c.k_summary) + b * c.k_summary_sb : nullptr;
-  auto summary_of = [&](int t) __attribute__((always_inline)) {
-    int4 k = make_int4(0, 0, 0, 0);
-    if (summary && t >= lo && t < hi) {
-      k = summary[(long long)t * kSub];
-      if (kSub > 1 && t * kSub + 1 < a.summaries) {
-        const int4 n = summary[(long long)t * kSub + 1];
-        k = make_int4(min(k.x, n.x), max(k.y, n.y), min(k.z, n.z), max(k.w, n.w));
-      }
-    }
-    return k;
-  };
-  const int4 first_summary = summary_of(lo / 64 * 64 + lane);
-
-  // by the caller's order, or later rows first: with an order of tokens they see more keys, and
-  // the longest work should not start last
-  int tile_of_rows = a.row_tiles - 1 - (int)row_tile;
-  if (kWaves > 1 && c.row_order) tile_of_rows = uniform(c.row_order[b * c.row_order_sb + row_tile]);
-  tile_of_rows = min(max(tile_of_rows, 0), a.row_tiles - 1);
-  const int row = (tile_of_rows * kWaves + wave) * 32 + lq;
-  const bool inside = row < a.rows;
-  const int token = inside ? (int)((uint32_t)row / (uint32_t)a.group) : 0;
-  const int head = kvh * a.group + (inside ? row - token * a.group : 0);
-  const int d = c.d, k_len = c.k_len, axes = c.axes;
-
-  // this row's document and order (rows outside the tensor read token 0's), its Q and positions,
-  // all asked for before any is used
-  int qdoc = 0, qord = 0;
-  if (c.q_documents) qdoc = c.q_documents[b * c.q_tokens_sb + token];
-  if (c.q_order) qord = c.q_order[b * c.q_tokens_sb + token];
-  const T* qrow = static_cast<const T*>(c.q) + b * c.q_sb + (long long)token * c.q_st + head * c.q_sh;
-  constexpr int kQ = kD / (2 * kPer);
-  typedef T TVec __attribute__((ext_vector_type(kPer)));
-  TVec qf[kQ];
-#pragma unroll
-  for (int m = 0; m < kQ; ++m) {
-    const int at = (2 * m + lh) * kPer;
-    qf[m] = TVec{};
-    if (at < d) qf[m] = *reinterpret_cast<const TVec*>(qrow + at);
-  }
-  float qpos[kMaxAxes], slope[kMaxAxes];
-#pragma unroll
-  for (int x = 0; x < kMaxAxes; ++x) {
-    qpos[x] = 0.f, slope[x] = 0.f;
-    if (x < axes) {
-      qpos[x] = c.q_positions[b * c.q_positions_sb + (long long)token * axes + x];
-      slope[x] = c.slopes[head * axes + x];
-    }
-  }
-
-  const bool live = inside && qdoc >= 0;
-  Range mine, all_rows;
-  mine.dmin = wave_min_int(live ? qdoc : 0x7fffffff);
-  mine.dmax = wave_max_int(live ? qdoc : -1);
-  mine.omin = wave_min_int(live ? qord : 0x7fffffff);
-  mine.omax = wave_max_int(live ? qord : (int)0x80000000);
-  all_rows = mine;
-  if constexpr (kWaves > 1) {
-    if (lane == 0) ranges[wave] = mine;
-  }
-  // keys of calls without documents or orders have 0
-  if (tid < 64) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) docs_s[i][tid] = 0, ords_s[i][tid] = 0;
-  }
-  __syncthreads();
-  if constexpr (kWaves > 1) {
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-      all_rows.dmin = min(all_rows.dmin, ranges[w].dmin);
-      all_rows.dmax = max(all_rows.dmax, ranges[w].dmax);
-      all_rows.omin = min(all_rows.omin, ranges[w].omin);
-      all_rows.omax = max(all_rows.omax, ranges[w].omax);
-    }
-  }
-
-  // Scores stay "raw" until the exponential: score in log2 units =
-  // raw * to_log2 (+ a constant that cancels), to_log2 > 0:
-  //   no cap   raw = +- q . k (Q negated for a negative scale), to_log2 = |scale| log2 e
-  //   cap      raw = -1 / (1 + e^2x), x = scale q . k / cap, as cap tanh x = cap (1 + 2 raw);
-  //            fp32: raw = tanh x
-  const bool capped = c.cap > 0.f;
-  const float scale = c.scale == 0.f ? 1.f : c.scale;
-  const float to_log2 = (capped ? (k16 ? 2.f * c.cap : c.cap) : fabsf(scale)) * kLog2e;
-  const float by_cap = capped ? scale / c.cap * (k16 ? 2.f * kLog2e : 1.f) : 0.f;
-  const bool negate = !capped && scale < 0.f;
-#pragma unroll
-  for (int m = 0; m < kQ; ++m) {
-    if (negate) qf[m] = -qf[m];
-    if (c.scale == 0.f) qf[m] = TVec{};
-  }
-  // the B operand of the distances: 1 and -position; slopes in raw units
-#pragma unroll
-  for (int x = 0; x < kMaxAxes; ++x) {
-    qpos[x] = x < axes ? (lh == 0 ? 1.f : -qpos[x]) : 0.f;
-    slope[x] = slope[x] * kLog2e / to_log2;
-  }
-
-  // Staging: load i of a tile fills 1024 bytes, whole rows; wave w issues loads w, w + kWaves, ..
-  // The loads of a whole tile share a resource based at the wave's first row, and a scalar offset
-  // leads to the rows of each; in the last, partial tile each has a resource of its own that ends
-  // with the last key.  Lanes of channels past d load from nowhere.
-  const char* kbase = reinterpret_cast<const char*>(static_cast<const T*>(c.k) + b * c.k_sb + (long long)kvh * c.k_sh);
-  const char* vbase = reinterpret_cast<const char*>(static_cast<const T*>(c.v) + b * c.v_sb + (long long)kvh * c.v_sh);
-  const uint32_t k_row = (uint32_t)(c.k_st * (long long)sizeof(T)), v_row = (uint32_t)(c.v_st * (long long)sizeof(T));
-  const uint32_t staged_at = (uint32_t)(size_t)(lds_void*)&staged[0][0] + wave * 1024;
-  constexpr int kRows = 64 / kPlaces;  // rows of a load
-  const int row_bytes = d * (int)sizeof(T);
-  auto load_tile = [&](int tile, int buf) __attribute__((always_inline)) {
-    const int first = tile * kTile, rem = min(k_len - first, kTile), mine = wave * kRows;
-    const uint32_t to = __builtin_amdgcn_readfirstlane(staged_at + buf * 2 * kPart);
-    const char* kt = kbase + (unsigned long long)(uint32_t)(first + mine) * k_row;
-    const char* vt = vbase + (unsigned long long)(uint32_t)(first + mine) * v_row;
-    auto lane_offset = [&](int j, uint32_t row) {
-      const int r = lane / kPlaces, chunk = (lane % kPlaces) ^ swizzle<kPitch>((wave + kWaves * j) * kRows + r);
-      return chunk * kPer < d ? (int)(r * row) + chunk * 16 : kNowhere;
-    };
-    if (rem == kTile) {
-      const int4v rk = resource(kt, (long long)(kTile - mine - 1) * k_row + row_bytes);
-      const int4v rv = resource(vt, (long long)(kTile - mine - 1) * v_row + row_bytes);
-      unroll<kLoads>([&](auto jc) {
-        constexpr int j = decltype(jc)::value;
-        load_to_lds_16<j * kWaves * 1024>(to, lane_offset(j, k_row), rk, (int)(j * kWaves * kRows * k_row));
-        load_to_lds_16<j * kWaves * 1024 + kPart>(to, lane_offset(j, v_row), rv, (int)(j * kWaves * kRows * v_row));
-      });
-    } else {
-      unroll<kLoads>([&](auto jc) {
-        constexpr int j = decltype(jc)::value;
-        const int rows = rem - mine - j * kWaves * kRows;
-        const unsigned long long at = j * kWaves * kRows;
-        load_to_lds_16<j * kWaves * 1024>(
-            to, lane_offset(j, k_row), resource(kt + at * k_row, rows > 0 ? (long long)(rows - 1) * k_row + row_bytes : 0), 0);
-        load_to_lds_16<j * kWaves * 1024 + kPart>(
-            to, lane_offset(j, v_row), resource(vt + at * v_row, rows > 0 ? (long long)(rows - 1) * v_row + row_bytes : 0), 0);
-      });
-    }
-    if (wave == kWaves - 1) {
-      if (c.k_documents)
-        load_to_lds_4(&docs_s[buf][0], lane * 4,
-                      resource(c.k_documents + b * c.k_tokens_sb + first, rem * 4));
-      if (c.k_order)
-        load_to_lds_4(&ords_s[buf][0], lane * 4,
-                      resource(c.k_order + b * c.k_tokens_sb + first, rem * 4));
-      if (axes) {
-        const int4v rp = resource(c.k_positions + b * c.k_positions_sb + (long long)first * axes, rem * axes * 4);
-#pragma unroll
-        for (int x = 0; x < kMaxAxes; ++x)
-          if (x < axes) load_to_lds_4(&pos_s[buf][64 * x], (64 * x + lane) * 4, rp);
-      }
-    }
-  };
-
-  floatx16 o[kO];
-  float m_run, l_run;  // running maximum (raw) and sum of this half's keys
-  float base;          // exponent of a score: raw * to_log2 + base
-  bool mixed_seen;
-
-  // one staged tile; whole: every row sees every key.  careful: in a mixed tile, products
-  // of keys that a row does not see are left out one by one (their V may be infinite or NaN)
-  auto attend = [&](int buf, int tile, bool whole, auto careful_c) __attribute__((always_inline)) {
-    constexpr bool careful = decltype(careful_c)::value;
-    // Byte places of this lane's operands: row lq (K) or the row and chunk of its V operand, in
-    // chunk order from the permutation's exclusive or, which all further chunks keep.  Formed
-    // anew for each tile, as keeping all of them would take the registers of the operands.
-    int k_at = buf * 2 * kPart + lq * kPitch + ((lh ^ swizzle<kPitch>(lq)) << 4);
-    int v_at = buf * 2 * kPart + kPart;
-    if constexpr (k16) {
-      const int r = 4 * lh + ((lq & 15) >> 2);
-      v_at += r * kPitch + (((2 * (lq >> 4) + ((lq & 3) >> 1)) ^ swizzle<kPitch>(r)) << 4) + 8 * (lq & 1);
-    } else {
-      v_at += 4 * lh * kPitch + (((lq >> 2) ^ lh) << 4) + 4 * (lq & 3);
-    }
-    asm volatile("" : "+v"(k_at), "+v"(v_at));
-    const char* all = &staged[0][0];
-    floatx16 s[kSub];
-    TVec kf[kSub][kQ];
-#pragma unroll
-    for (int u = 0; u < kSub; ++u)
-#pragma unroll
-      for (int m = 0; m < kQ; ++m)
-        kf[u][m] = *reinterpret_cast<const TVec*>(all + (k_at ^ (m << 5)) + 32 * u * kPitch);
-    __builtin_amdgcn_sched_barrier(0);  // all reads in flight before the first product waits
-#pragma unroll
-    for (int u = 0; u < kSub; ++u)
-#pragma unroll
-      for (int v = 0; v < 16; ++v) s[u][v] = 0.f;
-#pragma unroll
-    for (int m = 0; m < kQ; ++m)
-#pragma unroll
-      for (int u = 0; u < kSub; ++u) {
-        if constexpr (k16) {
-          s[u] = Ty::mfma(kf[u][m], qf[m], s[u]);
-        } else {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) s[u] = __builtin_amdgcn_mfma_f32_32x32x2f32(kf[u][m][j], qf[m][j], s[u], 0, 0, 0);
-        }
-      }
-    // V^T fragments by transposing LDS reads, in flight during the softmax: within a group of 16
-    // lanes, lane i's element j is element i % 4 of the 8 bytes that lane 4 j + i / 4 addressed,
-    // so with V row-major the lane that addresses V[key0 + r / 4][d0 + 4 (r % 4) ..] (r its place
-    // in the group) hands element j of lane i the value V[key0 + j][d0 + i]: the A operand's row
-    // d0 + i, k = j
-    short8v vf[k16 && !careful ? 2 * kSub : 1][k16 && !careful ? kO : 1];
-    auto read_v = [&](int mm, int x) {
-      // key0 = 16 mm + 4 lh (+ 8: the permutation's bit 1), d0 = 32 x + 16 (lq / 16)
-      auto tr = [&](int upper) {
-        typedef __attribute__((address_space(3))) short4v lds_short4v;
-        return __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (lds_short4v*)(all + (v_at ^ (x << 6) ^ (upper << 5)) + (16 * mm + 8 * upper) * kPitch));
-      };
-      const short4v f0 = tr(0), f1 = tr(1);
-      return short8v{f0[0], f0[1], f0[2], f0[3], f1[0], f1[1], f1[2], f1[3]};
-    };
-    if constexpr (k16 && !careful) {
-#pragma unroll
-      for (int mm = 0; mm < 2 * kSub; ++mm)
-#pragma unroll
-        for (int x = 0; x < kO; ++x) vf[mm][x] = read_v(mm, x);
-      __builtin_amdgcn_sched_barrier(0);
-    }
-    if (capped) {
-#pragma unroll
-      for (int u = 0; u < kSub; ++u)
-#pragma unroll
-        for (int v = 0; v < 16; ++v) {
-          const float x = s[u][v] * by_cap;
-          s[u][v] = k16 ? __builtin_amdgcn_rcpf(-1.f - __builtin_amdgcn_exp2f(x)) : tanhf(x);
-        }
-    }
-    // distances from the matrix cores: position(j) * 1 + 1 * -position(i), exact in fp32
-#pragma unroll
-    for (int x = 0; x < kMaxAxes; ++x)
-      if (x < axes)
-#pragma unroll
-        for (int u = 0; u < kSub; ++u) {
-          floatx16 apart;
-#pragma unroll
-          for (int v = 0; v < 16; ++v) apart[v] = 0.f;
-          const float kp = pos_s[buf][(32 * u + lq) * axes + x];
-          apart = __builtin_amdgcn_mfma_f32_32x32x2f32(lh == 0 ? kp : 1.f, qpos[x], apart, 0, 0, 0);
-#pragma unroll
-          for (int v = 0; v < 16; ++v) s[u][v] = fmaf(-slope[x], fabsf(apart[v]), s[u][v]);
-        }
-    // register v of block u holds key 32 u + 8 (v / 4) + 4 lh + v % 4
-    uint32_t seen = 0xffffffffu;
-    if (!whole) {
-      mixed_seen = true;
-      const int rem = k_len - tile * kTile;
-#pragma unroll
-      for (int u = 0; u < kSub; ++u)
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const int key = 32 * u + 8 * g + 4 * lh;
-          const int4v kd = *reinterpret_cast<const int4v*>(&docs_s[buf][key]);
-          const int4v ko = *reinterpret_cast<const int4v*>(&ords_s[buf][key]);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const bool see = kd[i] == qdoc && ko[i] <= qord && key + i < rem;
-            s[u][4 * g + i] = see ? s[u][4 * g + i] : -INFINITY;
-            if (careful && !see) seen &= ~(1u << (16 * u + 4 * g + i));
-          }
-        }
-    }
-    float top = s[0][0];
-#pragma unroll
-    for (int u = 0; u < kSub; ++u)
-#pragma unroll
-      for (int v = 0; v < 16; ++v) top = __builtin_elementwise_maximum(top, s[u][v]);
-    top = halves_max(top);
-    if (!__all((top - m_run) * to_log2 <= kLazyLog2)) {  // false at first, and for NaN
-      const float m_new = fmaxf(m_run, top);
-      const float alpha = m_run == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m_run - m_new) * to_log2);
-      l_run *= alpha;
-#pragma unroll
-      for (int x = 0; x < kO; ++x)
-#pragma unroll
-        for (int v = 0; v < 16; ++v) o[x][v] *= alpha;
-      m_run = m_new;
-      base = Ty::kShift - (m_run == -INFINITY ? 0.f : m_run * to_log2);
-    }
-#pragma unroll
-    for (int u = 0; u < kSub; ++u)
-#pragma unroll
-      for (int v = 0; v < 16; ++v) s[u][v] = __builtin_amdgcn_exp2f(fmaf(s[u][v], to_log2, base));
-    TVec p[2 * kSub];
-    if constexpr (k16) {
-#pragma unroll
-      for (int mm = 0; mm < 2 * kSub; ++mm)
-#pragma unroll
-        for (int j = 0; j < 8; j += 2) {
-          const float2v f = {s[mm >> 1][8 * (mm & 1) + j], s[mm >> 1][8 * (mm & 1) + j + 1]};
-          const auto two = __builtin_convertvector(f, typename Ty::Two);
-          p[mm][j] = two[0], p[mm][j + 1] = two[1];
-          l_run = Ty::add_both(two, l_run);  // the sum of what the product uses
-        }
-    } else {
-#pragma unroll
-      for (int u = 0; u < kSub; ++u)
-#pragma unroll
-        for (int v = 0; v < 16; ++v) l_run += s[u][v];
-    }
-    if (careful && !whole) {
-#pragma unroll 1
-      for (int key = 0; key < kTile; ++key) {
-        const int u0 = key >> 5, v0 = ((key & 31) >> 3) * 4 + (key & 3), from = lq + 32 * ((key >> 2) & 1);
-        float pr = 0.f;
-#pragma unroll
-        for (int u = 0; u < kSub; ++u)
-#pragma unroll
-          for (int v = 0; v < 16; ++v)
-            if (u == u0 && v == v0) pr = (float)(T)s[u][v];
-        pr = __shfl(pr, from, kWave);
-        const bool see = (__shfl(seen, from, kWave) >> (16 * u0 + v0)) & 1;
-#pragma unroll
-        for (int x = 0; x < kO; ++x)
-#pragma unroll
-          for (int v = 0; v < 16; ++v) {
-            if (v % 4 == 0) __builtin_amdgcn_sched_barrier(0);  // few values at a time
-            const int at = 32 * x + 8 * (v >> 2) + 4 * lh + (v & 3);
-            const T value = *reinterpret_cast<const T*>(staged[buf] + kPart + key * kPitch + ((at / kPer) ^ swizzle<kPitch>(key)) * 16 +
-                                                        at % kPer * (int)sizeof(T));
-            if (see) o[x][v] = fmaf(pr, (float)value, o[x][v]);
-          }
-      }
-      return;
-    }
-    if constexpr (k16) {
-#pragma unroll
-      for (int mm = 0; mm < 2 * kSub; ++mm)
-#pragma unroll
-        for (int x = 0; x < kO; ++x)
-          o[x] = Ty::mfma(__builtin_bit_cast(TVec, careful ? read_v(mm, x) : vf[careful ? 0 : mm][careful ? 0 : x]), p[mm], o[x]);
-    } else {
-      // step e takes keys 8 (e / 4) + 4 lh + e % 4: register e of s
-#pragma unroll
-      for (int u = 0; u < kSub; ++u)
-#pragma unroll
-        for (int e = 0; e < 16; ++e)
-#pragma unroll
-          for (int x = 0; x < kO; ++x) {
-            const float f = *reinterpret_cast<const float*>(
-                all + (v_at ^ (x << 7) ^ ((e & 3) << 6) ^ (((e >> 2) & 1) << 5)) +
-                (32 * u + 8 * (e >> 2) + (e & 3)) * kPitch);
-            o[x] = __builtin_amdgcn_mfma_f32_32x32x2f32(f, s[u][e], o[x], 0, 0, 0);
-          }
-    }
-  };
-
-  // the tiles that some row of the workgroup may see
-  int chunk = 0;
-  unsigned long long todo = 0, any_word = 0, whole_word = 0;
-  auto sort_tiles = [&](const int4 k) __attribute__((always_inline)) {
-    const int t = chunk * 64 + lane;
-    const bool here = t >= lo && t < hi;
-    auto may_see = [&](const Range& r) {
-      return here && k.y >= 0 && k.x <= r.dmax && k.y >= r.dmin && k.z <= r.omax;
-    };
-    todo = __ballot(may_see(all_rows));
-    any_word = __ballot(may_see(mine));
-    whole_word = __ballot(here && k.x == k.y && mine.dmin == mine.dmax && k.x == mine.dmin && k.w <= mine.omin &&
-                          (t + 1) * kTile <= k_len);
-  };
-  struct Next {
-    int tile;
-    bool any, whole;
-  };
-  auto next_tile = [&]() __attribute__((always_inline)) -> Next {
-    while (todo == 0) {
-      ++chunk;
-      if (chunk * 64 >= hi) return Next{-1, false, false};
-      sort_tiles(summary_of(chunk * 64 + lane));
-    }
-    const int bit = __builtin_ctzll(todo);
-    todo &= todo - 1;
-    return Next{chunk * 64 + bit, (bool)((any_word >> bit) & 1), (bool)((whole_word >> bit) & 1)};
-  };
-
-  auto walk = [&](auto careful_c) __attribute__((always_inline)) {
-#pragma unroll
-    for (int x = 0; x < kO; ++x)
-#pragma unroll
-      for (int v = 0; v < 16; ++v) o[x][v] = 0.f;
-    m_run = -INFINITY, l_run = 0.f, base = Ty::kShift, mixed_seen = false;
-    chunk = lo / 64;
-    sort_tiles(decltype(careful_c)::value ? summary_of(lo / 64 * 64 + lane) : first_summary);
-    Next now = next_tile();
-    if (now.tile >= 0) load_tile(now.tile, 0);
-    int buf = 0;
-    while (now.tile >= 0) {
-      const Next then = next_tile();
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's share of tile `now` is in LDS
-      __syncthreads();  // everyone's is, and everyone is done with the other buffer
-      if (then.tile >= 0) load_tile(then.tile, buf ^ 1);
-      if (now.any) attend(buf, now.tile, now.whole, careful_c);
-      buf ^= 1;
-      now = then;
-    }
-  };
-  walk(std::integral_constant<bool, false>{});
-  // 0 * V of an unseen key is NaN where V is not finite: then all over again, with care
-  bool bad = false;
-  if (mixed_seen && live) {
-#pragma unroll
-    for (int x = 0; x < kO; ++x)
-#pragma unroll
-      for (int v = 0; v < 16; ++v) bad |= !(fabsf(o[x][v]) < INFINITY);
-  }
-  // also the barrier before the buffers are filled again
-  if (__syncthreads_or(bad)) walk(std::integral_constant<bool, true>{});
-
-  l_run = halves_sum(l_run);
-  if (!inside) return;
-  // register v of block x holds channel 32 x + 8 (v / 4) + 4 lh + v % 4
-  if (a.splits == 1) {
-    const bool empty = !live || l_run == 0.f;
-    const float inv = 1.f / l_run;
-    T* orow = static_cast<T*>(c.out) + b * c.o_sb + (long long)token * c.o_st + head * c.o_sh;
-#pragma unroll
-    for (int x = 0; x < kO; ++x)
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int at = 32 * x + 8 * g + 4 * lh;
-        typedef T Four __attribute__((ext_vector_type(4)));
-        Four y;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) y[i] = empty ? (T)0.f : (T)(o[x][4 * g + i] * inv);
-        if (at < d) *reinterpret_cast<Four*>(orow + at) = y;
-      }
-  } else {
-    const long long part = ((long long)bh * a.rows + row) * a.splits + split;
-    if (lh == 0) {
-      a.part_ml[2 * part] = live ? m_run * to_log2 : -INFINITY;
-      a.part_ml[2 * part + 1] = live ? l_run : 0.f;
-    }
-    float* prow = a.part_o + part * d;
-#pragma unroll
-    for (int x = 0; x < kO; ++x)
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int at = 32 * x + 8 * g + 4 * lh;
-        const float4 y = make_float4(o[x][4 * g], o[x][4 * g + 1], o[x][4 * g + 2], o[x][4 * g + 3]);
-        if (at < d) *reinterpret_cast<float4*>(prow + at) = live ? y : make_float4(0.f, 0.f, 0.f, 0.f);
-      }
-  }
-}
-
-// Joins the splits of a row, in their order: four waves per row, each every fourth split with two
-// channels per lane, then the four in order.
-constexpr int kMaxSplits = 256;
-template <int kDtype>
-__global__ __launch_bounds__(256) void join_kernel(const Args a) {
-  typedef typename Type<kDtype>::T T;
-  __shared__ float weight[kMaxSplits], tops[4], sums[4];
-  __shared__ float2 parts[4][kWave];
-  const musc_masked_attention& c = a.c;
-  const long long r = blockIdx.x;
-  const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
-  const int splits = a.splits;
-  // the largest of the maxima, each split's factor and the sum; a part without keys has sum 0
-  // (one whose scores are NaN has its sum NaN)
-  const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + r * splits;
-  const float2 mine = tid < splits ? ml[tid] : make_float2(-INFINITY, 0.f);
-  const float top_here = wave_max(mine.x);
-  if (lane == 0) tops[wave] = top_here;
-  __syncthreads();
-  const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-  const float w = mine.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(mine.x - top);
-  if (tid < splits) weight[tid] = w;
-  const float sum_here = wave_sum(mine.y == 0.f ? 0.f : w * mine.y);
-  if (lane == 0) sums[wave] = sum_here;
-  __syncthreads();
-  const float sum = sums[0] + sums[1] + sums[2] + sums[3];
-  const bool ok = 2 * lane < c.d;
-  const float* at = a.part_o + r * splits * c.d + (ok ? 2 * lane : 0);
-  float2 y = make_float2(0.f, 0.f);
-#pragma unroll 4
-  for (int s = wave; s < splits; s += 4) {
-    const float2 p = *reinterpret_cast<const float2*>(at + (long long)s * c.d);
-    const float f = weight[s];
-    if (f != 0.f) y.x = fmaf(f, p.x, y.x), y.y = fmaf(f, p.y, y.y);
-  }
-  parts[wave][lane] = y;
-  __syncthreads();
-  if (wave != 0 || !ok) return;
-#pragma unroll
-  for (int i = 1; i < 4; ++i) y.x += parts[i][lane].x, y.y += parts[i][lane].y;
-  const float inv = 1.f / sum;
-  const long long bh = r / a.rows;
-  const int row = (int)(r % a.rows), token = row / a.group;
-  const int head = (int)(bh % c.kv_heads) * a.group + row % a.group;
-  typedef T Two __attribute__((ext_vector_type(2)));
-  Two out;
-  out[0] = sum == 0.f ? (T)0.f : (T)(y.x * inv);
-  out[1] = sum == 0.f ? (T)0.f : (T)(y.y * inv);
-  T* orow = static_cast<T*>(c.out) + (bh / c.kv_heads) * c.o_sb + (long long)token * c.o_st + head * c.o_sh;
-  *reinterpret_cast<Two*>(orow + 2 * lane) = out;
 }
 
 // Shape of the launch: rows per workgroup, tiles and splits.
@@ -857,26 +153,6 @@ int check(const musc_masked_attention* c) {
   return MUSC_OK;
 }
 
-template <int kDtype, int kD>
-void launch(const Args& a, int waves, hipStream_t stream) {
-  const dim3 grid((unsigned)align_up((size_t)a.units, kXcds));
-  if (waves == 1)
-    hipLaunchKernelGGL((masked_attention_kernel<kDtype, kD, 1>), grid, dim3(kWave), 0, stream, a);
-  else
-    hipLaunchKernelGGL((masked_attention_kernel<kDtype, kD, 4>), grid, dim3(4 * kWave), 0, stream, a);
-}
-
-template <int kDtype>
-void launch(const Args& a, int waves, hipStream_t stream) {
-  if (a.c.d <= 64) launch<kDtype, 64>(a, waves, stream);
-  else if (a.c.d <= 96) launch<kDtype, 96>(a, waves, stream);
-  else launch<kDtype, 128>(a, waves, stream);
-  if (a.splits > 1) {
-    const long long rows = (long long)a.c.batch * a.c.kv_heads * a.rows;
-    hipLaunchKernelGGL((join_kernel<kDtype>), dim3((unsigned)rows), dim3(256), 0, stream, a);
-  }
-}
-
 }  // namespace mattn
 }  // namespace musc
 
@@ -941,8 +217,8 @@ extern "C" int musc_masked_attention_fwd(const musc_masked_attention* c, void* w
     a.part_o = reinterpret_cast<float*>(static_cast<char*>(workspace) +
                                         align_up((size_t)c->batch * c->kv_heads * a.rows * a.splits * 2 * sizeof(float), 256));
   }
-  if (c->dtype == MUSC_DTYPE_F32) mattn::launch<MUSC_DTYPE_F32>(a, waves, stream);
-  else if (c->dtype == MUSC_DTYPE_F16) mattn::launch<MUSC_DTYPE_F16>(a, waves, stream);
-  else mattn::launch<MUSC_DTYPE_BF16>(a, waves, stream);
+  if (c->dtype == MUSC_DTYPE_F32) mattn::launch_f32(a, waves, stream);
+  else if (c->dtype == MUSC_DTYPE_F16) mattn::launch_f16(a, waves, stream);
+  else mattn::launch_bf16(a, waves, stream);
   return check_launch();
 }

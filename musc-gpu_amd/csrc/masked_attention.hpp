@@ -1,0 +1,148 @@
+// Softmax attention over the keys that a query may see, for packed images, padded batches,
+// prefixes and frames, with an optional cap on the scores and an optional bias by distance:
+//
+//   score(i, j) = c(scale q_i . k_j) - sum_a slope[head, a] |p_a(i) - p_a(j)|
+//   c(s)        = cap tanh(s / cap), or s
+//   seen(i, j)  = document(i) == document(j) >= 0 and order(j) <= order(i)
+//   out_i       = sum_seen e^(score - max) v_j / sum_seen e^(score - max); zeros if none is seen
+//
+// One pass over the keys with the running maximum and sum of the softmax.  As in the
+// unmasked kernels a wave forms S^T = K Q^T, so that a lane owns one query row and its
+// maximum, sum and probabilities stay in its registers; O^T += V^T P^T follows with P in
+// place.  A row is a (token, head of the group) pair: the heads that share a key head are
+// neighbouring rows, so K and V are read once for all of them.
+//
+// Keys come in tiles of kTile.  A small summary of the keys (per 32 of them the range of
+// documents and orders, made once per batch) sorts a tile, for the rows of a wave, into unseen
+// (skipped without reading K or V), seen whole (no mask is evaluated) and mixed (each score is
+// tested).  64 tiles are sorted at a time, one per lane.
+//
+// Few rows (a new token, a pooling latent): the keys are split over workgroups of one wave
+// that write (maximum, sum, output) parts, and a second kernel joins them in a fixed order.
+#pragma once
+
+#include <hip/hip_bf16.h>
+#include <hip/hip_fp16.h>
+
+#include <type_traits>
+
+#include "common.hpp"
+
+namespace musc {
+namespace mattn {
+
+typedef float floatx16 __attribute__((ext_vector_type(16)));
+typedef float float2v __attribute__((ext_vector_type(2)));
+typedef int int4v __attribute__((ext_vector_type(4)));
+typedef short short4v __attribute__((ext_vector_type(4)));
+typedef short short8v __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(3))) void lds_void;
+
+constexpr int kBufferFlags = 0x00020000;   // buffer resource word 3 for raw byte-addressed loads
+constexpr int kNowhere = 0x7fffff00;       // a byte offset past every extent: such loads give zeros
+constexpr float kLazyLog2 = 8.f;           // the running maximum moves once a tile exceeds it by this
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kSummaryKeys = 32;
+constexpr int kMaxAxes = 3;
+constexpr int kMaxSplits = 256;
+constexpr int kRowTile = 128;  // rows of a workgroup of four waves
+
+template <int kDtype>
+struct Type;
+template <>
+struct Type<MUSC_DTYPE_F32> {
+  typedef float T;
+  static constexpr int kTile = 32;
+  static constexpr float kShift = 0.f;
+};
+template <>
+struct Type<MUSC_DTYPE_F16> {
+  typedef _Float16 T;
+  typedef T Vec __attribute__((ext_vector_type(8)));
+  typedef T Two __attribute__((ext_vector_type(2)));
+  static constexpr int kTile = 64;
+  // probabilities are formed 2^7 times as large, at most 2^15 with the slack: entries down to
+  // 2^-21 of the largest stay normal fp16 numbers
+  static constexpr float kShift = 7.f;
+  static __device__ __forceinline__ floatx16 mfma(Vec a, Vec b, floatx16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ float add_both(Two p, float sum) {
+    return __builtin_amdgcn_fdot2(p, Two{(T)1.f, (T)1.f}, sum, false);
+  }
+};
+template <>
+struct Type<MUSC_DTYPE_BF16> {
+  typedef __bf16 T;
+  typedef T Vec __attribute__((ext_vector_type(8)));
+  typedef T Two __attribute__((ext_vector_type(2)));
+  static constexpr int kTile = 64;
+  static constexpr float kShift = 0.f;
+  static __device__ __forceinline__ floatx16 mfma(Vec a, Vec b, floatx16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ float add_both(Two p, float sum) {
+    return __builtin_amdgcn_fdot2_f32_bf16(p, Two{(T)1.f, (T)1.f}, sum, false);
+  }
+};
+
+// Keys of a tile: workgroups of one wave take 32, so that four of them fit a CU's LDS.
+template <int kDtype, int kWaves>
+constexpr int tile_keys() {
+  return kWaves == 1 ? 32 : Type<kDtype>::kTile;
+}
+
+// Staged rows of K and V: 128, 256 or 512 bytes, their 16-byte chunks permuted by the row so
+// that the lanes one LDS read serves together touch different banks: 16 neighbouring rows of
+// one chunk (K's operands) take 16 places of a 256-byte window, and so do 4 neighbouring rows
+// of 4 chunks (V's transposing reads).  Chunk c of row r is at place c ^ swizzle(r).
+template <int kPitch>
+__device__ __forceinline__ constexpr int swizzle(int r) {
+  return kPitch == 128 ? (((r >> 1) & 1) << 2) | ((r >> 2) & 3) : ((r & 3) << 2) | ((r >> 2) & 3);
+}
+
+struct Args {
+  musc_masked_attention c;
+  int group, rows, row_tiles, key_tiles, splits, summaries, heads_at_once;
+  long long units;
+  float* part_ml;  // (units in (b, kv head), rows, split) x (maximum, sum)
+  float* part_o;   // the same x d
+};
+
+__device__ __forceinline__ float halves_max(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __builtin_elementwise_maximum(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float halves_sum(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+// Minimum over the wave by lane-crossing moves (no LDS): lanes get their neighbours 1, 2, 4, 8 to
+// the left within rows of 16, then the rows' last lanes go on to the next rows; lane 63 has it.
+template <int kMove, int kRows>
+__device__ __forceinline__ int min_with(int v) {
+  return min(v, __builtin_amdgcn_update_dpp(0x7fffffff, v, kMove, kRows, 0xf, false));
+}
+__device__ __forceinline__ int wave_min_int(int v) {
+  v = min_with<0x111, 0xf>(v);
+  v = min_with<0x112, 0xf>(v);
+  v = min_with<0x114, 0xf>(v);
+  v = min_with<0x118, 0xf>(v);
+  v = min_with<0x142, 0xa>(v);
+  v = min_with<0x143, 0xc>(v);
+  return __builtin_amdgcn_readlane(v, 63);
+}
+__device__ __forceinline__ int wave_max_int(int v) { return ~wave_min_int(~v); }
+
+// The documents and orders of a set of rows: what a tile is compared with.
+struct Range {
+  int dmin, dmax, omin, omax;
+};
+
+// The kernels of one storage type, each compiled in its own file (launch_all below).
+void launch_f32(const Args& a, int waves, hipStream_t stream);
+void launch_f16(const Args& a, int waves, hipStream_t stream);
+void launch_bf16(const Args& a, int waves, hipStream_t stream);
+
+}  // namespace mattn
+}  // namespace musc

@@ -33,12 +33,13 @@ COMMON = ['-O3', '-std=c++17', '-fPIC', f'--offload-arch={ARCH}', f'-DMUSC_TARGE
           '-Wno-unused-function', '-Wno-unused-variable', '-Wno-unused-but-set-variable'] + DEVICE_FLAGS
 
 
-# Per-file device flags.  attention.hip and masked_attention.hip: the online softmax rescales the MFMA
+# Per-file device flags.  attention.hip and masked_attention_*.hip: the online softmax rescales the MFMA
 # accumulators with VALU instructions, so they must live in VGPRs; left to its
 # heuristics the compiler puts them in AGPRs and moves every value back and forth
 # (157 v_accvgpr moves per 32-key block in the fp16 kernel).
-FILE_FLAGS = {'attention.hip': ['-mllvm', '-amdgpu-mfma-vgpr-form'],
-              'masked_attention.hip': ['-mllvm', '-amdgpu-mfma-vgpr-form']}
+FILE_FLAGS = {name: ['-mllvm', '-amdgpu-mfma-vgpr-form']
+              for name in ('attention.hip', 'masked_attention_f32.hip', 'masked_attention_f16.hip',
+                           'masked_attention_bf16.hip')}
 
 
 def _compile(src: str, verbose: bool) -> str:
