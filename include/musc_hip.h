@@ -403,25 +403,26 @@ typedef struct musc_masked_attention {
   long long q_positions_sb, k_positions_sb;
   const float* slopes;
   int axes;               /* 0: no bias; at most 3 */
-  /* Order in which groups of 128 (token, head) rows are begun, from musc_token_schedule, at
-   * b * row_order_sb (int32); NULL: later rows first.  Results do not depend on it. */
-  const int* row_order;
-  long long row_order_sb;
+  /* self-attention: musc_token_schedule's block for heads / kv_heads, batch entry b's at
+   * b * schedule_sb (ints); NULL: none.  Which rows are begun first, and how many workgroups share
+   * a row's keys, goes by it. */
+  const int* schedule;
+  long long schedule_sb;
 } musc_masked_attention;
 
 /* Summary of (batch, t) documents and orders (NULL: none): four int32 per group of 32 keys,
  * (batch, ceil(t / 32), 4).  Made again when a document or order changes. */
 int musc_token_summary(const int* documents, const int* order, int batch, int t, int* summary, hipStream_t stream);
-/* Orders of the row groups of self-attention over these tokens, those that see most keys first,
- * for heads / kv_heads = 1, 2, 4 and 8 one after the other: (batch, 2, n) int32 each with n =
- * ceil(t * heads / kv_heads / 128), the first n of a batch entry the order, the others its work in
- * groups of 32 keys.  t up to MUSC_SCHEDULE_MAX_TOKENS (MUSC_ERR_UNSUPPORTED beyond: so many row
- * groups need no order). */
+/* Schedules of self-attention over these tokens (its groups of 128 (token, head) rows, those that
+ * see most keys first, and long ones in parts) for heads / kv_heads = 1, 2, 4 and 8 one after the
+ * other: batch blocks of 4 + 3 n + (9 n + 4) / 5 int32 each, n = ceil(t * heads / kv_heads / 128).  Made again when a
+ * document or order changes.  t up to MUSC_SCHEDULE_MAX_TOKENS (MUSC_ERR_UNSUPPORTED beyond: so many
+ * row groups need no schedule). */
 #define MUSC_SCHEDULE_MAX_TOKENS 65536
-int musc_token_schedule(const int* documents, const int* order, const int* summary, int batch, int t, int* row_order,
+int musc_token_schedule(const int* documents, const int* order, const int* summary, int batch, int t, int* schedule,
                         hipStream_t stream);
-/* Few rows are split over their keys and joined through a workspace (16-byte aligned; 0 bytes
- * where nothing is split).  Every row of q, k, v and out starts on 16 bytes; 64 rows of K and V
+/* Few rows, and long row groups among few, are split over their keys and joined through a workspace
+ * (16-byte aligned; 0 bytes where nothing is split).  Every row of q, k, v and out starts on 16 bytes; 64 rows of K and V
  * span less than 2 GiB (MUSC_ERR_UNSUPPORTED). */
 int musc_masked_attention_workspace_bytes(const musc_masked_attention* call, size_t* out);
 int musc_masked_attention_fwd(const musc_masked_attention* call, void* workspace, size_t workspace_bytes,

@@ -30,12 +30,13 @@ __global__ __launch_bounds__(256) void token_summary_kernel(const int* __restric
   if (threadIdx.x % kSummaryKeys == 0) summary[g] = s;
 }
 
-// Self-attention's row tiles for 1, 2, 4 and 8 query heads per key head, one after the other:
-// (batch, 2, row_tiles) int32 each.
+// Schedules of self-attention for 1, 2, 4 and 8 query heads per key head, one after the other,
+// a block (see schedule_block) per batch entry.
 struct Schedule {
   int batch, t, groups;
-  int tiles[4];      // row tiles
+  int tiles[4];        // row tiles
   long long first[5];  // (batch entry, row tile) pairs before this number of heads
+  long long at[4];     // first int of its blocks
   __device__ __forceinline__ int which(long long i) const { return (i >= first[1]) + (i >= first[2]) + (i >= first[3]); }
 };
 
@@ -60,21 +61,36 @@ __global__ __launch_bounds__(kWave) void row_work_kernel(const int* __restrict__
   }
 #pragma unroll
   for (int off = 32; off >= 1; off >>= 1) count += __shfl_xor(count, off, kWave);
-  if (lane == 0) out[2 * s.first[w] + (2LL * b + 1) * s.tiles[w] + tile] = count;
+  if (lane == 0) out[s.at[w] + b * schedule_block(s.tiles[w]) + kScheduleHead + tile] = count;
 }
 
-// The row tiles by their work, most first (later ones first where it is the same).
+// The row tiles by their work, most first (later ones first where it is the same): whole, and as
+// jobs, where a tile of more than 5/4 of the mean work is listed in up to 8 parts, by the work of a
+// part.  At most 9/5 n jobs.
 __global__ __launch_bounds__(256) void row_order_kernel(const Schedule s, int* __restrict__ out) {
-  const long long at = (long long)blockIdx.x * 256 + threadIdx.x;
-  if (at >= s.first[4]) return;
-  const int w = s.which(at), n = s.tiles[w];
-  const int i = (int)(at - s.first[w]), b = i / n, tile = i % n;
-  int* mine = out + 2 * s.first[w] + 2LL * b * n;
-  const int* work = mine + n;
-  const int here = work[tile];
-  int rank = 0;
-  for (int j = 0; j < n; ++j) rank += work[j] > here || (work[j] == here && j > tile);
-  mine[rank] = tile;
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= s.first[4]) return;
+  const int w = s.which(i), n = s.tiles[w];
+  const int b = (int)((i - s.first[w]) / n), tile = (int)((i - s.first[w]) % n);
+  int* block = out + s.at[w] + b * schedule_block(n);
+  const int* work = block + kScheduleHead;
+  long long total = 0;
+  for (int j = 0; j < n; ++j) total += work[j];
+  const int most = (int)max((5 * total + 4LL * n - 1) / (4LL * n), 8LL);  // of a part
+  auto parts_of = [&](int x) { return min(max((x + most - 1) / most, 1), kMaxParts); };
+  const int here = work[tile], parts = parts_of(here), size = (here + parts - 1) / parts;
+  int rank = 0, first = 0, all = 0;
+  for (int j = 0; j < n; ++j) {
+    const int x = work[j], p = parts_of(x), each = (x + p - 1) / p;
+    rank += x > here || (x == here && j > tile);
+    first += each > size || (each == size && j > tile) ? p : 0;
+    all += p;
+  }
+  block[kScheduleHead + n + rank] = tile;
+  block[kScheduleHead + 2 * n + tile] = first | parts << 24;
+  int* jobs = block + kScheduleHead + 3 * n + first;
+  for (int p = 0; p < parts; ++p) jobs[p] = tile | p << 20 | (parts - 1) << 23;
+  if (tile == 0) block[0] = all;
 }
 
 // Shape of the launch: rows per workgroup, tiles and splits.
@@ -89,18 +105,28 @@ int plan(const musc_masked_attention& c, Args& a, int& waves) {
   a.row_tiles = (int)((rows + 32 * waves - 1) / (32 * waves));
   a.key_tiles = (c.k_len + tile - 1) / tile;
   a.summaries = (c.k_len + kSummaryKeys - 1) / kSummaryKeys;
-  const long long whole = (long long)c.batch * c.kv_heads * a.row_tiles;
-  long long splits = 1;
-  const long long want = waves == 1 ? 2048 : 512;
-  if (whole < want / 2) splits = (want + whole - 1) / whole;
-  if (splits > a.key_tiles) splits = a.key_tiles;
-  if (splits > kMaxSplits) splits = kMaxSplits;
-  a.splits = splits < 1 ? 1 : (int)splits;
-  a.units = whole * a.splits;
+  const long long heads = (long long)c.batch * c.kv_heads, whole = heads * a.row_tiles;
+  // workgroups that the card holds at a time
+  a.slots = waves == 1 ? 1024 : c.dtype != MUSC_DTYPE_F32 && c.d <= 64 ? 768 : 512;
+  a.splits = 1, a.jobs = a.row_tiles, a.in_parts = 0;
+  if (waves > 1 && c.schedule) {
+    // Long row tiles in parts where all begin at once and the longest ends last: 4 packed images,
+    // fp32 (416 row tiles, 512 places), 204 -> 144 us; with more row tiles than places short ones
+    // fill up behind long ones (12 packed images, fp16, 1184 for 768: 106 us whole, 110 in parts).
+    a.in_parts = whole < a.slots;
+    if (a.in_parts) a.jobs = (int)schedule_jobs(a.row_tiles);
+  } else if (whole < (waves == 1 ? 1024 : 256)) {
+    // few rows: their keys in splits of at least one tile (4 where four waves share the tiles)
+    long long splits = ((waves == 1 ? 2048 : 512) + whole - 1) / whole;
+    const int least = waves == 1 ? 1 : 4;
+    if (splits > a.key_tiles / least) splits = a.key_tiles / least;
+    if (splits > kMaxSplits) splits = kMaxSplits;
+    a.splits = splits < 1 ? 1 : (int)splits;
+  }
+  a.units = heads * a.jobs * a.splits;
   // Heads that an XCD (32 CUs, 2 or 3 workgroups each) works on together: enough for two rounds of
   // workgroups, so that short work fills the gaps of long work, and no more, as they share its L2.
   // 0: the heads do not divide over the XCDs.
-  const long long heads = (long long)c.batch * c.kv_heads;
   a.heads_at_once = 0;
   if (heads % kXcds == 0) {
     const long long enough = (128 + a.row_tiles - 1) / a.row_tiles, per_xcd = heads / kXcds;
@@ -110,10 +136,15 @@ int plan(const musc_masked_attention& c, Args& a, int& waves) {
   return MUSC_OK;
 }
 
+// Rows that write parts: of every split, or of every job.
+size_t part_rows(const Args& a) {
+  const size_t heads = (size_t)a.c.batch * a.c.kv_heads;
+  if (a.in_parts) return heads * a.jobs * kRowTile;
+  return a.splits == 1 ? 0 : heads * a.rows * a.splits;
+}
 size_t part_bytes(const Args& a) {
-  if (a.splits == 1) return 0;
-  const size_t parts = (size_t)a.c.batch * a.c.kv_heads * a.rows * a.splits;
-  return align_up(parts * 2 * sizeof(float), 256) + parts * a.c.d * sizeof(float);
+  const size_t rows = part_rows(a);
+  return rows ? align_up(rows * 2 * sizeof(float), 256) + rows * a.c.d * sizeof(float) : 0;
 }
 
 // 16-byte vectors from every row of a tensor
@@ -145,10 +176,10 @@ int check(const musc_masked_attention* c) {
   const uintptr_t words = reinterpret_cast<uintptr_t>(c->q_documents) | reinterpret_cast<uintptr_t>(c->k_documents) |
                           reinterpret_cast<uintptr_t>(c->q_order) | reinterpret_cast<uintptr_t>(c->k_order) |
                           reinterpret_cast<uintptr_t>(c->q_positions) | reinterpret_cast<uintptr_t>(c->k_positions) |
-                          reinterpret_cast<uintptr_t>(c->slopes) | reinterpret_cast<uintptr_t>(c->row_order);
+                          reinterpret_cast<uintptr_t>(c->slopes) | reinterpret_cast<uintptr_t>(c->schedule);
   if ((words & 3) || (reinterpret_cast<uintptr_t>(c->k_summary) & 15)) return MUSC_ERR_INVALID_ARG;
   if ((c->q_tokens_sb | c->k_tokens_sb | c->q_positions_sb | c->k_positions_sb | c->k_summary_sb |
-       c->row_order_sb) < 0)
+       c->schedule_sb) < 0)
     return MUSC_ERR_INVALID_ARG;
   return MUSC_OK;
 }
@@ -174,23 +205,25 @@ extern "C" int musc_token_summary(const int* documents, const int* order, int ba
 }
 
 extern "C" int musc_token_schedule(const int* documents, const int* order, const int* summary, int batch, int t,
-                                   int* row_order, hipStream_t stream) {
-  if (!documents || !summary || !row_order || batch < 0 || t < 0) return MUSC_ERR_INVALID_ARG;
+                                   int* schedule, hipStream_t stream) {
+  if (!documents || !summary || !schedule || batch < 0 || t < 0) return MUSC_ERR_INVALID_ARG;
   if (((reinterpret_cast<uintptr_t>(documents) | reinterpret_cast<uintptr_t>(order) |
-        reinterpret_cast<uintptr_t>(row_order)) & 3) || (reinterpret_cast<uintptr_t>(summary) & 15))
+        reinterpret_cast<uintptr_t>(schedule)) & 3) || (reinterpret_cast<uintptr_t>(summary) & 15))
     return MUSC_ERR_INVALID_ARG;
   if (t > MUSC_SCHEDULE_MAX_TOKENS) return MUSC_ERR_UNSUPPORTED;
   if (batch == 0 || t == 0) return MUSC_OK;
-  mattn::Schedule s{batch, t, (t + mattn::kSummaryKeys - 1) / mattn::kSummaryKeys, {}, {}};
+  mattn::Schedule s{};
+  s.batch = batch, s.t = t, s.groups = (t + mattn::kSummaryKeys - 1) / mattn::kSummaryKeys;
   for (int w = 0; w < 4; ++w) {
     s.tiles[w] = (t + (mattn::kRowTile >> w) - 1) / (mattn::kRowTile >> w);
     s.first[w + 1] = s.first[w] + (long long)batch * s.tiles[w];
+    if (w < 3) s.at[w + 1] = s.at[w] + batch * mattn::schedule_block(s.tiles[w]);
   }
   if (s.first[4] >= (0x100000000LL >> 8)) return MUSC_ERR_UNSUPPORTED;
   hipLaunchKernelGGL(mattn::row_work_kernel, dim3((unsigned)s.first[4]), dim3(kWave), 0, stream, documents, order,
-                     reinterpret_cast<const int4*>(summary), s, row_order);
+                     reinterpret_cast<const int4*>(summary), s, schedule);
   hipLaunchKernelGGL(mattn::row_order_kernel, dim3((unsigned)((s.first[4] + 255) / 256)), dim3(256), 0, stream, s,
-                     row_order);
+                     schedule);
   return check_launch();
 }
 
@@ -215,7 +248,7 @@ extern "C" int musc_masked_attention_fwd(const musc_masked_attention* c, void* w
     if (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16) return MUSC_ERR_WORKSPACE;
     a.part_ml = static_cast<float*>(workspace);
     a.part_o = reinterpret_cast<float*>(static_cast<char*>(workspace) +
-                                        align_up((size_t)c->batch * c->kv_heads * a.rows * a.splits * 2 * sizeof(float), 256));
+                                        align_up(mattn::part_rows(a) * 2 * sizeof(float), 256));
   }
   if (c->dtype == MUSC_DTYPE_F32) mattn::launch_f32(a, waves, stream);
   else if (c->dtype == MUSC_DTYPE_F16) mattn::launch_f16(a, waves, stream);

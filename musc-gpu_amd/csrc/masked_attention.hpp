@@ -46,6 +46,11 @@ constexpr int kSummaryKeys = 32;
 constexpr int kMaxAxes = 3;
 constexpr int kMaxSplits = 256;
 constexpr int kRowTile = 128;  // rows of a workgroup of four waves
+// Schedule of n row tiles, in ints: head (jobs), work (n), row tiles by their work (n), first job
+// | parts << 24 of each row tile (n), jobs (row tile | part << 20 | (parts - 1) << 23).
+constexpr int kScheduleHead = 4, kMaxParts = 8;
+__host__ __device__ inline long long schedule_jobs(long long n) { return (9 * n + 4) / 5; }
+__host__ __device__ inline long long schedule_block(long long n) { return kScheduleHead + 3 * n + schedule_jobs(n); }
 
 template <int kDtype>
 struct Type;
@@ -104,6 +109,9 @@ __device__ __forceinline__ constexpr int swizzle(int r) {
 struct Args {
   musc_masked_attention c;
   int group, rows, row_tiles, key_tiles, splits, summaries, heads_at_once;
+  int jobs;      // workgroups of a head and split: its row tiles, or the schedule's jobs
+  int in_parts;  // jobs may be parts of a row tile's keys
+  int slots;     // workgroups that the card holds at a time
   long long units;
   float* part_ml;  // (units in (b, kv head), rows, split) x (maximum, sum)
   float* part_o;   // the same x d

@@ -59,24 +59,24 @@ __global__ __launch_bounds__(kWaves * kWave, kWaves == 1 ? 1 : kD == 64 && kDtyp
   const musc_masked_attention& c = a.c;
   // uniform numbers in scalar registers (the divisions leave them in vector ones)
   const auto uniform = [](long long x) { return __builtin_amdgcn_readfirstlane((int)x); };
-  uint32_t split, row_tile, bh;
+  uint32_t split, job, bh;
   if (a.heads_at_once) {
     // one XCD works on heads_at_once heads together, row tile by row tile (the longest first)
     const uint32_t per_xcd = (uint32_t)(c.batch * c.kv_heads) / kXcds, local = blockIdx.x / kXcds;
-    const uint32_t of_group = (uint32_t)(a.heads_at_once * a.row_tiles * a.splits);
+    const uint32_t of_group = (uint32_t)(a.heads_at_once * a.jobs * a.splits);
     const uint32_t group = uniform(local / of_group), in_group = local - group * of_group;
     const uint32_t first = group * a.heads_at_once, at_once = min((uint32_t)a.heads_at_once, per_xcd - first);
     const uint32_t rest = uniform(in_group / a.splits);
     split = in_group - rest * a.splits;
-    row_tile = uniform(rest / at_once);
-    bh = blockIdx.x % kXcds * per_xcd + first + (rest - row_tile * at_once);
+    job = uniform(rest / at_once);
+    bh = blockIdx.x % kXcds * per_xcd + first + (rest - job * at_once);
   } else {
     const uint32_t unit = (blockIdx.x % kXcds) * (gridDim.x / kXcds) + blockIdx.x / kXcds;
     if (unit >= (uint32_t)a.units) return;
     const uint32_t rest = uniform(unit / a.splits);
     split = unit - rest * a.splits;
-    bh = uniform(rest / a.row_tiles);
-    row_tile = rest - bh * a.row_tiles;
+    bh = uniform(rest / a.jobs);
+    job = rest - bh * a.jobs;
   }
   const int b = uniform(bh / c.kv_heads), kvh = bh - b * c.kv_heads;
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid % kWave;
@@ -99,10 +99,21 @@ __global__ __launch_bounds__(kWaves * kWave, kWaves == 1 ? 1 : kD == 64 && kDtyp
   };
   const int4 first_summary = summary_of(lo / 64 * 64 + lane);
 
-  // by the caller's order, or later rows first: with an order of tokens they see more keys, and
-  // the longest work should not start last
-  int tile_of_rows = a.row_tiles - 1 - (int)row_tile;
-  if (kWaves > 1 && c.row_order) tile_of_rows = uniform(c.row_order[b * c.row_order_sb + row_tile]);
+  // the row tile, or the part of its keys, that the schedule names; without one later rows first:
+  // with an order of tokens they see more keys, and the longest work should not start last
+  int tile_of_rows = a.row_tiles - 1 - (int)job, part = 0, parts = 1;
+  if (kWaves > 1 && c.schedule) {
+    const int* schedule = c.schedule + b * c.schedule_sb;
+    if (a.in_parts) {
+      const int jobs = schedule[0], j = schedule[kScheduleHead + 3 * a.row_tiles + job];
+      if ((int)job >= jobs) return;
+      tile_of_rows = uniform(j & 0xfffff);
+      part = uniform((j >> 20) & 7);
+      parts = uniform(((j >> 23) & 7) + 1);
+    } else {
+      tile_of_rows = uniform(schedule[kScheduleHead + a.row_tiles + job]);
+    }
+  }
   tile_of_rows = min(max(tile_of_rows, 0), a.row_tiles - 1);
   const int row = (tile_of_rows * kWaves + wave) * 32 + lq;
   const bool inside = row < a.rows;
@@ -244,7 +255,7 @@ __global__ __launch_bounds__(kWaves * kWave, kWaves == 1 ? 1 : kD == 64 && kDtyp
 
   // one staged tile; whole: every row sees every key.  careful: in a mixed tile, products
   // of keys that a row does not see are left out one by one (their V may be infinite or NaN)
-  auto attend = [&](int buf, int tile, bool whole, auto careful_c) __attribute__((always_inline)) {
+  auto attend = [&](int buf, bool whole, auto careful_c) __attribute__((always_inline)) {
     constexpr bool careful = decltype(careful_c)::value;
     // Byte places of this lane's operands: row lq (K) or the row and chunk of its V operand, in
     // chunk order from the permutation's exclusive or, which all further chunks keep.  Formed
@@ -332,7 +343,6 @@ __global__ __launch_bounds__(kWaves * kWave, kWaves == 1 ? 1 : kD == 64 && kDtyp
     uint32_t seen = 0xffffffffu;
     if (!whole) {
       mixed_seen = true;
-      const int rem = k_len - tile * kTile;
 #pragma unroll
       for (int u = 0; u < kSub; ++u)
 #pragma unroll
@@ -342,7 +352,7 @@ __global__ __launch_bounds__(kWaves * kWave, kWaves == 1 ? 1 : kD == 64 && kDtyp
           const int4v ko = *reinterpret_cast<const int4v*>(&ords_s[buf][key]);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const bool see = kd[i] == qdoc && ko[i] <= qord && key + i < rem;
+            const bool see = kd[i] == qdoc && ko[i] <= qord;
             s[u][4 * g + i] = see ? s[u][4 * g + i] : -INFINITY;
             if (careful && !see) seen &= ~(1u << (16 * u + 4 * g + i));
           }
@@ -434,7 +444,7 @@ __global__ __launch_bounds__(kWaves * kWave, kWaves == 1 ? 1 : kD == 64 && kDtyp
   };
 
   // the tiles that some row of the workgroup may see
-  int chunk = 0;
+  int chunk = 0, tiles_seen = 0;
   unsigned long long todo = 0, any_word = 0, whole_word = 0;
   auto sort_tiles = [&](const int4 k) __attribute__((always_inline)) {
     const int t = chunk * 64 + lane;
@@ -443,6 +453,11 @@ __global__ __launch_bounds__(kWaves * kWave, kWaves == 1 ? 1 : kD == 64 && kDtyp
       return here && k.y >= 0 && k.x <= r.dmax && k.y >= r.dmin && k.z <= r.omax;
     };
     todo = __ballot(may_see(all_rows));
+    if (kWaves > 1 && parts > 1) {  // every parts-th of them
+      const int number = tiles_seen + __popcll(todo & ((1ull << lane) - 1));
+      tiles_seen += __popcll(todo);
+      todo = __ballot(((todo >> lane) & 1) && number % parts == part);
+    }
     any_word = __ballot(may_see(mine));
     whole_word = __ballot(here && k.x == k.y && mine.dmin == mine.dmax && k.x == mine.dmin && k.w <= mine.omin &&
                           (t + 1) * kTile <= k_len);
@@ -468,7 +483,8 @@ __global__ __launch_bounds__(kWaves * kWave, kWaves == 1 ? 1 : kD == 64 && kDtyp
 #pragma unroll
       for (int v = 0; v < 16; ++v) o[x][v] = 0.f;
     m_run = -INFINITY, l_run = 0.f, base = Ty::kShift, mixed_seen = false;
-    chunk = lo / 64;
+    if (decltype(careful_c)::value && !c.k_documents && tid < 64) docs_s[0][tid] = docs_s[1][tid] = 0;
+    chunk = lo / 64, tiles_seen = 0;
     sort_tiles(decltype(careful_c)::value ? summary_of(lo / 64 * 64 + lane) : first_summary);
     Next now = next_tile();
     if (now.tile >= 0) load_tile(now.tile, 0);
@@ -476,9 +492,12 @@ __global__ __launch_bounds__(kWaves * kWave, kWaves == 1 ? 1 : kD == 64 && kDtyp
     while (now.tile >= 0) {
       const Next then = next_tile();
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's share of tile `now` is in LDS
+      // what lies behind the last key is of no document
+      if ((now.tile + 1) * kTile > k_len && wave == kWaves - 1 && lane < kTile && now.tile * kTile + lane >= k_len)
+        docs_s[buf][lane] = -1;
       __syncthreads();  // everyone's is, and everyone is done with the other buffer
       if (then.tile >= 0) load_tile(then.tile, buf ^ 1);
-      if (now.any) attend(buf, now.tile, now.whole, careful_c);
+      if (now.any) attend(buf, now.whole, careful_c);
       buf ^= 1;
       now = then;
     }
@@ -498,7 +517,7 @@ __global__ __launch_bounds__(kWaves * kWave, kWaves == 1 ? 1 : kD == 64 && kDtyp
   l_run = halves_sum(l_run);
   if (!inside) return;
   // register v of block x holds channel 32 x + 8 (v / 4) + 4 lh + v % 4
-  if (a.splits == 1) {
+  if (a.splits == 1 && parts == 1) {
     const bool empty = !live || l_run == 0.f;
     const float inv = 1.f / l_run;
     T* orow = static_cast<T*>(c.out) + b * c.o_sb + (long long)token * c.o_st + head * c.o_sh;
@@ -514,12 +533,13 @@ __global__ __launch_bounds__(kWaves * kWave, kWaves == 1 ? 1 : kD == 64 && kDtyp
         if (at < d) *reinterpret_cast<Four*>(orow + at) = y;
       }
   } else {
-    const long long part = ((long long)bh * a.rows + row) * a.splits + split;
+    const long long at_row = a.splits > 1 ? ((long long)bh * a.rows + row) * a.splits + split
+                                          : ((long long)bh * a.jobs + job) * kRowTile + row % kRowTile;
     if (lh == 0) {
-      a.part_ml[2 * part] = live ? m_run * to_log2 : -INFINITY;
-      a.part_ml[2 * part + 1] = live ? l_run : 0.f;
+      a.part_ml[2 * at_row] = live ? m_run * to_log2 : -INFINITY;
+      a.part_ml[2 * at_row + 1] = live ? l_run : 0.f;
     }
-    float* prow = a.part_o + part * d;
+    float* prow = a.part_o + at_row * d;
 #pragma unroll
     for (int x = 0; x < kO; ++x)
 #pragma unroll
@@ -582,6 +602,52 @@ __global__ __launch_bounds__(256) void join_kernel(const Args a) {
   *reinterpret_cast<Two*>(orow + 2 * lane) = out;
 }
 
+// Joins the parts of the row tiles that were done in parts, in their order: a workgroup per row
+// tile, four channels of a row per thread.
+template <int kDtype>
+__global__ __launch_bounds__(256) void join_parts_kernel(const Args a) {
+  typedef typename Type<kDtype>::T T;
+  const musc_masked_attention& c = a.c;
+  const int tile = blockIdx.x % a.row_tiles, bh = blockIdx.x / a.row_tiles, b = bh / c.kv_heads;
+  const int entry = c.schedule[b * c.schedule_sb + kScheduleHead + 2 * a.row_tiles + tile];
+  const int job = entry & 0xffffff, parts = min((entry >> 24) & 15, kMaxParts);
+  if (parts <= 1 || job + parts > a.jobs) return;
+  const int first_row = tile * kRowTile, rows = min(kRowTile, a.rows - first_row);
+  const int of_row = c.d / 4;
+  const long long first = ((long long)bh * a.jobs + job) * kRowTile;
+  for (int e = threadIdx.x; e < rows * of_row; e += 256) {
+    const int r = e / of_row, at = e % of_row * 4;
+    float m[kMaxParts], l[kMaxParts], top = -INFINITY;
+    float4 p[kMaxParts];
+#pragma unroll
+    for (int i = 0; i < kMaxParts; ++i) {
+      m[i] = -INFINITY, l[i] = 0.f, p[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (i < parts) {
+        const long long from = first + i * kRowTile + r;
+        const float2 ml = reinterpret_cast<const float2*>(a.part_ml)[from];
+        m[i] = ml.x, l[i] = ml.y;
+        p[i] = *reinterpret_cast<const float4*>(a.part_o + from * c.d + at);
+      }
+      top = fmaxf(top, m[i]);
+    }
+    float sum = 0.f;
+    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < kMaxParts; ++i) {
+      if (l[i] == 0.f) continue;  // nothing seen (a part whose scores are NaN has its sum NaN)
+      const float w = __builtin_amdgcn_exp2f(m[i] - top);
+      sum = fmaf(w, l[i], sum);
+      y.x = fmaf(w, p[i].x, y.x), y.y = fmaf(w, p[i].y, y.y), y.z = fmaf(w, p[i].z, y.z), y.w = fmaf(w, p[i].w, y.w);
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    const int row = first_row + r, token = row / a.group;
+    const int head = bh % c.kv_heads * a.group + row % a.group;
+    typedef T Four __attribute__((ext_vector_type(4)));
+    const Four out = {(T)(y.x * inv), (T)(y.y * inv), (T)(y.z * inv), (T)(y.w * inv)};
+    *reinterpret_cast<Four*>(static_cast<T*>(c.out) + b * c.o_sb + (long long)token * c.o_st + head * c.o_sh + at) = out;
+  }
+}
+
 template <int kDtype, int kD, int kMode>
 void launch(const Args& a, int waves, hipStream_t stream) {
   const dim3 grid((unsigned)align_up((size_t)a.units, kXcds));
@@ -605,6 +671,8 @@ void launch_all(const Args& a, int waves, hipStream_t stream) {
   if (a.c.d <= 64) launch<kDtype, 64>(a, waves, stream);
   else if (a.c.d <= 96) launch<kDtype, 96>(a, waves, stream);
   else launch<kDtype, 128>(a, waves, stream);
+  if (a.in_parts)
+    hipLaunchKernelGGL((join_parts_kernel<kDtype>), dim3((unsigned)(a.units / a.jobs * a.row_tiles)), dim3(256), 0, stream, a);
   if (a.splits > 1) {
     const long long rows = (long long)a.c.batch * a.c.kv_heads * a.rows;
     hipLaunchKernelGGL((join_kernel<kDtype>), dim3((unsigned)rows), dim3(256), 0, stream, a);

@@ -35,8 +35,8 @@ class Tokens:
     positions  float32 (T, axes) or (B, T, axes), up to 3 axes, for the bias by distance.
 
     The tensors are kept, not copied.  As keys they are also summarised (32 at a time) when the
-    object is made, on the current stream, and the groups of rows of self-attention over them put
-    in the order of their work; call refresh() after changing them in place.  queries_only leaves
+    object is made, on the current stream, and self-attention over them is scheduled (its longest
+    rows first, in parts where there are few); call refresh() after changing them in place.  queries_only leaves
     that out."""
 
     def __init__(self, documents=None, order=None, positions=None, queries_only: bool = False):
@@ -60,17 +60,17 @@ class Tokens:
                                           or positions.device != documents.device):
                 raise ValueError('positions must have the tokens of documents')
         self.documents, self.order, self.positions, self.summary = documents, order, positions, None
-        self._row_order = None
+        self._schedule = None
         if documents is not None and not queries_only:
             b, t = documents.shape if documents.dim() == 2 else (1, documents.shape[0])
             self.summary = torch.empty((b, -(-t // SUMMARY_KEYS), 4), dtype=torch.int32, device=documents.device)
             if 0 < t <= SCHEDULE_MAX_TOKENS:
-                # one after the other for 1, 2, 4 and 8 query heads per key head
+                # blocks for 1, 2, 4 and 8 query heads per key head, of n row groups each
                 tiles = [-(-t * group // ROW_TILE) for group in SCHEDULE_GROUPS]
-                self._row_order = torch.empty((b * 2 * sum(tiles),), dtype=torch.int32, device=documents.device)
-                starts = [b * 2 * sum(tiles[:i]) for i in range(len(tiles))]
-                self._row_order_at = {g: (self._row_order.data_ptr() + 4 * at, 2 * n)
-                                      for g, at, n in zip(SCHEDULE_GROUPS, starts, tiles)}
+                blocks = [4 + 3 * n + (9 * n + 4) // 5 for n in tiles]
+                self._schedule = torch.empty((b * sum(blocks),), dtype=torch.int32, device=documents.device)
+                self._schedule_of = {group: (self._schedule.data_ptr() + 4 * b * sum(blocks[:i]), blocks[i])
+                                     for i, group in enumerate(SCHEDULE_GROUPS)}
             self.refresh()
 
     def refresh(self) -> None:
@@ -82,10 +82,10 @@ class Tokens:
             rt.check(rt.library().musc_token_summary(
                 docs.data_ptr(), None if self.order is None else self.order.data_ptr(), self.summary.shape[0],
                 docs.shape[-1], self.summary.data_ptr(), rt.stream(docs.device)), 'musc_token_summary')
-            if self._row_order is not None:
+            if self._schedule is not None:
                 rt.check(rt.library().musc_token_schedule(
                     docs.data_ptr(), None if self.order is None else self.order.data_ptr(), self.summary.data_ptr(),
-                    self.summary.shape[0], docs.shape[-1], self._row_order.data_ptr(), rt.stream(docs.device)),
+                    self.summary.shape[0], docs.shape[-1], self._schedule.data_ptr(), rt.stream(docs.device)),
                     'musc_token_schedule')
 
 
@@ -187,14 +187,14 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: f
         return o
     if not tk:
         return o.zero_()
-    order_ptr = order_sb = 0
-    if queries is keys and kdocs is not None and keys._row_order is not None:
-        order_ptr, order_sb = keys._row_order_at.get(h // hk, (0, 0))
-        order_sb = order_sb if k_sb else 0
+    schedule = schedule_sb = 0
+    if queries is keys and keys._schedule is not None:
+        schedule, schedule_sb = keys._schedule_of.get(h // hk, (0, 0))
+        schedule_sb = schedule_sb if k_sb else 0
     call = rt.PACK_MASKED_ATTENTION.pack(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), *qs, *ks, *vs, *os_, _STORAGE[dtype], b, tq, tk, h, hk, d,
         scale, cap, qd_ptr, qo_ptr, kd_ptr, ko_ptr, q_sb, k_sb, sum_ptr, sum_sb, qp_ptr, kp_ptr, qp_sb, kp_sb, slope_ptr,
-        axes, order_ptr, order_sb)
+        axes, schedule, schedule_sb)
     lib, need, ws = rt.library(), ctypes.c_size_t(), None
     rt.check(lib.musc_masked_attention_workspace_bytes(call, ctypes.byref(need)), 'musc_masked_attention_workspace_bytes')
     if need.value:

@@ -56,7 +56,7 @@ class MaskedAttention(ctypes.Structure):
         + [('q_tokens_sb', ctypes.c_longlong), ('k_tokens_sb', ctypes.c_longlong), ('k_summary', ctypes.c_void_p),
            ('k_summary_sb', ctypes.c_longlong), ('q_positions', ctypes.c_void_p), ('k_positions', ctypes.c_void_p),
            ('q_positions_sb', ctypes.c_longlong), ('k_positions_sb', ctypes.c_longlong), ('slopes', ctypes.c_void_p),
-           ('axes', ctypes.c_int), ('row_order', ctypes.c_void_p), ('row_order_sb', ctypes.c_longlong)])
+           ('axes', ctypes.c_int), ('schedule', ctypes.c_void_p), ('schedule_sb', ctypes.c_longlong)])
 
 
 # The same as bytes: packing 45 fields at once takes 4 us less than setting them one by one

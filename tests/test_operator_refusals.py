@@ -89,7 +89,7 @@ def attention_call(**kw):
     (dict(q_order=4096, k_order=4096), INVALID), (dict(q_documents=4098, k_documents=4096, k_summary=4096), INVALID),
     (dict(q_documents=4096, k_documents=4096, k_summary=4096, q_order=4096), INVALID),
     (dict(axes=4), UNSUPPORTED), (dict(axes=1), INVALID), (dict(axes=1, q_positions=4096, k_positions=4096), INVALID),
-    (dict(q_tokens_sb=-1), INVALID), (dict(row_order=4098), INVALID), (dict(row_order_sb=-1), INVALID), (dict(batch=1 << 20, kv_heads=2, q_len=1 << 20), UNSUPPORTED)])
+    (dict(q_tokens_sb=-1), INVALID), (dict(schedule=4098), INVALID), (dict(schedule_sb=-2), INVALID), (dict(batch=1 << 20, kv_heads=2, q_len=1 << 20), UNSUPPORTED)])
 def test_masked_attention(lib, change, code):
     need = ctypes.c_size_t()
     call = ctypes.byref(attention_call(**change))
@@ -127,11 +127,11 @@ def test_token_summary(lib, args, code):
 
 
 @pytest.mark.parametrize('change,code', [
-    (dict(documents=None), INVALID), (dict(summary=None), INVALID), (dict(rows=None), INVALID),
+    (dict(documents=None), INVALID), (dict(summary=None), INVALID), (dict(schedule=None), INVALID), (dict(schedule=ctypes.c_void_p(4098)), INVALID),
     (dict(batch=-1), INVALID), (dict(t=-1), INVALID), (dict(summary=ctypes.c_void_p(4104)), INVALID),
     (dict(order=ctypes.c_void_p(4098)), INVALID), (dict(batch=0), OK), (dict(t=0), OK),
     (dict(batch=1 << 12, t=1 << 16), UNSUPPORTED), (dict(t=65537), UNSUPPORTED)])
 def test_token_schedule(lib, change, code):
-    a = dict(documents=P, order=None, summary=P, batch=1, t=64, rows=P, stream=None)
+    a = dict(documents=P, order=None, summary=P, batch=1, t=64, schedule=P, stream=None)
     a.update(change)
     assert lib.musc_token_schedule(*a.values()) == code
