@@ -34,10 +34,11 @@ __device__ __forceinline__ int4v resource(const void* base, long long bytes) {
                __builtin_amdgcn_readfirstlane((int)bytes), kBufferFlags};
 }
 
-// kWaves waves of 32 rows each; kD: head width rounded up to 64, 96 or 128; kMode: kCapped and
-// kBiased in any combination (without them their tests and registers are not in the key loop:
-// 155 -> 127 us for 256 workgroups of 128 tiles, one per CU, fp16, kD = 64).
-constexpr int kCapped = 1, kBiased = 2;
+// kWaves waves of 32 rows each; kD: head width rounded up to 64, 96 or 128; kMode: kCapped,
+// kBiased and, with four waves, kInParts in any combination (without them their tests and registers
+// are not in the key loop: 155 -> 127 us for 256 workgroups of 128 tiles, one per CU, fp16, kD = 64;
+// kInParts alone costs 3 to 8 %).
+constexpr int kCapped = 1, kBiased = 2, kInParts = 4;
 template <int kDtype, int kD, int kWaves, int kMode>
 __global__ __launch_bounds__(kWaves * kWave, kWaves == 1 ? 1 : kD == 64 && kDtype != MUSC_DTYPE_F32 ? 3 : 2) void masked_attention_kernel(const Args a) {
   using Ty = Type<kDtype>;
@@ -101,10 +102,11 @@ __global__ __launch_bounds__(kWaves * kWave, kWaves == 1 ? 1 : kD == 64 && kDtyp
 
   // the row tile, or the part of its keys, that the schedule names; without one later rows first:
   // with an order of tokens they see more keys, and the longest work should not start last
+  constexpr bool in_parts = (kMode & kInParts) != 0;
   int tile_of_rows = a.row_tiles - 1 - (int)job, part = 0, parts = 1;
   if (kWaves > 1 && c.schedule) {
     const int* schedule = c.schedule + b * c.schedule_sb;
-    if (a.in_parts) {
+    if constexpr (in_parts) {
       const int jobs = schedule[0], j = schedule[kScheduleHead + 3 * a.row_tiles + job];
       if ((int)job >= jobs) return;
       tile_of_rows = uniform(j & 0xfffff);
@@ -255,7 +257,7 @@ __global__ __launch_bounds__(kWaves * kWave, kWaves == 1 ? 1 : kD == 64 && kDtyp
 
   // one staged tile; whole: every row sees every key.  careful: in a mixed tile, products
   // of keys that a row does not see are left out one by one (their V may be infinite or NaN)
-  auto attend = [&](int buf, bool whole, auto careful_c) __attribute__((always_inline)) {
+  auto attend = [&](int buf, int tile, bool whole, auto careful_c) __attribute__((always_inline)) {
     constexpr bool careful = decltype(careful_c)::value;
     // Byte places of this lane's operands: row lq (K) or the row and chunk of its V operand, in
     // chunk order from the permutation's exclusive or, which all further chunks keep.  Formed
@@ -343,6 +345,7 @@ __global__ __launch_bounds__(kWaves * kWave, kWaves == 1 ? 1 : kD == 64 && kDtyp
     uint32_t seen = 0xffffffffu;
     if (!whole) {
       mixed_seen = true;
+      const int rem = k_len - tile * kTile;
 #pragma unroll
       for (int u = 0; u < kSub; ++u)
 #pragma unroll
@@ -352,7 +355,7 @@ __global__ __launch_bounds__(kWaves * kWave, kWaves == 1 ? 1 : kD == 64 && kDtyp
           const int4v ko = *reinterpret_cast<const int4v*>(&ords_s[buf][key]);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const bool see = kd[i] == qdoc && ko[i] <= qord;
+            const bool see = kd[i] == qdoc && ko[i] <= qord && key + i < rem;
             s[u][4 * g + i] = see ? s[u][4 * g + i] : -INFINITY;
             if (careful && !see) seen &= ~(1u << (16 * u + 4 * g + i));
           }
@@ -453,7 +456,7 @@ __global__ __launch_bounds__(kWaves * kWave, kWaves == 1 ? 1 : kD == 64 && kDtyp
       return here && k.y >= 0 && k.x <= r.dmax && k.y >= r.dmin && k.z <= r.omax;
     };
     todo = __ballot(may_see(all_rows));
-    if (kWaves > 1 && parts > 1) {  // every parts-th of them
+    if (in_parts && parts > 1) {  // every parts-th of them
       const int number = tiles_seen + __popcll(todo & ((1ull << lane) - 1));
       tiles_seen += __popcll(todo);
       todo = __ballot(((todo >> lane) & 1) && number % parts == part);
@@ -483,7 +486,6 @@ __global__ __launch_bounds__(kWaves * kWave, kWaves == 1 ? 1 : kD == 64 && kDtyp
 #pragma unroll
       for (int v = 0; v < 16; ++v) o[x][v] = 0.f;
     m_run = -INFINITY, l_run = 0.f, base = Ty::kShift, mixed_seen = false;
-    if (decltype(careful_c)::value && !c.k_documents && tid < 64) docs_s[0][tid] = docs_s[1][tid] = 0;
     chunk = lo / 64, tiles_seen = 0;
     sort_tiles(decltype(careful_c)::value ? summary_of(lo / 64 * 64 + lane) : first_summary);
     Next now = next_tile();
@@ -492,12 +494,9 @@ __global__ __launch_bounds__(kWaves * kWave, kWaves == 1 ? 1 : kD == 64 && kDtyp
     while (now.tile >= 0) {
       const Next then = next_tile();
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's share of tile `now` is in LDS
-      // what lies behind the last key is of no document
-      if ((now.tile + 1) * kTile > k_len && wave == kWaves - 1 && lane < kTile && now.tile * kTile + lane >= k_len)
-        docs_s[buf][lane] = -1;
       __syncthreads();  // everyone's is, and everyone is done with the other buffer
       if (then.tile >= 0) load_tile(then.tile, buf ^ 1);
-      if (now.any) attend(buf, now.whole, careful_c);
+      if (now.any) attend(buf, now.tile, now.whole, careful_c);
       buf ^= 1;
       now = then;
     }
@@ -517,7 +516,7 @@ __global__ __launch_bounds__(kWaves * kWave, kWaves == 1 ? 1 : kD == 64 && kDtyp
   l_run = halves_sum(l_run);
   if (!inside) return;
   // register v of block x holds channel 32 x + 8 (v / 4) + 4 lh + v % 4
-  if (a.splits == 1 && parts == 1) {
+  if (in_parts ? parts == 1 : a.splits == 1) {
     const bool empty = !live || l_run == 0.f;
     const float inv = 1.f / l_run;
     T* orow = static_cast<T*>(c.out) + b * c.o_sb + (long long)token * c.o_st + head * c.o_sh;
@@ -533,8 +532,8 @@ __global__ __launch_bounds__(kWaves * kWave, kWaves == 1 ? 1 : kD == 64 && kDtyp
         if (at < d) *reinterpret_cast<Four*>(orow + at) = y;
       }
   } else {
-    const long long at_row = a.splits > 1 ? ((long long)bh * a.rows + row) * a.splits + split
-                                          : ((long long)bh * a.jobs + job) * kRowTile + row % kRowTile;
+    const long long at_row = !in_parts ? ((long long)bh * a.rows + row) * a.splits + split
+                                       : ((long long)bh * a.jobs + job) * kRowTile + row % kRowTile;
     if (lh == 0) {
       a.part_ml[2 * at_row] = live ? m_run * to_log2 : -INFINITY;
       a.part_ml[2 * at_row + 1] = live ? l_run : 0.f;
@@ -653,6 +652,8 @@ void launch(const Args& a, int waves, hipStream_t stream) {
   const dim3 grid((unsigned)align_up((size_t)a.units, kXcds));
   if (waves == 1)
     hipLaunchKernelGGL((masked_attention_kernel<kDtype, kD, 1, kMode>), grid, dim3(kWave), 0, stream, a);
+  else if (a.in_parts)
+    hipLaunchKernelGGL((masked_attention_kernel<kDtype, kD, 4, kMode | kInParts>), grid, dim3(4 * kWave), 0, stream, a);
   else
     hipLaunchKernelGGL((masked_attention_kernel<kDtype, kD, 4, kMode>), grid, dim3(4 * kWave), 0, stream, a);
 }
