@@ -466,13 +466,22 @@ int musc_rmsnorm_rows_8bit(const void* x, long long x_stride, const void* residu
  *   frequency (pairs,) float64 on the device, turns per unit of position; axis (pairs,) int32 on
  *             the device, each in [0, axes).
  * pairs <= 256, d <= 512, q_heads + k_heads <= 1024 (MUSC_ERR_UNSUPPORTED beyond). */
-int musc_rotary(const void* q, int q_heads, long long q_sb, long long q_st, long long q_sh,
-                void* q_out, long long qo_sb, long long qo_st, long long qo_sh,
-                const void* k, int k_heads, long long k_sb, long long k_st, long long k_sh,
-                void* k_out, long long ko_sb, long long ko_st, long long ko_sh,
-                int dtype, int batch, int t, int d, const void* positions, int int_positions,
-                long long pos_sb, int axes, const double* frequency, const int* axis, int pairs,
-                int adjacent, int inverse, hipStream_t stream);
+typedef struct musc_rotary_call {
+  const void* q;
+  long long q_sb, q_st, q_sh;
+  void* q_out;
+  long long q_ob, q_ot, q_oh;
+  const void* k;
+  long long k_sb, k_st, k_sh;
+  void* k_out;
+  long long k_ob, k_ot, k_oh;
+  const void* positions;
+  long long pos_sb;
+  const double* frequency;
+  const int* axis;
+  int q_heads, k_heads, dtype, batch, t, d, int_positions, axes, pairs, adjacent, inverse;
+} musc_rotary_call;
+int musc_rotary(const musc_rotary_call* call, hipStream_t stream);
 
 #define MUSC_ACT_QUICK_GELU 0  /* x * sigmoid(1.702 x), transformer.py:32-35 (fp16: the
                                   three torch ops' roundings: 1.702 x, sigmoid, product) */

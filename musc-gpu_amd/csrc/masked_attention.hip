@@ -108,8 +108,14 @@ int plan(const musc_masked_attention& c, Args& a, int& waves) {
   const long long heads = (long long)c.batch * c.kv_heads, whole = heads * a.row_tiles;
   // workgroups that the card holds at a time
   a.slots = waves == 1 ? 1024 : c.dtype != MUSC_DTYPE_F32 && c.d <= 64 ? 768 : 512;
-  a.splits = 1, a.jobs = a.row_tiles, a.in_parts = 0;
-  if (waves > 1 && c.schedule) {
+  a.splits = 1, a.jobs = a.row_tiles, a.in_parts = 0, a.teams = 1;
+  // Few rows over up to 2048 keys (1024 of wide heads): the waves of one workgroup share them and
+  // join in LDS, without a second launch.  One row, 1369 keys, 16 heads of 64: 17.1 us in
+  // workgroups of one wave and a join, 12.9 us so, host time included.
+  const int teams = teams_of((c.d <= 64 ? 64 : 128) * (c.dtype == MUSC_DTYPE_F32 ? 4 : 2));
+  if (waves == 1 && a.key_tiles <= kTeamTiles * teams) a.teams = teams;
+  if (a.teams > 1) {
+  } else if (waves > 1 && c.schedule) {
     // Long row tiles in parts where all begin at once and the longest ends last: 4 packed images,
     // fp32 (416 row tiles, 512 places), 204 -> 144 us; with more row tiles than places short ones
     // fill up behind long ones (12 packed images, fp16, 1184 for 768: 106 us whole, 110 in parts).

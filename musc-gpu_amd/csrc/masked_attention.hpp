@@ -46,6 +46,10 @@ constexpr int kSummaryKeys = 32;
 constexpr int kMaxAxes = 3;
 constexpr int kMaxSplits = 256;
 constexpr int kRowTile = 128;  // rows of a workgroup of four waves
+// Waves of a workgroup that share few rows' keys, for staged rows of `pitch` bytes: two tiles of 32
+// keys each in 128 KiB of LDS.
+constexpr int teams_of(int pitch) { return 131072 / (4 * 32 * pitch); }
+constexpr int kTeamTiles = 8;  // tiles of such a wave at most
 // Schedule of n row tiles, in ints: head (jobs), work (n), row tiles by their work (n), first job
 // | parts << 24 of each row tile (n), jobs (row tile | part << 20 | (parts - 1) << 23).
 constexpr int kScheduleHead = 4, kMaxParts = 8;
@@ -111,6 +115,7 @@ struct Args {
   int group, rows, row_tiles, key_tiles, splits, summaries, heads_at_once;
   int jobs;      // workgroups of a head and split: its row tiles, or the schedule's jobs
   int in_parts;  // jobs may be parts of a row tile's keys
+  int teams;     // waves that share few rows' keys within a workgroup
   int slots;     // workgroups that the card holds at a time
   long long units;
   float* part_ml;  // (units in (b, kv head), rows, split) x (maximum, sum)

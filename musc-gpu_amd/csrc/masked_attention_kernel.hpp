@@ -37,10 +37,14 @@ __device__ __forceinline__ int4v resource(const void* base, long long bytes) {
 // kWaves waves of 32 rows each; kD: head width rounded up to 64, 96 or 128; kMode: kCapped,
 // kBiased and, with four waves, kInParts in any combination (without them their tests and registers
 // are not in the key loop: 155 -> 127 us for 256 workgroups of 128 tiles, one per CU, fp16, kD = 64;
-// kInParts alone costs 3 to 8 %).
-constexpr int kCapped = 1, kBiased = 2, kInParts = 4;
-template <int kDtype, int kD, int kWaves, int kMode>
-__global__ __launch_bounds__(kWaves * kWave, kWaves == 1 ? 1 : kD == 64 && kDtype != MUSC_DTYPE_F32 ? 3 : 2) void masked_attention_kernel(const Args a) {
+// kInParts alone costs 3 to 8 %).  kTeams > 1 (with one wave): that many waves take every n-th tile of
+// the same rows, each with its own place in LDS and at its own pace, and join their parts there.
+// kEither: a cap and a bias if the call has them, tested per tile (for the kernels of few rows and
+// of parts, which wait for memory or for one another).
+constexpr int kCapped = 1, kBiased = 2, kInParts = 4, kEither = 8;
+template <int kDtype, int kD, int kWaves, int kTeams, int kMode>
+__global__ __launch_bounds__(kWaves * kTeams * kWave, kWaves == 1 ? 1 : kD == 64 && kDtype != MUSC_DTYPE_F32 ? 3 : 2) void masked_attention_kernel(
+    const Args a) {
   using Ty = Type<kDtype>;
   typedef typename Ty::T T;
   constexpr bool k16 = kDtype != MUSC_DTYPE_F32;
@@ -52,9 +56,9 @@ __global__ __launch_bounds__(kWaves * kWave, kWaves == 1 ? 1 : kD == 64 && kDtyp
   constexpr int kLoads = kPart / 1024 / kWaves;             // loads of K (and of V) per wave
   static_assert(kLoads * kWaves * 1024 == kPart, "whole loads per wave");
   constexpr int kO = kD / 32;
-  __shared__ __attribute__((aligned(1024))) char staged[2][2 * kPart];
-  __shared__ __attribute__((aligned(16))) int docs_s[2][64], ords_s[2][64];
-  __shared__ float pos_s[2][64 * kMaxAxes];
+  __shared__ __attribute__((aligned(1024))) char staged[2 * kTeams][2 * kPart];
+  __shared__ __attribute__((aligned(16))) int docs_s[2 * kTeams][64], ords_s[2 * kTeams][64];
+  __shared__ float pos_s[2 * kTeams][64 * kMaxAxes];
   __shared__ Range ranges[kWaves];
 
   const musc_masked_attention& c = a.c;
@@ -80,7 +84,9 @@ __global__ __launch_bounds__(kWaves * kWave, kWaves == 1 ? 1 : kD == 64 && kDtyp
     job = rest - bh * a.jobs;
   }
   const int b = uniform(bh / c.kv_heads), kvh = bh - b * c.kv_heads;
-  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid % kWave;
+  const int tid = threadIdx.x, lane = tid % kWave;
+  const int team = kTeams > 1 ? __builtin_amdgcn_readfirstlane(tid / kWave) : 0;
+  const int wave = kTeams > 1 ? 0 : __builtin_amdgcn_readfirstlane(tid / kWave);
   const int lq = lane & 31, lh = lane >> 5;
 
   // tiles of this split, 64 sorted at a time by the keys' summary; the first 64 are asked for now
@@ -103,7 +109,7 @@ __global__ __launch_bounds__(kWaves * kWave, kWaves == 1 ? 1 : kD == 64 && kDtyp
   // the row tile, or the part of its keys, that the schedule names; without one later rows first:
   // with an order of tokens they see more keys, and the longest work should not start last
   constexpr bool in_parts = (kMode & kInParts) != 0;
-  int tile_of_rows = a.row_tiles - 1 - (int)job, part = 0, parts = 1;
+  int tile_of_rows = a.row_tiles - 1 - (int)job, part = team, parts = kTeams;
   if (kWaves > 1 && c.schedule) {
     const int* schedule = c.schedule + b * c.schedule_sb;
     if constexpr (in_parts) {
@@ -121,7 +127,7 @@ __global__ __launch_bounds__(kWaves * kWave, kWaves == 1 ? 1 : kD == 64 && kDtyp
   const bool inside = row < a.rows;
   const int token = inside ? (int)((uint32_t)row / (uint32_t)a.group) : 0;
   const int head = kvh * a.group + (inside ? row - token * a.group : 0);
-  const int d = c.d, k_len = c.k_len, axes = kMode & kBiased ? c.axes : 0;
+  const int d = c.d, k_len = c.k_len, axes = kMode & (kBiased | kEither) ? c.axes : 0;
 
   // this row's document and order (rows outside the tensor read token 0's), its Q and positions,
   // all asked for before any is used
@@ -159,9 +165,9 @@ __global__ __launch_bounds__(kWaves * kWave, kWaves == 1 ? 1 : kD == 64 && kDtyp
     if (lane == 0) ranges[wave] = mine;
   }
   // keys of calls without documents or orders have 0
-  if (tid < 64) {
+  if (wave == 0) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) docs_s[i][tid] = 0, ords_s[i][tid] = 0;
+    for (int i = 0; i < 2; ++i) docs_s[2 * team + i][lane] = 0, ords_s[2 * team + i][lane] = 0;
   }
   __syncthreads();
   if constexpr (kWaves > 1) {
@@ -179,7 +185,7 @@ __global__ __launch_bounds__(kWaves * kWave, kWaves == 1 ? 1 : kD == 64 && kDtyp
   //   no cap   raw = +- q . k (Q negated for a negative scale), to_log2 = |scale| log2 e
   //   cap      raw = -1 / (1 + e^2x), x = scale q . k / cap, as cap tanh x = cap (1 + 2 raw);
   //            fp32: raw = tanh x
-  constexpr bool capped = (kMode & kCapped) != 0;
+  const bool capped = (kMode & kCapped) != 0 || ((kMode & kEither) != 0 && c.cap > 0.f);
   const float scale = c.scale == 0.f ? 1.f : c.scale;
   const float to_log2 = (capped ? (k16 ? 2.f * c.cap : c.cap) : fabsf(scale)) * kLog2e;
   const float by_cap = capped ? scale / c.cap * (k16 ? 2.f * kLog2e : 1.f) : 0.f;
@@ -456,7 +462,7 @@ __global__ __launch_bounds__(kWaves * kWave, kWaves == 1 ? 1 : kD == 64 && kDtyp
       return here && k.y >= 0 && k.x <= r.dmax && k.y >= r.dmin && k.z <= r.omax;
     };
     todo = __ballot(may_see(all_rows));
-    if (in_parts && parts > 1) {  // every parts-th of them
+    if ((in_parts || kTeams > 1) && parts > 1) {  // every parts-th of them
       const int number = tiles_seen + __popcll(todo & ((1ull << lane) - 1));
       tiles_seen += __popcll(todo);
       todo = __ballot(((todo >> lane) & 1) && number % parts == part);
@@ -489,12 +495,13 @@ __global__ __launch_bounds__(kWaves * kWave, kWaves == 1 ? 1 : kD == 64 && kDtyp
     chunk = lo / 64, tiles_seen = 0;
     sort_tiles(decltype(careful_c)::value ? summary_of(lo / 64 * 64 + lane) : first_summary);
     Next now = next_tile();
-    if (now.tile >= 0) load_tile(now.tile, 0);
-    int buf = 0;
+    int buf = 2 * team;
+    if (now.tile >= 0) load_tile(now.tile, buf);
     while (now.tile >= 0) {
       const Next then = next_tile();
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's share of tile `now` is in LDS
-      __syncthreads();  // everyone's is, and everyone is done with the other buffer
+      if constexpr (kTeams > 1) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      else __syncthreads();  // everyone's is, and everyone is done with the other buffer
       if (then.tile >= 0) load_tile(then.tile, buf ^ 1);
       if (now.any) attend(buf, now.tile, now.whole, careful_c);
       buf ^= 1;
@@ -511,9 +518,50 @@ __global__ __launch_bounds__(kWaves * kWave, kWaves == 1 ? 1 : kD == 64 && kDtyp
       for (int v = 0; v < 16; ++v) bad |= !(fabsf(o[x][v]) < INFINITY);
   }
   // also the barrier before the buffers are filled again
-  if (__syncthreads_or(bad)) walk(std::integral_constant<bool, true>{});
+  if (kTeams > 1 ? __any(bad) : __syncthreads_or(bad)) walk(std::integral_constant<bool, true>{});
 
   l_run = halves_sum(l_run);
+  if constexpr (kTeams > 1) {
+    // each team's (maximum, sum) and output in its own place, then all of them in order
+    constexpr int kPlace = kPart;  // floats of a team's place: four tiles' bytes
+    static_assert(32 * kD + 64 <= kPlace, "a team's output fits its place");
+    float* places = reinterpret_cast<float*>(&staged[0][0]);
+    float* mine_at = places + team * kPlace;
+#pragma unroll
+    for (int x = 0; x < kO; ++x)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<float4*>(mine_at + lq * kD + 32 * x + 8 * g + 4 * lh) =
+            make_float4(o[x][4 * g], o[x][4 * g + 1], o[x][4 * g + 2], o[x][4 * g + 3]);
+    if (lh == 0) {
+      mine_at[32 * kD + 2 * lq] = live ? m_run * to_log2 : -INFINITY;
+      mine_at[32 * kD + 2 * lq + 1] = live ? l_run : 0.f;
+    }
+    __syncthreads();
+    for (int e = tid; e < a.rows * (d / 4); e += kTeams * kWave) {
+      const int r = e / (d / 4), at = e % (d / 4) * 4;
+      float top = -INFINITY, sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < kTeams; ++i) top = fmaxf(top, places[i * kPlace + 32 * kD + 2 * r]);
+      float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int i = 0; i < kTeams; ++i) {
+        const float* from = places + i * kPlace;
+        const float l = from[32 * kD + 2 * r + 1];
+        if (l == 0.f) continue;  // nothing seen (a part whose scores are NaN has its sum NaN)
+        const float w = __builtin_amdgcn_exp2f(from[32 * kD + 2 * r] - top);
+        const float4 p = *reinterpret_cast<const float4*>(from + r * kD + at);
+        sum = fmaf(w, l, sum);
+        y.x = fmaf(w, p.x, y.x), y.y = fmaf(w, p.y, y.y), y.z = fmaf(w, p.z, y.z), y.w = fmaf(w, p.w, y.w);
+      }
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      const int t = (int)((uint32_t)r / (uint32_t)a.group), h = kvh * a.group + (r - t * a.group);
+      typedef T Four __attribute__((ext_vector_type(4)));
+      *reinterpret_cast<Four*>(static_cast<T*>(c.out) + b * c.o_sb + (long long)t * c.o_st + h * c.o_sh + at) =
+          Four{(T)(y.x * inv), (T)(y.y * inv), (T)(y.z * inv), (T)(y.w * inv)};
+    }
+    return;
+  }
   if (!inside) return;
   // register v of block x holds channel 32 x + 8 (v / 4) + 4 lh + v % 4
   if (in_parts ? parts == 1 : a.splits == 1) {
@@ -647,24 +695,35 @@ __global__ __launch_bounds__(256) void join_parts_kernel(const Args a) {
   }
 }
 
+// Few rows, or rows in parts.
 template <int kDtype, int kD, int kMode>
-void launch(const Args& a, int waves, hipStream_t stream) {
-  const dim3 grid((unsigned)align_up((size_t)a.units, kXcds));
-  if (waves == 1)
-    hipLaunchKernelGGL((masked_attention_kernel<kDtype, kD, 1, kMode>), grid, dim3(kWave), 0, stream, a);
-  else if (a.in_parts)
-    hipLaunchKernelGGL((masked_attention_kernel<kDtype, kD, 4, kMode | kInParts>), grid, dim3(4 * kWave), 0, stream, a);
+void launch_special(const Args& a, int waves, const dim3& grid, hipStream_t stream) {
+  constexpr int kTeams = teams_of((kD <= 64 ? 64 : 128) * (kDtype == MUSC_DTYPE_F32 ? 4 : 2));
+  if (a.teams > 1)
+    hipLaunchKernelGGL((masked_attention_kernel<kDtype, kD, 1, kTeams, kMode>), grid, dim3(kTeams * kWave), 0, stream, a);
+  else if (waves == 1)
+    hipLaunchKernelGGL((masked_attention_kernel<kDtype, kD, 1, 1, kMode>), grid, dim3(kWave), 0, stream, a);
   else
-    hipLaunchKernelGGL((masked_attention_kernel<kDtype, kD, 4, kMode>), grid, dim3(4 * kWave), 0, stream, a);
+    hipLaunchKernelGGL((masked_attention_kernel<kDtype, kD, 4, 1, kMode | kInParts>), grid, dim3(4 * kWave), 0, stream, a);
 }
 
 template <int kDtype, int kD>
 void launch(const Args& a, int waves, hipStream_t stream) {
+  const dim3 grid((unsigned)align_up((size_t)a.units, kXcds));
   const int mode = (a.c.cap > 0.f ? kCapped : 0) | (a.c.axes ? kBiased : 0);
-  if (mode == 0) launch<kDtype, kD, 0>(a, waves, stream);
-  else if (mode == kCapped) launch<kDtype, kD, kCapped>(a, waves, stream);
-  else if (mode == kBiased) launch<kDtype, kD, kBiased>(a, waves, stream);
-  else launch<kDtype, kD, kCapped | kBiased>(a, waves, stream);
+  if (waves == 1 || a.in_parts) {
+    constexpr int kWide = kD <= 64 ? 64 : 128;
+    if (mode == 0) launch_special<kDtype, kWide, 0>(a, waves, grid, stream);
+    else launch_special<kDtype, kWide, kEither>(a, waves, grid, stream);
+  } else if (mode == 0) {
+    hipLaunchKernelGGL((masked_attention_kernel<kDtype, kD, 4, 1, 0>), grid, dim3(4 * kWave), 0, stream, a);
+  } else if (mode == kCapped) {
+    hipLaunchKernelGGL((masked_attention_kernel<kDtype, kD, 4, 1, kCapped>), grid, dim3(4 * kWave), 0, stream, a);
+  } else if (mode == kBiased) {
+    hipLaunchKernelGGL((masked_attention_kernel<kDtype, kD, 4, 1, kBiased>), grid, dim3(4 * kWave), 0, stream, a);
+  } else {
+    hipLaunchKernelGGL((masked_attention_kernel<kDtype, kD, 4, 1, kCapped | kBiased>), grid, dim3(4 * kWave), 0, stream, a);
+  }
 }
 
 template <int kDtype>

@@ -149,14 +149,12 @@ void launch(const Args& a, bool adjacent, bool vec, dim3 grid, hipStream_t strea
 
 using namespace musc;
 
-extern "C" int musc_rotary(const void* q, int q_heads, long long q_sb, long long q_st, long long q_sh, void* q_out,
-                           long long qo_sb, long long qo_st, long long qo_sh, const void* k, int k_heads,
-                           long long k_sb, long long k_st, long long k_sh, void* k_out, long long ko_sb,
-                           long long ko_st, long long ko_sh, int dtype, int batch, int t, int d,
-                           const void* positions, int int_positions, long long pos_sb, int axes,
-                           const double* frequency, const int* axis, int pairs, int adjacent, int inverse,
-                           hipStream_t stream) {
+extern "C" int musc_rotary(const musc_rotary_call* call, hipStream_t stream) {
   using namespace rotary;
+  if (!call) return MUSC_ERR_INVALID_ARG;
+  const auto& [q, q_sb, q_st, q_sh, q_out, qo_sb, qo_st, qo_sh, k, k_sb, k_st, k_sh, k_out, ko_sb, ko_st, ko_sh, positions,
+               pos_sb, frequency, axis, q_heads, k_heads, dtype, batch, t, d, int_positions, axes, pairs, adjacent,
+               inverse] = *call;
   if (!q || !q_out || !positions || !frequency || !axis || batch < 0 || t < 0 || q_heads < 1 || k_heads < 0 ||
       axes < 1 || pairs < 1 || d < 2 * pairs || pos_sb < 0)
     return MUSC_ERR_INVALID_ARG;

@@ -44,6 +44,7 @@ class RotaryAxes:
         self.head_dim, self.pairs, self.axes, self.adjacent = int(head_dim), pairs, len(sections), bool(adjacent)
         self.frequency = torch.tensor(turns, dtype=torch.float64, device=device)
         self.axis = torch.tensor(axis, dtype=torch.int32, device=device)
+        self.frequency_ptr, self.axis_ptr = self.frequency.data_ptr(), self.axis.data_ptr()
 
 
 def _head_rows(x, name, axes):
@@ -68,7 +69,7 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, axe
     rt.require_no_gradient(q, k)
     index = q.get_device()
     b, t, h, d = q2.shape
-    k2, ko, k_args = None, None, (None, 0, 0, 0, 0, None, 0, 0, 0)
+    k2, ko, k_heads, k_args = None, None, 0, (0, 0, 0, 0, 0, 0, 0, 0)
     if k is not None:
         k2 = _head_rows(k, 'k', axes)
         if k2.shape[0] != b or k2.shape[1] != t or k2.dtype != q2.dtype or k2.get_device() != index:
@@ -86,13 +87,14 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, axe
     if k2 is not None:
         ko = rt.output_like(out[1] if out is not None else None, k2, 'k_out')
         if k2.shape[2]:
-            k_args = (k2.data_ptr(), k2.shape[2], *rt.token_strides(k2), ko.data_ptr(), *rt.token_strides(ko))
+            k_heads = k2.shape[2]
+            k_args = (k2.data_ptr(), *rt.token_strides(k2), ko.data_ptr(), *rt.token_strides(ko))
         out = out[0] if out is not None else None
     qo = rt.output_like(out, q2, 'q_out')
     if b and t and h:
-        rt.check(rt.library().musc_rotary(
-            q2.data_ptr(), h, *rt.token_strides(q2), qo.data_ptr(), *rt.token_strides(qo), *k_args, _STORAGE[q2.dtype], b, t,
-            d, positions.data_ptr(), positions.dtype == torch.int32, 0 if len(shape) == 2 else t * axes.axes, axes.axes,
-            axes.frequency.data_ptr(), axes.axis.data_ptr(), axes.pairs, axes.adjacent, inverse,
-            rt.current_stream(index)), 'musc_rotary')
+        call = rt.PACK_ROTARY.pack(
+            q2.data_ptr(), *rt.token_strides(q2), qo.data_ptr(), *rt.token_strides(qo), *k_args, positions.data_ptr(),
+            0 if len(shape) == 2 else t * axes.axes, axes.frequency_ptr, axes.axis_ptr, h, k_heads, _STORAGE[q2.dtype], b, t,
+            d, positions.dtype == torch.int32, axes.axes, axes.pairs, axes.adjacent, inverse)
+        rt.check(rt.library().musc_rotary(call, rt.current_stream(index)), 'musc_rotary')
     return qo if k is None else (qo, ko)

@@ -59,9 +59,22 @@ class MaskedAttention(ctypes.Structure):
            ('axes', ctypes.c_int), ('schedule', ctypes.c_void_p), ('schedule_sb', ctypes.c_longlong)])
 
 
+class RotaryCall(ctypes.Structure):
+    """musc_rotary_call of include/musc_hip.h, field by field."""
+    _fields_ = (
+        [field for x in 'qk' for name, s in ((x, ('sb', 'st', 'sh')), (f'{x}_out', ('ob', 'ot', 'oh')))
+         for field in [(name, ctypes.c_void_p)] + [(f'{x}_{y}', ctypes.c_longlong) for y in s]]
+        + [('positions', ctypes.c_void_p), ('pos_sb', ctypes.c_longlong), ('frequency', ctypes.c_void_p),
+           ('axis', ctypes.c_void_p)]
+        + [(n, ctypes.c_int) for n in ('q_heads', 'k_heads', 'dtype', 'batch', 't', 'd', 'int_positions', 'axes', 'pairs',
+                                       'adjacent', 'inverse')])
+
+
 # The same as bytes: packing 45 fields at once takes 4 us less than setting them one by one
 PACK_MASKED_ATTENTION = struct.Struct('@4P12q7i2f4P2qPq2P2qPiPq')
+PACK_ROTARY = struct.Struct('@P3qP3qP3qP3qPqPP11i4x')
 assert PACK_MASKED_ATTENTION.size == ctypes.sizeof(MaskedAttention)
+assert PACK_ROTARY.size == ctypes.sizeof(RotaryCall)
 
 
 # Every symbol include/musc_hip.h declares, with its ctypes signature.
@@ -104,8 +117,7 @@ SIGNATURES = {
     'musc_masked_attention_fwd': (_i, [_vp, _vp, _sz, _vp]),
     'musc_rmsnorm_rows': (_i, [_vp, _ll, _vp, _ll, _vp, _vp, _i, _i, _i, _i, _f, _vp, _vp]),
     'musc_rmsnorm_rows_8bit': (_i, [_vp, _ll, _vp, _ll, _vp, _vp, _i, _i, _i, _i, _f, _i, _i, _vp, _vp, _vp]),
-    'musc_rotary': (_i, [_vp, _i, _ll, _ll, _ll, _vp, _ll, _ll, _ll, _vp, _i, _ll, _ll, _ll, _vp, _ll, _ll, _ll,
-                         _i, _i, _i, _i, _vp, _i, _ll, _i, _vp, _vp, _i, _i, _i, _vp]),
+    'musc_rotary': (_i, [_vp, _vp]),
     'musc_activation': (_i, [_vp, _vp, _i, _i, _ll, _vp]),
     'musc_calibrate_mfma_f32': (_i, [_vp, _i, _i, ctypes.POINTER(ctypes.c_double), _vp]),
     'musc_calibrate_mfma_f16': (_i, [_vp, _i, _i, ctypes.POINTER(ctypes.c_double), _vp]),

@@ -45,23 +45,27 @@ def test_rmsnorm_eight_bits(lib, change, code):
     assert lib.musc_rmsnorm_rows_8bit(*eight_args(**change)) == code
 
 
-def rotary_args(**kw):
-    a = dict(q=P, qh=2, qsb=512, qst=128, qsh=64, qo=P, qob=512, qot=128, qoh=64, k=None, kh=0, ksb=0, kst=0, ksh=0,
-             ko=None, kob=0, kot=0, koh=0, dt=0, batch=1, t=4, d=64, pos=P, ints=0, psb=0, axes=2, freq=P, axis=P, pairs=32,
-             adjacent=0, inverse=0, stream=None)
-    a.update(kw)
-    return list(a.values())
+def rotary_call(**kw):
+    from musc_hip import _runtime as rt
+    c = rt.RotaryCall()
+    c.q = c.q_out = c.positions = c.frequency = c.axis = 4096
+    c.q_sb, c.q_st, c.q_sh, c.q_ob, c.q_ot, c.q_oh = 512, 128, 64, 512, 128, 64
+    c.q_heads, c.batch, c.t, c.d, c.axes, c.pairs = 2, 1, 4, 64, 2, 32
+    for name, value in kw.items():
+        setattr(c, name, value)
+    return c
 
 
 @pytest.mark.parametrize('change,code', [
-    (dict(q=None), INVALID), (dict(qo=None), INVALID), (dict(pos=None), INVALID), (dict(freq=None), INVALID),
-    (dict(axis=None), INVALID), (dict(pairs=33), INVALID), (dict(pairs=0), INVALID), (dict(axes=0), INVALID),
-    (dict(qh=0), INVALID), (dict(kh=1), INVALID), (dict(qst=-1), INVALID), (dict(dt=3), INVALID), (dict(psb=-1), INVALID),
-    (dict(q=ctypes.c_void_p(4098)), INVALID), (dict(freq=ctypes.c_void_p(4100)), INVALID),
-    (dict(d=520), UNSUPPORTED), (dict(qh=1025), UNSUPPORTED), (dict(batch=65536, t=65536), UNSUPPORTED),
+    (dict(q=0), INVALID), (dict(q_out=0), INVALID), (dict(positions=0), INVALID), (dict(frequency=0), INVALID),
+    (dict(axis=0), INVALID), (dict(pairs=33), INVALID), (dict(pairs=0), INVALID), (dict(axes=0), INVALID),
+    (dict(q_heads=0), INVALID), (dict(k_heads=1), INVALID), (dict(q_st=-1), INVALID), (dict(dtype=3), INVALID),
+    (dict(pos_sb=-1), INVALID), (dict(q=4098), INVALID), (dict(frequency=4100), INVALID),
+    (dict(d=520), UNSUPPORTED), (dict(q_heads=1025), UNSUPPORTED), (dict(batch=65536, t=65536), UNSUPPORTED),
     (dict(d=512, pairs=256, t=0), OK), (dict(batch=0), OK)])
 def test_rotary(lib, change, code):
-    assert lib.musc_rotary(*rotary_args(**change)) == code
+    assert lib.musc_rotary(ctypes.byref(rotary_call(**change)), None) == code
+    assert lib.musc_rotary(None, None) == INVALID
 
 
 def attention_call(**kw):
@@ -111,11 +115,14 @@ def test_masked_attention_workspace(lib):
     assert lib.musc_masked_attention_fwd(one, ctypes.c_void_p(4100), need, None) == WORKSPACE
 
 
-def test_packed_call_is_the_structure(lib):
+def test_packed_calls_are_the_structures(lib):
     from musc_hip import _runtime as rt
     values = list(range(1, 24)) + [0.5, 2.0] + list(range(26, 42))
     packed = rt.MaskedAttention.from_buffer_copy(rt.PACK_MASKED_ATTENTION.pack(*values))
     assert [getattr(packed, name) for name, _ in rt.MaskedAttention._fields_] == values
+    values = list(range(1, 32))
+    packed = rt.RotaryCall.from_buffer_copy(rt.PACK_ROTARY.pack(*values))
+    assert [getattr(packed, name) for name, _ in rt.RotaryCall._fields_] == values
 
 
 @pytest.mark.parametrize('args,code', [
