@@ -418,7 +418,7 @@ int musc_token_summary(const int* documents, const int* order, int batch, int t,
  * other: batch blocks of 4 + 3 n + (9 n + 4) / 5 int32 each, n = ceil(t * heads / kv_heads / 128).  Made again when a
  * document or order changes.  t up to MUSC_SCHEDULE_MAX_TOKENS (MUSC_ERR_UNSUPPORTED beyond: so many
  * row groups need no schedule). */
-#define MUSC_SCHEDULE_MAX_TOKENS 65536
+#define MUSC_SCHEDULE_MAX_TOKENS 16384
 int musc_token_schedule(const int* documents, const int* order, const int* summary, int batch, int t, int* schedule,
                         hipStream_t stream);
 /* Few rows, and long row groups among few, are split over their keys and joined through a workspace

@@ -67,30 +67,53 @@ __global__ __launch_bounds__(kWave) void row_work_kernel(const int* __restrict__
 // The row tiles by their work, most first (later ones first where it is the same): whole, and as
 // jobs, where a tile of more than 5/4 of the mean work is listed in up to 8 parts, by the work of a
 // part.  At most 9/5 n jobs.
-__global__ __launch_bounds__(256) void row_order_kernel(const Schedule s, int* __restrict__ out) {
-  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-  if (i >= s.first[4]) return;
-  const int w = s.which(i), n = s.tiles[w];
-  const int b = (int)((i - s.first[w]) / n), tile = (int)((i - s.first[w]) % n);
+// One workgroup per schedule.  Every row tile finds its place by looking at all of them in LDS: 1024
+// tiles, 1024 threads.
+constexpr int kMostTiles = MUSC_SCHEDULE_MAX_TOKENS * 8 / kRowTile;
+__global__ __launch_bounds__(1024) void row_order_kernel(const Schedule s, int* __restrict__ out) {
+  __shared__ int2 tiles[kMostTiles];  // work, work of a part * 8 + parts - 1
+  __shared__ long long sums[16];
+  __shared__ int counts[16];
+  const int w = blockIdx.x % 4, b = blockIdx.x / 4, n = s.tiles[w], lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
   int* block = out + s.at[w] + b * schedule_block(n);
   const int* work = block + kScheduleHead;
-  long long total = 0;
-  for (int j = 0; j < n; ++j) total += work[j];
-  const int most = (int)max((5 * total + 4LL * n - 1) / (4LL * n), 8LL);  // of a part
-  auto parts_of = [&](int x) { return min(max((x + most - 1) / most, 1), kMaxParts); };
-  const int here = work[tile], parts = parts_of(here), size = (here + parts - 1) / parts;
-  int rank = 0, first = 0, all = 0;
-  for (int j = 0; j < n; ++j) {
-    const int x = work[j], p = parts_of(x), each = (x + p - 1) / p;
-    rank += x > here || (x == here && j > tile);
-    first += each > size || (each == size && j > tile) ? p : 0;
-    all += p;
+  double total = 0;  // whole numbers below 2^53
+  for (int j = threadIdx.x; j < n; j += 1024) total += work[j];
+  total = wave_sum(total);
+  if (lane == 0) sums[wave] = (long long)total;
+  __syncthreads();
+  long long all_work = 0;
+  for (int i = 0; i < 16; ++i) all_work += sums[i];
+  const int most = (int)max((5 * all_work + 4LL * n - 1) / (4LL * n), 8LL);  // of a part
+  float jobs_here = 0.f;
+  for (int j = threadIdx.x; j < n; j += 1024) {
+    const int x = work[j], parts = min(max((x + most - 1) / most, 1), kMaxParts);
+    tiles[j] = make_int2(x, (x + parts - 1) / parts * 8 + parts - 1);
+    jobs_here += parts;
   }
-  block[kScheduleHead + n + rank] = tile;
-  block[kScheduleHead + 2 * n + tile] = first | parts << 24;
-  int* jobs = block + kScheduleHead + 3 * n + first;
-  for (int p = 0; p < parts; ++p) jobs[p] = tile | p << 20 | (parts - 1) << 23;
-  if (tile == 0) block[0] = all;
+  jobs_here = wave_sum(jobs_here);
+  if (lane == 0) counts[wave] = (int)jobs_here;
+  __syncthreads();
+  for (int tile = threadIdx.x; tile < n; tile += 1024) {
+    const int2 here = tiles[tile];
+    const int size = here.y >> 3, parts = (here.y & 7) + 1;
+    int rank = 0, first = 0;
+    for (int j = 0; j < n; ++j) {
+      const int2 x = tiles[j];
+      const int each = x.y >> 3;
+      rank += x.x > here.x || (x.x == here.x && j > tile);
+      first += each > size || (each == size && j > tile) ? (x.y & 7) + 1 : 0;
+    }
+    block[kScheduleHead + n + rank] = tile;
+    block[kScheduleHead + 2 * n + tile] = first | parts << 24;
+    int* jobs = block + kScheduleHead + 3 * n + first;
+    for (int p = 0; p < parts; ++p) jobs[p] = tile | p << 20 | (parts - 1) << 23;
+  }
+  if (threadIdx.x == 0) {
+    int jobs = 0;
+    for (int i = 0; i < 16; ++i) jobs += counts[i];
+    block[0] = jobs;
+  }
 }
 
 // Shape of the launch: rows per workgroup, tiles and splits.
@@ -225,10 +248,10 @@ extern "C" int musc_token_schedule(const int* documents, const int* order, const
     s.first[w + 1] = s.first[w] + (long long)batch * s.tiles[w];
     if (w < 3) s.at[w + 1] = s.at[w] + batch * mattn::schedule_block(s.tiles[w]);
   }
-  if (s.first[4] >= (0x100000000LL >> 8)) return MUSC_ERR_UNSUPPORTED;
+  if (s.first[4] >= (0x100000000LL >> 10)) return MUSC_ERR_UNSUPPORTED;
   hipLaunchKernelGGL(mattn::row_work_kernel, dim3((unsigned)s.first[4]), dim3(kWave), 0, stream, documents, order,
                      reinterpret_cast<const int4*>(summary), s, schedule);
-  hipLaunchKernelGGL(mattn::row_order_kernel, dim3((unsigned)((s.first[4] + 255) / 256)), dim3(256), 0, stream, s,
+  hipLaunchKernelGGL(mattn::row_order_kernel, dim3((unsigned)batch * 4), dim3(1024), 0, stream, s,
                      schedule);
   return check_launch();
 }

@@ -19,7 +19,7 @@ _STORAGE = {torch.float32: rt.DTYPE_F32, torch.float16: rt.DTYPE_F16, torch.bflo
 SUMMARY_KEYS = 32
 ROW_TILE = 128
 SCHEDULE_GROUPS = (1, 2, 4, 8)
-SCHEDULE_MAX_TOKENS = 65536
+SCHEDULE_MAX_TOKENS = 16384
 
 
 class Tokens:

@@ -469,10 +469,52 @@ def bench_preprocess(args):
     return res
 
 
+def bench_packed_block(args):
+    """The norms, rotary positions and masked attention of one encoder block over --n images of
+    their own sizes (sides of 13 to 40 patches) packed into one sequence, 16 heads of 64."""
+    import random
+
+    from musc_hip import _layers_hip
+    from musc_hip._masked_attention_hip import Tokens, masked_attention
+    from musc_hip._rotary_hip import RotaryAxes, rotary
+    dev = torch.device('cuda:0')
+    dtype = torch.float16 if args.dtype == 'fp16' else torch.float32
+    rng = random.Random(2)
+    grids = [(rng.randint(13, 40), rng.randint(13, 40)) for _ in range(args.n)]
+    docs = torch.cat([torch.full((h * w,), i, dtype=torch.int32) for i, (h, w) in enumerate(grids)]).to(dev)
+    pos = torch.cat([torch.cartesian_prod(torch.arange(h), torch.arange(w)) for h, w in grids]).float().to(dev)
+    t, heads, d, width = len(docs), 16, 64, 1024
+    tokens, axes = Tokens(docs, positions=pos), RotaryAxes(d, (16, 16), base=100.0, device=dev)
+    slopes = (2.0 ** -torch.arange(1, heads + 1, device=dev).div(2)).unsqueeze(1).expand(heads, 2).contiguous()
+    x, r = (torch.randn((1, t, width), device=dev).to(dtype) for _ in range(2))
+    q, k, v = torch.randn((1, t, 3 * heads, d), device=dev).to(dtype).split(heads, 2)
+    weight = torch.ones(width, device=dev)
+    steps = {'rms_norm': lambda: _layers_hip.rms_norm(x, weight, 1e-6, residual=r),
+             'rms_norm_quantized': lambda: _layers_hip.rms_norm_quantized(x, weight, 1e-6, residual=r, group=128),
+             'rotary': lambda: rotary(q, k, pos, axes),
+             'masked_attention': lambda: masked_attention(q, k, v, 0.125, keys=tokens),
+             'masked_attention_biased': lambda: masked_attention(q, k, v, 0.125, keys=tokens, slopes=slopes)}
+    size, us = x.element_size(), {}
+    for name, step in steps.items():
+        for _ in range(3):
+            step()
+        e0, e1 = _events()
+        e0.record()
+        for _ in range(10 * args.iters):
+            step()
+        e1.record()
+        torch.cuda.synchronize()
+        us[name] = e0.elapsed_time(e1) * 1e3 / (10 * args.iters)
+    flop = 4.0 * heads * d * sum((h * w) ** 2 for h, w in grids)
+    return {'kernel': 'packed_block', 'dtype': args.dtype, 'images': args.n, 'tokens': t, 'us': us,
+            'masked_attention_tflops': flop / us['masked_attention'] / 1e6,
+            'rms_norm_gbps': 4 * size * t * width / us['rms_norm'] / 1e3, 'rotary_gbps': 4 * size * t * width / us['rotary'] / 1e3}
+
+
 def main():
     ap = argparse.ArgumentParser()
     ap.add_argument('kernels', nargs='+', choices=['msm', 'lnamd', 'super_fast', 'attention', 'copy', 'e2e',
-                                                     'mfma_peak', 'hbm', 'preprocess'])
+                                                     'mfma_peak', 'hbm', 'preprocess', 'packed_block'])
     ap.add_argument('--n', type=int, default=83)
     ap.add_argument('--p', type=int, default=1369)
     ap.add_argument('--c', type=int, default=1024)
@@ -491,7 +533,7 @@ def main():
     args = ap.parse_args()
     table = {'msm': bench_msm, 'lnamd': bench_lnamd, 'super_fast': bench_super_fast, 'attention': bench_attention,
              'copy': bench_copy, 'e2e': bench_e2e, 'mfma_peak': bench_mfma_peak, 'hbm': bench_hbm,
-             'preprocess': bench_preprocess}
+             'preprocess': bench_preprocess, 'packed_block': bench_packed_block}
     for name in args.kernels:
         print(json.dumps(table[name](args)), flush=True)
 

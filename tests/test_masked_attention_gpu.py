@@ -391,3 +391,45 @@ def test_refusals(device):
     wide = torch.zeros((1, 4, 1, 136), device=device, dtype=torch.float16)
     with pytest.raises(ValueError, match='head width'):
         masked_attention(wide, wide, wide, 1.0)
+
+
+@pytest.mark.parametrize('dtype', [torch.float16, torch.float32])
+@pytest.mark.parametrize('sizes', [[1000, 10, 20, 700, 5], [64] * 12 + [900], [3000]])
+@pytest.mark.parametrize('h,hk', [(2, 2), (4, 2), (8, 2), (16, 2), (6, 2)])
+def test_long_documents_among_short_ones(device, sizes, h, hk, dtype):
+    # row tiles in parts (few of them, of very different work), with 1, 2, 4, 8 and 3 heads a key head
+    docs = torch.repeat_interleave(torch.arange(len(sizes)), torch.tensor(sizes))
+    t = len(docs)
+    q, k, v = heads(device, dtype, 1, t, t, h, hk, 64)
+    pos = torch.arange(t).float()[:, None]
+    order = torch.arange(t)
+    slopes = torch.full((h, 1), 0.01)
+    tokens = Tokens(i32(docs, device), i32(order, device), pos.to(device))
+    got = masked_attention(q, k, v, 0.3, keys=tokens, slopes=slopes.to(device), cap=30.0)
+    rows = torch.randperm(t, generator=torch.Generator().manual_seed(1))[:300]
+    check(got[:, rows], q[:, rows], k, v, 0.3, seen=see(docs[rows], docs, order[rows], order), cap=30.0, slopes=slopes,
+          qpos=pos[rows][None], kpos=pos[None])
+    assert torch.equal(got, masked_attention(q, k, v, 0.3, keys=tokens, slopes=slopes.to(device), cap=30.0))
+    v[0, 5, 0, 3] = float('nan')          # seen by later rows of the first document only
+    got = masked_attention(q, k, v, 0.3, keys=tokens)
+    bad = torch.isnan(got).any(-1).any(-1)[0].cpu()
+    assert bad[5:sizes[0]].all() and not bad[:5].any() and not bad[sizes[0]:].any()
+
+
+def test_schedule_is_a_permutation(device):
+    for sizes in ([1], [128], [129, 300, 4], [2000] + [10] * 100, [16384]):
+        docs = i32(torch.repeat_interleave(torch.arange(len(sizes)), torch.tensor(sizes)), device)
+        tokens = Tokens(docs)
+        at = 0
+        for group in (1, 2, 4, 8):
+            n = -(-len(docs) * group // 128)
+            block = tokens._schedule[at:at + 4 + 3 * n + (9 * n + 4) // 5].cpu()
+            at += len(block)
+            work, order, first, jobs = block[4:4 + n], block[4 + n:4 + 2 * n], block[4 + 2 * n:4 + 3 * n], block[4 + 3 * n:]
+            assert sorted(order.tolist()) == list(range(n)) and (work[order.long()].diff() <= 0).all()
+            jobs = jobs[:block[0]].tolist()
+            parts = [x >> 24 for x in first.tolist()]
+            assert sum(parts) == len(jobs) and max(parts) <= 8
+            for tile, x in enumerate(first.tolist()):
+                assert jobs[x & 0xffffff:(x & 0xffffff) + (x >> 24)] == [
+                    tile | p << 20 | ((x >> 24) - 1) << 23 for p in range(x >> 24)]

@@ -137,7 +137,7 @@ def test_token_summary(lib, args, code):
     (dict(documents=None), INVALID), (dict(summary=None), INVALID), (dict(schedule=None), INVALID), (dict(schedule=ctypes.c_void_p(4098)), INVALID),
     (dict(batch=-1), INVALID), (dict(t=-1), INVALID), (dict(summary=ctypes.c_void_p(4104)), INVALID),
     (dict(order=ctypes.c_void_p(4098)), INVALID), (dict(batch=0), OK), (dict(t=0), OK),
-    (dict(batch=1 << 12, t=1 << 16), UNSUPPORTED), (dict(t=65537), UNSUPPORTED)])
+    (dict(batch=1 << 14, t=1 << 14), UNSUPPORTED), (dict(t=16385), UNSUPPORTED)])
 def test_token_schedule(lib, change, code):
     a = dict(documents=P, order=None, summary=P, batch=1, t=64, schedule=P, stream=None)
     a.update(change)
