@@ -161,7 +161,8 @@ int plan(const musc_masked_attention& c, Args& a, int& waves) {
     const long long enough = (128 + a.row_tiles - 1) / a.row_tiles, per_xcd = heads / kXcds;
     a.heads_at_once = (int)(enough < per_xcd ? enough : per_xcd);
   }
-  if (a.units >= (0x100000000LL >> 8)) return MUSC_ERR_UNSUPPORTED;  // 256 threads each in one grid dimension
+  // a grid dimension holds fewer than 2^32 threads, 256 or (teams) up to 512 a workgroup
+  if (a.units >= (0x100000000LL >> (a.teams > 1 ? 9 : 8))) return MUSC_ERR_UNSUPPORTED;
   return MUSC_OK;
 }
 

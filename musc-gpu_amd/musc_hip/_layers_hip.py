@@ -83,6 +83,8 @@ def _rms(x, weight, eps, residual, dtype, group):
     rt.require_no_gradient(x, weight, residual)
     width = x.shape[-1]
     rows = x.numel() // width
+    if rows > 0x7fffffff:
+        raise ValueError('x has more than 2^31 - 1 rows')
     w_ptr, w_dtype = None, rt.DTYPE_F32
     if weight is not None:
         rt.require_device_tensor(weight, 'weight')

@@ -4,7 +4,7 @@ The fused block attention of _attention_hip sees every token of one image; here 
 the keys of its own document (an image of a packed batch, the live part of a padded one) whose
 order is not past its own (a prefix, a causal text, the frames of a clip), and the scores may
 be capped by a tanh and lowered with the distance of two tokens.  The reference's blocks pass
-masks to torch's math path (models/backbone/open_clip/transformer.py:228-234); nothing here
+masks to torch's math path (models/backbone/open_clip/transformer.py:232-234); nothing here
 writes the logits or a mask to memory.
 """
 from __future__ import annotations
@@ -75,7 +75,7 @@ class Tokens:
 
     def refresh(self) -> None:
         """Summarises the keys again, on the current stream, after a change of documents or order."""
-        if self.summary is None:
+        if self.summary is None or not self.summary.numel():
             return
         docs = self.documents
         with torch.cuda.device(docs.device):
@@ -124,7 +124,8 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: f
     keys, queries: the Tokens of both sides; queries defaults to keys (self-attention), no keys at
     all lets every query see every key.  A query that sees no key gets zeros.
     cap > 0: scores become cap tanh(score / cap) before the bias.  slopes: float32 (heads, axes),
-    needs positions on both sides.  No backward pass."""
+    needs positions on both sides.  out: the tensor to write, rows on 16 bytes; it may not overlap q, k
+    or v.  No backward pass."""
     for name, x in (('q', q), ('k', k), ('v', v)):
         rt.require_device_tensor(x, name)
         if x.dim() != 4:

@@ -1,8 +1,8 @@
 """Rotary positions with several axes (time, height, width) on MI355X (libmusc_hip musc_rotary).
 
 For encoders of images and video of any size, whose blocks turn q and k by the token's place
-instead of adding a position embedding of one grid (the reference's encoder has only the
-latter, models/backbone/open_clip/transformer.py:391-398).  q and k are read in place from a
+instead of adding a position embedding of one grid (the reference's encoder does the latter).
+q and k are read in place from a
 packed projection; all heads of a token share its angles, whose whole turns are taken off in
 float64.
 """

@@ -367,6 +367,17 @@ def test_two_streams_and_threads(device):
             assert torch.equal(a, want[0]) and torch.equal(b, want[1])
 
 
+def test_no_tokens(device):
+    empty = Tokens(torch.zeros((0,), dtype=torch.int32, device=device), torch.zeros((0,), dtype=torch.int32, device=device))
+    q, k, v = (x.half().to(device) for x in torch.zeros((3, 2, 0, 4, 64)))
+    assert masked_attention(q, k, v, 1.0, keys=empty).shape == (2, 0, 4, 64)
+    one = torch.ones((2, 3, 4, 64), dtype=torch.float16, device=device)
+    docs = i32([0, 0, 0], device)
+    side = Tokens(docs, docs, queries_only=True)
+    assert (masked_attention(one, k, v, 1.0, keys=empty, queries=side) == 0).all()
+    assert masked_attention(one[:0], one[:0], one[:0], 1.0, keys=Tokens(docs)).shape == (0, 3, 4, 64)
+
+
 def test_refusals(device):
     q, k, v = heads(device, torch.float16, 1, 4, 4, 2, 2, 64)
     docs = i32([0, 0, 1, 1], device)
