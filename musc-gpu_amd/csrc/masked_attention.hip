@@ -139,10 +139,12 @@ int plan(const musc_masked_attention& c, Args& a, int& waves) {
   if (waves == 1 && a.key_tiles <= kTeamTiles * teams) a.teams = teams;
   if (a.teams > 1) {
   } else if (waves > 1 && c.schedule) {
-    // Long row tiles in parts where all begin at once and the longest ends last: 4 packed images,
-    // fp32 (416 row tiles, 512 places), 204 -> 144 us; with more row tiles than places short ones
-    // fill up behind long ones (12 packed images, fp16, 1184 for 768: 106 us whole, 110 in parts).
-    a.in_parts = whole < a.slots;
+    // Long row tiles in parts where all begin at once, so that the longest ends last, and are long
+    // enough to pay for a join: 4 packed images, fp32 (416 row tiles, 512 places), 204 -> 144 us; three
+    // documents of 2000, 1000 and 1000 tokens, 8 heads, fp16, bias, 102 -> 76 us, but of 500 tokens in
+    // all 23 -> 28.  With more row tiles than places short ones fill up behind long ones (12 packed
+    // images, fp16, 1184 for 768: 106 us whole, 110 in parts).
+    a.in_parts = whole < a.slots && (c.dtype == MUSC_DTYPE_F32 || c.k_len >= 2048);
     if (a.in_parts) a.jobs = (int)schedule_jobs(a.row_tiles);
   } else if (whole < (waves == 1 ? 1024 : 256)) {
     // few rows: their keys in splits of at least one tile (4 where four waves share the tiles)

@@ -2,9 +2,8 @@
 
 For encoders of images and video of any size, whose blocks turn q and k by the token's place
 instead of adding a position embedding of one grid (the reference's encoder does the latter).
-q and k are read in place from a
-packed projection; all heads of a token share its angles, whose whole turns are taken off in
-float64.
+q and k are read in place from a packed projection; all heads of a token share its angles, whose
+whole turns are taken off in float64.
 """
 from __future__ import annotations
 
@@ -42,8 +41,11 @@ class RotaryAxes:
                 turns.append(float(base) ** -exponent / (2 * math.pi))
                 axis.append(a)
         self.head_dim, self.pairs, self.axes, self.adjacent = int(head_dim), pairs, len(sections), bool(adjacent)
-        self.frequency = torch.tensor(turns, dtype=torch.float64, device=device)
-        self.axis = torch.tensor(axis, dtype=torch.int32, device=device)
+        both = torch.zeros(2 * pairs, dtype=torch.float64)       # one copy to the device for the two
+        both[:pairs] = torch.tensor(turns, dtype=torch.float64)
+        both[pairs:].view(torch.int32)[:pairs] = torch.tensor(axis, dtype=torch.int32)
+        both = both.to(device)
+        self.frequency, self.axis = both[:pairs], both[pairs:].view(torch.int32)[:pairs]
         self.frequency_ptr, self.axis_ptr = self.frequency.data_ptr(), self.axis.data_ptr()
 
 

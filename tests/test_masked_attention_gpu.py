@@ -405,7 +405,7 @@ def test_refusals(device):
 
 
 @pytest.mark.parametrize('dtype', [torch.float16, torch.float32])
-@pytest.mark.parametrize('sizes', [[1000, 10, 20, 700, 5], [64] * 12 + [900], [3000]])
+@pytest.mark.parametrize('sizes', [[1000, 10, 20, 700, 5], [64] * 12 + [900], [1800, 400, 30], [3000]])
 @pytest.mark.parametrize('h,hk', [(2, 2), (4, 2), (8, 2), (16, 2), (6, 2)])
 def test_long_documents_among_short_ones(device, sizes, h, hk, dtype):
     # row tiles in parts (few of them, of very different work), with 1, 2, 4, 8 and 3 heads a key head
