@@ -10,6 +10,9 @@ include/musc_hip.h); nothing here computes on the CPU.
   _aggregation_cache.RadiusAggregationCache     per-division statistics reuse
   _epilogue_hip.maps_and_scores                 layer/radius means, upsampling, image scores
   pipeline.score_pool                           tokens -> maps + image scores, fused
+  _layers_hip.rms_norm, rms_norm_quantized      root-mean-square norm of packed encoders, 8-bit output
+  _rotary_hip.RotaryAxes, rotary                rotary positions over several axes
+  _masked_attention_hip.Tokens, masked_attention  packed images, padded rows, prefixes, caches
 """
 from ._backend import configure_backend, select_backend  # noqa: F401
 
