@@ -108,7 +108,7 @@ def _heads(x, per):
     strides = rt.token_strides(x)
     if x.stride(3) == 1 and not x.data_ptr() % 16 and not (strides[0] | strides[1] | strides[2]) % per:
         return x, strides
-    x = x.contiguous()
+    x = x.clone(memory_format=torch.contiguous_format)  # also where it is contiguous and starts off 16 bytes
     return x, rt.token_strides(x)
 
 

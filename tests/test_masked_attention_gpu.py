@@ -287,6 +287,14 @@ def test_layouts(device, dtype):
     check(masked_attention(turned, one, v, 0.125), turned, one, v, 0.125)
 
 
+def test_contiguous_inputs_off_16_bytes(device):
+    b, t, h, d = 2, 40, 3, 64
+    g = torch.Generator().manual_seed(18)
+    flat = torch.randn(3 * b * t * h * d + 4, generator=g).to(torch.float16).to(device)
+    q, k, v = (flat[1 + i + i * b * t * h * d:][:b * t * h * d].view(b, t, h, d) for i in range(3))
+    check(masked_attention(q, k, v, 0.125), q, k, v, 0.125)
+
+
 @pytest.mark.parametrize('dtype', [torch.float16, torch.float32])
 def test_agrees_with_unmasked_attention(device, dtype):
     from musc_hip import _attention_hip
