@@ -133,7 +133,7 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: f
     if rt.elsewhere(q):
         with torch.cuda.device(q.device):
             return masked_attention(q, k, v, scale, keys, queries, cap, slopes, out)
-    rt.require_no_gradient(q, k, v, slopes)
+    rt.require_no_gradient(q, k, v, slopes, out)
     dtype, index = q.dtype, q.get_device()
     if dtype not in _STORAGE:
         raise ValueError('q must be float32, float16 or bfloat16')
@@ -171,6 +171,7 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: f
         kpos, qpos = keys.positions, queries.positions
         if kpos is None or qpos is None:
             raise ValueError('slopes need positions of keys and queries')
+        rt.require_no_gradient(kpos, qpos)
         axes = kpos.shape[-1]
         rt.require_device_tensor(slopes, 'slopes')
         if (slopes.dtype != torch.float32 or slopes.get_device() != index or qpos.shape[-1] != axes

@@ -68,7 +68,7 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, axe
     if rt.elsewhere(q):
         with torch.cuda.device(q.device):
             return rotary(q, k, positions, axes, inverse, out)
-    rt.require_no_gradient(q, k)
+    rt.require_no_gradient(q, k, positions, *(out if isinstance(out, (tuple, list)) else (out,)))
     index = q.get_device()
     b, t, h, d = q2.shape
     k2, ko, k_heads, k_args = None, None, 0, (0, 0, 0, 0, 0, 0, 0, 0)

@@ -287,6 +287,17 @@ def test_layouts(device, dtype):
     check(masked_attention(turned, one, v, 0.125), turned, one, v, 0.125)
 
 
+def test_refuses_gradients_of_positions_and_out(device):
+    q, k, v = heads(device, torch.float16, 1, 4, 4, 2, 2, 64)
+    pos, slopes = torch.zeros((4, 1), device=device, requires_grad=True), torch.ones((2, 1), device=device)
+    with pytest.raises(ValueError, match='backward'):
+        masked_attention(q, k, v, 1.0, keys=Tokens(positions=pos), slopes=slopes)
+    with pytest.raises(ValueError, match='backward'):
+        masked_attention(q, k, v, 1.0, out=torch.empty_like(q).requires_grad_())
+    with torch.no_grad():
+        masked_attention(q, k, v, 1.0, keys=Tokens(positions=pos), slopes=slopes)
+
+
 def test_contiguous_inputs_off_16_bytes(device):
     b, t, h, d = 2, 40, 3, 64
     g = torch.Generator().manual_seed(18)

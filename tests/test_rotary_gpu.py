@@ -172,3 +172,13 @@ def test_refusals(device):
             RotaryAxes(64, bad, device=device)
     with pytest.raises(RuntimeError, match='implemented range'):
         rotary(torch.zeros((1, 1, 1, 1024), device=device), None, pos[:1], RotaryAxes(1024, (4, 4), device=device))
+
+
+def test_refuses_gradients_of_positions_and_out(device):
+    q, pos = torch.zeros((1, 4, 2, 64), device=device), torch.zeros((4, 2), device=device)
+    axes = RotaryAxes(64, (16, 16), device=device)
+    for out in (torch.empty_like(q).requires_grad_(), None):
+        with pytest.raises(ValueError, match='backward'):
+            rotary(q, None, pos if out is not None else pos.clone().requires_grad_(), axes, out=out)
+    with pytest.raises(ValueError, match='backward'):
+        rotary(q, q.clone(), pos, axes, out=(torch.empty_like(q), torch.empty_like(q).requires_grad_()))
