@@ -99,4 +99,6 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, axe
             0 if len(shape) == 2 else t * axes.axes, axes.frequency_ptr, axes.axis_ptr, h, k_heads, _STORAGE[q2.dtype], b, t,
             d, positions.dtype == torch.int32, axes.axes, axes.pairs, axes.adjacent, inverse)
         rt.check(rt.library().musc_rotary(call, rt.current_stream(index)), 'musc_rotary')
+    elif k_heads:
+        rotary(k2, None, positions, axes, inverse, ko)
     return qo if k is None else (qo, ko)

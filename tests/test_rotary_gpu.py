@@ -182,3 +182,12 @@ def test_refuses_gradients_of_positions_and_out(device):
             rotary(q, None, pos if out is not None else pos.clone().requires_grad_(), axes, out=out)
     with pytest.raises(ValueError, match='backward'):
         rotary(q, q.clone(), pos, axes, out=(torch.empty_like(q), torch.empty_like(q).requires_grad_()))
+
+
+def test_keys_without_queries(device):
+    q, k = normal((2, 5, 0, 64), torch.float16, 12, device), normal((2, 5, 3, 64), torch.float16, 13, device)
+    pos = torch.arange(10).float().view(5, 2)
+    axes = RotaryAxes(64, (16, 16), device=device)
+    q_out, k_out = rotary(q, k, pos.to(device), axes)
+    assert q_out.shape == q.shape
+    check(k_out, k, pos, (16, 16), 10000.0, False, False)
