@@ -20,6 +20,7 @@ SUMMARY_KEYS = 32
 ROW_TILE = 128
 SCHEDULE_GROUPS = (1, 2, 4, 8)
 SCHEDULE_MAX_TOKENS = 16384
+SCHEDULE_MAX_TILES = 1 << 22   # of all batch entries; more run unscheduled
 
 
 class Tokens:
@@ -64,9 +65,9 @@ class Tokens:
         if documents is not None and not queries_only:
             b, t = documents.shape if documents.dim() == 2 else (1, documents.shape[0])
             self.summary = torch.empty((b, -(-t // SUMMARY_KEYS), 4), dtype=torch.int32, device=documents.device)
-            if 0 < t <= SCHEDULE_MAX_TOKENS:
-                # blocks for 1, 2, 4 and 8 query heads per key head, of n row groups each
-                tiles = [-(-t * group // ROW_TILE) for group in SCHEDULE_GROUPS]
+            # blocks for 1, 2, 4 and 8 query heads per key head, of n row groups each
+            tiles = [-(-t * group // ROW_TILE) for group in SCHEDULE_GROUPS]
+            if 0 < t <= SCHEDULE_MAX_TOKENS and b * sum(tiles) < SCHEDULE_MAX_TILES:
                 blocks = [4 + 3 * n + (9 * n + 4) // 5 for n in tiles]
                 self._schedule = torch.empty((b * sum(blocks),), dtype=torch.int32, device=documents.device)
                 self._schedule_of = {group: (self._schedule.data_ptr() + 4 * b * sum(blocks[:i]), blocks[i])

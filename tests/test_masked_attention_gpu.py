@@ -298,6 +298,15 @@ def test_refuses_gradients_of_positions_and_out(device):
         masked_attention(q, k, v, 1.0, keys=Tokens(positions=pos), slopes=slopes)
 
 
+def test_more_batch_entries_than_a_schedule_takes(device):
+    b = (1 << 20) + 5                                            # one token each: its output is its value
+    docs = torch.zeros((b, 1), dtype=torch.int32, device=device)
+    docs[::3] = -1
+    v = torch.randn((b, 1, 1, 8), device=device).half()
+    out = masked_attention(v, v, v, 1.0, keys=Tokens(docs))
+    assert torch.equal(out, v * (docs >= 0)[..., None, None])
+
+
 def test_contiguous_inputs_off_16_bytes(device):
     b, t, h, d = 2, 40, 3, 64
     g = torch.Generator().manual_seed(18)
