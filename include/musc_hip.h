@@ -378,7 +378,8 @@ int musc_layernorm_rows(const void* x, const void* residual, void* sum_out,
  *   score(i, j) = c(scale q_i . k_j) - sum_a slopes[head][a] |q_position[i][a] - k_position[j][a]|
  *   c(s) = cap tanh(s / cap) for cap > 0, else s
  *   seen(i, j) = document(i) == document(j), both >= 0, and order(j) <= order(i)
- *   out_i = softmax over the seen keys of score(i, .) times V; zeros where none is seen.
+ *   out_i = softmax over the seen keys of score(i, .) times V; zeros where none is seen, or where
+ *   all seen scores are minus infinity.
  * fp32 scores, softmax statistics and accumulation; the probabilities are rounded to 16-bit
  * types for their product with V.  What unseen keys hold (infinities and NaN among it) has no
  * effect.  No other call's result depends on it, and nothing is kept between calls. */

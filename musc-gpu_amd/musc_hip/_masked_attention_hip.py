@@ -123,7 +123,8 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: f
     float16 or bfloat16, D up to 128 in steps of 16 bytes; views of a packed projection are read
     in place where each row starts on 16 bytes, and copied otherwise.
     keys, queries: the Tokens of both sides; queries defaults to keys (self-attention), no keys at
-    all lets every query see every key.  A query that sees no key gets zeros.
+    all lets every query see every key.  A query that sees no key gets zeros, as does one whose seen
+    scores are all minus infinity.
     cap > 0: scores become cap tanh(score / cap) before the bias.  slopes: float32 (heads, axes),
     needs positions on both sides.  out: the tensor to write, rows on 16 bytes; it may not overlap q, k
     or v.  No backward pass."""

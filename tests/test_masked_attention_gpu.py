@@ -307,6 +307,17 @@ def test_more_batch_entries_than_a_schedule_takes(device):
     assert torch.equal(out, v * (docs >= 0)[..., None, None])
 
 
+@pytest.mark.parametrize('tq,tk', [(1, 40), (1, 5000), (200, 200)])
+def test_scores_of_minus_infinity(device, tq, tk):
+    q, k, v = heads(device, torch.float16, 1, tq, tk, 1, 1, 64)
+    q[..., 0] = 1.0
+    q[0, 0, 0, 0] = 0.5
+    k[0, :, 0, 0] = float('-inf')
+    assert (masked_attention(q, k, v, 0.125) == 0).all()
+    k[0, tk // 2, 0, 0] = 0.0                                    # one key left: its value
+    assert torch.equal(masked_attention(q, k, v, 0.125), v[:, tk // 2:tk // 2 + 1].expand(1, tq, 1, 64))
+
+
 def test_contiguous_inputs_off_16_bytes(device):
     b, t, h, d = 2, 40, 3, 64
     g = torch.Generator().manual_seed(18)
