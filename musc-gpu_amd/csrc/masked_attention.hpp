@@ -33,7 +33,7 @@
 // reciprocal), 256 of each kind with a bias over two axes; the two kinds run beside one another
 // little.  16 frames of 1024 patches, 16 heads of 128, bf16: 1075 us, 1.09 PFLOP/s, a product of
 // 8192^3 1.14.  8192 tokens, 16 heads of 64, fp16: 340 us, 0.81 PFLOP/s; with a bias over two axes
-// 460, with a cap 440 us.  A single token over 32768 keys: HBM, 5.1 TB/s of the 5.2 of a large copy.
+// 475, with a cap 450 us.  Single tokens over long caches: HBM, at the 5.2 TB/s of a large copy.
 // fp32: its matrix instructions, 127 TFLOP/s of the 153 of a product of 8192^3.
 #pragma once
 
