@@ -415,8 +415,8 @@ typedef struct musc_masked_attention {
  * (batch, ceil(t / 32), 4).  Made again when a document or order changes. */
 int musc_token_summary(const int* documents, const int* order, int batch, int t, int* summary, hipStream_t stream);
 /* Schedules of self-attention over these tokens (its groups of 128 (token, head) rows, those that
- * see most keys first, and long ones in parts) for heads / kv_heads = 1, 2, 4 and 8 one after the
- * other: batch blocks of 4 + 3 n + (9 n + 4) / 5 int32 each, n = ceil(t * heads / kv_heads / 128).  Made again when a
+ * see most keys first, long ones in parts, and those of two documents in two) for heads / kv_heads = 1, 2, 4 and 8 one after the
+ * other: batch blocks of 4 + 5 n + (9 n + 4) / 5 + n / 4 int32 each, n = ceil(t * heads / kv_heads / 128).  Made again when a
  * document or order changes.  t up to MUSC_SCHEDULE_MAX_TOKENS (MUSC_ERR_UNSUPPORTED beyond: so many
  * row groups need no schedule). */
 #define MUSC_SCHEDULE_MAX_TOKENS 16384

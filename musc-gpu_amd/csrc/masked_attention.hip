@@ -40,43 +40,72 @@ struct Schedule {
   __device__ __forceinline__ int which(long long i) const { return (i >= first[1]) + (i >= first[2]) + (i >= first[3]); }
 };
 
-// Work of each row tile: the groups of 32 keys that its rows may see.  One wave per tile.
+// Work of each row tile: the groups of 32 keys that its rows may see; and the document's start or end
+// within it whose two sides have the least work each, if that is at most 3/4.  One wave per tile.
 __global__ __launch_bounds__(kWave) void row_work_kernel(const int* __restrict__ documents, const int* __restrict__ order,
                                                          const int4* __restrict__ summary, const Schedule s,
                                                          int* __restrict__ out) {
   const int w = s.which(blockIdx.x), lane = threadIdx.x;
   const int i = (int)(blockIdx.x - s.first[w]), b = i / s.tiles[w], tile = i % s.tiles[w];
   const int first = tile * (kRowTile >> w), last = min(first + (kRowTile >> w), s.t) - 1;
-  Range r = {0x7fffffff, -1, 0x7fffffff, (int)0x80000000};
-  for (int k = first + lane; k <= last; k += kWave) {
-    const int doc = documents[(long long)b * s.t + k], ord = order ? order[(long long)b * s.t + k] : 0;
-    if (doc < 0) continue;
-    r = Range{min(r.dmin, doc), max(r.dmax, doc), min(r.omin, ord), max(r.omax, ord)};
-  }
-  r = Range{wave_min_int(r.dmin), wave_max_int(r.dmax), wave_min_int(r.omin), wave_max_int(r.omax)};
-  int count = 0;
-  for (int g = lane; g < s.groups; g += kWave) {
-    const int4 k = summary[(long long)b * s.groups + g];
-    count += k.y >= 0 && k.x <= r.dmax && k.y >= r.dmin && k.z <= r.omax;
-  }
+  int* block = out + s.at[w] + b * schedule_block(s.tiles[w]);
+  const int* docs = documents + (long long)b * s.t;
+  const int4* keys = summary + (long long)b * s.groups;
+  // groups that some token of from .. to - 1 may see
+  auto work = [&](int from, int to) {
+    Range r = {0x7fffffff, -1, 0x7fffffff, (int)0x80000000};
+    for (int k = from + lane; k < to; k += kWave) {
+      const int doc = docs[k], ord = order ? order[(long long)b * s.t + k] : 0;
+      if (doc < 0) continue;
+      r = Range{min(r.dmin, doc), max(r.dmax, doc), min(r.omin, ord), max(r.omax, ord)};
+    }
+    r = Range{wave_min_int(r.dmin), wave_max_int(r.dmax), wave_min_int(r.omin), wave_max_int(r.omax)};
+    int count = 0;
+    for (int g = lane; g < s.groups; g += kWave) {
+      const int4 k = keys[g];
+      count += k.y >= 0 && k.x <= r.dmax && k.y >= r.dmin && k.z <= r.omax;
+    }
 #pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) count += __shfl_xor(count, off, kWave);
-  if (lane == 0) out[s.at[w] + b * schedule_block(s.tiles[w]) + kScheduleHead + tile] = count;
+    for (int off = 32; off >= 1; off >>= 1) count += __shfl_xor(count, off, kWave);
+    return count;
+  };
+  const int count = work(first, last + 1);
+  // the end of the first document and the start of the last one: where a cut may halve the work
+  int ends = last + 1, starts = first;
+  for (int k = first + lane; k <= last; k += kWave) {
+    if (docs[k] != docs[first]) ends = min(ends, k);
+    if (docs[k] != docs[last]) starts = max(starts, k + 1);
+  }
+  ends = wave_min_int(ends), starts = wave_max_int(starts);
+  int cut = 0, least = count * 3 / 4;
+  if (ends <= last)
+    for (int i = 0; i < (ends == starts ? 1 : 2); ++i) {
+      const int at = i == 0 ? ends : starts, before = work(first, at), from = work(at, last + 1);
+      if (max(before, from) > least) continue;
+      least = max(before, from);
+      cut = (at - first) << w | before << 7 | from << 17;
+    }
+  if (lane == 0) block[kScheduleHead + 3 * s.tiles[w] + schedule_jobs(s.tiles[w]) + tile] = cut;
+  if (lane == 0) block[kScheduleHead + tile] = count;
 }
 
 // The row tiles by their work, most first (later ones first where it is the same): whole, and as
 // jobs, where a tile of more than 5/4 of the mean work is listed in up to 8 parts, by the work of a
-// part.  At most 9/5 n jobs.
+// part.  At most 9/5 n jobs.  And in pieces: the tiles of the most work, above the mean and n / 4 of them
+// at most, cut where row_work_kernel found it worth while.
 // One workgroup per schedule.  Every row tile finds its place by looking at all of them in LDS: 1024
 // tiles, 1024 threads.
 constexpr int kMostTiles = MUSC_SCHEDULE_MAX_TOKENS * 8 / kRowTile;
 __global__ __launch_bounds__(1024) void row_order_kernel(const Schedule s, int* __restrict__ out) {
   __shared__ int2 tiles[kMostTiles];  // work, work of a part * 8 + parts - 1
+  __shared__ int cut[kMostTiles];     // of the cuts, first those worth while, then the n / 4 most
   __shared__ long long sums[16];
   __shared__ int counts[16];
   const int w = blockIdx.x % 4, b = blockIdx.x / 4, n = s.tiles[w], lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
   int* block = out + s.at[w] + b * schedule_block(n);
   const int* work = block + kScheduleHead;
+  const int* cuts = block + kScheduleHead + 3 * n + schedule_jobs(n);
+  int* pieces = block + kScheduleHead + 4 * n + schedule_jobs(n);
   double total = 0;  // whole numbers below 2^53
   for (int j = threadIdx.x; j < n; j += 1024) total += work[j];
   total = wave_sum(total);
@@ -90,20 +119,40 @@ __global__ __launch_bounds__(1024) void row_order_kernel(const Schedule s, int* 
     const int x = work[j], parts = min(max((x + most - 1) / most, 1), kMaxParts);
     tiles[j] = make_int2(x, (x + parts - 1) / parts * 8 + parts - 1);
     jobs_here += parts;
+    cut[j] = (long long)x * n > all_work ? cuts[j] : 0;
   }
   jobs_here = wave_sum(jobs_here);
   if (lane == 0) counts[wave] = (int)jobs_here;
   __syncthreads();
+  static_assert(kMostTiles <= 1024, "one row tile per thread");
+  int mine = threadIdx.x < n ? cut[threadIdx.x] : 0, more = 0;
+  if (mine)
+    for (int j = 0; j < n; ++j)
+      more += cut[j] && (tiles[j].x > tiles[threadIdx.x].x || (tiles[j].x == tiles[threadIdx.x].x && j > (int)threadIdx.x));
+  if (more >= n / 4) mine = 0;
+  __syncthreads();
+  if (threadIdx.x < n) cut[threadIdx.x] = mine;
+  const float cut_here = wave_sum(mine ? 1.f : 0.f);
+  if (lane == 0) sums[wave] = (long long)cut_here;
+  __syncthreads();
   for (int tile = threadIdx.x; tile < n; tile += 1024) {
     const int2 here = tiles[tile];
     const int size = here.y >> 3, parts = (here.y & 7) + 1;
-    int rank = 0, first = 0;
+    // this tile's pieces: all of it, or its rows before the cut and those from it on
+    const int at = cut[tile] & 127, before = at ? (cut[tile] >> 7) & 1023 : here.x, from = cut[tile] >> 17;
+    int rank = 0, first = 0, rank_before = at && from >= before, rank_from = at && before > from;
     for (int j = 0; j < n; ++j) {
       const int2 x = tiles[j];
       const int each = x.y >> 3;
       rank += x.x > here.x || (x.x == here.x && j > tile);
       first += each > size || (each == size && j > tile) ? (x.y & 7) + 1 : 0;
+      if (j == tile) continue;
+      const int x_from = cut[j] ? cut[j] >> 17 : -1, x_before = cut[j] ? (cut[j] >> 7) & 1023 : x.x, later = j > tile;
+      rank_before += (x_before + later > before) + (x_from + later > before);
+      rank_from += (x_before + later > from) + (x_from + later > from);
     }
+    pieces[rank_before] = tile | (at ? at - 1 : kRowTile - 1) << 17;
+    if (at) pieces[rank_from] = tile | at << 10 | (kRowTile - 1) << 17;
     block[kScheduleHead + n + rank] = tile;
     block[kScheduleHead + 2 * n + tile] = first | parts << 24;
     int* jobs = block + kScheduleHead + 3 * n + first;
@@ -111,8 +160,9 @@ __global__ __launch_bounds__(1024) void row_order_kernel(const Schedule s, int* 
   }
   if (threadIdx.x == 0) {
     int jobs = 0;
-    for (int i = 0; i < 16; ++i) jobs += counts[i];
-    block[0] = jobs;
+    long long cut_tiles = 0;
+    for (int i = 0; i < 16; ++i) jobs += counts[i], cut_tiles += sums[i];
+    block[0] = jobs, block[1] = n + (int)cut_tiles;
   }
 }
 
@@ -131,7 +181,7 @@ int plan(const musc_masked_attention& c, Args& a, int& waves) {
   const long long heads = (long long)c.batch * c.kv_heads, whole = heads * a.row_tiles;
   // workgroups that the card holds at a time
   a.slots = waves == 1 ? 1024 : c.dtype != MUSC_DTYPE_F32 && c.d <= 64 ? 768 : 512;
-  a.splits = 1, a.jobs = a.row_tiles, a.in_parts = 0, a.teams = 1;
+  a.splits = 1, a.jobs = a.row_tiles, a.in_parts = 0, a.in_pieces = 0, a.teams = 1;
   // Few rows over up to 2048 keys (1024 of wide heads): the waves of one workgroup share them and
   // join in LDS, without a second launch.  One row, 1369 keys, 16 heads of 64: 17.1 us in
   // workgroups of one wave and a join, 12.9 us so, host time included.
@@ -146,6 +196,8 @@ int plan(const musc_masked_attention& c, Args& a, int& waves) {
     // images, fp16, 1184 for 768: 106 us whole, 110 in parts).
     a.in_parts = whole < a.slots && (c.dtype == MUSC_DTYPE_F32 || c.k_len >= 2048);
     if (a.in_parts) a.jobs = (int)schedule_jobs(a.row_tiles);
+    a.in_pieces = !a.in_parts && !c.q_order && whole < 4LL * a.slots;
+    if (a.in_pieces) a.jobs = (int)schedule_pieces(a.row_tiles);
   } else if (whole < (waves == 1 ? 1024 : 256)) {
     // few rows: their keys in splits of at least one tile (4 where four waves share the tiles)
     long long splits = ((waves == 1 ? 2048 : 512) + whole - 1) / whole;

@@ -66,11 +66,15 @@ constexpr int kRowTile = 128;  // rows of a workgroup of four waves
 // keys each in 128 KiB of LDS.
 constexpr int teams_of(int pitch) { return 131072 / (4 * 32 * pitch); }
 constexpr int kTeamTiles = 8;  // tiles of such a wave at most
-// Schedule of n row tiles, in ints: head (jobs), work (n), row tiles by their work (n), first job
-// | parts << 24 of each row tile (n), jobs (row tile | part << 20 | (parts - 1) << 23).
+// Schedule of n row tiles, in ints: head (jobs, pieces), work (n), row tiles by their work (n), first
+// job | parts << 24 of each row tile (n), jobs (row tile | part << 20 | (parts - 1) << 23), cuts (n: row |
+// work before it << 7 | work from it on << 17, or 0), pieces (row tile | first row << 10 | last row << 17).
 constexpr int kScheduleHead = 4, kMaxParts = 8;
 __host__ __device__ inline long long schedule_jobs(long long n) { return (9 * n + 4) / 5; }
-__host__ __device__ inline long long schedule_block(long long n) { return kScheduleHead + 3 * n + schedule_jobs(n); }
+__host__ __device__ inline long long schedule_pieces(long long n) { return n + n / 4; }
+__host__ __device__ inline long long schedule_block(long long n) {
+  return kScheduleHead + 4 * n + schedule_jobs(n) + schedule_pieces(n);
+}
 
 template <int kDtype>
 struct Type;
@@ -131,6 +135,7 @@ struct Args {
   int group, rows, row_tiles, key_tiles, splits, summaries, heads_at_once;
   int jobs;      // workgroups of a head and split: its row tiles, or the schedule's jobs
   int in_parts;  // jobs may be parts of a row tile's keys
+  int in_pieces; // jobs may be the rows of a row tile before or from a document's start on
   int teams;     // waves that share few rows' keys within a workgroup
   int slots;     // workgroups that the card holds at a time
   long long units;

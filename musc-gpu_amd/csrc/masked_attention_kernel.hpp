@@ -110,6 +110,7 @@ __global__ __launch_bounds__(kWaves * kTeams * kWave, kWaves == 1 ? 1 : kD == 64
   // with an order of tokens they see more keys, and the longest work should not start last
   constexpr bool in_parts = (kMode & kInParts) != 0;
   int tile_of_rows = a.row_tiles - 1 - (int)job, part = team, parts = kTeams;
+  int first_row = 0, last_row = kRowTile - 1;
   if (kWaves > 1 && c.schedule) {
     const int* schedule = c.schedule + b * c.schedule_sb;
     if constexpr (in_parts) {
@@ -119,12 +120,18 @@ __global__ __launch_bounds__(kWaves * kTeams * kWave, kWaves == 1 ? 1 : kD == 64
       part = uniform((j >> 20) & 7);
       parts = uniform(((j >> 23) & 7) + 1);
     } else {
-      tile_of_rows = uniform(schedule[kScheduleHead + a.row_tiles + job]);
+      const int pieces = schedule[1];
+      const int e = schedule[kScheduleHead + job + (a.in_pieces ? 4 * a.row_tiles + (int)schedule_jobs(a.row_tiles) : a.row_tiles)];
+      if (a.in_pieces) {
+        if ((int)job >= pieces) return;
+        first_row = uniform((e >> 10) & 127), last_row = uniform((e >> 17) & 127);
+      }
+      tile_of_rows = uniform(e & 1023);
     }
   }
   tile_of_rows = min(max(tile_of_rows, 0), a.row_tiles - 1);
   const int row = (tile_of_rows * kWaves + wave) * 32 + lq;
-  const bool inside = row < a.rows;
+  const bool inside = row < a.rows && (in_parts || kWaves == 1 || (wave * 32 + lq >= first_row && wave * 32 + lq <= last_row));
   const int token = inside ? (int)((uint32_t)row / (uint32_t)a.group) : 0;
   const int head = kvh * a.group + (inside ? row - token * a.group : 0);
   const int d = c.d, k_len = c.k_len, axes = kMode & (kBiased | kEither) ? c.axes : 0;

@@ -68,7 +68,7 @@ class Tokens:
             # blocks for 1, 2, 4 and 8 query heads per key head, of n row groups each
             tiles = [-(-t * group // ROW_TILE) for group in SCHEDULE_GROUPS]
             if 0 < t <= SCHEDULE_MAX_TOKENS and b * sum(tiles) < SCHEDULE_MAX_TILES:
-                blocks = [4 + 3 * n + (9 * n + 4) // 5 for n in tiles]
+                blocks = [4 + 5 * n + (9 * n + 4) // 5 + n // 4 for n in tiles]
                 self._schedule = torch.empty((b * sum(blocks),), dtype=torch.int32, device=documents.device)
                 self._schedule_of = {group: (self._schedule.data_ptr() + 4 * b * sum(blocks[:i]), blocks[i])
                                      for i, group in enumerate(SCHEDULE_GROUPS)}

@@ -467,15 +467,17 @@ def test_long_documents_among_short_ones(device, sizes, h, hk, dtype):
 
 
 def test_schedule_is_a_permutation(device):
-    for sizes in ([1], [128], [129, 300, 4], [2000] + [10] * 100, [16384]):
-        docs = i32(torch.repeat_interleave(torch.arange(len(sizes)), torch.tensor(sizes)), device)
+    for sizes in ([1], [128], [129, 300, 4], [2000] + [10] * 100, [700, 900, 1000], [300, -1, 77] * 30, [16384]):
+        docs = i32(torch.repeat_interleave(torch.arange(len(sizes)), torch.tensor(sizes).abs()), device)
+        docs[::50] -= sum(n < 0 for n in sizes)                  # some padding
         tokens = Tokens(docs)
         at = 0
         for group in (1, 2, 4, 8):
             n = -(-len(docs) * group // 128)
-            block = tokens._schedule[at:at + 4 + 3 * n + (9 * n + 4) // 5].cpu()
+            block = tokens._schedule[at:at + 4 + 5 * n + (9 * n + 4) // 5 + n // 4].cpu()
             at += len(block)
             work, order, first, jobs = block[4:4 + n], block[4 + n:4 + 2 * n], block[4 + 2 * n:4 + 3 * n], block[4 + 3 * n:]
+            cuts, pieces = jobs[(9 * n + 4) // 5:][:n].tolist(), jobs[(9 * n + 4) // 5 + n:][:block[1]].tolist()
             assert sorted(order.tolist()) == list(range(n)) and (work[order.long()].diff() <= 0).all()
             jobs = jobs[:block[0]].tolist()
             parts = [x >> 24 for x in first.tolist()]
@@ -483,3 +485,18 @@ def test_schedule_is_a_permutation(device):
             for tile, x in enumerate(first.tolist()):
                 assert jobs[x & 0xffffff:(x & 0xffffff) + (x >> 24)] == [
                     tile | p << 20 | ((x >> 24) - 1) << 23 for p in range(x >> 24)]
+            # pieces: every row of every tile once, those of the most work first, cut between documents
+            rows = sorted((x & 1023, x >> 10 & 127, x >> 17) for x in pieces)
+            whole = [(t, 0, 127) for t in range(n)]
+            for t, low, high in rows:
+                if low:
+                    assert (t, 0, low - 1) in rows and high == 127 and not low % group
+                    token = t * 128 // group + low // group
+                    assert docs[token] != docs[token - 1] and cuts[t] & 127 == low
+                    whole[t] = (t, 0, low - 1)
+            assert rows == sorted(whole + [x for x in rows if x[1]]) and len(rows) <= n + n // 4
+            of = {(t, bool(low)): cuts[t] >> 17 if low else cuts[t] >> 7 & 1023 if high < 127 else int(work[t]) for t, low, high in rows}
+            sizes_of = [of[x & 1023, bool(x >> 10 & 127)] for x in pieces]
+            assert sizes_of == sorted(sizes_of, reverse=True)
+            if sizes == [700, 900, 1000]:
+                assert len(rows) > n
