@@ -382,7 +382,7 @@ int musc_layernorm_rows(const void* x, const void* residual, void* sum_out,
  *   all seen scores are minus infinity.
  * fp32 scores, softmax statistics and accumulation; the probabilities are rounded to 16-bit
  * types for their product with V.  What unseen keys hold (infinities and NaN among it) has no
- * effect.  No other call's result depends on it, and nothing is kept between calls. */
+ * effect, but for the order of some fp32 sums where it is not finite.  No other call's result depends on it, and nothing is kept between calls. */
 typedef struct musc_masked_attention {
   const void *q, *k, *v;  /* heads of d channels at b * sb + token * st + head * sh (elements) */
   void* out;

@@ -189,13 +189,17 @@ int plan(const musc_masked_attention& c, Args& a, int& waves) {
   if (waves == 1 && a.key_tiles <= kTeamTiles * teams) a.teams = teams;
   if (a.teams > 1) {
   } else if (waves > 1 && c.schedule) {
-    // Long row tiles in parts where all begin at once, so that the longest ends last, and are long
-    // enough to pay for a join: 4 packed images, fp32 (416 row tiles, 512 places), 204 -> 144 us; three
-    // documents of 2000, 1000 and 1000 tokens, 8 heads, fp16, bias, 102 -> 76 us, but of 500 tokens in
-    // all 23 -> 28.  With more row tiles than places short ones fill up behind long ones (12 packed
-    // images, fp16, 1184 for 768: 106 us whole, 110 in parts).
-    a.in_parts = whole < a.slots && (c.dtype == MUSC_DTYPE_F32 || c.k_len >= 2048);
+    // Where all row tiles begin at once the longest ends last.  With an order of tokens their lengths
+    // differ most: long ones go in parts, if long enough to pay for a join (fp16, 8 heads of 64: three
+    // causal documents of 4000 tokens in all 45 us, in pieces 58; of 1000 20 us either way).  So do those
+    // of fp32 with narrow heads, whose tiles take longest (4 packed images 227 us, in pieces 256; four
+    // documents of 1000 tokens in all 47, 60; three 69, 54).
+    a.in_parts = whole < a.slots && (c.q_order ? c.dtype == MUSC_DTYPE_F32 || c.k_len >= 2048 : c.dtype == MUSC_DTYPE_F32 && c.d <= 64);
     if (a.in_parts) a.jobs = (int)schedule_jobs(a.row_tiles);
+    // Without an order the longest tiles are those that end one document and begin the next: cut there
+    // (fp16, 16 heads of 64: 12 packed images 99 us whole, 87 in pieces; three documents of 1500 tokens in
+    // all 49, 29, of 2500 with a bias 66 in parts, 46 in pieces).  Few rounds only: listed but empty
+    // pieces cost a little, and short tiles fill up behind long ones.
     a.in_pieces = !a.in_parts && !c.q_order && whole < 4LL * a.slots;
     if (a.in_pieces) a.jobs = (int)schedule_pieces(a.row_tiles);
   } else if (whole < (waves == 1 ? 1024 : 256)) {

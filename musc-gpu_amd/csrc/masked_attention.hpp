@@ -20,8 +20,9 @@
 //
 // Rows and keys are shared out three ways:
 //   many rows   four waves of 32 rows each on the same tiles.  Row tiles are begun in the order of
-//               their work (musc_token_schedule); where all begin at once the long ones are done in
-//               parts (kInParts) that a second kernel joins;
+//               their work (musc_token_schedule); those of two documents are cut between them, or, with an
+//               order of tokens and where all begin at once, long ones are done in parts of their keys
+//               (kInParts) that a second kernel joins;
 //   few rows    (a new token, a pooling latent) over up to 2048 keys: the waves of one workgroup take
 //               every n-th tile of the same rows and join in LDS (kTeams);
 //   few rows over more keys: one wave each on a stretch of the keys, four of them on a CU, joined by

@@ -466,6 +466,32 @@ def test_long_documents_among_short_ones(device, sizes, h, hk, dtype):
     assert bad[5:sizes[0]].all() and not bad[:5].any() and not bad[sizes[0]:].any()
 
 
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('h,hk,d', [(2, 2, 64), (4, 1, 128), (8, 1, 96)])
+def test_row_tiles_of_two_documents(device, h, hk, d, dtype):
+    # long documents that meet inside row tiles, with padding and a single token between them
+    sizes = [[330, 6, 517, 1, 490], [200, 0, 500, 300, 344]]
+    docs = torch.stack([torch.repeat_interleave(torch.tensor([4, -1, 2, 9, 3]), torch.tensor(n)) for n in sizes])
+    t = docs.shape[1]
+    q, k, v = heads(device, dtype, 2, t, t, h, hk, d)
+    tokens = Tokens(i32(docs, device))
+    seen = see(docs, docs)
+    out = torch.full_like(q, 7.0)
+    got = masked_attention(q, k, v, 0.1, keys=tokens, out=out)
+    check(got, q, k, v, 0.1, seen=seen)
+    assert (got[docs.to(device) < 0] == 0).all()
+    v[0, 3], k[1, 300] = float('nan'), float('inf')       # of the first document, and of the second entry's second
+    held = masked_attention(q, k, v, 0.1, keys=tokens)
+    same = torch.ones((2, t), dtype=torch.bool)
+    same[0, :330], same[1, 200:700] = False, False
+    # not to the bit: a workgroup that meets an unseen NaN adds its mixed tiles' products one by one, in
+    # fp32 as the matrix instructions do but in another order, which the tolerance's n 2^-24 W covers
+    for b in range(2):
+        rows = same[b].nonzero()[:, 0]
+        check(held[b:b + 1, rows], q[b:b + 1, rows], k[b:b + 1], v[b:b + 1], 0.1, seen=seen[b:b + 1, rows])
+    assert torch.isnan(held[0, :330]).all() and torch.isnan(held[1, 200:700]).any(-1).all()
+
+
 def test_schedule_is_a_permutation(device):
     for sizes in ([1], [128], [129, 300, 4], [2000] + [10] * 100, [700, 900, 1000], [300, -1, 77] * 30, [16384]):
         docs = i32(torch.repeat_interleave(torch.arange(len(sizes)), torch.tensor(sizes).abs()), device)
