@@ -93,77 +93,69 @@ __global__ __launch_bounds__(kWave) void row_work_kernel(const int* __restrict__
 // jobs, where a tile of more than 5/4 of the mean work is listed in up to 8 parts, by the work of a
 // part.  At most 9/5 n jobs.  And in pieces: the tiles of the most work, above the mean and n / 4 of them
 // at most, cut where row_work_kernel found it worth while.
-// One workgroup per schedule.  Every row tile finds its place by looking at all of them in LDS: 1024
-// tiles, 1024 threads.
+// Every row tile finds its places by looking at all of them in LDS: 1024 tiles, 1024 threads.  A
+// schedule is shared by `slices` workgroups, which all form the same numbers and write their own tiles'.
 constexpr int kMostTiles = MUSC_SCHEDULE_MAX_TOKENS * 8 / kRowTile;
-__global__ __launch_bounds__(1024) void row_order_kernel(const Schedule s, int* __restrict__ out) {
-  __shared__ int2 tiles[kMostTiles];  // work, work of a part * 8 + parts - 1
-  __shared__ int cut[kMostTiles];     // of the cuts, first those worth while, then the n / 4 most
+__global__ __launch_bounds__(1024) void row_order_kernel(const Schedule s, int slices, int* __restrict__ out) {
+  static_assert(kMostTiles <= 1024, "one row tile per thread");
+  // Per tile, keys that are larger for what comes first: work << 10 | tile (whole), then (work of a part
+  // << 10 | tile) << 3 | parts - 1, then the whole key's form for the tile's pieces (-1: not cut).
+  __shared__ int4 keys[kMostTiles];
   __shared__ long long sums[16];
-  __shared__ int counts[16];
-  const int w = blockIdx.x % 4, b = blockIdx.x / 4, n = s.tiles[w], lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  __shared__ int counts[16], cuts_here[16];
+  const int slice = blockIdx.x % slices, w = blockIdx.x / slices % 4, b = blockIdx.x / slices / 4;
+  const int n = s.tiles[w], j = threadIdx.x, lane = j % kWave, wave = j / kWave;
   int* block = out + s.at[w] + b * schedule_block(n);
-  const int* work = block + kScheduleHead;
-  const int* cuts = block + kScheduleHead + 3 * n + schedule_jobs(n);
-  int* pieces = block + kScheduleHead + 4 * n + schedule_jobs(n);
-  double total = 0;  // whole numbers below 2^53
-  for (int j = threadIdx.x; j < n; j += 1024) total += work[j];
-  total = wave_sum(total);
+  const int x = j < n ? block[kScheduleHead + j] : 0;
+  const double total = wave_sum((double)x);  // whole numbers below 2^53
   if (lane == 0) sums[wave] = (long long)total;
   __syncthreads();
   long long all_work = 0;
   for (int i = 0; i < 16; ++i) all_work += sums[i];
   const int most = (int)max((5 * all_work + 4LL * n - 1) / (4LL * n), 8LL);  // of a part
-  float jobs_here = 0.f;
-  for (int j = threadIdx.x; j < n; j += 1024) {
-    const int x = work[j], parts = min(max((x + most - 1) / most, 1), kMaxParts);
-    tiles[j] = make_int2(x, (x + parts - 1) / parts * 8 + parts - 1);
-    jobs_here += parts;
-    cut[j] = (long long)x * n > all_work ? cuts[j] : 0;
-  }
-  jobs_here = wave_sum(jobs_here);
-  if (lane == 0) counts[wave] = (int)jobs_here;
+  const int parts = j < n ? min(max((x + most - 1) / most, 1), kMaxParts) : 0;
+  int cut = j < n && (long long)x * n > all_work ? block[kScheduleHead + 3 * n + schedule_jobs(n) + j] : 0;
+  const float jobs_here = wave_sum((float)parts), cut_here = wave_sum(cut ? 1.f : 0.f);
+  if (lane == 0) counts[wave] = (int)jobs_here, cuts_here[wave] = (int)cut_here;
+  keys[j] = make_int4(x << 10 | j, 0, 0, cut);
   __syncthreads();
-  static_assert(kMostTiles <= 1024, "one row tile per thread");
-  int mine = threadIdx.x < n ? cut[threadIdx.x] : 0, more = 0;
-  if (mine)
-    for (int j = 0; j < n; ++j)
-      more += cut[j] && (tiles[j].x > tiles[threadIdx.x].x || (tiles[j].x == tiles[threadIdx.x].x && j > (int)threadIdx.x));
-  if (more >= n / 4) mine = 0;
-  __syncthreads();
-  if (threadIdx.x < n) cut[threadIdx.x] = mine;
-  const float cut_here = wave_sum(mine ? 1.f : 0.f);
-  if (lane == 0) sums[wave] = (long long)cut_here;
-  __syncthreads();
-  for (int tile = threadIdx.x; tile < n; tile += 1024) {
-    const int2 here = tiles[tile];
-    const int size = here.y >> 3, parts = (here.y & 7) + 1;
-    // this tile's pieces: all of it, or its rows before the cut and those from it on
-    const int at = cut[tile] & 127, before = at ? (cut[tile] >> 7) & 1023 : here.x, from = cut[tile] >> 17;
-    int rank = 0, first = 0, rank_before = at && from >= before, rank_from = at && before > from;
-    for (int j = 0; j < n; ++j) {
-      const int2 x = tiles[j];
-      const int each = x.y >> 3;
-      rank += x.x > here.x || (x.x == here.x && j > tile);
-      first += each > size || (each == size && j > tile) ? (x.y & 7) + 1 : 0;
-      if (j == tile) continue;
-      const int x_from = cut[j] ? cut[j] >> 17 : -1, x_before = cut[j] ? (cut[j] >> 7) & 1023 : x.x, later = j > tile;
-      rank_before += (x_before + later > before) + (x_from + later > before);
-      rank_from += (x_before + later > from) + (x_from + later > from);
-    }
-    pieces[rank_before] = tile | (at ? at - 1 : kRowTile - 1) << 17;
-    if (at) pieces[rank_from] = tile | at << 10 | (kRowTile - 1) << 17;
-    block[kScheduleHead + n + rank] = tile;
-    block[kScheduleHead + 2 * n + tile] = first | parts << 24;
-    int* jobs = block + kScheduleHead + 3 * n + first;
-    for (int p = 0; p < parts; ++p) jobs[p] = tile | p << 20 | (parts - 1) << 23;
+  int jobs = 0, cut_tiles = 0;
+  for (int i = 0; i < 16; ++i) jobs += counts[i], cut_tiles += cuts_here[i];
+  if (cut_tiles > n / 4) {  // the most work only
+    int more = 0;
+    if (cut)
+      for (int i = 0; i < n; ++i) more += keys[i].w && keys[i].x > (x << 10 | j);
+    if (more >= n / 4) cut = 0;
+    cut_tiles = n / 4;
+    __syncthreads();
   }
-  if (threadIdx.x == 0) {
-    int jobs = 0;
-    long long cut_tiles = 0;
-    for (int i = 0; i < 16; ++i) jobs += counts[i], cut_tiles += sums[i];
-    block[0] = jobs, block[1] = n + (int)cut_tiles;
+  const int whole = x << 10 | j, part = parts ? ((x + parts - 1) / parts << 10 | j) << 3 | (parts - 1) : 0;
+  // the rows of a cut tile before the cut and from it on; the later piece of equal ones begins first
+  const int before = cut ? ((cut >> 7) & 1023) << 10 | j : whole, from = cut ? cut >> 17 << 10 | j : -1;
+  keys[j] = make_int4(whole, part, before, from);
+  __syncthreads();
+  if (slice == 0 && j == 0) block[0] = jobs, block[1] = n + cut_tiles;
+  const int per = kMostTiles / slices, tile = slice * per + j;
+  if (j >= per || tile >= n) return;
+  const int4 here = keys[tile];
+  int rank = 0, first = 0, rank_before = here.w >= here.z, rank_from = 0;
+  for (int i = 0; i < n; ++i) {
+    const int4 k = keys[i];
+    rank += k.x > here.x;
+    first += k.y > here.y ? (k.y & 7) + 1 : 0;
+    rank_before += (k.z > here.z) + (k.w > here.z);
+    if (here.w >= 0) rank_from += (k.z > here.w) + (k.w > here.w);
   }
+  rank_before -= here.w > here.z;  // counted above
+  const int at = here.w >= 0 ? block[kScheduleHead + 3 * n + schedule_jobs(n) + tile] & 127 : 0;
+  int* pieces = block + kScheduleHead + 4 * n + schedule_jobs(n);
+  pieces[rank_before] = tile | (at ? at - 1 : kRowTile - 1) << 17;
+  if (at) pieces[rank_from] = tile | at << 10 | (kRowTile - 1) << 17;
+  block[kScheduleHead + n + rank] = tile;
+  const int of = (here.y & 7) + 1;
+  block[kScheduleHead + 2 * n + tile] = first | of << 24;
+  int* jobs_at = block + kScheduleHead + 3 * n + first;
+  for (int p = 0; p < of; ++p) jobs_at[p] = tile | p << 20 | (of - 1) << 23;
 }
 
 // Shape of the launch: rows per workgroup, tiles and splits.
@@ -310,7 +302,8 @@ extern "C" int musc_token_schedule(const int* documents, const int* order, const
   if (s.first[4] >= (0x100000000LL >> 10)) return MUSC_ERR_UNSUPPORTED;
   hipLaunchKernelGGL(mattn::row_work_kernel, dim3((unsigned)s.first[4]), dim3(kWave), 0, stream, documents, order,
                      reinterpret_cast<const int4*>(summary), s, schedule);
-  hipLaunchKernelGGL(mattn::row_order_kernel, dim3((unsigned)batch * 4), dim3(1024), 0, stream, s,
+  const int slices = s.tiles[3] > 256 ? 4 : 1;  // 1370 tokens 8 us, 4096 14; 9465 30, 16384 48 (one workgroup: 151)
+  hipLaunchKernelGGL(mattn::row_order_kernel, dim3((unsigned)(batch * 4 * slices)), dim3(1024), 0, stream, s, slices,
                      schedule);
   return check_launch();
 }

@@ -493,7 +493,7 @@ def test_row_tiles_of_two_documents(device, h, hk, d, dtype):
 
 
 def test_schedule_is_a_permutation(device):
-    for sizes in ([1], [128], [129, 300, 4], [2000] + [10] * 100, [700, 900, 1000], [300, -1, 77] * 30, [16384]):
+    for sizes in ([1], [128], [129, 300, 4], [2000] + [10] * 100, [700, 900, 1000], [300, -1, 77] * 30, [3000, 2500, 1200, 90], [150] * 109, [16384]):
         docs = i32(torch.repeat_interleave(torch.arange(len(sizes)), torch.tensor(sizes).abs()), device)
         docs[::50] -= sum(n < 0 for n in sizes)                  # some padding
         tokens = Tokens(docs)
