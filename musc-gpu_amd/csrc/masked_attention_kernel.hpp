@@ -17,15 +17,18 @@ __device__ __forceinline__ void unroll(F f) {
 
 // Loads straight from memory into LDS, lane l's 16 (or 4) bytes to `to` (+ kTo) + 16 l (or
 // 4 l), `to` uniform.  From inline assembly, as the compiler, which cannot tell the two buffers apart,
-// would wait for them before reading the other one; the loop waits for them itself.
+// would wait for them before reading the other one; the loop waits for them itself.  The resource
+// comes out of vector registers (v_readfirstlane), and a vector-memory instruction may read it from the
+// fifth wait state after that on, which the compiler does not see to for an asm statement: the scalar
+// instruction and s_nop 3 are five.  (M0 needs one.)
 template <int kTo>
 __device__ __forceinline__ void load_to_lds_16(uint32_t to, int offset, int4v from, int from_offset) {
-  asm volatile("s_add_u32 m0, %0, %4\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+  asm volatile("s_add_u32 m0, %0, %4\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
                :: "s"(to), "v"(offset), "s"(from), "s"(from_offset), "i"(kTo) : "memory", "m0", "scc");
 }
 __device__ __forceinline__ void load_to_lds_4(const void* place, int offset, int4v from) {
   const uint32_t to = __builtin_amdgcn_readfirstlane((uint32_t)(size_t)(lds_void*)place);
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dword %1, %2, 0 offen lds"
                :: "s"(to), "v"(offset), "s"(from) : "memory", "m0");
 }
 __device__ __forceinline__ int4v resource(const void* base, long long bytes) {
