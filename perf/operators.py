@@ -207,8 +207,6 @@ def prepare(case, seed):
         return _prepare_attention(case, g, normal)
     if case['op'] == 'rotary':
         return _prepare_rotary(case, g, normal)
-    if own:
-        _package()
     rows, width = case['rows'], case['width']
     scale = torch.exp(torch.randn((rows, 1), generator=g, device=DEV) * 0.5)
     return dict(case=case, x=(normal(rows, width).float() * scale).to(dtype),
@@ -336,6 +334,7 @@ def _rotated(x, cos, sin, adjacent):
 def _norm(state):
     case, x, r, w = state['case'], state['x'], state['residual'], state['weight']
     if own:
+        _package()
         from musc_hip import _layers_hip
         if case['eight']:
             return _layers_hip.rms_norm_quantized(x, w, EPS, residual=r, group=case['group'])
