@@ -59,6 +59,9 @@ constexpr int kBufferFlags = 0x00020000;   // buffer resource word 3 for raw byt
 constexpr int kNowhere = 0x7fffff00;       // a byte offset past every extent: such loads give zeros
 constexpr float kLazyLog2 = 8.f;           // the running maximum moves once a tile exceeds it by this
 constexpr float kLog2e = 1.4426950408889634f;
+// 16-bit types: the largest cap whose tanh is formed by one exponential and one reciprocal.  Its error,
+// cap 2^-21 in the score, is then at most an eighth of what rounding a probability to fp16 (2^-11) may do.
+constexpr float kSmallCap = 128.f;
 constexpr int kSummaryKeys = 32;
 constexpr int kMaxAxes = 3;
 constexpr int kMaxSplits = 256;

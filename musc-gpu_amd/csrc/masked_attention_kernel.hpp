@@ -43,8 +43,10 @@ __device__ __forceinline__ int4v resource(const void* base, long long bytes) {
 // kInParts alone costs 3 to 8 %).  kTeams > 1 (with one wave): that many waves take every n-th tile of
 // the same rows, each with its own place in LDS and at its own pace, and join their parts there.
 // kEither: a cap and a bias if the call has them, tested per tile (for the kernels of few rows and
-// of parts, which wait for memory or for one another).
-constexpr int kCapped = 1, kBiased = 2, kInParts = 4, kEither = 8;
+// of parts, which wait for memory or for one another).  kLargeCap (16-bit types, with kEither): the cap is past
+// kSmallCap; kernels of their own, as tanhf beside the other form costs registers (parts of fp16 heads of 64:
+// 76 spilled instead of 17): 8192 tokens, 16 heads of 64, fp16, 730 us past kSmallCap, 450 up to it.
+constexpr int kCapped = 1, kBiased = 2, kInParts = 4, kEither = 8, kLargeCap = 16;
 template <int kDtype, int kD, int kWaves, int kTeams, int kMode>
 __global__ __launch_bounds__(kWaves * kTeams * kWave, kWaves == 1 ? 1 : kD == 64 && kDtype != MUSC_DTYPE_F32 ? 3 : 2) void masked_attention_kernel(
     const Args a) {
@@ -193,12 +195,14 @@ __global__ __launch_bounds__(kWaves * kTeams * kWave, kWaves == 1 ? 1 : kD == 64
   // Scores stay "raw" until the exponential: score in log2 units =
   // raw * to_log2 (+ a constant that cancels), to_log2 > 0:
   //   no cap   raw = +- q . k (Q negated for a negative scale), to_log2 = |scale| log2 e
-  //   cap      raw = -1 / (1 + e^2x), x = scale q . k / cap, as cap tanh x = cap (1 + 2 raw);
-  //            fp32: raw = tanh x
+  //   cap      raw = -1 / (1 + e^2x), x = scale q . k / cap, as cap tanh x = cap (1 + 2 raw): off by
+  //            cap 2^-21 however small the score is, so in 16-bit types up to kSmallCap only;
+  //            raw = tanh x above it and in fp32, off by the score's own 2^-21
   const bool capped = (kMode & kCapped) != 0 || ((kMode & kEither) != 0 && c.cap > 0.f);
+  constexpr bool by_exponential = k16 && (kMode & kLargeCap) == 0;
   const float scale = c.scale == 0.f ? 1.f : c.scale;
-  const float to_log2 = (capped ? (k16 ? 2.f * c.cap : c.cap) : fabsf(scale)) * kLog2e;
-  const float by_cap = capped ? scale / c.cap * (k16 ? 2.f * kLog2e : 1.f) : 0.f;
+  const float to_log2 = (capped ? (by_exponential ? 2.f * c.cap : c.cap) : fabsf(scale)) * kLog2e;
+  const float by_cap = capped ? scale / c.cap * (by_exponential ? 2.f * kLog2e : 1.f) : 0.f;
   const bool negate = !capped && scale < 0.f;
 #pragma unroll
   for (int m = 0; m < kQ; ++m) {
@@ -340,7 +344,7 @@ __global__ __launch_bounds__(kWaves * kTeams * kWave, kWaves == 1 ? 1 : kD == 64
 #pragma unroll
         for (int v = 0; v < 16; ++v) {
           const float x = s[u][v] * by_cap;
-          s[u][v] = k16 ? __builtin_amdgcn_rcpf(-1.f - __builtin_amdgcn_exp2f(x)) : tanhf(x);
+          s[u][v] = by_exponential ? __builtin_amdgcn_rcpf(-1.f - __builtin_amdgcn_exp2f(x)) : tanhf(x);
         }
     }
     // distances from the matrix cores: position(j) * 1 + 1 * -position(i), exact in fp32
@@ -728,7 +732,7 @@ __global__ __launch_bounds__(256) void join_parts_kernel(const Args a) {
   }
 }
 
-// Few rows, or rows in parts.
+// Few rows, rows in parts, or a large cap.
 template <int kDtype, int kD, int kMode>
 void launch_special(const Args& a, int waves, const dim3& grid, hipStream_t stream) {
   constexpr int kTeams = teams_of((kD <= 64 ? 64 : 128) * (kDtype == MUSC_DTYPE_F32 ? 4 : 2));
@@ -736,16 +740,21 @@ void launch_special(const Args& a, int waves, const dim3& grid, hipStream_t stre
     hipLaunchKernelGGL((masked_attention_kernel<kDtype, kD, 1, kTeams, kMode>), grid, dim3(kTeams * kWave), 0, stream, a);
   else if (waves == 1)
     hipLaunchKernelGGL((masked_attention_kernel<kDtype, kD, 1, 1, kMode>), grid, dim3(kWave), 0, stream, a);
-  else
+  else if (a.in_parts)
     hipLaunchKernelGGL((masked_attention_kernel<kDtype, kD, 4, 1, kMode | kInParts>), grid, dim3(4 * kWave), 0, stream, a);
+  else if constexpr ((kMode & kLargeCap) != 0)
+    hipLaunchKernelGGL((masked_attention_kernel<kDtype, kD, 4, 1, kMode>), grid, dim3(4 * kWave), 0, stream, a);
 }
 
 template <int kDtype, int kD>
 void launch(const Args& a, int waves, hipStream_t stream) {
   const dim3 grid((unsigned)align_up((size_t)a.units, kXcds));
   const int mode = (a.c.cap > 0.f ? kCapped : 0) | (a.c.axes ? kBiased : 0);
+  constexpr int kWide = kD <= 64 ? 64 : 128;
+  if constexpr (kDtype != MUSC_DTYPE_F32) {
+    if (a.c.cap > kSmallCap) return launch_special<kDtype, kWide, kEither | kLargeCap>(a, waves, grid, stream);
+  }
   if (waves == 1 || a.in_parts) {
-    constexpr int kWide = kD <= 64 ? 64 : 128;
     if (mode == 0) launch_special<kDtype, kWide, 0>(a, waves, grid, stream);
     else launch_special<kDtype, kWide, kEither>(a, waves, grid, stream);
   } else if (mode == 0) {
