@@ -70,8 +70,8 @@ class Tokens:
             if 0 < t <= SCHEDULE_MAX_TOKENS and b * sum(tiles) < SCHEDULE_MAX_TILES:
                 blocks = [4 + 5 * n + (9 * n + 4) // 5 + n // 4 for n in tiles]
                 self._schedule = torch.empty((b * sum(blocks),), dtype=torch.int32, device=documents.device)
-                self._schedule_of = {group: (self._schedule.data_ptr() + 4 * b * sum(blocks[:i]), blocks[i])
-                                     for i, group in enumerate(SCHEDULE_GROUPS)}
+                # bytes before a group's blocks (no address: copies have their own), ints of a block
+                self._schedule_of = {group: (4 * b * sum(blocks[:i]), blocks[i]) for i, group in enumerate(SCHEDULE_GROUPS)}
             self.refresh()
 
     def refresh(self) -> None:
@@ -192,9 +192,9 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: f
     if not tk:
         return o.zero_()
     schedule = schedule_sb = 0
-    if queries is keys and keys._schedule is not None:
-        schedule, schedule_sb = keys._schedule_of.get(h // hk, (0, 0))
-        schedule_sb = schedule_sb if k_sb else 0
+    if queries is keys and keys._schedule is not None and h // hk in keys._schedule_of:
+        before, block = keys._schedule_of[h // hk]
+        schedule, schedule_sb = keys._schedule.data_ptr() + before, block if k_sb else 0
     call = rt.PACK_MASKED_ATTENTION.pack(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), *qs, *ks, *vs, *os_, _STORAGE[dtype], b, tq, tk, h, hk, d,
         scale, cap, qd_ptr, qo_ptr, kd_ptr, ko_ptr, q_sb, k_sb, sum_ptr, sum_sb, qp_ptr, kp_ptr, qp_sb, kp_sb, slope_ptr,

@@ -46,7 +46,6 @@ class RotaryAxes:
         both[pairs:].view(torch.int32)[:pairs] = torch.tensor(axis, dtype=torch.int32)
         both = both.to(device)
         self.frequency, self.axis = both[:pairs], both[pairs:].view(torch.int32)[:pairs]
-        self.frequency_ptr, self.axis_ptr = self.frequency.data_ptr(), self.axis.data_ptr()
 
 
 def _head_rows(x, name, axes):
@@ -96,7 +95,7 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, axe
     if b and t and h:
         call = rt.PACK_ROTARY.pack(
             q2.data_ptr(), *rt.token_strides(q2), qo.data_ptr(), *rt.token_strides(qo), *k_args, positions.data_ptr(),
-            0 if len(shape) == 2 else t * axes.axes, axes.frequency_ptr, axes.axis_ptr, h, k_heads, _STORAGE[q2.dtype], b, t,
+            0 if len(shape) == 2 else t * axes.axes, axes.frequency.data_ptr(), axes.axis.data_ptr(), h, k_heads, _STORAGE[q2.dtype], b, t,
             d, positions.dtype == torch.int32, axes.axes, axes.pairs, axes.adjacent, inverse)
         rt.check(rt.library().musc_rotary(call, rt.current_stream(index)), 'musc_rotary')
     elif k_heads:
