@@ -38,7 +38,8 @@ class Tokens:
     The tensors are kept, not copied.  As keys they are also summarised (32 at a time) when the
     object is made, on the current stream, and self-attention over them is scheduled (its longest
     rows first, in parts where there are few); call refresh() after changing them in place.  queries_only leaves
-    that out."""
+    that out.  Calls on another stream than the one it was made on keep its memory until they are done, also
+    where the object goes before; that stream waits for what made it as the caller says, as with any tensor."""
 
     def __init__(self, documents=None, order=None, positions=None, queries_only: bool = False):
         for name, x, dtype in (('documents', documents, torch.int32), ('order', order, torch.int32),
@@ -61,7 +62,10 @@ class Tokens:
                                           or positions.device != documents.device):
                 raise ValueError('positions must have the tokens of documents')
         self.documents, self.order, self.positions, self.summary = documents, order, positions, None
-        self._schedule = None
+        self._schedule = self._made_on = None
+        for x in (documents, positions):
+            if x is not None:
+                self._made_on = rt.current_stream(x.get_device())
         if documents is not None and not queries_only:
             b, t = documents.shape if documents.dim() == 2 else (1, documents.shape[0])
             self.summary = torch.empty((b, -(-t // SUMMARY_KEYS), 4), dtype=torch.int32, device=documents.device)
@@ -74,11 +78,22 @@ class Tokens:
                 self._schedule_of = {group: (4 * b * sum(blocks[:i]), blocks[i]) for i, group in enumerate(SCHEDULE_GROUPS)}
             self.refresh()
 
+    def __getstate__(self):
+        return {**self.__dict__, '_made_on': None}      # a copy's tensors may be of any stream
+
+    def used_on(self, stream: int, device: torch.device) -> None:
+        """Keeps the tensors' memory for work just begun on `stream`, the device's current one."""
+        if stream != self._made_on:
+            for x in (self.documents, self.order, self.positions, self.summary, self._schedule):
+                if x is not None:
+                    x.record_stream(torch.cuda.current_stream(device))
+
     def refresh(self) -> None:
         """Summarises the keys again, on the current stream, after a change of documents or order."""
         if self.summary is None or not self.summary.numel():
             return
         docs = self.documents
+        self.used_on(rt.current_stream(docs.get_device()), docs.device)
         with torch.cuda.device(docs.device):
             rt.check(rt.library().musc_token_summary(
                 docs.data_ptr(), None if self.order is None else self.order.data_ptr(), self.summary.shape[0],
@@ -203,6 +218,11 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: f
     rt.check(lib.musc_masked_attention_workspace_bytes(call, ctypes.byref(need)), 'musc_masked_attention_workspace_bytes')
     if need.value:
         ws = torch.empty(need.value, dtype=torch.uint8, device=q.device)
-    rt.check(lib.musc_masked_attention_fwd(call, None if ws is None else ws.data_ptr(), need.value,
-                                           rt.current_stream(index)), 'musc_masked_attention_fwd')
+    stream = rt.current_stream(index)
+    rt.check(lib.musc_masked_attention_fwd(call, None if ws is None else ws.data_ptr(), need.value, stream),
+             'musc_masked_attention_fwd')
+    if keys is not _EVERY:
+        keys.used_on(stream, q.device)
+    if queries is not keys:
+        queries.used_on(stream, q.device)
     return o

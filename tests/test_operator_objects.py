@@ -5,7 +5,7 @@ import pickle
 import pytest
 import torch
 
-from musc_hip import _masked_attention_hip, _runtime
+from musc_hip import _runtime
 from musc_hip._masked_attention_hip import Tokens
 from musc_hip._rotary_hip import RotaryAxes
 
@@ -13,6 +13,7 @@ from musc_hip._rotary_hip import RotaryAxes
 @pytest.fixture
 def on_cpu(monkeypatch):
     monkeypatch.setattr(_runtime, 'require_device_tensor', lambda t, name: None)
+    monkeypatch.setattr(_runtime, 'current_stream', lambda index: 0)
     monkeypatch.setattr(Tokens, 'refresh', lambda self: None)
 
 

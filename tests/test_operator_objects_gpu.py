@@ -24,3 +24,27 @@ def test_copies_outlive_the_original(device):
     for a, b in zip(got, want):
         assert torch.equal(a, b)
     assert filler
+
+
+def test_tokens_dropped_while_another_stream_works_with_them(device):
+    g = torch.Generator().manual_seed(2)
+    t = 1500
+    q, k, v = (torch.randn((1, t, 2, 64), generator=g).half().to(device) for _ in range(3))
+    ids = torch.arange(t, dtype=torch.int32) // 400
+    docs = ids.to(device)
+    want = masked_attention(q, k, v, 0.125, keys=Tokens(docs))
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        masked_attention(q, k, v, 0.125, keys=Tokens(docs))            # what a first call on a stream sets up
+    torch.cuda.synchronize()
+    tokens = Tokens(ids.to(device))
+    sizes = [x.numel() for x in (tokens.summary, tokens._schedule, tokens.documents)]
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(50_000_000)                                   # tens of milliseconds
+        got = masked_attention(q, k, v, 0.125, keys=tokens)
+    del tokens
+    filler = [torch.zeros((n,), dtype=torch.int32, device=device) for n in sizes * 8]
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
+    assert filler
