@@ -243,7 +243,12 @@ def require_device_tensor(t: torch.Tensor, name: str) -> None:
 
 
 def require_no_gradient(*tensors) -> None:
-    """Operators without a backward pass refuse inputs that ask for one."""
+    """Operators without a backward pass refuse inputs that ask for one, and those that carry a
+    forward-mode tangent (which no_grad does not turn off)."""
+    if torch.autograd.forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
+                raise ValueError('this operator has no derivative: call it on the primal of a dual tensor')
     if not torch.is_grad_enabled():
         return
     for t in tensors:
