@@ -141,3 +141,11 @@ def test_two_graphs_of_one_batch(device):
         eager = masked_attention(*one, 0.1, keys=tokens)
         torch.cuda.synchronize()
         assert torch.equal(kept[0], want[0]) and torch.equal(kept[1], want[1]) and torch.equal(eager, want[0])
+
+
+@pytest.mark.parametrize('scale,cap', [(1e39, 0.0), (-1e300, 0.0), (1.0, 1e39), (float('inf'), 0.0), (1.0, float('inf')),
+                                       (2.0 ** 61, 0.0), (1.0, 2.0 ** 61), (1.0, float('nan'))])
+def test_refuses_scales_and_caps_past_the_range(device, scale, cap):
+    q, k, v = heads(device, torch.float16, 1, 4, 4, 2, 2, 64)
+    with pytest.raises(ValueError):
+        masked_attention(q, k, v, scale, cap=cap)
