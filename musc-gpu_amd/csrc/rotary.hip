@@ -24,7 +24,8 @@ namespace rotary {
 constexpr int kThreads = 256;
 constexpr int kMaxPairs = 256;
 constexpr int kMaxTokens = 16;  // tokens of a workgroup
-constexpr int kTable = 2048;    // (token, pair) entries of a workgroup at most
+constexpr int kTable = 256;     // (token, pair) entries of a workgroup: one sincos per thread, or one token's pairs
+static_assert(kTable >= kThreads && kTable >= kMaxPairs, "a workgroup's angles fit the table");
 
 struct Side {
   const void* x;
