@@ -9,7 +9,9 @@
 // One pass over the keys with the running maximum and sum of the softmax.  As in the
 // unmasked kernels a wave forms S^T = K Q^T, so that a lane owns one query row and its
 // maximum, sum and probabilities stay in its registers; O^T += V^T P^T follows with P in
-// place.  A row is a (token, head of the group) pair: the heads that share a key head are
+// place.  16-bit types round P to the storage type for that product, and the sum is of the rounded
+// values: half a step of each probability, with which an output is 1.1 to 1.3 times as far from float64 as
+// rounding the output alone leaves it, for a product of 8 (fp32: 1) times the rate.  A row is a (token, head of the group) pair: the heads that share a key head are
 // neighbouring rows, so K and V are read once for all of them.
 //
 // Keys come in tiles of 64 (fp32, and workgroups of one wave: 32), staged in LDS straight from
@@ -32,10 +34,12 @@
 // of matrix instructions and about 650 of vector ones (per score: multiply-add, exponential of two
 // slots, half a maximum, half a conversion, half a sum), 770 more with a cap (exponential and
 // reciprocal), 256 of each kind with a bias over two axes; the two kinds run beside one another
-// little.  16 frames of 1024 patches, 16 heads of 128, bf16: 1075 us, 1.09 PFLOP/s, a product of
-// 8192^3 1.14.  8192 tokens, 16 heads of 64, fp16: 340 us, 0.81 PFLOP/s; with a bias over two axes
-// 475, with a cap 450 us.  Single tokens over long caches: HBM, at the 5.2 TB/s of a large copy.
-// fp32: its matrix instructions, 127 TFLOP/s of the 153 of a product of 8192^3.
+// little.  16 frames of 1024 patches, 16 heads of 128, bf16: 1075 to 1125 us by card, 1.04 to 1.09 PFLOP/s, a
+// product of 8192^3 1.14.  8192 tokens, 16 heads of 64, fp16: 336 us, 0.82 PFLOP/s; with a bias over two axes
+// 475, with a cap of up to 128 450, above 730 us.  Single tokens over long caches: HBM, at the 5.2 TB/s of a
+// large copy.  fp32: its matrix instructions, 127 to 133 TFLOP/s (8192 tokens, 8 heads of 64, 96 and 128) of the
+// 153 of a product of 8192^3; the four-wave kernels of heads past 96 spill 46 to 75 registers.  One document of
+// few row tiles leaves CUs idle: a schedule takes the place of splits of the keys, see plan().
 #pragma once
 
 #include <hip/hip_bf16.h>

@@ -122,7 +122,8 @@ def rms_norm(x: torch.Tensor, weight, eps: float, residual: torch.Tensor | None 
 
     With `residual`, returns (s, rms_norm(s)) where s = x + residual rounded to x's dtype, in
     one pass; otherwise rms_norm(x).  weight: one value per column in x's dtype or float32, or
-    None.  No backward pass."""
+    None.  The sum of squares is float32: a row whose squares overflow it (bfloat16 and float32 values
+    past about 1e17) comes out as zeros.  No derivative."""
     return _rms(x, weight, eps, residual, None, 0)
 
 

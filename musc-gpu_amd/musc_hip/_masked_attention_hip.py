@@ -140,9 +140,9 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: f
     keys, queries: the Tokens of both sides; queries defaults to keys (self-attention), no keys at
     all lets every query see every key.  A query that sees no key gets zeros, as does one whose seen
     scores are all minus infinity.
-    cap > 0: scores become cap tanh(score / cap) before the bias.  slopes: float32 (heads, axes),
+    cap > 0 (up to 2^60; 16-bit types are quickest up to 128): scores become cap tanh(score / cap) before the bias.  slopes: float32 (heads, axes),
     needs positions on both sides.  out: the tensor to write, rows on 16 bytes; it may not overlap q, k
-    or v.  No backward pass."""
+    or v.  No derivative."""
     for name, x in (('q', q), ('k', k), ('v', v)):
         rt.require_device_tensor(x, name)
         if x.dim() != 4:

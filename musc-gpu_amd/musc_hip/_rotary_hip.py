@@ -23,8 +23,8 @@ class RotaryAxes:
     columns of (time, height, width) positions); their sum R may leave channels from 2 R on as
     they are.  Pair i of n in its axis's section turns base ** -(i / n) radians per unit of
     position; with `shared`, pair i of all R turns base ** -(i / R).  Pairs are channels
-    (i, R + i), or (2 i, 2 i + 1) with `adjacent`.  Kept by the caller and used by any call with
-    the same head width."""
+    (i, R + i), or (2 i, 2 i + 1) with `adjacent`.  Kept by the caller, as a weight is, and used by
+    any call with the same head width."""
 
     def __init__(self, head_dim: int, sections, base: float = 10000.0, shared: bool = False, adjacent: bool = False,
                  device='cuda'):
@@ -62,7 +62,7 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, axe
     q (B, T, heads, D), k (B, T, kv_heads, D), any strides with a contiguous last dimension;
     positions (T, axes) or (B, T, axes), float32 or int32.  inverse turns back (the transpose).
     out: the tensors to write, (q_out, k_out) or q_out; they may be q and k themselves, and may
-    not overlap them otherwise.  No backward pass."""
+    not overlap them otherwise.  No derivative."""
     q2 = _head_rows(q, 'q', axes)
     if rt.elsewhere(q):
         with torch.cuda.device(q.device):
