@@ -249,7 +249,8 @@ int check(const musc_masked_attention* c) {
   if (!aligned(c->q, c->q_sb, c->q_st, c->q_sh, per) || !aligned(c->k, c->k_sb, c->k_st, c->k_sh, per) ||
       !aligned(c->v, c->v_sb, c->v_st, c->v_sh, per) || !aligned(c->out, c->o_sb, c->o_st, c->o_sh, per))
     return MUSC_ERR_INVALID_ARG;
-  if ((63 * c->k_st + c->d) * size > kNowhere - 16 || (63 * c->v_st + c->d) * size > kNowhere - 16)
+  if (c->k_st > kNowhere || c->v_st > kNowhere || (63 * c->k_st + c->d) * size > kNowhere - 16 ||
+      (63 * c->v_st + c->d) * size > kNowhere - 16)
     return MUSC_ERR_UNSUPPORTED;
   // documents on both sides and the keys' summary, or none; orders and positions likewise
   if (!c->q_documents != !c->k_documents || !c->k_documents != !c->k_summary) return MUSC_ERR_INVALID_ARG;

@@ -1,5 +1,7 @@
-"""The objects that a model keeps for its packed encoder, copied and pickled with it (CPU only)."""
+"""The objects that a model keeps for its packed encoder, copied and pickled with it, and strides that no
+memory has (CPU only)."""
 import copy
+import ctypes
 import pickle
 
 import pytest
@@ -51,3 +53,13 @@ def test_copies_hold_no_address_of_the_original(on_cpu, make, copied):
     for name, x in vars(was).items():
         if isinstance(x, torch.Tensor):
             assert getattr(other, name).data_ptr() != x.data_ptr() and getattr(other, name).shape == x.shape
+
+
+@pytest.mark.parametrize('side', ['k_st', 'v_st'])
+@pytest.mark.parametrize('stride', [1 << 28, 1 << 58, 1 << 60, (1 << 63) - 64])
+def test_row_strides_past_any_tile_are_refused(side, stride):
+    # 63 rows of 2^58 elements wrap around 64 bits
+    from test_operator_refusals import UNSUPPORTED, attention_call
+    need = ctypes.c_size_t()
+    call = ctypes.byref(attention_call(**{side: stride}))
+    assert _runtime.library().musc_masked_attention_workspace_bytes(call, ctypes.byref(need)) == UNSUPPORTED
