@@ -486,6 +486,12 @@ typedef struct musc_rotary_call {
   int q_heads, k_heads, dtype, batch, t, d, int_positions, axes, pairs, adjacent, inverse;
 } musc_rotary_call;
 int musc_rotary(const musc_rotary_call* call, hipStream_t stream);
+/* The same of heads that are normed first: y = x weight / sqrt(mean(x^2) + eps) over a head's d channels,
+ * in fp32 and not rounded before it is turned.  q_weight, k_weight: d values of the dtype given with each
+ * (the call's or MUSC_DTYPE_F32) at head * weight_sh, 0 for one row that all heads share; NULL for 1.
+ * The sum of squares is fp32: heads whose squares overflow it give y = 0. */
+int musc_norm_rotary(const musc_rotary_call* call, const void* q_weight, long long q_weight_sh, int q_weight_dtype,
+                     const void* k_weight, long long k_weight_sh, int k_weight_dtype, float eps, hipStream_t stream);
 
 #define MUSC_ACT_QUICK_GELU 0  /* x * sigmoid(1.702 x), transformer.py:32-35 (fp16: the
                                   three torch ops' roundings: 1.702 x, sigmoid, product) */

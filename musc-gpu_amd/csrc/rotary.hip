@@ -12,8 +12,14 @@
 // turns are taken off in float64, so far positions keep the angle's 24 bits.  16384 tokens of 32 + 8
 // heads of 128, bf16: 61-68 us = 4.9-5.5 TB/s (a large copy 5.2); 4 x 1370 tokens of 16 + 16 heads of
 // 64, fp16: 10 us; 8 tokens 3.9 us, the latency of a sincos and two reads.
+//
+// norm_rotary_kernel norms each head of q and k before that, in the same pass:
+//
+//   y = x w / sqrt(mean(x^2) + eps)                  fp32, turned before its one rounding
 #include <hip/hip_bf16.h>
 #include <hip/hip_fp16.h>
+
+#include <type_traits>
 
 #include "common.hpp"
 #include "storage.hpp"
@@ -48,18 +54,9 @@ struct Args {
 
 __device__ __forceinline__ uint32_t over(uint32_t x, uint32_t reciprocal) { return reciprocal ? __umulhi(x, reciprocal) : x; }
 
-// kVec: vectors of 16 bytes; otherwise one pair, or one copied channel, per thread.
-template <int kDtype, bool kAdjacent, bool kVec>
-__global__ __launch_bounds__(kThreads) void rotary_kernel(const Args a) {
-  using S = Storage<kDtype>;
-  typedef typename S::T T;
-  constexpr int N = S::N;
-  __shared__ float2 table[kTable];
-  __shared__ long long at_b[kMaxTokens];
-  __shared__ int at_t[kMaxTokens];
-  const long long first = linear_block() * a.tokens, total = (long long)a.batch * a.t;
-  if (first >= total) return;
-  const int here = (int)min((long long)a.tokens, total - first);
+// Cosines and sines of `here` tokens from the workgroup's first on, and where those tokens are.
+__device__ __forceinline__ void form_angles(const Args& a, long long first, int here, float2* table, long long* at_b,
+                                            int* at_t) {
   const int pairs = a.pairs;
   for (int e = threadIdx.x; e < here * pairs; e += kThreads) {
     const int token = e / pairs, i = e % pairs;
@@ -77,6 +74,22 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(const Args a) {
       at_t[token] = (int)t;
     }
   }
+}
+
+// kVec: vectors of 16 bytes; otherwise one pair, or one copied channel, per thread.
+template <int kDtype, bool kAdjacent, bool kVec>
+__global__ __launch_bounds__(kThreads) void rotary_kernel(const Args a) {
+  using S = Storage<kDtype>;
+  typedef typename S::T T;
+  constexpr int N = S::N;
+  __shared__ float2 table[kTable];
+  __shared__ long long at_b[kMaxTokens];
+  __shared__ int at_t[kMaxTokens];
+  const long long first = linear_block() * a.tokens, total = (long long)a.batch * a.t;
+  if (first >= total) return;
+  const int here = (int)min((long long)a.tokens, total - first);
+  const int pairs = a.pairs;
+  form_angles(a, first, here, table, at_b, at_t);
   __syncthreads();
   const int heads = a.q.heads + a.k.heads;
   const int all = here * heads * a.items;
@@ -136,6 +149,201 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(const Args a) {
   }
 }
 
+struct Norm {
+  const void* w[2];   // of q and k, or null
+  long long w_sh[2];  // elements between the weights of two heads, 0: shared
+  int w_dtype[2];
+  uint32_t by_heads[2];
+  float eps;
+  int lane_bits;      // a head is held by 2^lane_bits neighbouring lanes
+};
+
+// Sum over groups of 2^bits neighbouring lanes, by lane-crossing moves up to 16 of them.
+__device__ __forceinline__ float group_sum(float v, int bits) {
+  const auto with = [&](auto move) {
+    v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), decltype(move)::value, 0xf, 0xf, true));
+  };
+  if (bits > 0) with(std::integral_constant<int, 0xb1>{});   // lane ^ 1
+  if (bits > 1) with(std::integral_constant<int, 0x4e>{});   // lane ^ 2
+  if (bits > 2) with(std::integral_constant<int, 0x141>{});  // the other half of 8
+  if (bits > 3) with(std::integral_constant<int, 0x140>{});  // the other half of 16
+  if (bits > 4) v += __shfl_xor(v, 16, kWave);
+  if (bits > 5) v += __shfl_xor(v, 32, kWave);
+  return v;
+}
+
+// N values of a weight in the storage type or fp32.
+template <int kDtype, int N>
+__device__ __forceinline__ void load_weight(const void* w, int dtype, long long at, float (&v)[N]) {
+  typedef typename Storage<kDtype>::T T;
+  if (dtype == kDtype) {
+    typedef T Vec __attribute__((ext_vector_type(N)));
+    const Vec x = *reinterpret_cast<const Vec*>(static_cast<const T*>(w) + at);
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = (float)x[j];
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; j += 4) {
+      const float4 x = *reinterpret_cast<const float4*>(static_cast<const float*>(w) + at + j);
+      v[j] = x.x, v[j + 1] = x.y, v[j + 2] = x.z, v[j + 3] = x.w;
+    }
+  }
+}
+
+// Vectors of N elements: a lane holds one of a head's turned items (two vectors of a half each, or
+// one of neighbouring pairs) or one vector of the channels that do not turn.  The loads of kHeads heads
+// are in flight together, the first ones while the angles are formed.
+template <int kDtype, bool kAdjacent, int N>
+__global__ __launch_bounds__(kThreads) void norm_rotary_kernel(const Args a, const Norm n) {
+  typedef typename Storage<kDtype>::T T;
+  typedef T Vec __attribute__((ext_vector_type(N)));
+  constexpr int kHeads = 4;
+  __shared__ float2 table[kTable];
+  __shared__ long long at_b[kMaxTokens];
+  __shared__ int at_t[kMaxTokens];
+  const long long first = linear_block() * a.tokens, total = (long long)a.batch * a.t;
+  if (first >= total) return;
+  const int here = (int)min((long long)a.tokens, total - first);
+  const int pairs = a.pairs, tid = threadIdx.x;
+  if (tid < here) {
+    at_b[tid] = (first + tid) / a.t;
+    at_t[tid] = (int)((first + tid) % a.t);
+  }
+  __syncthreads();
+  const int group = tid >> n.lane_bits, item = tid & ((1 << n.lane_bits) - 1), groups = kThreads >> n.lane_bits;
+  const int turned = kAdjacent ? 2 * pairs / N : pairs / N;
+  const bool live = item < a.items, turns = item < turned, two = !kAdjacent && turns;
+  const int c0 = turns ? item * N : 2 * pairs + (item - turned) * N, c1 = pairs + item * N;
+  bool formed = false;
+#pragma unroll 1
+  for (int which = 0; which < 2; ++which) {
+    const Side& side = which ? a.k : a.q;
+    const int heads = side.heads, all = here * heads;
+    const void* w = n.w[which];
+    float w0[N], w1[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) w0[j] = w1[j] = 1.f;
+    if (w && live && n.w_sh[which] == 0) {
+      load_weight<kDtype, N>(w, n.w_dtype[which], c0, w0);
+      if (two) load_weight<kDtype, N>(w, n.w_dtype[which], c1, w1);
+    }
+    for (int from = 0; from < all; from += kHeads * groups) {
+      Vec x0[kHeads], x1[kHeads];
+      int token[kHeads], head[kHeads];
+#pragma unroll
+      for (int u = 0; u < kHeads; ++u) {
+        const int h = from + u * groups + group;
+        x0[u] = Vec{}, x1[u] = Vec{};
+        token[u] = over(h, n.by_heads[which]);
+        head[u] = h - token[u] * heads;
+        if (live && h < all) {
+          const T* x = static_cast<const T*>(side.x) + at_b[token[u]] * side.sb + at_t[token[u]] * side.st + head[u] * side.sh;
+          x0[u] = *reinterpret_cast<const Vec*>(x + c0);
+          if (two) x1[u] = *reinterpret_cast<const Vec*>(x + c1);
+        }
+      }
+      if (!formed) {
+        form_angles(a, first, here, table, at_b, at_t);
+        __syncthreads();
+        formed = true;
+      }
+#pragma unroll
+      for (int u = 0; u < kHeads; ++u) {
+        float q = 0.f, v0[N], v1[N];
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+          v0[j] = (float)x0[u][j], v1[j] = (float)x1[u][j];
+          q = fmaf(v0[j], v0[j], q);
+          if (!kAdjacent) q = fmaf(v1[j], v1[j], q);
+        }
+        const float rstd = 1.f / sqrtf(group_sum(q, n.lane_bits) / (float)a.dim + n.eps);
+        const int h = from + u * groups + group;
+        if (!live || h >= all) continue;
+        if (w && n.w_sh[which]) {
+          load_weight<kDtype, N>(w, n.w_dtype[which], head[u] * n.w_sh[which] + c0, w0);
+          if (two) load_weight<kDtype, N>(w, n.w_dtype[which], head[u] * n.w_sh[which] + c1, w1);
+        }
+#pragma unroll
+        for (int j = 0; j < N; ++j) v0[j] = v0[j] * rstd * w0[j], v1[j] = v1[j] * rstd * w1[j];
+        T* y = static_cast<T*>(side.y) + at_b[token[u]] * side.ob + at_t[token[u]] * side.ot + head[u] * side.oh;
+        Vec y0, y1;
+        if (turns) {
+          const float2* cs = table + token[u] * pairs + (kAdjacent ? item * (N / 2) : item * N);
+          if constexpr (kAdjacent) {
+#pragma unroll
+            for (int j = 0; j < N; j += 2) {
+              const float2 r = cs[j / 2];
+              const float p = v0[j];
+              v0[j] = p * r.x - v0[j + 1] * r.y;
+              v0[j + 1] = v0[j + 1] * r.x + p * r.y;
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+              const float2 r = cs[j];
+              const float p = v0[j];
+              v0[j] = p * r.x - v1[j] * r.y;
+              v1[j] = v1[j] * r.x + p * r.y;
+            }
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < N; ++j) y0[j] = (T)v0[j], y1[j] = (T)v1[j];
+        *reinterpret_cast<Vec*>(y + c0) = y0;
+        if (two) *reinterpret_cast<Vec*>(y + c1) = y1;
+      }
+    }
+  }
+}
+
+// Any alignment: a wave a head, a pair or a channel that does not turn per lane at a time, in two passes.
+template <int kDtype, bool kAdjacent>
+__global__ __launch_bounds__(kThreads) void norm_rotary_any_kernel(const Args a, const Norm n) {
+  using S = Storage<kDtype>;
+  typedef typename S::T T;
+  __shared__ float2 table[kTable];
+  __shared__ long long at_b[kMaxTokens];
+  __shared__ int at_t[kMaxTokens];
+  const long long first = linear_block() * a.tokens, total = (long long)a.batch * a.t;
+  if (first >= total) return;
+  const int here = (int)min((long long)a.tokens, total - first);
+  const int pairs = a.pairs, lane = threadIdx.x % kWave;
+  form_angles(a, first, here, table, at_b, at_t);
+  __syncthreads();
+  const int heads = a.q.heads + a.k.heads;
+  for (int h = threadIdx.x / kWave; h < here * heads; h += kThreads / kWave) {
+    const int token = h / heads, which = h % heads >= a.q.heads;
+    const int head = h % heads - (which ? a.q.heads : 0);
+    const Side& side = which ? a.k : a.q;
+    const T* x = static_cast<const T*>(side.x) + at_b[token] * side.sb + at_t[token] * side.st + head * side.sh;
+    T* y = static_cast<T*>(side.y) + at_b[token] * side.ob + at_t[token] * side.ot + head * side.oh;
+    float q = 0.f;
+    for (int c = lane; c < a.dim; c += kWave) {
+      const float v = S::one(x[c]);
+      q = fmaf(v, v, q);
+    }
+    const float rstd = 1.f / sqrtf(group_sum(q, 6) / (float)a.dim + n.eps);
+    const auto normed = [&](int c) {
+      const long long at = head * n.w_sh[which] + c;
+      const float w = !n.w[which]                    ? 1.f
+                      : n.w_dtype[which] == kDtype ? S::one(static_cast<const T*>(n.w[which])[at])
+                                                   : static_cast<const float*>(n.w[which])[at];
+      return S::one(x[c]) * rstd * w;
+    };
+    for (int i = lane; i < a.items; i += kWave) {
+      if (i >= pairs) {
+        y[pairs + i] = S::round(normed(pairs + i));
+      } else {
+        const int c0 = kAdjacent ? 2 * i : i, c1 = kAdjacent ? c0 + 1 : pairs + i;
+        const float2 r = table[token * pairs + i];
+        const float p = normed(c0), s = normed(c1);
+        y[c0] = S::round(p * r.x - s * r.y);
+        y[c1] = S::round(s * r.x + p * r.y);
+      }
+    }
+  }
+}
+
 template <int kDtype>
 void launch(const Args& a, bool adjacent, bool vec, dim3 grid, hipStream_t stream) {
   if (adjacent) {
@@ -147,13 +355,31 @@ void launch(const Args& a, bool adjacent, bool vec, dim3 grid, hipStream_t strea
   }
 }
 
-}  // namespace rotary
-}  // namespace musc
+// vec: elements of a vector, 0 for any alignment.
+template <int kDtype>
+void launch_normed(const Args& a, const Norm& n, bool adjacent, int vec, dim3 grid, hipStream_t stream) {
+#define MUSC_NORM_ROTARY(...) hipLaunchKernelGGL((__VA_ARGS__), grid, dim3(kThreads), 0, stream, a, n)
+  if (vec == 0) {
+    if (adjacent) MUSC_NORM_ROTARY(norm_rotary_any_kernel<kDtype, true>);
+    else MUSC_NORM_ROTARY(norm_rotary_any_kernel<kDtype, false>);
+    return;
+  }
+  if constexpr (kDtype != MUSC_DTYPE_F32) {
+    if (vec == 8) {
+      if (adjacent) MUSC_NORM_ROTARY(norm_rotary_kernel<kDtype, true, 8>);
+      else MUSC_NORM_ROTARY(norm_rotary_kernel<kDtype, false, 8>);
+      return;
+    }
+  }
+  if (adjacent) MUSC_NORM_ROTARY(norm_rotary_kernel<kDtype, true, 4>);
+  else MUSC_NORM_ROTARY(norm_rotary_kernel<kDtype, false, 4>);
+#undef MUSC_NORM_ROTARY
+}
 
-using namespace musc;
+inline uint32_t reciprocal(long long n) { return n > 1 ? (uint32_t)((0x100000000ULL + n - 1) / n) : 0; }
 
-extern "C" int musc_rotary(const musc_rotary_call* call, hipStream_t stream) {
-  using namespace rotary;
+// Checks a call and fills in what both kernels' arguments share.
+int arguments(const musc_rotary_call* call, Args& a) {
   if (!call) return MUSC_ERR_INVALID_ARG;
   const auto& [q, q_sb, q_st, q_sh, q_out, qo_sb, qo_st, qo_sh, k, k_sb, k_st, k_sh, k_out, ko_sb, ko_st, ko_sh, positions,
                pos_sb, frequency, axis, q_heads, k_heads, dtype, batch, t, d, int_positions, axes, pairs, adjacent,
@@ -175,13 +401,6 @@ extern "C" int musc_rotary(const musc_rotary_call* call, hipStream_t stream) {
   if ((reinterpret_cast<uintptr_t>(positions) & 3) || (reinterpret_cast<uintptr_t>(frequency) & 7) ||
       (reinterpret_cast<uintptr_t>(axis) & 3))
     return MUSC_ERR_INVALID_ARG;
-  if (total == 0) return MUSC_OK;
-  const int n = dtype == MUSC_DTYPE_F32 ? 4 : 8;
-  const long long strides = q_sb | q_st | q_sh | qo_sb | qo_st | qo_sh |
-                            (k_heads ? k_sb | k_st | k_sh | ko_sb | ko_st | ko_sh : 0);
-  const bool vec = data % 16 == 0 && strides % n == 0 && d % n == 0 && (adjacent ? 2 * pairs : pairs) % n == 0 &&
-                   (2 * pairs) % n == 0;
-  Args a{};
   a.q = Side{q, q_out, q_sb, q_st, q_sh, qo_sb, qo_st, qo_sh, q_heads};
   a.k = Side{k, k_out, k_sb, k_st, k_sh, ko_sb, ko_st, ko_sh, k_heads};
   a.positions = positions;
@@ -189,21 +408,85 @@ extern "C" int musc_rotary(const musc_rotary_call* call, hipStream_t stream) {
   a.frequency = frequency;
   a.axis = axis;
   a.batch = batch, a.t = t, a.axes = axes, a.pairs = pairs, a.dim = d, a.int_positions = int_positions;
-  a.items = vec ? (adjacent ? 2 * pairs / n : pairs / n) + (d - 2 * pairs) / n : pairs + (d - 2 * pairs);
-  a.by_items = a.items > 1 ? (uint32_t)((0x100000000ULL + a.items - 1) / a.items) : 0;
-  a.by_heads = heads > 1 ? (uint32_t)((0x100000000ULL + heads - 1) / heads) : 0;
   a.sign = inverse ? -1.f : 1.f;
   // tokens of a workgroup: one sincos per thread, while there are workgroups for every CU
-  int tokens = kThreads / pairs > 1 ? kThreads / pairs : 1;
-  if (tokens > kMaxTokens) tokens = kMaxTokens;
-  while (tokens > 1 && total / tokens < 512) --tokens;
+  a.tokens = kThreads / pairs > 1 ? kThreads / pairs : 1;
+  if (a.tokens > kMaxTokens) a.tokens = kMaxTokens;
+  while (a.tokens > 1 && total / a.tokens < 512) --a.tokens;
+  return MUSC_OK;
+}
+
+// Whether every vector of n elements starts on its own size.
+bool vectors(const musc_rotary_call& c, int n) {
+  const uintptr_t data = reinterpret_cast<uintptr_t>(c.q) | reinterpret_cast<uintptr_t>(c.q_out) |
+                         (c.k_heads ? reinterpret_cast<uintptr_t>(c.k) | reinterpret_cast<uintptr_t>(c.k_out) : 0);
+  const long long strides = c.q_sb | c.q_st | c.q_sh | c.q_ob | c.q_ot | c.q_oh |
+                            (c.k_heads ? c.k_sb | c.k_st | c.k_sh | c.k_ob | c.k_ot | c.k_oh : 0);
+  return data % (n * (c.dtype == MUSC_DTYPE_F32 ? 4 : 2)) == 0 && strides % n == 0 && c.d % n == 0 &&
+         (c.adjacent ? 2 * c.pairs : c.pairs) % n == 0;
+}
+int items_of(const musc_rotary_call& c, int n) {
+  return n ? (c.adjacent ? 2 * c.pairs / n : c.pairs / n) + (c.d - 2 * c.pairs) / n : c.pairs + (c.d - 2 * c.pairs);
+}
+
+}  // namespace rotary
+}  // namespace musc
+
+using namespace musc;
+
+extern "C" int musc_rotary(const musc_rotary_call* call, hipStream_t stream) {
+  using namespace rotary;
+  Args a{};
+  if (const int rc = arguments(call, a)) return rc;
+  const long long total = (long long)a.batch * a.t, heads = (long long)a.q.heads + a.k.heads;
+  if (total == 0) return MUSC_OK;
+  const int n = call->dtype == MUSC_DTYPE_F32 ? 4 : 8;
+  const bool vec = vectors(*call, n), adjacent = call->adjacent;
+  a.items = items_of(*call, vec ? n : 0);
+  a.by_items = reciprocal(a.items);
+  a.by_heads = reciprocal(heads);
   // the reciprocals divide exactly below 2^32 / divisor (one token: 2^19 * 2^10 at most)
   const long long per_token = heads * a.items, divisor = heads > a.items ? heads : a.items;
-  while (tokens > 1 && tokens * per_token * divisor > 0xffffffffLL) --tokens;
-  a.tokens = tokens;
-  const dim3 grid = linear_grid((total + tokens - 1) / tokens);
-  if (dtype == MUSC_DTYPE_F32) launch<MUSC_DTYPE_F32>(a, adjacent, vec, grid, stream);
-  else if (dtype == MUSC_DTYPE_F16) launch<MUSC_DTYPE_F16>(a, adjacent, vec, grid, stream);
+  while (a.tokens > 1 && a.tokens * per_token * divisor > 0xffffffffLL) --a.tokens;
+  const dim3 grid = linear_grid((total + a.tokens - 1) / a.tokens);
+  if (call->dtype == MUSC_DTYPE_F32) launch<MUSC_DTYPE_F32>(a, adjacent, vec, grid, stream);
+  else if (call->dtype == MUSC_DTYPE_F16) launch<MUSC_DTYPE_F16>(a, adjacent, vec, grid, stream);
   else launch<MUSC_DTYPE_BF16>(a, adjacent, vec, grid, stream);
+  return check_launch();
+}
+
+extern "C" int musc_norm_rotary(const musc_rotary_call* call, const void* q_weight, long long q_weight_sh,
+                                int q_weight_dtype, const void* k_weight, long long k_weight_sh, int k_weight_dtype,
+                                float eps, hipStream_t stream) {
+  using namespace rotary;
+  Args a{};
+  if (const int rc = arguments(call, a)) return rc;
+  Norm n{{q_weight, a.k.heads ? k_weight : nullptr}, {q_weight_sh, k_weight_sh}, {q_weight_dtype, k_weight_dtype}};
+  const int dtype = call->dtype;
+  if (!(eps >= 0.f)) return MUSC_ERR_INVALID_ARG;
+  // largest vectors (of up to 64 lanes a head) that start on their own size, weights on 16 bytes at most
+  int vec = dtype == MUSC_DTYPE_F32 ? 4 : 8;
+  while (vec >= 4 && (!vectors(*call, vec) || items_of(*call, vec) > kWave)) vec /= 2;
+  for (int i = 0; i < 2; ++i) {
+    if (!n.w[i]) continue;
+    const int size = n.w_dtype[i] == MUSC_DTYPE_F32 ? 4 : 2;
+    if (n.w_dtype[i] != dtype && n.w_dtype[i] != MUSC_DTYPE_F32) return MUSC_ERR_INVALID_ARG;
+    const uintptr_t at = reinterpret_cast<uintptr_t>(n.w[i]);
+    if (at % size || n.w_sh[i] < 0) return MUSC_ERR_INVALID_ARG;
+    const int bytes = vec * size < 16 ? vec * size : 16;
+    if (vec >= 4 && (at % bytes || n.w_sh[i] * size % bytes)) vec = 0;
+  }
+  const long long total = (long long)a.batch * a.t;
+  if (total == 0) return MUSC_OK;
+  if (vec < 4) vec = 0;
+  a.items = items_of(*call, vec);
+  while (vec && a.items > 1 << n.lane_bits) ++n.lane_bits;
+  n.by_heads[0] = reciprocal(a.q.heads), n.by_heads[1] = reciprocal(a.k.heads);
+  n.eps = eps;
+  const dim3 grid = linear_grid((total + a.tokens - 1) / a.tokens);
+  const bool adjacent = call->adjacent;
+  if (dtype == MUSC_DTYPE_F32) launch_normed<MUSC_DTYPE_F32>(a, n, adjacent, vec, grid, stream);
+  else if (dtype == MUSC_DTYPE_F16) launch_normed<MUSC_DTYPE_F16>(a, n, adjacent, vec, grid, stream);
+  else launch_normed<MUSC_DTYPE_BF16>(a, n, adjacent, vec, grid, stream);
   return check_launch();
 }

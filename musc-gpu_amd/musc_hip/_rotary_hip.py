@@ -3,7 +3,8 @@
 For encoders of images and video of any size, whose blocks turn q and k by the token's place
 instead of adding a position embedding of one grid (the reference's encoder does the latter).
 q and k are read in place from a packed projection; all heads of a token share its angles, whose
-whole turns are taken off in float64.
+whole turns are taken off in float64.  norm_rotary takes the root-mean-square norm of every head first, in
+the same pass (musc_norm_rotary).
 """
 from __future__ import annotations
 
@@ -55,18 +56,25 @@ def _head_rows(x, name, axes):
     return x if x.stride(-1) == 1 else x.contiguous()
 
 
-def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, axes: RotaryAxes, inverse: bool = False,
-           out=None):
-    """(q, k) turned by their tokens' positions, or q alone where k is None.
+def _head_weight(weight, name, x):
+    """(tensor, elements between the weights of two heads, storage) of a head norm's weight."""
+    rt.require_device_tensor(weight, name)
+    rt.require_no_gradient(weight)
+    h, d = x.shape[2:]
+    if (weight.get_device() != x.get_device() or weight.dtype not in (x.dtype, torch.float32)
+            or (weight.shape != (d,) and weight.shape != (h, d))):
+        raise ValueError(f"{name} must be ({d},) or ({h}, {d}) on its input's device, in its dtype or float32")
+    weight = weight.contiguous()
+    if weight.data_ptr() % 16:
+        weight = weight.clone()     # read as 16-byte vectors
+    return weight, d if weight.dim() == 2 else 0, _STORAGE[weight.dtype]
 
-    q (B, T, heads, D), k (B, T, kv_heads, D), any strides with a contiguous last dimension;
-    positions (T, axes) or (B, T, axes), float32 or int32.  inverse turns back (the transpose).
-    out: the tensors to write, (q_out, k_out) or q_out; they may be q and k themselves, and may
-    not overlap them otherwise.  No derivative."""
+
+def _turn(q, k, positions, axes, inverse, out, norm):
     q2 = _head_rows(q, 'q', axes)
     if rt.elsewhere(q):
         with torch.cuda.device(q.device):
-            return rotary(q, k, positions, axes, inverse, out)
+            return _turn(q, k, positions, axes, inverse, out, norm)
     rt.require_no_gradient(q, k, positions, *(out if isinstance(out, (tuple, list)) else (out,)))
     index = q.get_device()
     b, t, h, d = q2.shape
@@ -85,6 +93,10 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, axe
     if axes.frequency.get_device() != index:
         raise ValueError("axes must be on q's device")
     positions = positions.contiguous()
+    weights = []
+    if norm is not None:
+        for weight, name, x in ((norm[0], 'q_weight', q2), (norm[1], 'k_weight', k2)):
+            weights.append((None, 0, rt.DTYPE_F32) if weight is None or x is None else _head_weight(weight, name, x))
     if k2 is not None:
         ko = rt.output_like(out[1] if out is not None else None, k2, 'k_out')
         if k2.shape[2]:
@@ -97,7 +109,37 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, axe
             q2.data_ptr(), *rt.token_strides(q2), qo.data_ptr(), *rt.token_strides(qo), *k_args, positions.data_ptr(),
             0 if len(shape) == 2 else t * axes.axes, axes.frequency.data_ptr(), axes.axis.data_ptr(), h, k_heads, _STORAGE[q2.dtype], b, t,
             d, positions.dtype == torch.int32, axes.axes, axes.pairs, axes.adjacent, inverse)
-        rt.check(rt.library().musc_rotary(call, rt.current_stream(index)), 'musc_rotary')
+        if norm is None:
+            rt.check(rt.library().musc_rotary(call, rt.current_stream(index)), 'musc_rotary')
+        else:
+            (qw, q_sh, q_type), (kw, k_sh, k_type) = weights
+            rt.check(rt.library().musc_norm_rotary(call, None if qw is None else qw.data_ptr(), q_sh, q_type,
+                                                   None if kw is None else kw.data_ptr(), k_sh, k_type, norm[2],
+                                                   rt.current_stream(index)), 'musc_norm_rotary')
     elif k_heads:
-        rotary(k2, None, positions, axes, inverse, ko)
+        _turn(k2, None, positions, axes, inverse, ko, None if norm is None else (norm[1], None, norm[2]))
     return qo if k is None else (qo, ko)
+
+
+def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, axes: RotaryAxes, inverse: bool = False,
+           out=None):
+    """(q, k) turned by their tokens' positions, or q alone where k is None.
+
+    q (B, T, heads, D), k (B, T, kv_heads, D), any strides with a contiguous last dimension;
+    positions (T, axes) or (B, T, axes), float32 or int32.  inverse turns back (the transpose).
+    out: the tensors to write, (q_out, k_out) or q_out; they may be q and k themselves, and may
+    not overlap them otherwise.  No derivative."""
+    return _turn(q, k, positions, axes, inverse, out, None)
+
+
+def norm_rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, axes: RotaryAxes, q_weight=None,
+                k_weight=None, eps: float = 1e-6, out=None):
+    """(q, k), or q alone where k is None, with every head's root-mean-square norm taken and then
+    turned by its token's position, in one pass and with one rounding.
+
+    y = x * weight / sqrt(mean(x^2) + eps) over the D channels of a head, in float32; then rotary's
+    rotation of y.  q_weight, k_weight: (D,) for all heads or (heads, D), in the input's dtype or
+    float32; None: 1.  The sum of squares is float32: a head whose squares overflow it (bfloat16 and
+    float32 values past about 1e18) comes out as zeros.  The other arguments, the outputs and what they may
+    overlap are rotary's.  No derivative."""
+    return _turn(q, k, positions, axes, False, out, (q_weight, k_weight, float(eps)))

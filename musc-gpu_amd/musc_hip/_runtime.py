@@ -118,6 +118,7 @@ SIGNATURES = {
     'musc_rmsnorm_rows': (_i, [_vp, _ll, _vp, _ll, _vp, _vp, _i, _i, _i, _i, _f, _vp, _vp]),
     'musc_rmsnorm_rows_8bit': (_i, [_vp, _ll, _vp, _ll, _vp, _vp, _i, _i, _i, _i, _f, _i, _i, _vp, _vp, _vp]),
     'musc_rotary': (_i, [_vp, _vp]),
+    'musc_norm_rotary': (_i, [_vp, _vp, _ll, _i, _vp, _ll, _i, _f, _vp]),
     'musc_activation': (_i, [_vp, _vp, _i, _i, _ll, _vp]),
     'musc_calibrate_mfma_f32': (_i, [_vp, _i, _i, ctypes.POINTER(ctypes.c_double), _vp]),
     'musc_calibrate_mfma_f16': (_i, [_vp, _i, _i, ctypes.POINTER(ctypes.c_double), _vp]),
