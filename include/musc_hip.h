@@ -432,6 +432,31 @@ int musc_masked_attention_workspace_bytes(const musc_masked_attention* call, siz
 int musc_masked_attention_fwd(const musc_masked_attention* call, void* workspace, size_t workspace_bytes,
                               hipStream_t stream);
 
+/* The same with a sliding window and sinks: of the keys above, query i sees
+ *   order(j) > order(i) - window (its own place and the window - 1 before it) or 0 <= order(j) < sinks.
+ * window >= 1, sinks >= 0, with orders on both sides.  Tiles that
+ * no row of a workgroup sees are not read.  call->schedule is not used. */
+int musc_window_attention_workspace_bytes(const musc_masked_attention* call, int window, int sinks, size_t* out);
+int musc_window_attention_fwd(const musc_masked_attention* call, int window, int sinks, void* workspace,
+                              size_t workspace_bytes, hipStream_t stream);
+
+/* The same after a prefix that the whole batch shares: every query that has a document (all of them
+ * in a call without documents) sees each of its len keys, and of the call's own keys those above.
+ * Where the entries have few rows each, the rows of all of them pass over the prefix together.
+ * k and v have heads of the call's d channels at token * st + head * sh, by the rules of the call's K and V;
+ * positions: float32 (len, axes) rows, needed with call->axes.  len >= 1; call->k_len may be 0 (no own
+ * keys; what is given of them is then not looked at).  call->schedule is not used. */
+typedef struct musc_attention_prefix {
+  const void *k, *v;
+  long long k_st, k_sh, v_st, v_sh;
+  const float* positions;
+  int len;
+} musc_attention_prefix;
+int musc_prefix_attention_workspace_bytes(const musc_masked_attention* call, const musc_attention_prefix* prefix,
+                                          size_t* out);
+int musc_prefix_attention_fwd(const musc_masked_attention* call, const musc_attention_prefix* prefix, void* workspace,
+                              size_t workspace_bytes, hipStream_t stream);
+
 /* Root-mean-square norm of the rows of (rows, width) x, row strides in elements (the last
  * dimension contiguous), dtype MUSC_DTYPE_F32, _F16 or _BF16, fp32 statistics:
  *   s = x + residual rounded to the dtype, written to the contiguous sum_out (residual == NULL:

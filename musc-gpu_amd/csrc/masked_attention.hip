@@ -158,6 +158,22 @@ __global__ __launch_bounds__(1024) void row_order_kernel(const Schedule s, int s
   for (int p = 0; p < of; ++p) jobs_at[p] = tile | p << 20 | (of - 1) << 23;
 }
 
+// The grid: what a workgroup's number means, and whether it fits.
+int finish(Args& a, long long heads, int waves) {
+  a.units = heads * a.jobs * a.splits;
+  // Heads that an XCD (32 CUs, 2 or 3 workgroups each) works on together: enough for two rounds of
+  // workgroups, so that short work fills the gaps of long work, and no more, as they share its L2.
+  // 0: the heads do not divide over the XCDs.
+  a.heads_at_once = 0;
+  if (heads % kXcds == 0) {
+    const long long enough = (128 + a.row_tiles - 1) / a.row_tiles, per_xcd = heads / kXcds;
+    a.heads_at_once = (int)(enough < per_xcd ? enough : per_xcd);
+  }
+  // a grid dimension holds fewer than 2^32 threads, 256 or (teams) up to 512 a workgroup
+  if (a.units >= (0x100000000LL >> (a.teams > 1 ? 9 : 8))) return MUSC_ERR_UNSUPPORTED;
+  return MUSC_OK;
+}
+
 // Shape of the launch: rows per workgroup, tiles and splits.
 int plan(const musc_masked_attention& c, Args& a, int& waves) {
   a.c = c;
@@ -205,25 +221,68 @@ int plan(const musc_masked_attention& c, Args& a, int& waves) {
     if (splits > kMaxSplits) splits = kMaxSplits;
     a.splits = splits < 1 ? 1 : (int)splits;
   }
-  a.units = heads * a.jobs * a.splits;
-  // Heads that an XCD (32 CUs, 2 or 3 workgroups each) works on together: enough for two rounds of
-  // workgroups, so that short work fills the gaps of long work, and no more, as they share its L2.
-  // 0: the heads do not divide over the XCDs.
-  a.heads_at_once = 0;
-  if (heads % kXcds == 0) {
-    const long long enough = (128 + a.row_tiles - 1) / a.row_tiles, per_xcd = heads / kXcds;
-    a.heads_at_once = (int)(enough < per_xcd ? enough : per_xcd);
+  return finish(a, heads, waves);
+}
+
+// Windows: the same shapes without a schedule, whose work does not know of the window.  Splits take every
+// n-th tile of those that a row tile sees.
+int plan_window(const musc_masked_attention& c, int window, int sinks, Args& a, int& waves) {
+  musc_masked_attention call = c;
+  call.schedule = nullptr;
+  a.window = window, a.sinks = sinks;
+  return plan(call, a, waves);
+}
+
+// Shape of one launch after a prefix: the rows of `batches` entries over p_tiles of the prefix and the own
+// keys, if any.
+int shape(Args& a, long long rows, int batches, bool of_prefix, bool of_own, int most_splits, int& waves) {
+  const musc_masked_attention& c = a.c;
+  if (rows > 0x7fffff00LL) return MUSC_ERR_UNSUPPORTED;
+  a.rows = (int)rows, a.batches = batches;
+  waves = rows <= 32 ? 1 : 4;
+  const int tile = waves == 1 || c.dtype == MUSC_DTYPE_F32 ? 32 : 64;
+  a.row_tiles = (int)((rows + 32 * waves - 1) / (32 * waves));
+  a.p_tiles = of_prefix ? (a.p.len + tile - 1) / tile : 0;
+  a.key_tiles = a.p_tiles + (of_own ? (c.k_len + tile - 1) / tile : 0);
+  a.summaries = (c.k_len + kSummaryKeys - 1) / kSummaryKeys;
+  a.jobs = a.row_tiles, a.teams = 1, a.splits = 1;
+  const long long heads = (long long)batches * c.kv_heads, whole = heads * a.row_tiles;
+  if (whole < (waves == 1 ? 1024 : 256)) {
+    long long splits = ((waves == 1 ? 2048 : 512) + whole - 1) / whole;
+    const int least = waves == 1 ? 1 : 4;
+    if (splits > a.key_tiles / least) splits = a.key_tiles / least;
+    if (splits > most_splits) splits = most_splits;
+    a.splits = splits < 1 ? 1 : (int)splits;
   }
-  // a grid dimension holds fewer than 2^32 threads, 256 or (teams) up to 512 a workgroup
-  if (a.units >= (0x100000000LL >> (a.teams > 1 ? 9 : 8))) return MUSC_ERR_UNSUPPORTED;
-  return MUSC_OK;
+  return finish(a, heads, waves);
+}
+
+// After a prefix: each entry's rows over it and their own keys in one launch, or, where the tiles of the
+// entries' few rows would leave places empty, the rows of all entries over the prefix, and then each entry's
+// over its own keys (more).
+int plan_prefix(const musc_masked_attention& c, const musc_attention_prefix& p, Args& a, int& waves, Args& more,
+                int& more_waves) {
+  a.c = c, a.p = p;
+  a.c.schedule = nullptr;
+  a.group = c.heads / c.kv_heads;
+  const long long rows = (long long)c.q_len * a.group, all = rows * c.batch;
+  if (p.len > 0x7fffff00 || c.k_len > 0x7fffff00) return MUSC_ERR_UNSUPPORTED;
+  const long long apart = c.batch * ((rows + kRowTile - 1) / kRowTile), together = (all + kRowTile - 1) / kRowTile;
+  a.stacked = c.batch > 1 && 2 * apart >= 3 * together && all * c.kv_heads < (1 << 24);
+  more = a;
+  if (!a.stacked) return shape(a, rows, c.batch, true, true, kMaxSplits, waves);
+  a.partial = 1;
+  if (const int rc = shape(a, all, 1, true, false, kMaxSplits / 2, waves)) return rc;
+  if (c.k_len == 0) return MUSC_OK;
+  more.partial = 1, more.stacked = 0;
+  return shape(more, rows, c.batch, false, true, kMaxSplits / 2, more_waves);
 }
 
 // Rows that write parts: of every split, or of every job.
 size_t part_rows(const Args& a) {
-  const size_t heads = (size_t)a.c.batch * a.c.kv_heads;
+  const size_t heads = (size_t)(a.batches ? a.batches : a.c.batch) * a.c.kv_heads;
   if (a.in_parts) return heads * a.jobs * kRowTile;
-  return a.splits == 1 ? 0 : heads * a.rows * a.splits;
+  return a.splits == 1 && !a.partial ? 0 : heads * a.rows * a.splits;
 }
 size_t part_bytes(const Args& a) {
   const size_t rows = part_rows(a);
@@ -235,10 +294,18 @@ inline bool aligned(const void* p, long long sb, long long st, long long sh, int
   return reinterpret_cast<uintptr_t>(p) % 16 == 0 && sb >= 0 && st >= 0 && sh >= 0 && (sb | st | sh) % per == 0;
 }
 
-int check(const musc_masked_attention* c) {
-  if (!c || !c->q || !c->k || !c->v || !c->out) return MUSC_ERR_INVALID_ARG;
+// 64 rows of K or V reach less than 2 GiB
+inline bool reachable(long long st, int d, int size) {
+  return st <= kNowhere && (63 * st + d) * size <= kNowhere - 16;
+}
+
+// keyless: there may be no own keys (k_len 0), after a prefix
+int check(const musc_masked_attention* c, bool keyless = false) {
+  if (!c || !c->q || !c->out) return MUSC_ERR_INVALID_ARG;
+  const bool keys = !keyless || c->k_len != 0;
+  if (keys && (!c->k || !c->v)) return MUSC_ERR_INVALID_ARG;
   if (c->dtype != MUSC_DTYPE_F32 && c->dtype != MUSC_DTYPE_F16 && c->dtype != MUSC_DTYPE_BF16) return MUSC_ERR_INVALID_ARG;
-  if (c->batch < 1 || c->q_len < 1 || c->k_len < 1 || c->heads < 1 || c->kv_heads < 1 || c->heads % c->kv_heads)
+  if (c->batch < 1 || c->q_len < 1 || (keys && c->k_len < 1) || c->heads < 1 || c->kv_heads < 1 || c->heads % c->kv_heads)
     return MUSC_ERR_INVALID_ARG;
   // scores, slopes and the cap are taken relative to one another
   const float least = 0x1p-60f, most = 0x1p60f;
@@ -246,17 +313,15 @@ int check(const musc_masked_attention* c) {
   if (!(fabsf(c->scale) <= most) || (c->scale != 0.f && fabsf(c->scale) < least)) return MUSC_ERR_INVALID_ARG;
   const int per = c->dtype == MUSC_DTYPE_F32 ? 4 : 8, size = 16 / per;
   if (c->d < 1 || c->d > 128 || c->d % per) return MUSC_ERR_UNSUPPORTED;
-  if (!aligned(c->q, c->q_sb, c->q_st, c->q_sh, per) || !aligned(c->k, c->k_sb, c->k_st, c->k_sh, per) ||
-      !aligned(c->v, c->v_sb, c->v_st, c->v_sh, per) || !aligned(c->out, c->o_sb, c->o_st, c->o_sh, per))
+  if (!aligned(c->q, c->q_sb, c->q_st, c->q_sh, per) || !aligned(c->out, c->o_sb, c->o_st, c->o_sh, per) ||
+      (keys && (!aligned(c->k, c->k_sb, c->k_st, c->k_sh, per) || !aligned(c->v, c->v_sb, c->v_st, c->v_sh, per))))
     return MUSC_ERR_INVALID_ARG;
-  if (c->k_st > kNowhere || c->v_st > kNowhere || (63 * c->k_st + c->d) * size > kNowhere - 16 ||
-      (63 * c->v_st + c->d) * size > kNowhere - 16)
-    return MUSC_ERR_UNSUPPORTED;
+  if (keys && (!reachable(c->k_st, c->d, size) || !reachable(c->v_st, c->d, size))) return MUSC_ERR_UNSUPPORTED;
   // documents on both sides and the keys' summary, or none; orders and positions likewise
-  if (!c->q_documents != !c->k_documents || !c->k_documents != !c->k_summary) return MUSC_ERR_INVALID_ARG;
-  if (!c->q_order != !c->k_order || (c->q_order && !c->q_documents)) return MUSC_ERR_INVALID_ARG;
+  if (keys && (!c->q_documents != !c->k_documents || !c->k_documents != !c->k_summary)) return MUSC_ERR_INVALID_ARG;
+  if ((keys && !c->q_order != !c->k_order) || (c->q_order && !c->q_documents)) return MUSC_ERR_INVALID_ARG;
   if (c->axes < 0 || c->axes > kMaxAxes) return MUSC_ERR_UNSUPPORTED;
-  if (c->axes && (!c->q_positions || !c->k_positions || !c->slopes)) return MUSC_ERR_INVALID_ARG;
+  if (c->axes && (!c->q_positions || (keys && !c->k_positions) || !c->slopes)) return MUSC_ERR_INVALID_ARG;
   const uintptr_t words = reinterpret_cast<uintptr_t>(c->q_documents) | reinterpret_cast<uintptr_t>(c->k_documents) |
                           reinterpret_cast<uintptr_t>(c->q_order) | reinterpret_cast<uintptr_t>(c->k_order) |
                           reinterpret_cast<uintptr_t>(c->q_positions) | reinterpret_cast<uintptr_t>(c->k_positions) |
@@ -266,6 +331,31 @@ int check(const musc_masked_attention* c) {
        c->schedule_sb) < 0)
     return MUSC_ERR_INVALID_ARG;
   return MUSC_OK;
+}
+
+int check_window(const musc_masked_attention* c, int window, int sinks) {
+  if (const int rc = check(c)) return rc;
+  return window < 1 || sinks < 0 || !c->q_order ? MUSC_ERR_INVALID_ARG : MUSC_OK;
+}
+
+int check_prefix(const musc_masked_attention* c, const musc_attention_prefix* p) {
+  if (const int rc = check(c, true)) return rc;
+  if (!p || !p->k || !p->v || p->len < 1) return MUSC_ERR_INVALID_ARG;
+  const int per = c->dtype == MUSC_DTYPE_F32 ? 4 : 8, size = 16 / per;
+  if (!aligned(p->k, 0, p->k_st, p->k_sh, per) || !aligned(p->v, 0, p->v_st, p->v_sh, per)) return MUSC_ERR_INVALID_ARG;
+  if (!reachable(p->k_st, c->d, size) || !reachable(p->v_st, c->d, size)) return MUSC_ERR_UNSUPPORTED;
+  if (c->axes && (!p->positions || (reinterpret_cast<uintptr_t>(p->positions) & 3))) return MUSC_ERR_INVALID_ARG;
+  return MUSC_OK;
+}
+
+// Places of a launch's parts in the workspace; returns the bytes they take.
+size_t place_parts(Args& a, char* at) {
+  const size_t bytes = part_bytes(a);
+  if (bytes) {
+    a.part_ml = reinterpret_cast<float*>(at);
+    a.part_o = reinterpret_cast<float*>(at + align_up(part_rows(a) * 2 * sizeof(float), 256));
+  }
+  return bytes;
 }
 
 }  // namespace mattn
@@ -329,14 +419,64 @@ extern "C" int musc_masked_attention_fwd(const musc_masked_attention* c, void* w
   int waves;
   if (const int rc = mattn::plan(*c, a, waves)) return rc;
   const size_t need = mattn::part_bytes(a);
-  if (need) {
-    if (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16) return MUSC_ERR_WORKSPACE;
-    a.part_ml = static_cast<float*>(workspace);
-    a.part_o = reinterpret_cast<float*>(static_cast<char*>(workspace) +
-                                        align_up(mattn::part_rows(a) * 2 * sizeof(float), 256));
-  }
+  if (need && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16)) return MUSC_ERR_WORKSPACE;
+  mattn::place_parts(a, static_cast<char*>(workspace));
   if (c->dtype == MUSC_DTYPE_F32) mattn::launch_f32(a, waves, stream);
   else if (c->dtype == MUSC_DTYPE_F16) mattn::launch_f16(a, waves, stream);
   else mattn::launch_bf16(a, waves, stream);
+  return check_launch();
+}
+
+extern "C" int musc_window_attention_workspace_bytes(const musc_masked_attention* c, int window, int sinks, size_t* out) {
+  if (!out) return MUSC_ERR_INVALID_ARG;
+  if (const int rc = mattn::check_window(c, window, sinks)) return rc;
+  mattn::Args a{};
+  int waves;
+  if (const int rc = mattn::plan_window(*c, window, sinks, a, waves)) return rc;
+  *out = mattn::part_bytes(a);
+  return MUSC_OK;
+}
+
+extern "C" int musc_window_attention_fwd(const musc_masked_attention* c, int window, int sinks, void* workspace,
+                                         size_t workspace_bytes, hipStream_t stream) {
+  if (const int rc = mattn::check_window(c, window, sinks)) return rc;
+  mattn::Args a{};
+  int waves;
+  if (const int rc = mattn::plan_window(*c, window, sinks, a, waves)) return rc;
+  const size_t need = mattn::part_bytes(a);
+  if (need && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16)) return MUSC_ERR_WORKSPACE;
+  mattn::place_parts(a, static_cast<char*>(workspace));
+  if (c->dtype == MUSC_DTYPE_F32) mattn::launch_window_f32(a, waves, stream);
+  else if (c->dtype == MUSC_DTYPE_F16) mattn::launch_window_f16(a, waves, stream);
+  else mattn::launch_window_bf16(a, waves, stream);
+  return check_launch();
+}
+
+extern "C" int musc_prefix_attention_workspace_bytes(const musc_masked_attention* c, const musc_attention_prefix* p,
+                                                     size_t* out) {
+  if (!out) return MUSC_ERR_INVALID_ARG;
+  if (const int rc = mattn::check_prefix(c, p)) return rc;
+  mattn::Args a{}, more{};
+  int waves, more_waves;
+  if (const int rc = mattn::plan_prefix(*c, *p, a, waves, more, more_waves)) return rc;
+  *out = align_up(mattn::part_bytes(a), 256) + (a.stacked && c->k_len ? mattn::part_bytes(more) : 0);
+  return MUSC_OK;
+}
+
+extern "C" int musc_prefix_attention_fwd(const musc_masked_attention* c, const musc_attention_prefix* p, void* workspace,
+                                         size_t workspace_bytes, hipStream_t stream) {
+  if (const int rc = mattn::check_prefix(c, p)) return rc;
+  mattn::Args a{}, more{};
+  int waves, more_waves = 0;
+  if (const int rc = mattn::plan_prefix(*c, *p, a, waves, more, more_waves)) return rc;
+  const bool two = a.stacked && c->k_len;
+  const size_t first = align_up(mattn::part_bytes(a), 256), need = first + (two ? mattn::part_bytes(more) : 0);
+  if (need && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16)) return MUSC_ERR_WORKSPACE;
+  mattn::place_parts(a, static_cast<char*>(workspace));
+  if (two) mattn::place_parts(more, static_cast<char*>(workspace) + first);
+  const mattn::Args* own = two ? &more : nullptr;
+  if (c->dtype == MUSC_DTYPE_F32) mattn::launch_prefix_f32(a, waves, own, more_waves, stream);
+  else if (c->dtype == MUSC_DTYPE_F16) mattn::launch_prefix_f16(a, waves, own, more_waves, stream);
+  else mattn::launch_prefix_bf16(a, waves, own, more_waves, stream);
   return check_launch();
 }

@@ -146,6 +146,13 @@ struct Args {
   int in_pieces; // jobs may be the rows of a row tile before or from a document's start on
   int teams;     // waves that share few rows' keys within a workgroup
   int slots;     // workgroups that the card holds at a time
+  int window, sinks;  // of windowed attention
+  // prefixed attention: the prefix, its tiles (the first ones, may be none), batch entries of the grid (1 where
+  // the rows of all are stacked), and whether the rows' parts are joined even if there is one
+  musc_attention_prefix p;
+  int p_tiles, batches, stacked, partial;
+  int more_splits;    // its join: parts of the second launch
+  float *more_ml, *more_o;
   long long units;
   float* part_ml;  // (units in (b, kv head), rows, split) x (maximum, sum)
   float* part_o;   // the same x d
@@ -185,6 +192,12 @@ struct Range {
 void launch_f32(const Args& a, int waves, hipStream_t stream);
 void launch_f16(const Args& a, int waves, hipStream_t stream);
 void launch_bf16(const Args& a, int waves, hipStream_t stream);
+void launch_window_f32(const Args& a, int waves, hipStream_t stream);
+void launch_window_f16(const Args& a, int waves, hipStream_t stream);
+void launch_window_bf16(const Args& a, int waves, hipStream_t stream);
+void launch_prefix_f32(const Args& a, int waves, const Args* more, int more_waves, hipStream_t stream);
+void launch_prefix_f16(const Args& a, int waves, const Args* more, int more_waves, hipStream_t stream);
+void launch_prefix_bf16(const Args& a, int waves, const Args* more, int more_waves, hipStream_t stream);
 
 }  // namespace mattn
 }  // namespace musc

@@ -46,7 +46,9 @@ __device__ __forceinline__ int4v resource(const void* base, long long bytes) {
 // of parts, which wait for memory or for one another).  kLargeCap (16-bit types, with kEither): the cap is past
 // kSmallCap; kernels of their own, as tanhf beside the other form costs registers (parts of fp16 heads of 64:
 // 76 spilled instead of 17): 8192 tokens, 16 heads of 64, fp16, 730 us past kSmallCap, 450 up to it.
-constexpr int kCapped = 1, kBiased = 2, kInParts = 4, kEither = 8, kLargeCap = 16;
+// kWindowed: keys behind the window and past the sinks are not seen either.  kPrefixed: the first a.p_tiles
+// tiles are of a prefix that the batch shares; a.stacked: all rows of the batch over those tiles.
+constexpr int kCapped = 1, kBiased = 2, kInParts = 4, kEither = 8, kLargeCap = 16, kWindowed = 32, kPrefixed = 64;
 template <int kDtype, int kD, int kWaves, int kTeams, int kMode>
 __global__ __launch_bounds__(kWaves * kTeams * kWave, kWaves == 1 ? 1 : kD == 64 && kDtype != MUSC_DTYPE_F32 ? 3 : 2) void masked_attention_kernel(
     const Args a) {
@@ -61,10 +63,13 @@ __global__ __launch_bounds__(kWaves * kTeams * kWave, kWaves == 1 ? 1 : kD == 64
   constexpr int kLoads = kPart / 1024 / kWaves;             // loads of K (and of V) per wave
   static_assert(kLoads * kWaves * 1024 == kPart, "whole loads per wave");
   constexpr int kO = kD / 32;
+  constexpr bool windowed = (kMode & kWindowed) != 0, prefixed = (kMode & kPrefixed) != 0;
   __shared__ __attribute__((aligned(1024))) char staged[2 * kTeams][2 * kPart];
   __shared__ __attribute__((aligned(16))) int docs_s[2 * kTeams][64], ords_s[2 * kTeams][64];
   __shared__ float pos_s[2 * kTeams][64 * kMaxAxes];
   __shared__ Range ranges[kWaves];
+  __shared__ unsigned long long chunks_s[windowed ? kWaves * kTeams : 1];
+  __shared__ int seen_s[windowed ? kWaves * kTeams : 1];
 
   const musc_masked_attention& c = a.c;
   // uniform numbers in scalar registers (the divisions leave them in vector ones)
@@ -72,7 +77,7 @@ __global__ __launch_bounds__(kWaves * kTeams * kWave, kWaves == 1 ? 1 : kD == 64
   uint32_t split, job, bh;
   if (a.heads_at_once) {
     // one XCD works on heads_at_once heads together, row tile by row tile (the longest first)
-    const uint32_t per_xcd = (uint32_t)(c.batch * c.kv_heads) / kXcds, local = blockIdx.x / kXcds;
+    const uint32_t per_xcd = (uint32_t)((prefixed ? a.batches : c.batch) * c.kv_heads) / kXcds, local = blockIdx.x / kXcds;
     const uint32_t of_group = (uint32_t)(a.heads_at_once * a.jobs * a.splits);
     const uint32_t group = uniform(local / of_group), in_group = local - group * of_group;
     const uint32_t first = group * a.heads_at_once, at_once = min((uint32_t)a.heads_at_once, per_xcd - first);
@@ -88,19 +93,24 @@ __global__ __launch_bounds__(kWaves * kTeams * kWave, kWaves == 1 ? 1 : kD == 64
     bh = uniform(rest / a.jobs);
     job = rest - bh * a.jobs;
   }
-  const int b = uniform(bh / c.kv_heads), kvh = bh - b * c.kv_heads;
+  // a shared prefix's heads are neighbours over the batch, so that an XCD reads it once for many of them
+  const int of_major = prefixed ? a.batches : c.kv_heads, major = uniform(bh / of_major), minor = bh - major * of_major;
+  const int b = prefixed ? minor : major, kvh = prefixed ? major : minor;
   const int tid = threadIdx.x, lane = tid % kWave;
   const int team = kTeams > 1 ? __builtin_amdgcn_readfirstlane(tid / kWave) : 0;
   const int wave = kTeams > 1 ? 0 : __builtin_amdgcn_readfirstlane(tid / kWave);
   const int lq = lane & 31, lh = lane >> 5;
 
-  // tiles of this split, 64 sorted at a time by the keys' summary; the first 64 are asked for now
-  const int lo = uniform((long long)a.key_tiles * split / a.splits);
-  const int hi = uniform((long long)a.key_tiles * (split + 1) / a.splits);
+  // tiles of this split (of a window: all of them, and every splits-th of those that are seen), 64 sorted
+  // at a time by the keys' summary; the first 64 are asked for now
+  const int lo = windowed ? 0 : uniform((long long)a.key_tiles * split / a.splits);
+  const int hi = windowed ? a.key_tiles : uniform((long long)a.key_tiles * (split + 1) / a.splits);
+  const int p_tiles = prefixed ? a.p_tiles : 0;
   const int4* summary = c.k_summary ? reinterpret_cast<const int4*>(c.k_summary) + b * c.k_summary_sb : nullptr;
   auto summary_of = [&](int t) __attribute__((always_inline)) {
     int4 k = make_int4(0, 0, 0, 0);
-    if (summary && t >= lo && t < hi) {
+    if (summary && t >= (prefixed ? max(lo, p_tiles) : lo) && t < hi) {
+      t -= p_tiles;
       k = summary[(long long)t * kSub];
       if (kSub > 1 && t * kSub + 1 < a.summaries) {
         const int4 n = summary[(long long)t * kSub + 1];
@@ -115,6 +125,7 @@ __global__ __launch_bounds__(kWaves * kTeams * kWave, kWaves == 1 ? 1 : kD == 64
   // with an order of tokens they see more keys, and the longest work should not start last
   constexpr bool in_parts = (kMode & kInParts) != 0;
   int tile_of_rows = a.row_tiles - 1 - (int)job, part = team, parts = kTeams;
+  if (windowed && kTeams == 1) part = (int)split, parts = a.splits;
   int first_row = 0, last_row = kRowTile - 1;
   if (kWaves > 1 && c.schedule) {
     const int* schedule = c.schedule + b * c.schedule_sb;
@@ -137,16 +148,21 @@ __global__ __launch_bounds__(kWaves * kTeams * kWave, kWaves == 1 ? 1 : kD == 64
   tile_of_rows = min(max(tile_of_rows, 0), a.row_tiles - 1);
   const int row = (tile_of_rows * kWaves + wave) * 32 + lq;
   const bool inside = row < a.rows && (in_parts || kWaves == 1 || (wave * 32 + lq >= first_row && wave * 32 + lq <= last_row));
-  const int token = inside ? (int)((uint32_t)row / (uint32_t)a.group) : 0;
+  int token = inside ? (int)((uint32_t)row / (uint32_t)a.group) : 0;
   const int head = kvh * a.group + (inside ? row - token * a.group : 0);
+  int qb = b;  // the batch entry of this row
+  if (prefixed && a.stacked) {
+    qb = (int)((uint32_t)token / (uint32_t)c.q_len);
+    token -= qb * c.q_len;
+  }
   const int d = c.d, k_len = c.k_len, axes = kMode & (kBiased | kEither) ? c.axes : 0;
 
   // this row's document and order (rows outside the tensor read token 0's), its Q and positions,
   // all asked for before any is used
   int qdoc = 0, qord = 0;
-  if (c.q_documents) qdoc = c.q_documents[b * c.q_tokens_sb + token];
-  if (c.q_order) qord = c.q_order[b * c.q_tokens_sb + token];
-  const T* qrow = static_cast<const T*>(c.q) + b * c.q_sb + (long long)token * c.q_st + head * c.q_sh;
+  if (c.q_documents) qdoc = c.q_documents[qb * c.q_tokens_sb + token];
+  if (c.q_order) qord = c.q_order[qb * c.q_tokens_sb + token];
+  const T* qrow = static_cast<const T*>(c.q) + qb * c.q_sb + (long long)token * c.q_st + head * c.q_sh;
   constexpr int kQ = kD / (2 * kPer);
   typedef T TVec __attribute__((ext_vector_type(kPer)));
   TVec qf[kQ];
@@ -161,7 +177,7 @@ __global__ __launch_bounds__(kWaves * kTeams * kWave, kWaves == 1 ? 1 : kD == 64
   for (int x = 0; x < kMaxAxes; ++x) {
     qpos[x] = 0.f, slope[x] = 0.f;
     if (x < axes) {
-      qpos[x] = c.q_positions[b * c.q_positions_sb + (long long)token * axes + x];
+      qpos[x] = c.q_positions[qb * c.q_positions_sb + (long long)token * axes + x];
       slope[x] = c.slopes[head * axes + x];
     }
   }
@@ -189,6 +205,49 @@ __global__ __launch_bounds__(kWaves * kTeams * kWave, kWaves == 1 ? 1 : kD == 64
       all_rows.dmax = max(all_rows.dmax, ranges[w].dmax);
       all_rows.omin = min(all_rows.omin, ranges[w].omin);
       all_rows.omax = max(all_rows.omax, ranges[w].omax);
+    }
+  }
+
+  // Of a window: the order of the first key in it; which 64s of tiles hold some that the workgroup's rows
+  // see (bit 63: all from the 63rd on), found by all waves before any of them has its accumulators; and of
+  // the splits only as many as there are such tiles (four of them for four waves) have work.
+  const auto window_from = [&](int order) { return __builtin_elementwise_sub_sat(order, a.window - 1); };
+  // this row's window: its first order and how many follow; and its sinks
+  const int qfirst = windowed ? window_from(qord) : 0;
+  const uint32_t qspan = windowed ? (uint32_t)qord - (uint32_t)qfirst : 0;
+  const uint32_t qsinks = windowed && qord >= 0 && a.sinks > 0 ? (uint32_t)min(qord, a.sinks - 1) + 1 : 0;
+  auto may_see_tile = [&](const int4 k, const Range& r) __attribute__((always_inline)) {
+    return k.y >= 0 && k.x <= r.dmax && k.y >= r.dmin && k.z <= r.omax &&
+           (!windowed || k.w >= window_from(r.omin) || (k.w >= 0 && k.z < a.sinks));
+  };
+  unsigned long long chunks = ~0ull;
+  if constexpr (windowed) {
+    if (hi > 64 || (kTeams == 1 && a.splits > 1)) {
+      constexpr int kAll = kWaves * kTeams;
+      const int self = __builtin_amdgcn_readfirstlane(tid / kWave);
+      unsigned long long here = 0;
+      int seen_tiles = 0;
+#pragma unroll 4
+      for (int n = self; n * 64 < hi; n += kAll) {
+        const int t = n * 64 + lane;
+        const unsigned long long some = __ballot(t < hi && may_see_tile(summary_of(t), all_rows));
+        if (some) here |= 1ull << min(n, 63);
+        seen_tiles += __popcll(some);
+      }
+      if (lane == 0) chunks_s[self] = here, seen_s[self] = seen_tiles;
+      __syncthreads();
+      chunks = 0, seen_tiles = 0;
+#pragma unroll
+      for (int w = 0; w < kAll; ++w) chunks |= chunks_s[w], seen_tiles += seen_s[w];
+      if (kTeams == 1 && a.splits > 1) {
+        seen_tiles = __builtin_amdgcn_readfirstlane(seen_tiles);
+        parts = max(min(parts, kWaves == 1 ? seen_tiles : (seen_tiles + 3) / 4), 1);
+        if (part >= parts) {  // the whole workgroup
+          if (inside && lh == 0)
+            reinterpret_cast<float2*>(a.part_ml)[((long long)bh * a.rows + row) * a.splits + split] = make_float2(-INFINITY, 0.f);
+          return;
+        }
+      }
     }
   }
 
@@ -222,15 +281,25 @@ __global__ __launch_bounds__(kWaves * kTeams * kWave, kWaves == 1 ? 1 : kD == 64
   // with the last key.  Lanes of channels past d load from nowhere.
   const char* kbase = reinterpret_cast<const char*>(static_cast<const T*>(c.k) + b * c.k_sb + (long long)kvh * c.k_sh);
   const char* vbase = reinterpret_cast<const char*>(static_cast<const T*>(c.v) + b * c.v_sb + (long long)kvh * c.v_sh);
-  const uint32_t k_row = (uint32_t)(c.k_st * (long long)sizeof(T)), v_row = (uint32_t)(c.v_st * (long long)sizeof(T));
+  const uint32_t own_k_row = (uint32_t)(c.k_st * (long long)sizeof(T)), own_v_row = (uint32_t)(c.v_st * (long long)sizeof(T));
+  const char *pkbase = kbase, *pvbase = vbase;
+  uint32_t p_k_row = 0, p_v_row = 0;
+  if constexpr (prefixed) {
+    pkbase = reinterpret_cast<const char*>(static_cast<const T*>(a.p.k) + (long long)kvh * a.p.k_sh);
+    pvbase = reinterpret_cast<const char*>(static_cast<const T*>(a.p.v) + (long long)kvh * a.p.v_sh);
+    p_k_row = (uint32_t)(a.p.k_st * (long long)sizeof(T)), p_v_row = (uint32_t)(a.p.v_st * (long long)sizeof(T));
+  }
   const uint32_t staged_at = (uint32_t)(size_t)(lds_void*)&staged[0][0] + wave * 1024;
   constexpr int kRows = 64 / kPlaces;  // rows of a load
   const int row_bytes = d * (int)sizeof(T);
   auto load_tile = [&](int tile, int buf) __attribute__((always_inline)) {
-    const int first = tile * kTile, rem = min(k_len - first, kTile), mine = wave * kRows;
+    const bool shared = prefixed && tile < p_tiles;
+    const int first = (shared ? tile : tile - p_tiles) * kTile, mine = wave * kRows;
+    const int rem = min((shared ? a.p.len : k_len) - first, kTile);
+    const uint32_t k_row = shared ? p_k_row : own_k_row, v_row = shared ? p_v_row : own_v_row;
     const uint32_t to = __builtin_amdgcn_readfirstlane(staged_at + buf * 2 * kPart);
-    const char* kt = kbase + (unsigned long long)(uint32_t)(first + mine) * k_row;
-    const char* vt = vbase + (unsigned long long)(uint32_t)(first + mine) * v_row;
+    const char* kt = (shared ? pkbase : kbase) + (unsigned long long)(uint32_t)(first + mine) * k_row;
+    const char* vt = (shared ? pvbase : vbase) + (unsigned long long)(uint32_t)(first + mine) * v_row;
     auto lane_offset = [&](int j, uint32_t row) {
       const int r = lane / kPlaces, chunk = (lane % kPlaces) ^ swizzle<kPitch>((wave + kWaves * j) * kRows + r);
       return chunk * kPer < d ? (int)(r * row) + chunk * 16 : kNowhere;
@@ -255,14 +324,15 @@ __global__ __launch_bounds__(kWaves * kTeams * kWave, kWaves == 1 ? 1 : kD == 64
       });
     }
     if (wave == kWaves - 1) {
-      if (c.k_documents)
+      if (c.k_documents && !shared)
         load_to_lds_4(&docs_s[buf][0], lane * 4,
                       resource(c.k_documents + b * c.k_tokens_sb + first, rem * 4));
-      if (c.k_order)
+      if (c.k_order && !shared)
         load_to_lds_4(&ords_s[buf][0], lane * 4,
                       resource(c.k_order + b * c.k_tokens_sb + first, rem * 4));
       if (axes) {
-        const int4v rp = resource(c.k_positions + b * c.k_positions_sb + (long long)first * axes, rem * axes * 4);
+        const float* positions = shared ? a.p.positions : c.k_positions + b * c.k_positions_sb;
+        const int4v rp = resource(positions + (long long)first * axes, rem * axes * 4);
 #pragma unroll
         for (int x = 0; x < kMaxAxes; ++x)
           if (x < axes) load_to_lds_4(&pos_s[buf][64 * x], (64 * x + lane) * 4, rp);
@@ -365,7 +435,8 @@ __global__ __launch_bounds__(kWaves * kTeams * kWave, kWaves == 1 ? 1 : kD == 64
     uint32_t seen = 0xffffffffu;
     if (!whole) {
       mixed_seen = true;
-      const int rem = k_len - tile * kTile;
+      const bool shared = prefixed && tile < p_tiles;
+      const int rem = shared ? a.p.len - tile * kTile : k_len - (tile - p_tiles) * kTile;
 #pragma unroll
       for (int u = 0; u < kSub; ++u)
 #pragma unroll
@@ -375,7 +446,10 @@ __global__ __launch_bounds__(kWaves * kTeams * kWave, kWaves == 1 ? 1 : kD == 64
           const int4v ko = *reinterpret_cast<const int4v*>(&ords_s[buf][key]);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const bool see = kd[i] == qdoc && ko[i] <= qord && key + i < rem;
+            const bool in = windowed ? (uint32_t)ko[i] - (uint32_t)qfirst <= qspan || (uint32_t)ko[i] < qsinks : ko[i] <= qord;
+            bool see = kd[i] == qdoc && in;
+            if (prefixed) see = see || shared;
+            see = see && key + i < rem;
             s[u][4 * g + i] = see ? s[u][4 * g + i] : -INFINITY;
             if (careful && !see) seen &= ~(1u << (16 * u + 4 * g + i));
           }
@@ -473,18 +547,19 @@ __global__ __launch_bounds__(kWaves * kTeams * kWave, kWaves == 1 ? 1 : kD == 64
   auto sort_tiles = [&](const int4 k) __attribute__((always_inline)) {
     const int t = chunk * 64 + lane;
     const bool here = t >= lo && t < hi;
-    auto may_see = [&](const Range& r) {
-      return here && k.y >= 0 && k.x <= r.dmax && k.y >= r.dmin && k.z <= r.omax;
-    };
+    const bool shared = prefixed && t < p_tiles;
+    auto may_see = [&](const Range& r) { return here && (shared ? r.dmax >= 0 : may_see_tile(k, r)); };
     todo = __ballot(may_see(all_rows));
-    if ((in_parts || kTeams > 1) && parts > 1) {  // every parts-th of them
+    if ((in_parts || kTeams > 1 || windowed) && parts > 1) {  // every parts-th of them
       const int number = tiles_seen + __popcll(todo & ((1ull << lane) - 1));
       tiles_seen += __popcll(todo);
       todo = __ballot(((todo >> lane) & 1) && number % parts == part);
     }
     any_word = __ballot(may_see(mine));
-    whole_word = __ballot(here && k.x == k.y && mine.dmin == mine.dmax && k.x == mine.dmin && k.w <= mine.omin &&
-                          (t + 1) * kTile <= k_len);
+    const bool in_window = !windowed || k.z >= window_from(mine.omax) || (k.z >= 0 && k.w < a.sinks);
+    const bool whole = k.x == k.y && mine.dmin == mine.dmax && k.x == mine.dmin && k.w <= mine.omin && in_window &&
+                       (t + 1 - p_tiles) * kTile <= k_len;
+    whole_word = __ballot(here && (shared ? (t + 1) * kTile <= a.p.len : whole));
   };
   struct Next {
     int tile;
@@ -493,6 +568,8 @@ __global__ __launch_bounds__(kWaves * kTeams * kWave, kWaves == 1 ? 1 : kD == 64
   auto next_tile = [&]() __attribute__((always_inline)) -> Next {
     while (todo == 0) {
       ++chunk;
+      if (windowed)
+        while (chunk * 64 < hi && !((chunks >> min(chunk, 63)) & 1)) ++chunk;
       if (chunk * 64 >= hi) return Next{-1, false, false};
       sort_tiles(summary_of(chunk * 64 + lane));
     }
@@ -601,7 +678,7 @@ __global__ __launch_bounds__(kWaves * kTeams * kWave, kWaves == 1 ? 1 : kD == 64
   }
   if (!inside) return;
   // register v of block x holds channel 32 x + 8 (v / 4) + 4 lh + v % 4
-  if (in_parts ? parts == 1 : a.splits == 1) {
+  if (in_parts ? parts == 1 : a.splits == 1 && !(prefixed && a.partial)) {
     const bool empty = !live || l_run == 0.f;
     const float inv = 1.f / l_run;
     T* orow = static_cast<T*>(c.out) + b * c.o_sb + (long long)token * c.o_st + head * c.o_sh;
@@ -686,6 +763,57 @@ __global__ __launch_bounds__(256) void join_kernel(const Args a) {
   *reinterpret_cast<Two*>(orow + 2 * lane) = out;
 }
 
+// Joins what the rows of prefixed attention have in a.splits parts of one launch and a.more_splits of
+// another, in their order: the kernel above over both.
+template <int kDtype>
+__global__ __launch_bounds__(256) void join_prefixed_kernel(const Args a) {
+  typedef typename Type<kDtype>::T T;
+  __shared__ float weight[kMaxSplits], tops[4], sums[4];
+  __shared__ float2 parts[4][kWave];
+  const musc_masked_attention& c = a.c;
+  const long long r = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
+  const int splits = a.splits, all = splits + a.more_splits;
+  float2 mine = make_float2(-INFINITY, 0.f);
+  if (tid < splits) mine = reinterpret_cast<const float2*>(a.part_ml)[r * splits + tid];
+  else if (tid < all) mine = reinterpret_cast<const float2*>(a.more_ml)[r * a.more_splits + tid - splits];
+  const float top_here = wave_max(mine.x);
+  if (lane == 0) tops[wave] = top_here;
+  __syncthreads();
+  const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+  const float w = mine.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(mine.x - top);
+  weight[tid] = w;
+  const float sum_here = wave_sum(mine.y == 0.f ? 0.f : w * mine.y);
+  if (lane == 0) sums[wave] = sum_here;
+  __syncthreads();
+  const float sum = sums[0] + sums[1] + sums[2] + sums[3];
+  const bool ok = 2 * lane < c.d;
+  const int at = ok ? 2 * lane : 0;
+  float2 y = make_float2(0.f, 0.f);
+#pragma unroll 4
+  for (int s = wave; s < all; s += 4) {
+    const float* from = s < splits ? a.part_o + (r * splits + s) * c.d : a.more_o + (r * a.more_splits + s - splits) * c.d;
+    const float2 p = *reinterpret_cast<const float2*>(from + at);
+    const float f = weight[s];
+    if (f != 0.f) y.x = fmaf(f, p.x, y.x), y.y = fmaf(f, p.y, y.y);
+  }
+  parts[wave][lane] = y;
+  __syncthreads();
+  if (wave != 0 || !ok) return;
+#pragma unroll
+  for (int i = 1; i < 4; ++i) y.x += parts[i][lane].x, y.y += parts[i][lane].y;
+  const float inv = 1.f / sum;
+  const int rows = c.q_len * a.group;  // of a batch entry and key head
+  const long long bh = r / rows;
+  const int row = (int)(r % rows), token = row / a.group;
+  const int b = (int)(bh % c.batch), head = (int)(bh / c.batch) * a.group + row % a.group;
+  typedef T Two __attribute__((ext_vector_type(2)));
+  Two out;
+  out[0] = sum == 0.f ? (T)0.f : (T)(y.x * inv);
+  out[1] = sum == 0.f ? (T)0.f : (T)(y.y * inv);
+  *reinterpret_cast<Two*>(static_cast<T*>(c.out) + b * c.o_sb + (long long)token * c.o_st + head * c.o_sh + 2 * lane) = out;
+}
+
 // Joins the parts of the row tiles that were done in parts, in their order: a workgroup per row
 // tile, four channels of a row per thread.
 template <int kDtype>
@@ -765,6 +893,74 @@ void launch(const Args& a, int waves, hipStream_t stream) {
     hipLaunchKernelGGL((masked_attention_kernel<kDtype, kD, 4, 1, kBiased>), grid, dim3(4 * kWave), 0, stream, a);
   } else {
     hipLaunchKernelGGL((masked_attention_kernel<kDtype, kD, 4, 1, kCapped | kBiased>), grid, dim3(4 * kWave), 0, stream, a);
+  }
+}
+
+// Windows and shared prefixes (kExtra): the same kernels with that mode, no parts of row tiles.
+template <int kDtype, int kD, int kMode>
+void launch_one(const Args& a, const dim3& grid, hipStream_t stream) {
+  hipLaunchKernelGGL((masked_attention_kernel<kDtype, kD, 4, 1, kMode>), grid, dim3(4 * kWave), 0, stream, a);
+}
+template <int kDtype, int kD, int kMode>
+void launch_few(const Args& a, const dim3& grid, hipStream_t stream) {
+  constexpr int kTeams = teams_of((kD <= 64 ? 64 : 128) * (kDtype == MUSC_DTYPE_F32 ? 4 : 2));
+  if constexpr ((kMode & kWindowed) != 0) {
+    if (a.teams > 1) {
+      hipLaunchKernelGGL((masked_attention_kernel<kDtype, kD, 1, kTeams, kMode>), grid, dim3(kTeams * kWave), 0, stream, a);
+      return;
+    }
+  }
+  hipLaunchKernelGGL((masked_attention_kernel<kDtype, kD, 1, 1, kMode>), grid, dim3(kWave), 0, stream, a);
+}
+template <int kDtype, int kD, int kExtra>
+void launch_extra(const Args& a, int waves, hipStream_t stream) {
+  const dim3 grid((unsigned)align_up((size_t)a.units, kXcds));
+  const int mode = (a.c.cap > 0.f ? kCapped : 0) | (a.c.axes ? kBiased : 0);
+  constexpr int kWide = kD <= 64 ? 64 : 128;
+  if constexpr (kDtype != MUSC_DTYPE_F32) {
+    if (a.c.cap > kSmallCap) {
+      if (waves == 1) launch_few<kDtype, kWide, kEither | kLargeCap | kExtra>(a, grid, stream);
+      else launch_one<kDtype, kWide, kEither | kLargeCap | kExtra>(a, grid, stream);
+      return;
+    }
+  }
+  if (waves == 1) {
+    if (mode == 0) launch_few<kDtype, kWide, kExtra>(a, grid, stream);
+    else launch_few<kDtype, kWide, kEither | kExtra>(a, grid, stream);
+  } else if (mode == 0) {
+    launch_one<kDtype, kD, kExtra>(a, grid, stream);
+  } else if (mode == kCapped) {
+    launch_one<kDtype, kD, kCapped | kExtra>(a, grid, stream);
+  } else if (mode == kBiased) {
+    launch_one<kDtype, kD, kBiased | kExtra>(a, grid, stream);
+  } else {
+    launch_one<kDtype, kD, kCapped | kBiased | kExtra>(a, grid, stream);
+  }
+}
+template <int kDtype, int kExtra>
+void launch_extra(const Args& a, int waves, hipStream_t stream) {
+  if (a.c.d <= 64) launch_extra<kDtype, 64, kExtra>(a, waves, stream);
+  else if (a.c.d <= 96) launch_extra<kDtype, 96, kExtra>(a, waves, stream);
+  else launch_extra<kDtype, 128, kExtra>(a, waves, stream);
+}
+template <int kDtype>
+void launch_windowed(const Args& a, int waves, hipStream_t stream) {
+  launch_extra<kDtype, kWindowed>(a, waves, stream);
+  if (a.splits > 1) {
+    const long long rows = (long long)a.c.batch * a.c.kv_heads * a.rows;
+    hipLaunchKernelGGL((join_kernel<kDtype>), dim3((unsigned)rows), dim3(256), 0, stream, a);
+  }
+}
+// One launch (more == null), or all rows over the prefix and then each entry's over its own keys.
+template <int kDtype>
+void launch_prefixed(const Args& a, int waves, const Args* more, int more_waves, hipStream_t stream) {
+  launch_extra<kDtype, kPrefixed>(a, waves, stream);
+  if (more) launch_extra<kDtype, kPrefixed>(*more, more_waves, stream);
+  if (a.splits > 1 || a.partial) {
+    Args both = a;
+    if (more) both.more_splits = more->splits, both.more_ml = more->part_ml, both.more_o = more->part_o;
+    const long long rows = (long long)a.c.batch * a.c.kv_heads * a.c.q_len * a.group;
+    hipLaunchKernelGGL((join_prefixed_kernel<kDtype>), dim3((unsigned)rows), dim3(256), 0, stream, both);
   }
 }
 

@@ -1,0 +1,7 @@
+// Masked attention with a window and sinks on fp16 storage (its matrix instructions, __builtin_amdgcn_mfma_*, are in
+// masked_attention_kernel.hpp).
+#include "masked_attention_kernel.hpp"
+
+void musc::mattn::launch_window_f16(const Args& a, int waves, hipStream_t stream) {
+  launch_windowed<MUSC_DTYPE_F16>(a, waves, stream);
+}

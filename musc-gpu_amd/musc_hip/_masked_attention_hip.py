@@ -10,6 +10,7 @@ writes the logits or a mask to memory.
 from __future__ import annotations
 
 import ctypes
+import operator
 
 import torch
 
@@ -128,29 +129,23 @@ def _heads(x, per):
     return x, rt.token_strides(x)
 
 
-def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float, keys: Tokens | None = None,
-                     queries: Tokens | None = None, cap: float = 0.0, slopes: torch.Tensor | None = None,
-                     out: torch.Tensor | None = None) -> torch.Tensor:
-    """softmax over the keys each query sees of c(scale q k^T) - sum_a slopes[h, a] |distance_a|,
-    times v; (B, Tq, heads, D).
+def _prefix_heads(x, name, q, hk, per):
+    """A prefix's K or V (P, kv_heads, D), copied where its rows do not start on 16 bytes, and its strides."""
+    if x.dim() != 3 or x.shape[1] != hk or x.shape[2] != q.shape[3] or x.dtype != q.dtype or x.get_device() != q.get_device():
+        raise ValueError(f"{name} must be (P, {hk}, {q.shape[3]}) in q's dtype on its device")
+    x, (_, st, sh) = _heads(x[None], per)
+    return x, st, sh
 
-    q (B, Tq, heads, D), k and v (B, Tk, kv_heads, D), heads a multiple of kv_heads, float32,
-    float16 or bfloat16, D up to 128 in steps of 16 bytes; views of a packed projection are read
-    in place where each row starts on 16 bytes, and copied otherwise.
-    keys, queries: the Tokens of both sides; queries defaults to keys (self-attention), no keys at
-    all lets every query see every key.  A query that sees no key gets zeros, as does one whose seen
-    scores are all minus infinity.
-    cap > 0 (up to 2^60; 16-bit types are quickest up to 128): scores become cap tanh(score / cap) before the bias.  slopes: float32 (heads, axes),
-    needs positions on both sides.  out: the tensor to write, rows on 16 bytes; it may not overlap q, k
-    or v.  No derivative."""
+
+def _attend(q, k, v, scale, keys, queries, cap, slopes, out, window=None, prefix=None):
     for name, x in (('q', q), ('k', k), ('v', v)):
         rt.require_device_tensor(x, name)
         if x.dim() != 4:
             raise ValueError(f'{name} must be a (B, T, heads, D) tensor')
     if rt.elsewhere(q):
         with torch.cuda.device(q.device):
-            return masked_attention(q, k, v, scale, keys, queries, cap, slopes, out)
-    rt.require_no_gradient(q, k, v, slopes, out)
+            return _attend(q, k, v, scale, keys, queries, cap, slopes, out, window, prefix)
+    rt.require_no_gradient(q, k, v, slopes, out, *(prefix or ()))
     dtype, index = q.dtype, q.get_device()
     if dtype not in _STORAGE:
         raise ValueError('q must be float32, float16 or bfloat16')
@@ -173,6 +168,8 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: f
     kdocs, qdocs, kord, qord = keys.documents, queries.documents, keys.order, queries.order
     if (kdocs is None) != (qdocs is None) or (kord is None) != (qord is None):
         raise ValueError('keys and queries must both have documents, and both an order, or neither')
+    if window is not None and kord is None:
+        raise ValueError('a window needs an order of keys and queries')
     q_sb = k_sb = sum_sb = qd_ptr = kd_ptr = qo_ptr = ko_ptr = sum_ptr = 0
     if kdocs is not None:
         if keys.summary is None:
@@ -198,31 +195,97 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: f
         qp_sb = _batch_stride('queries.positions', qpos, qpos.shape[:-1], b, tq, index)
         kp_sb = _batch_stride('keys.positions', kpos, kpos.shape[:-1], b, tk, index)
         qp_ptr, kp_ptr, slope_ptr = qpos.data_ptr(), kpos.data_ptr(), slopes.data_ptr()
+    before = None
+    if prefix is not None:
+        pk, pk_st, pk_sh = _prefix_heads(prefix[0], 'prefix_k', q, hk, per)
+        pv, pv_st, pv_sh = _prefix_heads(prefix[1], 'prefix_v', q, hk, per)
+        p, p_pos, p_ptr = pk.shape[1], prefix[2], 0
+        if pv.shape[1] != p:
+            raise ValueError('prefix_v must match prefix_k in shape')
+        if axes:
+            if p_pos is None:
+                raise ValueError('slopes need prefix_positions')
+            if p_pos.shape != (p, axes) or p_pos.dtype != torch.float32 or p_pos.get_device() != index:
+                raise ValueError(f"prefix_positions must be float32 ({p}, {axes}) on q's device")
+            p_pos = p_pos.contiguous()
+            p_ptr = p_pos.data_ptr()
+        if p:
+            before = rt.PACK_ATTENTION_PREFIX.pack(pk.data_ptr(), pv.data_ptr(), pk_st, pk_sh, pv_st, pv_sh, p_ptr, p)
     o = rt.output_like(out, q, 'out')
     os_ = rt.token_strides(o)
     if o.data_ptr() % 16 or (os_[0] | os_[1] | os_[2]) % per:
         raise ValueError('rows of out must start on 16 bytes')
     if not (b and tq and h):
         return o
-    if not tk:
+    if not tk and before is None:
         return o.zero_()
     schedule = schedule_sb = 0
-    if queries is keys and keys._schedule is not None and h // hk in keys._schedule_of:
-        before, block = keys._schedule_of[h // hk]
-        schedule, schedule_sb = keys._schedule.data_ptr() + before, block if k_sb else 0
+    if window is None and before is None and queries is keys and keys._schedule is not None and h // hk in keys._schedule_of:
+        first, block = keys._schedule_of[h // hk]
+        schedule, schedule_sb = keys._schedule.data_ptr() + first, block if k_sb else 0
     call = rt.PACK_MASKED_ATTENTION.pack(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), *qs, *ks, *vs, *os_, _STORAGE[dtype], b, tq, tk, h, hk, d,
         scale, cap, qd_ptr, qo_ptr, kd_ptr, ko_ptr, q_sb, k_sb, sum_ptr, sum_sb, qp_ptr, kp_ptr, qp_sb, kp_sb, slope_ptr,
         axes, schedule, schedule_sb)
+    # the entry point of the call, and what it takes beside it
+    name, more = 'masked', ()
+    if window is not None:
+        name, more = 'window', window
+    elif before is not None:
+        name, more = 'prefix', (before,)
     lib, need, ws = rt.library(), ctypes.c_size_t(), None
-    rt.check(lib.musc_masked_attention_workspace_bytes(call, ctypes.byref(need)), 'musc_masked_attention_workspace_bytes')
+    rt.check(getattr(lib, f'musc_{name}_attention_workspace_bytes')(call, *more, ctypes.byref(need)), f'musc_{name}_attention_workspace_bytes')
     if need.value:
         ws = torch.empty(need.value, dtype=torch.uint8, device=q.device)
     stream = rt.current_stream(index)
-    rt.check(lib.musc_masked_attention_fwd(call, None if ws is None else ws.data_ptr(), need.value, stream),
-             'musc_masked_attention_fwd')
+    rt.check(getattr(lib, f'musc_{name}_attention_fwd')(call, *more, None if ws is None else ws.data_ptr(), need.value, stream),
+             f'musc_{name}_attention_fwd')
     if keys is not _EVERY:
         keys.used_on(stream, q.device)
     if queries is not keys:
         queries.used_on(stream, q.device)
     return o
+
+
+def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float, keys: Tokens | None = None,
+                     queries: Tokens | None = None, cap: float = 0.0, slopes: torch.Tensor | None = None,
+                     out: torch.Tensor | None = None, window: int = 0, sinks: int = 0) -> torch.Tensor:
+    """softmax over the keys each query sees of c(scale q k^T) - sum_a slopes[h, a] |distance_a|,
+    times v; (B, Tq, heads, D).
+
+    q (B, Tq, heads, D), k and v (B, Tk, kv_heads, D), heads a multiple of kv_heads, float32,
+    float16 or bfloat16, D up to 128 in steps of 16 bytes; views of a packed projection are read
+    in place where each row starts on 16 bytes, and copied otherwise.
+    keys, queries: the Tokens of both sides; queries defaults to keys (self-attention), no keys at
+    all lets every query see every key.  A query that sees no key gets zeros, as does one whose seen
+    scores are all minus infinity.
+    cap > 0 (up to 2^60; 16-bit types are quickest up to 128): scores become cap tanh(score / cap) before the bias.  slopes: float32 (heads, axes),
+    needs positions on both sides.  out: the tensor to write, rows on 16 bytes; it may not overlap q, k
+    or v.
+    window > 0 (needs an order): of those keys a query sees the ones whose order is one of the last `window`, its
+    own among them, and the first `sinks` orders (0 .. sinks - 1), such as class or register tokens or a clip's first
+    frames; what no query sees is not read.  No derivative."""
+    if not (window or sinks):
+        return _attend(q, k, v, scale, keys, queries, cap, slopes, out)
+    window, sinks = operator.index(window), operator.index(sinks)
+    if not (0 < window < 1 << 31 and 0 <= sinks < 1 << 31):
+        raise ValueError('window and sinks must be whole numbers from 0 up, sinks only with a window')
+    return _attend(q, k, v, scale, keys, queries, cap, slopes, out, window=(window, sinks))
+
+
+def prefix_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, prefix_k: torch.Tensor, prefix_v: torch.Tensor,
+                     scale: float, keys: Tokens | None = None, queries: Tokens | None = None, cap: float = 0.0,
+                     slopes: torch.Tensor | None = None, prefix_positions: torch.Tensor | None = None,
+                     out: torch.Tensor | None = None) -> torch.Tensor:
+    """masked_attention of a batch whose entries all begin with the same keys (reference images, a common text):
+    every query sees the whole prefix and, of k and v, what keys and queries let it see; (B, Tq, heads, D).
+
+    prefix_k, prefix_v: (P, kv_heads, D), once for the batch; views are read in place as k and v are.
+    Single tokens and other short calls pass over the prefix together, so it is read once for all of them.
+    Queries without a document (negative ids, padding) get zeros.  k and v may have no tokens, and the
+    prefix none.  slopes need prefix_positions, float32 (P, axes), too.  The rest as for masked_attention.  No derivative."""
+    rt.require_device_tensor(prefix_k, 'prefix_k')
+    rt.require_device_tensor(prefix_v, 'prefix_v')
+    if prefix_positions is not None:
+        rt.require_device_tensor(prefix_positions, 'prefix_positions')
+    return _attend(q, k, v, scale, keys, queries, cap, slopes, out, prefix=(prefix_k, prefix_v, prefix_positions))

@@ -59,6 +59,12 @@ class MaskedAttention(ctypes.Structure):
            ('axes', ctypes.c_int), ('schedule', ctypes.c_void_p), ('schedule_sb', ctypes.c_longlong)])
 
 
+class AttentionPrefix(ctypes.Structure):
+    """musc_attention_prefix of include/musc_hip.h, field by field."""
+    _fields_ = ([(n, ctypes.c_void_p) for n in ('k', 'v')] + [(n, ctypes.c_longlong) for n in ('k_st', 'k_sh', 'v_st', 'v_sh')]
+                + [('positions', ctypes.c_void_p), ('len', ctypes.c_int)])
+
+
 class RotaryCall(ctypes.Structure):
     """musc_rotary_call of include/musc_hip.h, field by field."""
     _fields_ = (
@@ -72,8 +78,10 @@ class RotaryCall(ctypes.Structure):
 
 # The same as bytes: packing 45 fields at once takes 4 us less than setting them one by one
 PACK_MASKED_ATTENTION = struct.Struct('@4P12q7i2f4P2qPq2P2qPiPq')
+PACK_ATTENTION_PREFIX = struct.Struct('@2P4qPi4x')
 PACK_ROTARY = struct.Struct('@P3qP3qP3qP3qPqPP11i4x')
 assert PACK_MASKED_ATTENTION.size == ctypes.sizeof(MaskedAttention)
+assert PACK_ATTENTION_PREFIX.size == ctypes.sizeof(AttentionPrefix)
 assert PACK_ROTARY.size == ctypes.sizeof(RotaryCall)
 
 
@@ -115,6 +123,10 @@ SIGNATURES = {
     'musc_token_schedule': (_i, [_vp, _vp, _vp, _i, _i, _vp, _vp]),
     'musc_masked_attention_workspace_bytes': (_i, [_vp, ctypes.POINTER(_sz)]),
     'musc_masked_attention_fwd': (_i, [_vp, _vp, _sz, _vp]),
+    'musc_window_attention_workspace_bytes': (_i, [_vp, _i, _i, ctypes.POINTER(_sz)]),
+    'musc_window_attention_fwd': (_i, [_vp, _i, _i, _vp, _sz, _vp]),
+    'musc_prefix_attention_workspace_bytes': (_i, [_vp, _vp, ctypes.POINTER(_sz)]),
+    'musc_prefix_attention_fwd': (_i, [_vp, _vp, _vp, _sz, _vp]),
     'musc_rmsnorm_rows': (_i, [_vp, _ll, _vp, _ll, _vp, _vp, _i, _i, _i, _i, _f, _vp, _vp]),
     'musc_rmsnorm_rows_8bit': (_i, [_vp, _ll, _vp, _ll, _vp, _vp, _i, _i, _i, _i, _f, _i, _i, _vp, _vp, _vp]),
     'musc_rotary': (_i, [_vp, _vp]),

@@ -38,8 +38,8 @@ COMMON = ['-O3', '-std=c++17', '-fPIC', f'--offload-arch={ARCH}', f'-DMUSC_TARGE
 # heuristics the compiler puts them in AGPRs and moves every value back and forth
 # (157 v_accvgpr moves per 32-key block in the fp16 kernel).
 FILE_FLAGS = {name: ['-mllvm', '-amdgpu-mfma-vgpr-form']
-              for name in ('attention.hip', 'masked_attention_f32.hip', 'masked_attention_f16.hip',
-                           'masked_attention_bf16.hip')}
+              for name in ['attention.hip'] + [f'masked_attention_{kind}{storage}.hip' for kind in ('', 'window_', 'prefix_')
+                                               for storage in ('f32', 'f16', 'bf16')]}
 
 
 def _compile(src: str, verbose: bool) -> str:
