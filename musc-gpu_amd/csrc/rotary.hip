@@ -16,6 +16,10 @@
 // norm_rotary_kernel norms each head of q and k before that, in the same pass:
 //
 //   y = x w / sqrt(mean(x^2) + eps)                  fp32, turned before its one rounding
+//
+// a head's channels in 1 to 64 neighbouring lanes, whose sum of squares goes round by lane-crossing
+// moves: the same bound.  16384 tokens of 32 + 8 heads of 128, bf16: 61 us = 5.5 TB/s; 4 x 1370
+// tokens of 16 + 16 heads of 64, fp16: 12 us; 8 tokens 5 us.
 #include <hip/hip_bf16.h>
 #include <hip/hip_fp16.h>
 
@@ -153,7 +157,6 @@ struct Norm {
   const void* w[2];   // of q and k, or null
   long long w_sh[2];  // elements between the weights of two heads, 0: shared
   int w_dtype[2];
-  uint32_t by_heads[2];
   float eps;
   int lane_bits;      // a head is held by 2^lane_bits neighbouring lanes
 };
@@ -191,108 +194,131 @@ __device__ __forceinline__ void load_weight(const void* w, int dtype, long long 
 }
 
 // Vectors of N elements: a lane holds one of a head's turned items (two vectors of a half each, or
-// one of neighbouring pairs) or one vector of the channels that do not turn.  The loads of kHeads heads
-// are in flight together, the first ones while the angles are formed.
+// one of neighbouring pairs) or one vector of the channels that do not turn.  The first heads' loads are
+// in flight while the angles are formed; weights that heads share wait in LDS as fp32.  One head a lane at a
+// time and waves enough to hide its loads: two or four at a time take 64 and 84 us for the 16384 tokens.
 template <int kDtype, bool kAdjacent, int N>
 __global__ __launch_bounds__(kThreads) void norm_rotary_kernel(const Args a, const Norm n) {
   typedef typename Storage<kDtype>::T T;
   typedef T Vec __attribute__((ext_vector_type(N)));
-  constexpr int kHeads = 4;
   __shared__ float2 table[kTable];
-  __shared__ long long at_b[kMaxTokens];
-  __shared__ int at_t[kMaxTokens];
+  __shared__ __attribute__((aligned(16))) float weights[2][2 * kMaxPairs];
   const long long first = linear_block() * a.tokens, total = (long long)a.batch * a.t;
   if (first >= total) return;
   const int here = (int)min((long long)a.tokens, total - first);
   const int pairs = a.pairs, tid = threadIdx.x;
-  if (tid < here) {
-    at_b[tid] = (first + tid) / a.t;
-    at_t[tid] = (int)((first + tid) % a.t);
-  }
-  __syncthreads();
+  const uint32_t first_b = (uint32_t)first / (uint32_t)a.t, first_t = (uint32_t)first - first_b * (uint32_t)a.t;
+  // batch entry and place of the workgroup's token
+  const auto place = [&](int token, uint32_t& b, uint32_t& t) {
+    b = first_b, t = first_t + token;
+    if (t >= (uint32_t)a.t) b += t / (uint32_t)a.t, t %= (uint32_t)a.t;
+  };
+  // this thread's angle (there are no more of them): asked for before anything else
+  static_assert(kTable <= kThreads, "one angle a thread");
+  const int angle_token = (int)((uint32_t)tid / (uint32_t)pairs), pair = tid - angle_token * pairs;
+  const bool has_angle = angle_token < here;
+  int axis = 0;
+  double frequency = 0.;
+  if (has_angle) axis = a.axis[pair], frequency = a.frequency[pair];
+  const void *qw = n.w[0], *kw = n.w[1];
+  const bool q_each = qw && n.w_sh[0] != 0, k_each = kw && n.w_sh[1] != 0;  // weights of each head
   const int group = tid >> n.lane_bits, item = tid & ((1 << n.lane_bits) - 1), groups = kThreads >> n.lane_bits;
   const int turned = kAdjacent ? 2 * pairs / N : pairs / N;
-  const bool live = item < a.items, turns = item < turned, two = !kAdjacent && turns;
+  const bool turns = item < turned, two = !kAdjacent && turns;
   const int c0 = turns ? item * N : 2 * pairs + (item - turned) * N, c1 = pairs + item * N;
-  bool formed = false;
-#pragma unroll 1
-  for (int which = 0; which < 2; ++which) {
-    const Side& side = which ? a.k : a.q;
-    const int heads = side.heads, all = here * heads;
-    const void* w = n.w[which];
+  const int q_heads = a.q.heads, heads = q_heads + a.k.heads, all = here * heads;
+  for (int from = 0; from < all; from += groups) {
+    const int h = from + group, token = over(h, a.by_heads), of_both = h - token * heads;
+    const bool live = item < a.items && h < all, of_k = of_both >= q_heads, each = of_k ? k_each : q_each;
+    const int head = of_k ? of_both - q_heads : of_both;
+    const auto of = [&](auto field) { return of_k ? a.k.*field : a.q.*field; };
+    uint32_t b, t;
+    place(token, b, t);
+    Vec x0 = Vec{}, x1 = Vec{};
     float w0[N], w1[N];
 #pragma unroll
     for (int j = 0; j < N; ++j) w0[j] = w1[j] = 1.f;
-    if (w && live && n.w_sh[which] == 0) {
-      load_weight<kDtype, N>(w, n.w_dtype[which], c0, w0);
-      if (two) load_weight<kDtype, N>(w, n.w_dtype[which], c1, w1);
+    if (live) {
+      const T* x = static_cast<const T*>(of(&Side::x)) + b * of(&Side::sb) + t * of(&Side::st) + head * of(&Side::sh);
+      x0 = *reinterpret_cast<const Vec*>(x + c0);
+      if (two) x1 = *reinterpret_cast<const Vec*>(x + c1);
+      if (each) {
+        const int w_dtype = of_k ? n.w_dtype[1] : n.w_dtype[0];
+        const long long at = head * (of_k ? n.w_sh[1] : n.w_sh[0]);
+        load_weight<kDtype, N>(of_k ? kw : qw, w_dtype, at + c0, w0);
+        if (two) load_weight<kDtype, N>(of_k ? kw : qw, w_dtype, at + c1, w1);
+      }
     }
-    for (int from = 0; from < all; from += kHeads * groups) {
-      Vec x0[kHeads], x1[kHeads];
-      int token[kHeads], head[kHeads];
+    if (from == 0) {
+      int raw = 0;  // of the position, float or int
+      if (has_angle) {
+        uint32_t ab, at;
+        place(angle_token, ab, at);
+        raw = static_cast<const int*>(a.positions)[ab * a.pos_sb + (long long)at * a.axes + axis];
+      }
+      // half of the workgroup stages q's weight, the other one k's
+      const int which = __builtin_amdgcn_readfirstlane(tid / (kThreads / 2)), c = tid % (kThreads / 2) * 4;
+      if (c < a.dim) {
+        float w[4] = {1.f, 1.f, 1.f, 1.f};
+        if ((which ? kw : qw) && !(which ? k_each : q_each))
+          load_weight<kDtype, 4>(which ? kw : qw, which ? n.w_dtype[1] : n.w_dtype[0], c, w);
+        *reinterpret_cast<float4*>(&weights[which][c]) = make_float4(w[0], w[1], w[2], w[3]);
+      }
+      const double all_turns = (a.int_positions ? (double)raw : (double)__int_as_float(raw)) * frequency;
+      const float rest = (float)(all_turns - rint(all_turns));  // in [-1/2, 1/2]
+      if (has_angle) {
+        float s, cos;
+        sincospif(2.f * rest, &s, &cos);
+        table[tid] = make_float2(cos, a.sign * s);
+      }
+      __syncthreads();
+    }
+    float q = 0.f, v0[N], v1[N];
 #pragma unroll
-      for (int u = 0; u < kHeads; ++u) {
-        const int h = from + u * groups + group;
-        x0[u] = Vec{}, x1[u] = Vec{};
-        token[u] = over(h, n.by_heads[which]);
-        head[u] = h - token[u] * heads;
-        if (live && h < all) {
-          const T* x = static_cast<const T*>(side.x) + at_b[token[u]] * side.sb + at_t[token[u]] * side.st + head[u] * side.sh;
-          x0[u] = *reinterpret_cast<const Vec*>(x + c0);
-          if (two) x1[u] = *reinterpret_cast<const Vec*>(x + c1);
+    for (int j = 0; j < N; ++j) {
+      v0[j] = (float)x0[j], v1[j] = (float)x1[j];
+      q = fmaf(v0[j], v0[j], q);
+      if (!kAdjacent) q = fmaf(v1[j], v1[j], q);
+    }
+    const float rstd = 1.f / sqrtf(group_sum(q, n.lane_bits) / (float)a.dim + n.eps);
+    if (!live) continue;
+    if (!each) {
+      const float* w = weights[of_k ? 1 : 0];
+#pragma unroll
+      for (int j = 0; j < N; j += 4) {
+        const float4 f = *reinterpret_cast<const float4*>(w + c0 + j), g = *reinterpret_cast<const float4*>(w + (two ? c1 : c0) + j);
+        w0[j] = f.x, w0[j + 1] = f.y, w0[j + 2] = f.z, w0[j + 3] = f.w;
+        w1[j] = g.x, w1[j + 1] = g.y, w1[j + 2] = g.z, w1[j + 3] = g.w;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < N; ++j) v0[j] = v0[j] * rstd * w0[j], v1[j] = v1[j] * rstd * w1[j];
+    if (turns) {
+      const float2* cs = table + token * pairs + (kAdjacent ? item * (N / 2) : item * N);
+      if constexpr (kAdjacent) {
+#pragma unroll
+        for (int j = 0; j < N; j += 2) {
+          const float2 r = cs[j / 2];
+          const float p = v0[j];
+          v0[j] = p * r.x - v0[j + 1] * r.y;
+          v0[j + 1] = v0[j + 1] * r.x + p * r.y;
         }
-      }
-      if (!formed) {
-        form_angles(a, first, here, table, at_b, at_t);
-        __syncthreads();
-        formed = true;
-      }
-#pragma unroll
-      for (int u = 0; u < kHeads; ++u) {
-        float q = 0.f, v0[N], v1[N];
+      } else {
 #pragma unroll
         for (int j = 0; j < N; ++j) {
-          v0[j] = (float)x0[u][j], v1[j] = (float)x1[u][j];
-          q = fmaf(v0[j], v0[j], q);
-          if (!kAdjacent) q = fmaf(v1[j], v1[j], q);
+          const float2 r = cs[j];
+          const float p = v0[j];
+          v0[j] = p * r.x - v1[j] * r.y;
+          v1[j] = v1[j] * r.x + p * r.y;
         }
-        const float rstd = 1.f / sqrtf(group_sum(q, n.lane_bits) / (float)a.dim + n.eps);
-        const int h = from + u * groups + group;
-        if (!live || h >= all) continue;
-        if (w && n.w_sh[which]) {
-          load_weight<kDtype, N>(w, n.w_dtype[which], head[u] * n.w_sh[which] + c0, w0);
-          if (two) load_weight<kDtype, N>(w, n.w_dtype[which], head[u] * n.w_sh[which] + c1, w1);
-        }
-#pragma unroll
-        for (int j = 0; j < N; ++j) v0[j] = v0[j] * rstd * w0[j], v1[j] = v1[j] * rstd * w1[j];
-        T* y = static_cast<T*>(side.y) + at_b[token[u]] * side.ob + at_t[token[u]] * side.ot + head[u] * side.oh;
-        Vec y0, y1;
-        if (turns) {
-          const float2* cs = table + token[u] * pairs + (kAdjacent ? item * (N / 2) : item * N);
-          if constexpr (kAdjacent) {
-#pragma unroll
-            for (int j = 0; j < N; j += 2) {
-              const float2 r = cs[j / 2];
-              const float p = v0[j];
-              v0[j] = p * r.x - v0[j + 1] * r.y;
-              v0[j + 1] = v0[j + 1] * r.x + p * r.y;
-            }
-          } else {
-#pragma unroll
-            for (int j = 0; j < N; ++j) {
-              const float2 r = cs[j];
-              const float p = v0[j];
-              v0[j] = p * r.x - v1[j] * r.y;
-              v1[j] = v1[j] * r.x + p * r.y;
-            }
-          }
-        }
-#pragma unroll
-        for (int j = 0; j < N; ++j) y0[j] = (T)v0[j], y1[j] = (T)v1[j];
-        *reinterpret_cast<Vec*>(y + c0) = y0;
-        if (two) *reinterpret_cast<Vec*>(y + c1) = y1;
       }
     }
+    Vec y0, y1;
+#pragma unroll
+    for (int j = 0; j < N; ++j) y0[j] = (T)v0[j], y1[j] = (T)v1[j];
+    T* y = static_cast<T*>(of(&Side::y)) + b * of(&Side::ob) + t * of(&Side::ot) + head * of(&Side::oh);
+    *reinterpret_cast<Vec*>(y + c0) = y0;
+    if (two) *reinterpret_cast<Vec*>(y + c1) = y1;
   }
 }
 
@@ -480,8 +506,10 @@ extern "C" int musc_norm_rotary(const musc_rotary_call* call, const void* q_weig
   if (total == 0) return MUSC_OK;
   if (vec < 4) vec = 0;
   a.items = items_of(*call, vec);
+  // 8 workgroups a CU: 4 x 1370 tokens 12.2 us so, 12.6 with two; 3 x 900 of 72 channels in fp32 13.6 and 17.8
+  while (a.tokens > 1 && total / a.tokens < 2048) --a.tokens;
   while (vec && a.items > 1 << n.lane_bits) ++n.lane_bits;
-  n.by_heads[0] = reciprocal(a.q.heads), n.by_heads[1] = reciprocal(a.k.heads);
+  a.by_heads = reciprocal((long long)a.q.heads + a.k.heads);  // exact below 2^32 / heads: 16 tokens of 1024 at most
   n.eps = eps;
   const dim3 grid = linear_grid((total + a.tokens - 1) / a.tokens);
   const bool adjacent = call->adjacent;

@@ -56,18 +56,27 @@ def _head_rows(x, name, axes):
     return x if x.stride(-1) == 1 else x.contiguous()
 
 
-def _head_weight(weight, name, x):
+def _head_weight(weight, name, h, d, dtype, index):
     """(tensor, elements between the weights of two heads, storage) of a head norm's weight."""
     rt.require_device_tensor(weight, name)
     rt.require_no_gradient(weight)
-    h, d = x.shape[2:]
-    if (weight.get_device() != x.get_device() or weight.dtype not in (x.dtype, torch.float32)
-            or (weight.shape != (d,) and weight.shape != (h, d))):
+    per_head, w_dtype = weight.dim() == 2, weight.dtype
+    if (weight.get_device() != index or (w_dtype is not dtype and w_dtype is not torch.float32) or weight.dim() not in (1, 2)
+            or weight.shape[-1] != d or (per_head and weight.shape[0] != h)):
         raise ValueError(f"{name} must be ({d},) or ({h}, {d}) on its input's device, in its dtype or float32")
-    weight = weight.contiguous()
-    if weight.data_ptr() % 16:
-        weight = weight.clone()     # read as 16-byte vectors
-    return weight, d if weight.dim() == 2 else 0, _STORAGE[weight.dtype]
+    if not weight.is_contiguous() or weight.data_ptr() % 16:
+        weight = weight.clone(memory_format=torch.contiguous_format)     # read as 16-byte vectors
+    return weight, d if per_head else 0, _STORAGE[w_dtype]
+
+
+def _turned(out, x, name):
+    """(tensor to write, its strides as rt.token_strides has them)."""
+    if out is None:
+        out = torch.empty_like(x, memory_format=torch.contiguous_format)
+        _, t, h, d = x.shape
+        return out, (t * h * d, h * d, d)
+    out = rt.output_like(out, x, name)
+    return out, rt.token_strides(out)
 
 
 def _turn(q, k, positions, axes, inverse, out, norm):
@@ -76,43 +85,47 @@ def _turn(q, k, positions, axes, inverse, out, norm):
         with torch.cuda.device(q.device):
             return _turn(q, k, positions, axes, inverse, out, norm)
     rt.require_no_gradient(q, k, positions, *(out if isinstance(out, (tuple, list)) else (out,)))
-    index = q.get_device()
+    index, dtype = q.get_device(), q.dtype
     b, t, h, d = q2.shape
     k2, ko, k_heads, k_args = None, None, 0, (0, 0, 0, 0, 0, 0, 0, 0)
     if k is not None:
         k2 = _head_rows(k, 'k', axes)
-        if k2.shape[0] != b or k2.shape[1] != t or k2.dtype != q2.dtype or k2.get_device() != index:
+        kb, kt, hk, _ = k2.shape
+        if kb != b or kt != t or k2.dtype is not dtype or k2.get_device() != index:
             raise ValueError('k must match q in batch, tokens, dtype and device')
         if out is not None and len(out) != 2:
             raise ValueError('out must be (q_out, k_out)')
     rt.require_device_tensor(positions, 'positions')
-    shape = positions.shape
+    n, shared = axes.axes, positions.dim() == 2
     if (positions.dtype not in (torch.float32, torch.int32) or positions.get_device() != index
-            or (shape != (b, t, axes.axes) and shape != (t, axes.axes))):
-        raise ValueError(f"positions must be float32 or int32 of shape (T, {axes.axes}) or (B, T, {axes.axes}) on q's device")
+            or tuple(positions.shape) != ((t, n) if shared else (b, t, n))):
+        raise ValueError(f"positions must be float32 or int32 of shape (T, {n}) or (B, T, {n}) on q's device")
     if axes.frequency.get_device() != index:
         raise ValueError("axes must be on q's device")
     positions = positions.contiguous()
-    weights = []
+    qw = kw = None
+    q_sh = k_sh = 0
+    q_type = k_type = rt.DTYPE_F32
     if norm is not None:
-        for weight, name, x in ((norm[0], 'q_weight', q2), (norm[1], 'k_weight', k2)):
-            weights.append((None, 0, rt.DTYPE_F32) if weight is None or x is None else _head_weight(weight, name, x))
+        if norm[0] is not None:
+            qw, q_sh, q_type = _head_weight(norm[0], 'q_weight', h, d, dtype, index)
+        if norm[1] is not None and k is not None:
+            kw, k_sh, k_type = _head_weight(norm[1], 'k_weight', hk, d, dtype, index)
     if k2 is not None:
-        ko = rt.output_like(out[1] if out is not None else None, k2, 'k_out')
-        if k2.shape[2]:
-            k_heads = k2.shape[2]
-            k_args = (k2.data_ptr(), *rt.token_strides(k2), ko.data_ptr(), *rt.token_strides(ko))
+        ko, ko_strides = _turned(out[1] if out is not None else None, k2, 'k_out')
+        if hk:
+            k_heads = hk
+            k_args = (k2.data_ptr(), *rt.token_strides(k2), ko.data_ptr(), *ko_strides)
         out = out[0] if out is not None else None
-    qo = rt.output_like(out, q2, 'q_out')
+    qo, qo_strides = _turned(out, q2, 'q_out')
     if b and t and h:
         call = rt.PACK_ROTARY.pack(
-            q2.data_ptr(), *rt.token_strides(q2), qo.data_ptr(), *rt.token_strides(qo), *k_args, positions.data_ptr(),
-            0 if len(shape) == 2 else t * axes.axes, axes.frequency.data_ptr(), axes.axis.data_ptr(), h, k_heads, _STORAGE[q2.dtype], b, t,
-            d, positions.dtype == torch.int32, axes.axes, axes.pairs, axes.adjacent, inverse)
+            q2.data_ptr(), *rt.token_strides(q2), qo.data_ptr(), *qo_strides, *k_args, positions.data_ptr(), 0 if shared else t * n,
+            axes.frequency.data_ptr(), axes.axis.data_ptr(), h, k_heads, _STORAGE[dtype], b, t, d, positions.dtype is torch.int32, n,
+            axes.pairs, axes.adjacent, inverse)
         if norm is None:
             rt.check(rt.library().musc_rotary(call, rt.current_stream(index)), 'musc_rotary')
         else:
-            (qw, q_sh, q_type), (kw, k_sh, k_type) = weights
             rt.check(rt.library().musc_norm_rotary(call, None if qw is None else qw.data_ptr(), q_sh, q_type,
                                                    None if kw is None else kw.data_ptr(), k_sh, k_type, norm[2],
                                                    rt.current_stream(index)), 'musc_norm_rotary')

@@ -245,7 +245,7 @@ def current_stream(index: int) -> int:
 
 def elsewhere(x: torch.Tensor) -> bool:
     """Whether x lies on another GPU than the current one, which then has to be made current."""
-    return x.is_cuda and x.get_device() != torch.cuda.current_device()
+    return x.is_cuda and x.get_device() != torch._C._cuda_getDevice()
 
 
 def require_device_tensor(t: torch.Tensor, name: str) -> None:
@@ -275,6 +275,8 @@ def token_strides(x: torch.Tensor) -> tuple[int, int, int]:
     one element has none."""
     b, t, h, _ = x.shape
     sb, st, sh, _ = x.stride()
+    if b > 1 and t > 1 and h > 1:
+        return sb, st, sh
     return sb if b > 1 else 0, st if t > 1 else 0, sh if h > 1 else 0
 
 
