@@ -215,7 +215,9 @@ int plan(const musc_masked_attention& c, Args& a, int& waves) {
     if (a.in_pieces) a.jobs = (int)schedule_pieces(a.row_tiles);
   } else if (whole < (waves == 1 ? 1024 : 256)) {
     // few rows: their keys in splits of at least one tile (4 where four waves share the tiles)
-    long long splits = ((waves == 1 ? 2048 : 512) + whole - 1) / whole;
+    // (a window's first look over all tiles pays for fewer workgroups: 8 x 4096 of 32768 keys, 32 heads on 8 of
+    // 128, bf16, 2048 waves 45 us with the join, 1024 36, 512 37)
+    long long splits = ((waves == 1 ? (a.window ? 1024 : 2048) : 512) + whole - 1) / whole;
     const int least = waves == 1 ? 1 : 4;
     if (splits > a.key_tiles / least) splits = a.key_tiles / least;
     if (splits > kMaxSplits) splits = kMaxSplits;
@@ -233,49 +235,63 @@ int plan_window(const musc_masked_attention& c, int window, int sinks, Args& a, 
   return plan(call, a, waves);
 }
 
-// Shape of one launch after a prefix: the rows of `batches` entries over p_tiles of the prefix and the own
-// keys, if any.
-int shape(Args& a, long long rows, int batches, bool of_prefix, bool of_own, int most_splits, int& waves) {
+// Shape of the work after a prefix: the rows of `batches` entries, by `waves` waves, over its tiles and those
+// of the own keys, as given; a workgroup's waves sharing few rows' tiles (teams > 1), or the tiles in
+// splits, for `enough` workgroups.
+int shape(Args& a, long long rows, int batches, int waves, bool of_prefix, bool of_own, int teams, int enough) {
   const musc_masked_attention& c = a.c;
   if (rows > 0x7fffff00LL) return MUSC_ERR_UNSUPPORTED;
   a.rows = (int)rows, a.batches = batches;
-  waves = rows <= 32 ? 1 : 4;
   const int tile = waves == 1 || c.dtype == MUSC_DTYPE_F32 ? 32 : 64;
   a.row_tiles = (int)((rows + 32 * waves - 1) / (32 * waves));
   a.p_tiles = of_prefix ? (a.p.len + tile - 1) / tile : 0;
   a.key_tiles = a.p_tiles + (of_own ? (c.k_len + tile - 1) / tile : 0);
   a.summaries = (c.k_len + kSummaryKeys - 1) / kSummaryKeys;
-  a.jobs = a.row_tiles, a.teams = 1, a.splits = 1;
+  a.jobs = a.row_tiles, a.teams = teams, a.splits = 1;
   const long long heads = (long long)batches * c.kv_heads, whole = heads * a.row_tiles;
-  if (whole < (waves == 1 ? 1024 : 256)) {
-    long long splits = ((waves == 1 ? 2048 : 512) + whole - 1) / whole;
-    const int least = waves == 1 ? 1 : 4;
+  if (teams == 1 && 2 * whole <= enough) {
+    long long splits = (enough + whole - 1) / whole;
+    const int least = waves == 1 ? 1 : c.dtype == MUSC_DTYPE_F32 ? 2 : 4, most = a.partial ? kMaxSplits / 2 : kMaxSplits;
     if (splits > a.key_tiles / least) splits = a.key_tiles / least;
-    if (splits > most_splits) splits = most_splits;
+    if (splits > most) splits = most;
     a.splits = splits < 1 ? 1 : (int)splits;
   }
   return finish(a, heads, waves);
 }
 
-// After a prefix: each entry's rows over it and their own keys in one launch, or, where the tiles of the
-// entries' few rows would leave places empty, the rows of all entries over the prefix, and then each entry's
-// over its own keys (more).
-int plan_prefix(const musc_masked_attention& c, const musc_attention_prefix& p, Args& a, int& waves, Args& more,
-                int& more_waves) {
+// After a prefix: each entry's rows over it and their own keys, or, where the tiles of the entries' few rows
+// would leave places empty, the rows of all entries over the prefix and, in the same launch, each entry's over
+// its own keys (more), and a join.
+int plan_prefix(const musc_masked_attention& c, const musc_attention_prefix& p, Args& a, Args& more, int& waves) {
   a.c = c, a.p = p;
   a.c.schedule = nullptr;
   a.group = c.heads / c.kv_heads;
-  const long long rows = (long long)c.q_len * a.group, all = rows * c.batch;
+  const long long rows = (long long)c.q_len * a.group, all = rows * c.batch, heads = (long long)c.batch * c.kv_heads;
   if (p.len > 0x7fffff00 || c.k_len > 0x7fffff00) return MUSC_ERR_UNSUPPORTED;
+  const int teams = teams_of((c.d <= 64 ? 64 : 128) * (c.dtype == MUSC_DTYPE_F32 ? 4 : 2));
+  const long long tiles = (p.len + 31LL) / 32 + (c.k_len + 31LL) / 32;
+  // few rows, and up to two rounds of workgroups whose waves have a few tiles each: no join (2 single tokens
+  // after 300 keys, 16 heads of 64, fp16: 10 us, stacked and joined 20)
+  if (rows <= 32 && tiles <= kTeamTiles * teams && heads <= 512) {
+    more = a, waves = 1;
+    return shape(a, rows, c.batch, waves, true, true, teams, 0);
+  }
   const long long apart = c.batch * ((rows + kRowTile - 1) / kRowTile), together = (all + kRowTile - 1) / kRowTile;
   a.stacked = c.batch > 1 && 2 * apart >= 3 * together && all * c.kv_heads < (1 << 24);
-  more = a;
-  if (!a.stacked) return shape(a, rows, c.batch, true, true, kMaxSplits, waves);
+  if (!a.stacked) {
+    more = a, waves = rows <= 32 ? 1 : 4;
+    return shape(a, rows, c.batch, waves, true, true, 1, waves == 1 ? 1024 : 512);
+  }
+  // As many workgroups for each of the two as there are CUs: 32 single tokens after 16384 keys and over up to
+  // 700 of their own, 32 heads on 8 of 128, bf16: 36 us and 7 for the join; 512 of each 40 and 11; apart 25, 22
+  // and 11.
   a.partial = 1;
-  if (const int rc = shape(a, all, 1, true, false, kMaxSplits / 2, waves)) return rc;
+  waves = all <= 32 ? 1 : 4;
+  more = a;
+  more.stacked = 0;
+  if (const int rc = shape(a, all, 1, waves, true, false, 1, waves == 1 ? 1024 : 256)) return rc;
   if (c.k_len == 0) return MUSC_OK;
-  more.partial = 1, more.stacked = 0;
-  return shape(more, rows, c.batch, false, true, kMaxSplits / 2, more_waves);
+  return shape(more, rows, c.batch, waves, false, true, 1, waves == 1 ? 1024 : 256);
 }
 
 // Rows that write parts: of every split, or of every job.
@@ -457,8 +473,8 @@ extern "C" int musc_prefix_attention_workspace_bytes(const musc_masked_attention
   if (!out) return MUSC_ERR_INVALID_ARG;
   if (const int rc = mattn::check_prefix(c, p)) return rc;
   mattn::Args a{}, more{};
-  int waves, more_waves;
-  if (const int rc = mattn::plan_prefix(*c, *p, a, waves, more, more_waves)) return rc;
+  int waves;
+  if (const int rc = mattn::plan_prefix(*c, *p, a, more, waves)) return rc;
   *out = align_up(mattn::part_bytes(a), 256) + (a.stacked && c->k_len ? mattn::part_bytes(more) : 0);
   return MUSC_OK;
 }
@@ -467,16 +483,17 @@ extern "C" int musc_prefix_attention_fwd(const musc_masked_attention* c, const m
                                          size_t workspace_bytes, hipStream_t stream) {
   if (const int rc = mattn::check_prefix(c, p)) return rc;
   mattn::Args a{}, more{};
-  int waves, more_waves = 0;
-  if (const int rc = mattn::plan_prefix(*c, *p, a, waves, more, more_waves)) return rc;
+  int waves;
+  if (const int rc = mattn::plan_prefix(*c, *p, a, more, waves)) return rc;
   const bool two = a.stacked && c->k_len;
+  if (two && a.units + more.units >= (0x100000000LL >> 8) - 2 * kXcds) return MUSC_ERR_UNSUPPORTED;
   const size_t first = align_up(mattn::part_bytes(a), 256), need = first + (two ? mattn::part_bytes(more) : 0);
   if (need && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16)) return MUSC_ERR_WORKSPACE;
   mattn::place_parts(a, static_cast<char*>(workspace));
   if (two) mattn::place_parts(more, static_cast<char*>(workspace) + first);
   const mattn::Args* own = two ? &more : nullptr;
-  if (c->dtype == MUSC_DTYPE_F32) mattn::launch_prefix_f32(a, waves, own, more_waves, stream);
-  else if (c->dtype == MUSC_DTYPE_F16) mattn::launch_prefix_f16(a, waves, own, more_waves, stream);
-  else mattn::launch_prefix_bf16(a, waves, own, more_waves, stream);
+  if (c->dtype == MUSC_DTYPE_F32) mattn::launch_prefix_f32(a, own, waves, stream);
+  else if (c->dtype == MUSC_DTYPE_F16) mattn::launch_prefix_f16(a, own, waves, stream);
+  else mattn::launch_prefix_bf16(a, own, waves, stream);
   return check_launch();
 }

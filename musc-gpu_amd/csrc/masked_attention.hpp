@@ -151,11 +151,17 @@ struct Args {
   // the rows of all are stacked), and whether the rows' parts are joined even if there is one
   musc_attention_prefix p;
   int p_tiles, batches, stacked, partial;
-  int more_splits;    // its join: parts of the second launch
+  int more_splits;    // for the join: parts over the own keys
   float *more_ml, *more_o;
   long long units;
   float* part_ml;  // (units in (b, kv head), rows, split) x (maximum, sum)
   float* part_o;   // the same x d
+};
+
+// Two calls' work in one launch.
+struct TwoArgs {
+  Args first, second;
+  uint32_t first_blocks;
 };
 
 __device__ __forceinline__ float halves_max(float v) {
@@ -195,9 +201,9 @@ void launch_bf16(const Args& a, int waves, hipStream_t stream);
 void launch_window_f32(const Args& a, int waves, hipStream_t stream);
 void launch_window_f16(const Args& a, int waves, hipStream_t stream);
 void launch_window_bf16(const Args& a, int waves, hipStream_t stream);
-void launch_prefix_f32(const Args& a, int waves, const Args* more, int more_waves, hipStream_t stream);
-void launch_prefix_f16(const Args& a, int waves, const Args* more, int more_waves, hipStream_t stream);
-void launch_prefix_bf16(const Args& a, int waves, const Args* more, int more_waves, hipStream_t stream);
+void launch_prefix_f32(const Args& a, const Args* more, int waves, hipStream_t stream);
+void launch_prefix_f16(const Args& a, const Args* more, int waves, hipStream_t stream);
+void launch_prefix_bf16(const Args& a, const Args* more, int waves, hipStream_t stream);
 
 }  // namespace mattn
 }  // namespace musc

@@ -50,8 +50,7 @@ __device__ __forceinline__ int4v resource(const void* base, long long bytes) {
 // tiles are of a prefix that the batch shares; a.stacked: all rows of the batch over those tiles.
 constexpr int kCapped = 1, kBiased = 2, kInParts = 4, kEither = 8, kLargeCap = 16, kWindowed = 32, kPrefixed = 64;
 template <int kDtype, int kD, int kWaves, int kTeams, int kMode>
-__global__ __launch_bounds__(kWaves * kTeams * kWave, kWaves == 1 ? 1 : kD == 64 && kDtype != MUSC_DTYPE_F32 ? 3 : 2) void masked_attention_kernel(
-    const Args a) {
+__device__ __forceinline__ void attention_of_block(const Args& a, const uint32_t block, const uint32_t blocks) {
   using Ty = Type<kDtype>;
   typedef typename Ty::T T;
   constexpr bool k16 = kDtype != MUSC_DTYPE_F32;
@@ -77,16 +76,16 @@ __global__ __launch_bounds__(kWaves * kTeams * kWave, kWaves == 1 ? 1 : kD == 64
   uint32_t split, job, bh;
   if (a.heads_at_once) {
     // one XCD works on heads_at_once heads together, row tile by row tile (the longest first)
-    const uint32_t per_xcd = (uint32_t)((prefixed ? a.batches : c.batch) * c.kv_heads) / kXcds, local = blockIdx.x / kXcds;
+    const uint32_t per_xcd = (uint32_t)((prefixed ? a.batches : c.batch) * c.kv_heads) / kXcds, local = block / kXcds;
     const uint32_t of_group = (uint32_t)(a.heads_at_once * a.jobs * a.splits);
     const uint32_t group = uniform(local / of_group), in_group = local - group * of_group;
     const uint32_t first = group * a.heads_at_once, at_once = min((uint32_t)a.heads_at_once, per_xcd - first);
     const uint32_t rest = uniform(in_group / a.splits);
     split = in_group - rest * a.splits;
     job = uniform(rest / at_once);
-    bh = blockIdx.x % kXcds * per_xcd + first + (rest - job * at_once);
+    bh = block % kXcds * per_xcd + first + (rest - job * at_once);
   } else {
-    const uint32_t unit = (blockIdx.x % kXcds) * (gridDim.x / kXcds) + blockIdx.x / kXcds;
+    const uint32_t unit = (block % kXcds) * (blocks / kXcds) + block / kXcds;
     if (unit >= (uint32_t)a.units) return;
     const uint32_t rest = uniform(unit / a.splits);
     split = unit - rest * a.splits;
@@ -120,6 +119,16 @@ __global__ __launch_bounds__(kWaves * kTeams * kWave, kWaves == 1 ? 1 : kD == 64
     return k;
   };
   const int4 first_summary = summary_of(lo / 64 * 64 + lane);
+  // a window's tiles are all looked at before the first: each wave takes every n-th 64, the first ones
+  // asked for now too
+  constexpr int kAll = kWaves * kTeams, kAhead = !windowed ? 0 : kAll == 1 ? 16 : 4;
+  const int self = windowed ? __builtin_amdgcn_readfirstlane(tid / kWave) : 0;
+  const bool look = windowed && (hi > 64 || (kTeams == 1 && a.splits > 1));
+  int4 ahead[windowed ? kAhead : 1];
+  if (look) {
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) ahead[i] = summary_of((self + i * kAll) * 64 + lane);
+  }
 
   // the row tile, or the part of its keys, that the schedule names; without one later rows first:
   // with an order of tokens they see more keys, and the longest work should not start last
@@ -208,40 +217,39 @@ __global__ __launch_bounds__(kWaves * kTeams * kWave, kWaves == 1 ? 1 : kD == 64
     }
   }
 
-  // Of a window: the order of the first key in it; which 64s of tiles hold some that the workgroup's rows
+  // Of a window: the order of the first key in it, and which 64s of tiles hold some that the workgroup's rows
   // see (bit 63: all from the 63rd on), found by all waves before any of them has its accumulators; and of
   // the splits only as many as there are such tiles (four of them for four waves) have work.
   const auto window_from = [&](int order) { return __builtin_elementwise_sub_sat(order, a.window - 1); };
-  // this row's window: its first order and how many follow; and its sinks
-  const int qfirst = windowed ? window_from(qord) : 0;
-  const uint32_t qspan = windowed ? (uint32_t)qord - (uint32_t)qfirst : 0;
-  const uint32_t qsinks = windowed && qord >= 0 && a.sinks > 0 ? (uint32_t)min(qord, a.sinks - 1) + 1 : 0;
   auto may_see_tile = [&](const int4 k, const Range& r) __attribute__((always_inline)) {
     return k.y >= 0 && k.x <= r.dmax && k.y >= r.dmin && k.z <= r.omax &&
            (!windowed || k.w >= window_from(r.omin) || (k.w >= 0 && k.z < a.sinks));
   };
   unsigned long long chunks = ~0ull;
+  constexpr int kLeast = kDtype == MUSC_DTYPE_F32 ? 2 : 4;  // tiles of a split
   if constexpr (windowed) {
-    if (hi > 64 || (kTeams == 1 && a.splits > 1)) {
-      constexpr int kAll = kWaves * kTeams;
-      const int self = __builtin_amdgcn_readfirstlane(tid / kWave);
+    if (look) {
       unsigned long long here = 0;
       int seen_tiles = 0;
-#pragma unroll 4
-      for (int n = self; n * 64 < hi; n += kAll) {
-        const int t = n * 64 + lane;
-        const unsigned long long some = __ballot(t < hi && may_see_tile(summary_of(t), all_rows));
+      auto look_at = [&](int n, const int4 k) __attribute__((always_inline)) {
+        const unsigned long long some = __ballot(n * 64 + lane < hi && may_see_tile(k, all_rows));
         if (some) here |= 1ull << min(n, 63);
         seen_tiles += __popcll(some);
-      }
+      };
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) look_at(self + i * kAll, ahead[i]);
+#pragma unroll 4
+      for (int n = self + kAhead * kAll; n * 64 < hi; n += kAll) look_at(n, summary_of(n * 64 + lane));
       if (lane == 0) chunks_s[self] = here, seen_s[self] = seen_tiles;
       __syncthreads();
       chunks = 0, seen_tiles = 0;
 #pragma unroll
       for (int w = 0; w < kAll; ++w) chunks |= chunks_s[w], seen_tiles += seen_s[w];
+      chunks = (unsigned long long)(uint32_t)__builtin_amdgcn_readfirstlane((int)(chunks >> 32)) << 32 |
+               (uint32_t)__builtin_amdgcn_readfirstlane((int)chunks);
       if (kTeams == 1 && a.splits > 1) {
         seen_tiles = __builtin_amdgcn_readfirstlane(seen_tiles);
-        parts = max(min(parts, kWaves == 1 ? seen_tiles : (seen_tiles + 3) / 4), 1);
+        parts = max(min(parts, kWaves == 1 ? seen_tiles : (seen_tiles + kLeast - 1) / kLeast), 1);
         if (part >= parts) {  // the whole workgroup
           if (inside && lh == 0)
             reinterpret_cast<float2*>(a.part_ml)[((long long)bh * a.rows + row) * a.splits + split] = make_float2(-INFINITY, 0.f);
@@ -435,6 +443,12 @@ __global__ __launch_bounds__(kWaves * kTeams * kWave, kWaves == 1 ? 1 : kD == 64
     uint32_t seen = 0xffffffffu;
     if (!whole) {
       mixed_seen = true;
+      // this row's window: its first order and how many follow, and its sinks; formed anew, as v_at is
+      int order = qord;
+      if (windowed) asm volatile("" : "+v"(order));
+      const int qfirst = windowed ? window_from(order) : 0;
+      const uint32_t qspan = (uint32_t)order - (uint32_t)qfirst;
+      const uint32_t qsinks = windowed && order >= 0 && a.sinks > 0 ? (uint32_t)min(order, a.sinks - 1) + 1 : 0;
       const bool shared = prefixed && tile < p_tiles;
       const int rem = shared ? a.p.len - tile * kTile : k_len - (tile - p_tiles) * kTile;
 #pragma unroll
@@ -712,6 +726,21 @@ __global__ __launch_bounds__(kWaves * kTeams * kWave, kWaves == 1 ? 1 : kD == 64
   }
 }
 
+#define MUSC_MASKED_ATTENTION_BOUNDS \
+  __launch_bounds__(kWaves * kTeams * kWave, kWaves == 1 ? 1 : kD == 64 && kDtype != MUSC_DTYPE_F32 ? 3 : 2)
+template <int kDtype, int kD, int kWaves, int kTeams, int kMode>
+__global__ MUSC_MASKED_ATTENTION_BOUNDS void masked_attention_kernel(const Args a) {
+  attention_of_block<kDtype, kD, kWaves, kTeams, kMode>(a, blockIdx.x, gridDim.x);
+}
+// The same with the work of two calls side by side, the second's workgroups after the first's (whose number
+// is a multiple of the XCDs).
+template <int kDtype, int kD, int kWaves, int kTeams, int kMode>
+__global__ MUSC_MASKED_ATTENTION_BOUNDS void prefixed_attention_kernel(const TwoArgs two) {
+  const bool second = blockIdx.x >= two.first_blocks;
+  const uint32_t before = second ? two.first_blocks : 0, blocks = second ? gridDim.x - before : two.first_blocks;
+  attention_of_block<kDtype, kD, kWaves, kTeams, kMode>(second ? two.second : two.first, blockIdx.x - before, blocks);
+}
+
 // Joins the splits of a row, in their order: four waves per row, each every fourth split with two
 // channels per lane, then the four in order.
 template <int kDtype>
@@ -763,8 +792,8 @@ __global__ __launch_bounds__(256) void join_kernel(const Args a) {
   *reinterpret_cast<Two*>(orow + 2 * lane) = out;
 }
 
-// Joins what the rows of prefixed attention have in a.splits parts of one launch and a.more_splits of
-// another, in their order: the kernel above over both.
+// Joins what the rows of prefixed attention have in a.splits parts over the prefix and a.more_splits over
+// their own keys (or in parts over both), in their order: the kernel above over both.
 template <int kDtype>
 __global__ __launch_bounds__(256) void join_prefixed_kernel(const Args a) {
   typedef typename Type<kDtype>::T T;
@@ -897,66 +926,67 @@ void launch(const Args& a, int waves, hipStream_t stream) {
 }
 
 // Windows and shared prefixes (kExtra): the same kernels with that mode, no parts of row tiles.
-template <int kDtype, int kD, int kMode>
-void launch_one(const Args& a, const dim3& grid, hipStream_t stream) {
-  hipLaunchKernelGGL((masked_attention_kernel<kDtype, kD, 4, 1, kMode>), grid, dim3(4 * kWave), 0, stream, a);
+template <int kDtype, int kD, int kWaves, int kTeams, int kMode>
+void launch_one(const Args& a, const Args* more, hipStream_t stream) {
+  const size_t blocks = align_up((size_t)a.units, kXcds), all = blocks + (more ? align_up((size_t)more->units, kXcds) : 0);
+  if constexpr ((kMode & kPrefixed) != 0) {
+    const TwoArgs two{a, more ? *more : a, (uint32_t)blocks};
+    hipLaunchKernelGGL((prefixed_attention_kernel<kDtype, kD, kWaves, kTeams, kMode>), dim3((unsigned)all),
+                       dim3(kWaves * kTeams * kWave), 0, stream, two);
+  } else {
+    hipLaunchKernelGGL((masked_attention_kernel<kDtype, kD, kWaves, kTeams, kMode>), dim3((unsigned)all),
+                       dim3(kWaves * kTeams * kWave), 0, stream, a);
+  }
 }
 template <int kDtype, int kD, int kMode>
-void launch_few(const Args& a, const dim3& grid, hipStream_t stream) {
+void launch_few(const Args& a, const Args* more, hipStream_t stream) {
   constexpr int kTeams = teams_of((kD <= 64 ? 64 : 128) * (kDtype == MUSC_DTYPE_F32 ? 4 : 2));
-  if constexpr ((kMode & kWindowed) != 0) {
-    if (a.teams > 1) {
-      hipLaunchKernelGGL((masked_attention_kernel<kDtype, kD, 1, kTeams, kMode>), grid, dim3(kTeams * kWave), 0, stream, a);
-      return;
-    }
-  }
-  hipLaunchKernelGGL((masked_attention_kernel<kDtype, kD, 1, 1, kMode>), grid, dim3(kWave), 0, stream, a);
+  if (a.teams > 1) launch_one<kDtype, kD, 1, kTeams, kMode>(a, more, stream);
+  else launch_one<kDtype, kD, 1, 1, kMode>(a, more, stream);
 }
 template <int kDtype, int kD, int kExtra>
-void launch_extra(const Args& a, int waves, hipStream_t stream) {
-  const dim3 grid((unsigned)align_up((size_t)a.units, kXcds));
+void launch_extra(const Args& a, const Args* more, int waves, hipStream_t stream) {
   const int mode = (a.c.cap > 0.f ? kCapped : 0) | (a.c.axes ? kBiased : 0);
   constexpr int kWide = kD <= 64 ? 64 : 128;
   if constexpr (kDtype != MUSC_DTYPE_F32) {
     if (a.c.cap > kSmallCap) {
-      if (waves == 1) launch_few<kDtype, kWide, kEither | kLargeCap | kExtra>(a, grid, stream);
-      else launch_one<kDtype, kWide, kEither | kLargeCap | kExtra>(a, grid, stream);
+      if (waves == 1) launch_few<kDtype, kWide, kEither | kLargeCap | kExtra>(a, more, stream);
+      else launch_one<kDtype, kWide, 4, 1, kEither | kLargeCap | kExtra>(a, more, stream);
       return;
     }
   }
   if (waves == 1) {
-    if (mode == 0) launch_few<kDtype, kWide, kExtra>(a, grid, stream);
-    else launch_few<kDtype, kWide, kEither | kExtra>(a, grid, stream);
+    if (mode == 0) launch_few<kDtype, kWide, kExtra>(a, more, stream);
+    else launch_few<kDtype, kWide, kEither | kExtra>(a, more, stream);
   } else if (mode == 0) {
-    launch_one<kDtype, kD, kExtra>(a, grid, stream);
+    launch_one<kDtype, kD, 4, 1, kExtra>(a, more, stream);
   } else if (mode == kCapped) {
-    launch_one<kDtype, kD, kCapped | kExtra>(a, grid, stream);
+    launch_one<kDtype, kD, 4, 1, kCapped | kExtra>(a, more, stream);
   } else if (mode == kBiased) {
-    launch_one<kDtype, kD, kBiased | kExtra>(a, grid, stream);
+    launch_one<kDtype, kD, 4, 1, kBiased | kExtra>(a, more, stream);
   } else {
-    launch_one<kDtype, kD, kCapped | kBiased | kExtra>(a, grid, stream);
+    launch_one<kDtype, kD, 4, 1, kCapped | kBiased | kExtra>(a, more, stream);
   }
 }
 template <int kDtype, int kExtra>
-void launch_extra(const Args& a, int waves, hipStream_t stream) {
-  if (a.c.d <= 64) launch_extra<kDtype, 64, kExtra>(a, waves, stream);
-  else if (a.c.d <= 96) launch_extra<kDtype, 96, kExtra>(a, waves, stream);
-  else launch_extra<kDtype, 128, kExtra>(a, waves, stream);
+void launch_extra(const Args& a, const Args* more, int waves, hipStream_t stream) {
+  if (a.c.d <= 64) launch_extra<kDtype, 64, kExtra>(a, more, waves, stream);
+  else if (a.c.d <= 96) launch_extra<kDtype, 96, kExtra>(a, more, waves, stream);
+  else launch_extra<kDtype, 128, kExtra>(a, more, waves, stream);
 }
 template <int kDtype>
 void launch_windowed(const Args& a, int waves, hipStream_t stream) {
-  launch_extra<kDtype, kWindowed>(a, waves, stream);
+  launch_extra<kDtype, kWindowed>(a, nullptr, waves, stream);
   if (a.splits > 1) {
     const long long rows = (long long)a.c.batch * a.c.kv_heads * a.rows;
     hipLaunchKernelGGL((join_kernel<kDtype>), dim3((unsigned)rows), dim3(256), 0, stream, a);
   }
 }
-// One launch (more == null), or all rows over the prefix and then each entry's over its own keys.
+// more: the entries' own keys, beside all rows over the prefix.
 template <int kDtype>
-void launch_prefixed(const Args& a, int waves, const Args* more, int more_waves, hipStream_t stream) {
-  launch_extra<kDtype, kPrefixed>(a, waves, stream);
-  if (more) launch_extra<kDtype, kPrefixed>(*more, more_waves, stream);
-  if (a.splits > 1 || a.partial) {
+void launch_prefixed(const Args& a, const Args* more, int waves, hipStream_t stream) {
+  launch_extra<kDtype, kPrefixed>(a, more, waves, stream);
+  if (a.splits > 1 || a.stacked) {
     Args both = a;
     if (more) both.more_splits = more->splits, both.more_ml = more->part_ml, both.more_o = more->part_o;
     const long long rows = (long long)a.c.batch * a.c.kv_heads * a.c.q_len * a.group;

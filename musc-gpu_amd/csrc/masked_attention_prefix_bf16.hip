@@ -2,6 +2,6 @@
 // masked_attention_kernel.hpp).
 #include "masked_attention_kernel.hpp"
 
-void musc::mattn::launch_prefix_bf16(const Args& a, int waves, const Args* more, int more_waves, hipStream_t stream) {
-  launch_prefixed<MUSC_DTYPE_BF16>(a, waves, more, more_waves, stream);
+void musc::mattn::launch_prefix_bf16(const Args& a, const Args* more, int waves, hipStream_t stream) {
+  launch_prefixed<MUSC_DTYPE_BF16>(a, more, waves, stream);
 }

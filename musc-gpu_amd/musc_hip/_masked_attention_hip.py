@@ -129,11 +129,17 @@ def _heads(x, per):
     return x, rt.token_strides(x)
 
 
-def _prefix_heads(x, name, q, hk, per):
+def _prefix_heads(x, name, hk, d, dtype, index, per):
     """A prefix's K or V (P, kv_heads, D), copied where its rows do not start on 16 bytes, and its strides."""
-    if x.dim() != 3 or x.shape[1] != hk or x.shape[2] != q.shape[3] or x.dtype != q.dtype or x.get_device() != q.get_device():
-        raise ValueError(f"{name} must be (P, {hk}, {q.shape[3]}) in q's dtype on its device")
-    x, (_, st, sh) = _heads(x[None], per)
+    if x.dim() != 3 or x.dtype is not dtype or x.get_device() != index:
+        raise ValueError(f"{name} must be (P, {hk}, {d}) in q's dtype on its device")
+    p, heads, width = x.shape
+    if heads != hk or width != d:
+        raise ValueError(f"{name} must be (P, {hk}, {d}) in q's dtype on its device")
+    st, sh, last = x.stride()
+    st, sh = st if p > 1 else 0, sh if hk > 1 else 0
+    if last != 1 or x.data_ptr() % 16 or (st | sh) % per:
+        x, st, sh = x.clone(memory_format=torch.contiguous_format), hk * d, d
     return x, st, sh
 
 
@@ -197,10 +203,10 @@ def _attend(q, k, v, scale, keys, queries, cap, slopes, out, window=None, prefix
         qp_ptr, kp_ptr, slope_ptr = qpos.data_ptr(), kpos.data_ptr(), slopes.data_ptr()
     before = None
     if prefix is not None:
-        pk, pk_st, pk_sh = _prefix_heads(prefix[0], 'prefix_k', q, hk, per)
-        pv, pv_st, pv_sh = _prefix_heads(prefix[1], 'prefix_v', q, hk, per)
-        p, p_pos, p_ptr = pk.shape[1], prefix[2], 0
-        if pv.shape[1] != p:
+        pk, pk_st, pk_sh = _prefix_heads(prefix[0], 'prefix_k', hk, d, dtype, index, per)
+        pv, pv_st, pv_sh = _prefix_heads(prefix[1], 'prefix_v', hk, d, dtype, index, per)
+        p, p_pos, p_ptr = pk.shape[0], prefix[2], 0
+        if pv.shape[0] != p:
             raise ValueError('prefix_v must match prefix_k in shape')
         if axes:
             if p_pos is None:
