@@ -123,6 +123,46 @@ struct Type<MUSC_DTYPE_BF16> {
   }
 };
 
+// fp32 operands as two fp16 numbers each, x 2^n = hi + lo to 2^-22 of x, for windows and after prefixes: a
+// product of two is hi hi + hi lo + lo hi, off by 3 2^-22 of itself at most, at 3/16 of the fp32 instructions'
+// time.  n takes the largest of a row of Q, of a tile of K and of 32 channels of V over the tiles so far to
+// 2^13 .. 2^14, so what is below 2^-17 of that is off by 2^-39 of the largest instead.  Probabilities are
+// taken 2^7 times as large, as in fp16.  Tiles that hold infinities or NaN go by fp32 instructions.
+struct Split {
+  typedef _Float16 Vec __attribute__((ext_vector_type(8)));
+  static constexpr int kTop = 14, kLeast = -100, kInfinity = 0x7f800000;
+  static constexpr float kShift = 7.f;
+  static __device__ __forceinline__ floatx16 mfma(Vec a, Vec b, floatx16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+  }
+  // e with |x| < 2^e, from the bits of |x|; the smallest share kLeast
+  static __device__ __forceinline__ int exponent(int bits) { return max((bits >> 23) - 126, kLeast); }
+  static __device__ __forceinline__ float power(int e) { return __int_as_float((e + 127) << 23); }
+  typedef _Float16 Two __attribute__((ext_vector_type(2)));
+  // two of each: hi is opaque, or the compiler forms it a second time for lo
+  static __device__ __forceinline__ void split(float x, float y, float by, int j, Vec& hi, Vec& lo) {
+    Two h = __builtin_convertvector((float2v{x * by, y * by}), Two);
+    asm("" : "+v"(h));
+    hi[j] = h[0], hi[j + 1] = h[1];
+    lo[j] = (_Float16)fmaf(x, by, -(float)h[0]), lo[j + 1] = (_Float16)fmaf(y, by, -(float)h[1]);
+  }
+  template <typename F>
+  static __device__ __forceinline__ void split(const F& a, const F& b, float by, Vec& hi, Vec& lo) {
+    split(a[0], a[1], by, 0, hi, lo), split(a[2], a[3], by, 2, hi, lo);
+    split(b[0], b[1], by, 4, hi, lo), split(b[2], b[3], by, 6, hi, lo);
+  }
+  // By its series up to 0.3 (the next term is 2^-24 of it), and 1 - 2 / (1 + e^2x): off by 2^-20 of itself.
+  static __device__ __forceinline__ float tanh(float x) {
+    const float y = x * x;
+    float p = fmaf(y, 62.f / 2835.f, -17.f / 315.f);
+    p = fmaf(y, p, 2.f / 15.f);
+    p = fmaf(y, p, -1.f / 3.f);
+    const float near = fmaf(x * y, p, x);
+    const float far = fmaf(__builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * (2.f * kLog2e))), -2.f, 1.f);
+    return fabsf(x) < 0.3f ? near : far;
+  }
+};
+
 // Keys of a tile: workgroups of one wave take 32, so that four of them fit a CU's LDS.
 template <int kDtype, int kWaves>
 constexpr int tile_keys() {

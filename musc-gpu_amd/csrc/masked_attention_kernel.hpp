@@ -63,6 +63,9 @@ __device__ __forceinline__ void attention_of_block(const Args& a, const uint32_t
   static_assert(kLoads * kWaves * 1024 == kPart, "whole loads per wave");
   constexpr int kO = kD / 32;
   constexpr bool windowed = (kMode & kWindowed) != 0, prefixed = (kMode & kPrefixed) != 0;
+  // fp32 as three fp16 products, see Split in masked_attention.hpp
+  constexpr bool kSplit = !k16 && (windowed || prefixed);
+  constexpr float kShift = kSplit ? Split::kShift : Ty::kShift;
   __shared__ __attribute__((aligned(1024))) char staged[2 * kTeams][2 * kPart];
   __shared__ __attribute__((aligned(16))) int docs_s[2 * kTeams][64], ords_s[2 * kTeams][64];
   __shared__ float pos_s[2 * kTeams][64 * kMaxAxes];
@@ -276,6 +279,29 @@ __device__ __forceinline__ void attention_of_block(const Args& a, const uint32_t
     if (negate) qf[m] = -qf[m];
     if (c.scale == 0.f) qf[m] = TVec{};
   }
+  // split: this row's Q in 2^(q_exp - 14), and whether some row of the wave holds what cannot be split
+  Split::Vec qh[kSplit ? kQ / 2 : 1], ql[kSplit ? kQ / 2 : 1];
+  int q_exp = 0;
+  bool q_whole = true;
+  if constexpr (kSplit) {
+    float most = 0.f;
+#pragma unroll
+    for (int m = 0; m < kQ; ++m)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) most = __builtin_elementwise_maximum(most, fabsf(qf[m][j]));
+    most = halves_max(most);
+    q_whole = __all(most < INFINITY);
+    q_exp = Split::exponent(__float_as_int(most));
+    const float by = Split::power(Split::kTop - q_exp);
+#pragma unroll
+    for (int m = 0; m < kQ; m += 2) Split::split(qf[m], qf[m + 1], by, qh[m / 2], ql[m / 2]);
+    if (!q_whole) {  // then only their sum is used: infinities stay what they are
+#pragma unroll
+      for (int m = 0; m < kQ / 2; ++m)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) ql[m][j] = fabsf((float)qh[m][j]) < INFINITY ? ql[m][j] : (_Float16)0.f;
+    }
+  }
   // the B operand of the distances: 1 and -position; slopes in raw units
 #pragma unroll
   for (int x = 0; x < kMaxAxes; ++x) {
@@ -349,6 +375,7 @@ __device__ __forceinline__ void attention_of_block(const Args& a, const uint32_t
   };
 
   floatx16 o[kO];
+  int v_exp[kSplit ? kO : 1];  // split: o is in 2^(v_exp - 14)
   float m_run, l_run;  // running maximum (raw) and sum of this half's keys
   float base;          // exponent of a score: raw * to_log2 + base
   bool mixed_seen;
@@ -382,6 +409,41 @@ __device__ __forceinline__ void attention_of_block(const Args& a, const uint32_t
     for (int u = 0; u < kSub; ++u)
 #pragma unroll
       for (int v = 0; v < 16; ++v) s[u][v] = 0.f;
+    if constexpr (kSplit) {
+      float most = 0.f;
+#pragma unroll
+      for (int m = 0; m < kQ; ++m)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) most = __builtin_elementwise_maximum(most, fabsf(kf[0][m][j]));
+      const int bits = wave_max_int(__float_as_int(most));
+      int k_exp = Split::kTop;
+      if (!careful && q_whole && bits < Split::kInfinity) {
+        k_exp = Split::exponent(bits);
+        const float by = Split::power(Split::kTop - k_exp);
+#pragma unroll
+        for (int m = 0; m < kQ / 2; ++m) {
+          Split::Vec kh, kl;
+          Split::split(kf[0][2 * m], kf[0][2 * m + 1], by, kh, kl);
+          s[0] = Split::mfma(kl, qh[m], s[0]);
+          s[0] = Split::mfma(kh, ql[m], s[0]);
+          s[0] = Split::mfma(kh, qh[m], s[0]);
+          __builtin_amdgcn_sched_barrier(0);  // one pair's registers at a time
+        }
+      } else {
+#pragma unroll
+        for (int m = 0; m < kQ / 2; ++m) {
+          Split::Vec h = qh[m], l = ql[m];
+          asm volatile("" : "+v"(h), "+v"(l));  // Q's sums are formed here, not kept beside its parts
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            s[0] = __builtin_amdgcn_mfma_f32_32x32x2f32(kf[0][2 * m + j / 4][j % 4], (float)h[j] + (float)l[j], s[0], 0, 0, 0);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+      const int by = k_exp + q_exp - 2 * Split::kTop;
+#pragma unroll
+      for (int v = 0; v < 16; ++v) s[0][v] = __builtin_ldexpf(s[0][v], by);
+    } else {
 #pragma unroll
     for (int m = 0; m < kQ; ++m)
 #pragma unroll
@@ -393,6 +455,7 @@ __device__ __forceinline__ void attention_of_block(const Args& a, const uint32_t
           for (int j = 0; j < 4; ++j) s[u] = __builtin_amdgcn_mfma_f32_32x32x2f32(kf[u][m][j], qf[m][j], s[u], 0, 0, 0);
         }
       }
+    }
     // V^T fragments by transposing LDS reads, in flight during the softmax: within a group of 16
     // lanes, lane i's element j is element i % 4 of the 8 bytes that lane 4 j + i / 4 addressed,
     // so with V row-major the lane that addresses V[key0 + r / 4][d0 + 4 (r % 4) ..] (r its place
@@ -422,7 +485,7 @@ __device__ __forceinline__ void attention_of_block(const Args& a, const uint32_t
 #pragma unroll
         for (int v = 0; v < 16; ++v) {
           const float x = s[u][v] * by_cap;
-          s[u][v] = by_exponential ? __builtin_amdgcn_rcpf(-1.f - __builtin_amdgcn_exp2f(x)) : tanhf(x);
+          s[u][v] = by_exponential ? __builtin_amdgcn_rcpf(-1.f - __builtin_amdgcn_exp2f(x)) : kSplit ? Split::tanh(x) : tanhf(x);
         }
     }
     // distances from the matrix cores: position(j) * 1 + 1 * -position(i), exact in fp32
@@ -485,7 +548,7 @@ __device__ __forceinline__ void attention_of_block(const Args& a, const uint32_t
 #pragma unroll
         for (int v = 0; v < 16; ++v) o[x][v] *= alpha;
       m_run = m_new;
-      base = Ty::kShift - (m_run == -INFINITY ? 0.f : m_run * to_log2);
+      base = kShift - (m_run == -INFINITY ? 0.f : m_run * to_log2);
     }
 #pragma unroll
     for (int u = 0; u < kSub; ++u)
@@ -539,6 +602,49 @@ __device__ __forceinline__ void attention_of_block(const Args& a, const uint32_t
 #pragma unroll
         for (int x = 0; x < kO; ++x)
           o[x] = Ty::mfma(__builtin_bit_cast(TVec, careful ? read_v(mm, x) : vf[careful ? 0 : mm][careful ? 0 : x]), p[mm], o[x]);
+    } else if constexpr (kSplit) {
+      Split::Vec ph[2], pl[2];
+#pragma unroll
+      for (int g = 0; g < 2; ++g)
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) Split::split(s[0][8 * g + j], s[0][8 * g + j + 1], 1.f, j, ph[g], pl[g]);
+#pragma unroll
+      for (int x = 0; x < kO; ++x) {
+        float f[16];  // element e: key 8 (e / 4) + 4 lh + e % 4, channel 32 x + lq
+        float most = 0.f;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          f[e] = *reinterpret_cast<const float*>(
+              all + (v_at ^ (x << 7) ^ ((e & 3) << 6) ^ (((e >> 2) & 1) << 5)) + (8 * (e >> 2) + (e & 3)) * kPitch);
+          most = __builtin_elementwise_maximum(most, fabsf(f[e]));
+        }
+        const int bits = wave_max_int(__float_as_int(most));
+        if (!careful && bits < Split::kInfinity) {
+          const int here = Split::exponent(bits);
+          if (here > v_exp[x]) {
+#pragma unroll
+            for (int v = 0; v < 16; ++v) o[x][v] = __builtin_ldexpf(o[x][v], v_exp[x] - here);
+            v_exp[x] = here;
+          }
+          const float by = Split::power(Split::kTop - v_exp[x]);
+#pragma unroll
+          for (int g = 0; g < 2; ++g) {
+            Split::Vec vh, vl;
+            Split::split(float4{f[8 * g], f[8 * g + 1], f[8 * g + 2], f[8 * g + 3]},
+                         float4{f[8 * g + 4], f[8 * g + 5], f[8 * g + 6], f[8 * g + 7]}, by, vh, vl);
+            o[x] = Split::mfma(vl, ph[g], o[x]);
+            o[x] = Split::mfma(vh, pl[g], o[x]);
+            o[x] = Split::mfma(vh, ph[g], o[x]);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+        } else {
+          const float by = Split::power(Split::kTop - v_exp[x]);
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            o[x] = __builtin_amdgcn_mfma_f32_32x32x2f32(f[e] * by, s[0][e], o[x], 0, 0, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
     } else {
       // step e takes keys 8 (e / 4) + 4 lh + e % 4: register e of s
 #pragma unroll
@@ -597,7 +703,11 @@ __device__ __forceinline__ void attention_of_block(const Args& a, const uint32_t
     for (int x = 0; x < kO; ++x)
 #pragma unroll
       for (int v = 0; v < 16; ++v) o[x][v] = 0.f;
-    m_run = -INFINITY, l_run = 0.f, base = Ty::kShift, mixed_seen = false;
+    m_run = -INFINITY, l_run = 0.f, base = kShift, mixed_seen = false;
+    if constexpr (kSplit) {
+#pragma unroll
+      for (int x = 0; x < kO; ++x) v_exp[x] = decltype(careful_c)::value ? Split::kTop : Split::kLeast;
+    }
     chunk = lo / 64, tiles_seen = 0;
     sort_tiles(decltype(careful_c)::value ? summary_of(lo / 64 * 64 + lane) : first_summary);
     Next now = next_tile();
@@ -649,6 +759,12 @@ __device__ __forceinline__ void attention_of_block(const Args& a, const uint32_t
   if (kTeams > 1 ? __any(bad) : __syncthreads_or(bad)) walk(std::integral_constant<bool, true>{});
 
   l_run = halves_sum(l_run);
+  if constexpr (kSplit) {
+#pragma unroll
+    for (int x = 0; x < kO; ++x)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) o[x][v] = __builtin_ldexpf(o[x][v], v_exp[x] - Split::kTop);
+  }
   if constexpr (kTeams > 1) {
     // each team's (maximum, sum) and output in its own place, then all of them in order
     constexpr int kPlace = kPart;  // floats of a team's place: four tiles' bytes
