@@ -122,9 +122,11 @@ _EVERY = Tokens()
 
 def _heads(x, per):
     """x, copied where its rows do not start on 16 bytes (per elements), and its strides."""
-    strides = rt.token_strides(x)
-    if x.stride(3) == 1 and not x.data_ptr() % 16 and not (strides[0] | strides[1] | strides[2]) % per:
-        return x, strides
+    b, t, h, _ = x.shape
+    sb, st, sh, last = x.stride()
+    sb, st, sh = sb if b > 1 else 0, st if t > 1 else 0, sh if h > 1 else 0
+    if last == 1 and not x.data_ptr() % 16 and not (sb | st | sh) % per:
+        return x, (sb, st, sh)
     x = x.clone(memory_format=torch.contiguous_format)  # also where it is contiguous and starts off 16 bytes
     return x, rt.token_strides(x)
 
@@ -144,14 +146,18 @@ def _prefix_heads(x, name, hk, d, dtype, index, per):
 
 
 def _attend(q, k, v, scale, keys, queries, cap, slopes, out, window=None, prefix=None):
-    for name, x in (('q', q), ('k', k), ('v', v)):
-        rt.require_device_tensor(x, name)
-        if x.dim() != 4:
-            raise ValueError(f'{name} must be a (B, T, heads, D) tensor')
+    rt.require_device_tensor(q, 'q')
+    rt.require_device_tensor(k, 'k')
+    rt.require_device_tensor(v, 'v')
+    if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
+        raise ValueError('q, k and v must be (B, T, heads, D) tensors')
     if rt.elsewhere(q):
         with torch.cuda.device(q.device):
             return _attend(q, k, v, scale, keys, queries, cap, slopes, out, window, prefix)
-    rt.require_no_gradient(q, k, v, slopes, out, *(prefix or ()))
+    if slopes is out is prefix is None:
+        rt.require_no_gradient(q, k, v)
+    else:
+        rt.require_no_gradient(q, k, v, slopes, out, *(prefix or ()))
     dtype, index = q.dtype, q.get_device()
     if dtype not in _STORAGE:
         raise ValueError('q must be float32, float16 or bfloat16')
@@ -217,10 +223,13 @@ def _attend(q, k, v, scale, keys, queries, cap, slopes, out, window=None, prefix
             p_ptr = p_pos.data_ptr()
         if p:
             before = rt.PACK_ATTENTION_PREFIX.pack(pk.data_ptr(), pv.data_ptr(), pk_st, pk_sh, pv_st, pv_sh, p_ptr, p)
-    o = rt.output_like(out, q, 'out')
-    os_ = rt.token_strides(o)
-    if o.data_ptr() % 16 or (os_[0] | os_[1] | os_[2]) % per:
-        raise ValueError('rows of out must start on 16 bytes')
+    if out is None:
+        o, os_ = torch.empty_like(q, memory_format=torch.contiguous_format), (tq * h * d, h * d, d)
+    else:
+        o = rt.output_like(out, q, 'out')
+        os_ = rt.token_strides(o)
+        if o.data_ptr() % 16 or (os_[0] | os_[1] | os_[2]) % per:
+            raise ValueError('rows of out must start on 16 bytes')
     if not (b and tq and h):
         return o
     if not tk and before is None:

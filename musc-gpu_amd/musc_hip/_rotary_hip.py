@@ -14,6 +14,7 @@ import torch
 
 from . import _runtime as rt
 
+_F32 = torch.float32
 _STORAGE = {torch.float32: rt.DTYPE_F32, torch.float16: rt.DTYPE_F16, torch.bfloat16: rt.DTYPE_BF16}
 
 
@@ -50,85 +51,90 @@ class RotaryAxes:
 
 
 def _head_rows(x, name, axes):
+    """(x with a contiguous last dimension, its batch, tokens and heads, their strides as rt.token_strides has them)."""
     rt.require_device_tensor(x, name)
-    if x.dim() != 4 or x.shape[-1] != axes.head_dim or x.dtype not in _STORAGE:
+    if x.dim() != 4 or x.shape[3] != axes.head_dim or x.dtype not in _STORAGE:
         raise ValueError(f'{name} must be a (B, T, heads, {axes.head_dim}) float32, float16 or bfloat16 tensor')
-    return x if x.stride(-1) == 1 else x.contiguous()
+    if x.stride(3) != 1:
+        x = x.contiguous()
+    b, t, h, _ = x.shape
+    sb, st, sh, _ = x.stride()
+    return x, b, t, h, (sb if b > 1 else 0, st if t > 1 else 0, sh if h > 1 else 0)
 
 
 def _head_weight(weight, name, h, d, dtype, index):
-    """(tensor, elements between the weights of two heads, storage) of a head norm's weight."""
+    """(address, elements between the weights of two heads, storage, tensor) of a head norm's weight."""
     rt.require_device_tensor(weight, name)
-    rt.require_no_gradient(weight)
-    per_head, w_dtype = weight.dim() == 2, weight.dtype
-    if (weight.get_device() != index or (w_dtype is not dtype and w_dtype is not torch.float32) or weight.dim() not in (1, 2)
-            or weight.shape[-1] != d or (per_head and weight.shape[0] != h)):
+    w_dtype, dims, n = weight.dtype, weight.dim(), weight.numel()
+    if (weight.get_device() != index or (w_dtype is not dtype and w_dtype is not _F32)
+            or not (n == d if dims == 1 else dims == 2 and n == h * d and weight.shape[1] == d)):
         raise ValueError(f"{name} must be ({d},) or ({h}, {d}) on its input's device, in its dtype or float32")
-    if not weight.is_contiguous() or weight.data_ptr() % 16:
+    at = weight.data_ptr()
+    if at % 16 or not weight.is_contiguous():
         weight = weight.clone(memory_format=torch.contiguous_format)     # read as 16-byte vectors
-    return weight, d if per_head else 0, _STORAGE[w_dtype]
+        at = weight.data_ptr()
+    return at, d if dims == 2 else 0, _STORAGE[w_dtype], weight
 
 
-def _turned(out, x, name):
+def _turned(out, x, name, t, h, d):
     """(tensor to write, its strides as rt.token_strides has them)."""
     if out is None:
-        out = torch.empty_like(x, memory_format=torch.contiguous_format)
-        _, t, h, d = x.shape
-        return out, (t * h * d, h * d, d)
+        return torch.empty_like(x, memory_format=torch.contiguous_format), (t * h * d, h * d, d)
     out = rt.output_like(out, x, name)
     return out, rt.token_strides(out)
 
 
 def _turn(q, k, positions, axes, inverse, out, norm):
-    q2 = _head_rows(q, 'q', axes)
+    q2, b, t, h, q_strides = _head_rows(q, 'q', axes)
     if rt.elsewhere(q):
         with torch.cuda.device(q.device):
             return _turn(q, k, positions, axes, inverse, out, norm)
-    rt.require_no_gradient(q, k, positions, *(out if isinstance(out, (tuple, list)) else (out,)))
-    index, dtype = q.get_device(), q.dtype
-    b, t, h, d = q2.shape
+    if out is None:
+        rt.require_no_gradient(q, k, positions)
+    else:
+        rt.require_no_gradient(q, k, positions, *(out if isinstance(out, (tuple, list)) else (out,)))
+    index, dtype, d = q.get_device(), q.dtype, axes.head_dim
     k2, ko, k_heads, k_args = None, None, 0, (0, 0, 0, 0, 0, 0, 0, 0)
     if k is not None:
-        k2 = _head_rows(k, 'k', axes)
-        kb, kt, hk, _ = k2.shape
+        k2, kb, kt, hk, k_strides = _head_rows(k, 'k', axes)
         if kb != b or kt != t or k2.dtype is not dtype or k2.get_device() != index:
             raise ValueError('k must match q in batch, tokens, dtype and device')
         if out is not None and len(out) != 2:
             raise ValueError('out must be (q_out, k_out)')
     rt.require_device_tensor(positions, 'positions')
-    n, shared = axes.axes, positions.dim() == 2
-    if (positions.dtype not in (torch.float32, torch.int32) or positions.get_device() != index
-            or tuple(positions.shape) != ((t, n) if shared else (b, t, n))):
+    n, p_dtype, p_shape = axes.axes, positions.dtype, positions.shape
+    shared = len(p_shape) == 2
+    if ((p_dtype is not _F32 and p_dtype is not torch.int32) or positions.get_device() != index
+            or p_shape != ((t, n) if shared else (b, t, n))):
         raise ValueError(f"positions must be float32 or int32 of shape (T, {n}) or (B, T, {n}) on q's device")
-    if axes.frequency.get_device() != index:
+    frequency = axes.frequency
+    if frequency.get_device() != index:
         raise ValueError("axes must be on q's device")
     positions = positions.contiguous()
-    qw = kw = None
-    q_sh = k_sh = 0
-    q_type = k_type = rt.DTYPE_F32
+    qw = kw = (None, 0, 0, None)
     if norm is not None:
-        if norm[0] is not None:
-            qw, q_sh, q_type = _head_weight(norm[0], 'q_weight', h, d, dtype, index)
-        if norm[1] is not None and k is not None:
-            kw, k_sh, k_type = _head_weight(norm[1], 'k_weight', hk, d, dtype, index)
+        q_weight, k_weight, eps = norm
+        if q_weight is not None:
+            qw = _head_weight(q_weight, 'q_weight', h, d, dtype, index)
+        if k_weight is not None and k is not None:
+            kw = _head_weight(k_weight, 'k_weight', hk, d, dtype, index)
+        rt.require_no_gradient(qw[3], kw[3])
     if k2 is not None:
-        ko, ko_strides = _turned(out[1] if out is not None else None, k2, 'k_out')
+        ko, ko_strides = _turned(out[1] if out is not None else None, k2, 'k_out', t, hk, d)
         if hk:
             k_heads = hk
-            k_args = (k2.data_ptr(), *rt.token_strides(k2), ko.data_ptr(), *ko_strides)
+            k_args = (k2.data_ptr(), *k_strides, ko.data_ptr(), *ko_strides)
         out = out[0] if out is not None else None
-    qo, qo_strides = _turned(out, q2, 'q_out')
+    qo, qo_strides = _turned(out, q2, 'q_out', t, h, d)
     if b and t and h:
         call = rt.PACK_ROTARY.pack(
-            q2.data_ptr(), *rt.token_strides(q2), qo.data_ptr(), *qo_strides, *k_args, positions.data_ptr(), 0 if shared else t * n,
-            axes.frequency.data_ptr(), axes.axis.data_ptr(), h, k_heads, _STORAGE[dtype], b, t, d, positions.dtype is torch.int32, n,
+            q2.data_ptr(), *q_strides, qo.data_ptr(), *qo_strides, *k_args, positions.data_ptr(), 0 if shared else t * n,
+            frequency.data_ptr(), axes.axis.data_ptr(), h, k_heads, _STORAGE[dtype], b, t, d, p_dtype is torch.int32, n,
             axes.pairs, axes.adjacent, inverse)
         if norm is None:
             rt.check(rt.library().musc_rotary(call, rt.current_stream(index)), 'musc_rotary')
         else:
-            rt.check(rt.library().musc_norm_rotary(call, None if qw is None else qw.data_ptr(), q_sh, q_type,
-                                                   None if kw is None else kw.data_ptr(), k_sh, k_type, norm[2],
-                                                   rt.current_stream(index)), 'musc_norm_rotary')
+            rt.check(rt.library().musc_norm_rotary(call, *qw[:3], *kw[:3], eps, rt.current_stream(index)), 'musc_norm_rotary')
     elif k_heads:
         _turn(k2, None, positions, axes, inverse, ko, None if norm is None else (norm[1], None, norm[2]))
     return qo if k is None else (qo, ko)

@@ -21,6 +21,8 @@ import struct
 import threading
 
 import torch
+from torch import Tensor, is_grad_enabled
+from torch.autograd import forward_ad
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), 'libmusc_hip.so')
 
@@ -249,7 +251,7 @@ def elsewhere(x: torch.Tensor) -> bool:
 
 
 def require_device_tensor(t: torch.Tensor, name: str) -> None:
-    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+    if not isinstance(t, Tensor) or not t.is_cuda:
         raise ValueError(f'{name} must be a GPU tensor')
     if torch.version.hip is None:
         raise RuntimeError('musc_hip requires a ROCm build of PyTorch')
@@ -258,11 +260,11 @@ def require_device_tensor(t: torch.Tensor, name: str) -> None:
 def require_no_gradient(*tensors) -> None:
     """Operators without a backward pass refuse inputs that ask for one, and those that carry a
     forward-mode tangent (which no_grad does not turn off)."""
-    if torch.autograd.forward_ad._current_level >= 0:
+    if forward_ad._current_level >= 0:
         for t in tensors:
-            if t is not None and torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
                 raise ValueError('this operator has no derivative: call it on the primal of a dual tensor')
-    if not torch.is_grad_enabled():
+    if not is_grad_enabled():
         return
     for t in tensors:
         if t is not None and t.requires_grad:
