@@ -908,55 +908,91 @@ __global__ __launch_bounds__(256) void join_kernel(const Args a) {
   *reinterpret_cast<Two*>(orow + 2 * lane) = out;
 }
 
-// Joins what the rows of prefixed attention have in a.splits parts over the prefix and a.more_splits over
-// their own keys (or in parts over both), in their order: the kernel above over both.
-template <int kDtype>
-__global__ __launch_bounds__(256) void join_prefixed_kernel(const Args a) {
+// Joins the parts of windowed and prefixed attention's rows, a.splits and then a.more_splits of them, in
+// their order: kShare waves a row, each every kShare-th part with two channels per lane, then those in
+// order.  The first eight parts of a wave are asked for before their factors are formed.  Four waves for
+// few rows, else one (4160 rows of 18 parts, fp32: 9 us with four, 6 with one).
+template <int kDtype, bool kByKeyHead, int kShare>
+__global__ __launch_bounds__(256) void join_rows_kernel(const Args a, const long long all_rows) {
   typedef typename Type<kDtype>::T T;
-  __shared__ float weight[kMaxSplits], tops[4], sums[4];
-  __shared__ float2 parts[4][kWave];
+  __shared__ float2 shared[kShare > 1 ? 4 : 1][kWave];
   const musc_masked_attention& c = a.c;
-  const long long r = blockIdx.x;
-  const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
+  const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), part = wave % kShare;
+  const long long r = (long long)blockIdx.x * (4 / kShare) + wave / kShare;
+  if (r >= all_rows) return;  // whole workgroups with kShare > 1
   const int splits = a.splits, all = splits + a.more_splits;
-  float2 mine = make_float2(-INFINITY, 0.f);
-  if (tid < splits) mine = reinterpret_cast<const float2*>(a.part_ml)[r * splits + tid];
-  else if (tid < all) mine = reinterpret_cast<const float2*>(a.more_ml)[r * a.more_splits + tid - splits];
-  const float top_here = wave_max(mine.x);
-  if (lane == 0) tops[wave] = top_here;
-  __syncthreads();
-  const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-  const float w = mine.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(mine.x - top);
-  weight[tid] = w;
-  const float sum_here = wave_sum(mine.y == 0.f ? 0.f : w * mine.y);
-  if (lane == 0) sums[wave] = sum_here;
-  __syncthreads();
-  const float sum = sums[0] + sums[1] + sums[2] + sums[3];
   const bool ok = 2 * lane < c.d;
   const int at = ok ? 2 * lane : 0;
-  float2 y = make_float2(0.f, 0.f);
-#pragma unroll 4
-  for (int s = wave; s < all; s += 4) {
-    const float* from = s < splits ? a.part_o + (r * splits + s) * c.d : a.more_o + (r * a.more_splits + s - splits) * c.d;
-    const float2 p = *reinterpret_cast<const float2*>(from + at);
-    const float f = weight[s];
-    if (f != 0.f) y.x = fmaf(f, p.x, y.x), y.y = fmaf(f, p.y, y.y);
-  }
-  parts[wave][lane] = y;
-  __syncthreads();
-  if (wave != 0 || !ok) return;
+  const float *first_o = a.part_o + r * splits * c.d + at, *more_o = a.more_o + (r * a.more_splits - splits) * c.d + at;
+  auto load = [&](int s) __attribute__((always_inline)) {
+    return *reinterpret_cast<const float2*>((s < splits ? first_o : more_o) + (long long)s * c.d);
+  };
+  constexpr int kBatch = 8;
+  float2 p[kBatch];
 #pragma unroll
-  for (int i = 1; i < 4; ++i) y.x += parts[i][lane].x, y.y += parts[i][lane].y;
+  for (int i = 0; i < kBatch; ++i) p[i] = load(min(part + i * kShare, all - 1));
+  // the largest of the maxima, each part's factor and the sum; a part without keys has sum 0 (one whose
+  // scores are NaN has its sum NaN)
+  constexpr int kPer = kMaxSplits / kWave;
+  float w[kPer], l[kPer], top = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int s = i * kWave + lane;
+    float2 ml = make_float2(-INFINITY, 0.f);
+    if (s < splits) ml = reinterpret_cast<const float2*>(a.part_ml)[r * splits + s];
+    else if (s < all) ml = reinterpret_cast<const float2*>(a.more_ml)[r * a.more_splits + s - splits];
+    w[i] = ml.x, l[i] = ml.y;
+    top = fmaxf(top, ml.x);
+  }
+  top = wave_max(top);
+  float sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    w[i] = l[i] == 0.f ? 0.f : __builtin_amdgcn_exp2f(w[i] - top);
+    sum += l[i] == 0.f ? 0.f : w[i] * l[i];
+  }
+  sum = wave_sum(sum);
+  float2 y = make_float2(0.f, 0.f);
+  for (int from = part; from < all; from += kBatch * kShare) {
+    if (from != part) {
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) p[i] = load(min(from + i * kShare, all - 1));
+    }
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const int s = from + i * kShare;
+      const float of = s < kWave ? w[0] : s < 2 * kWave ? w[1] : s < 3 * kWave ? w[2] : w[3];
+      const float f = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(of), s % kWave));
+      if (s < all && f != 0.f) y.x = fmaf(f, p[i].x, y.x), y.y = fmaf(f, p[i].y, y.y);
+    }
+  }
+  if constexpr (kShare > 1) {
+    shared[wave][lane] = y;
+    __syncthreads();
+    if (wave != 0) return;
+#pragma unroll
+    for (int i = 1; i < kShare; ++i) y.x += shared[i][lane].x, y.y += shared[i][lane].y;
+  }
+  if (!ok) return;
   const float inv = 1.f / sum;
   const int rows = c.q_len * a.group;  // of a batch entry and key head
   const long long bh = r / rows;
   const int row = (int)(r % rows), token = row / a.group;
-  const int b = (int)(bh % c.batch), head = (int)(bh / c.batch) * a.group + row % a.group;
+  const int b = (int)(kByKeyHead ? bh % c.batch : bh / c.kv_heads);
+  const int head = (int)(kByKeyHead ? bh / c.batch : bh % c.kv_heads) * a.group + row % a.group;
   typedef T Two __attribute__((ext_vector_type(2)));
   Two out;
   out[0] = sum == 0.f ? (T)0.f : (T)(y.x * inv);
   out[1] = sum == 0.f ? (T)0.f : (T)(y.y * inv);
   *reinterpret_cast<Two*>(static_cast<T*>(c.out) + b * c.o_sb + (long long)token * c.o_st + head * c.o_sh + 2 * lane) = out;
+}
+template <int kDtype, bool kByKeyHead>
+void launch_join(const Args& a, hipStream_t stream) {
+  const long long rows = (long long)a.c.batch * a.c.kv_heads * a.c.q_len * a.group;
+  if (rows <= 1024)
+    hipLaunchKernelGGL((join_rows_kernel<kDtype, kByKeyHead, 4>), dim3((unsigned)rows), dim3(256), 0, stream, a, rows);
+  else
+    hipLaunchKernelGGL((join_rows_kernel<kDtype, kByKeyHead, 1>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream, a, rows);
 }
 
 // Joins the parts of the row tiles that were done in parts, in their order: a workgroup per row
@@ -1093,10 +1129,7 @@ void launch_extra(const Args& a, const Args* more, int waves, hipStream_t stream
 template <int kDtype>
 void launch_windowed(const Args& a, int waves, hipStream_t stream) {
   launch_extra<kDtype, kWindowed>(a, nullptr, waves, stream);
-  if (a.splits > 1) {
-    const long long rows = (long long)a.c.batch * a.c.kv_heads * a.rows;
-    hipLaunchKernelGGL((join_kernel<kDtype>), dim3((unsigned)rows), dim3(256), 0, stream, a);
-  }
+  if (a.splits > 1) launch_join<kDtype, false>(a, stream);
 }
 // more: the entries' own keys, beside all rows over the prefix.
 template <int kDtype>
@@ -1105,8 +1138,7 @@ void launch_prefixed(const Args& a, const Args* more, int waves, hipStream_t str
   if (a.splits > 1 || a.stacked) {
     Args both = a;
     if (more) both.more_splits = more->splits, both.more_ml = more->part_ml, both.more_o = more->part_o;
-    const long long rows = (long long)a.c.batch * a.c.kv_heads * a.c.q_len * a.group;
-    hipLaunchKernelGGL((join_prefixed_kernel<kDtype>), dim3((unsigned)rows), dim3(256), 0, stream, both);
+    launch_join<kDtype, true>(both, stream);
   }
 }
 
