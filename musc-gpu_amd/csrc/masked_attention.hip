@@ -195,6 +195,12 @@ int plan(const musc_masked_attention& c, Args& a, int& waves) {
   // workgroups of one wave and a join, 12.9 us so, host time included.
   const int teams = teams_of((c.d <= 64 ? 64 : 128) * (c.dtype == MUSC_DTYPE_F32 ? 4 : 2));
   if (waves == 1 && a.key_tiles <= kTeamTiles * teams) a.teams = teams;
+  // Of a window, if each order has one key or so, a row tile sees about so many tiles: few of them need no
+  // splits and join, which the host's time for a launch is lost on (3 us).  Where orders have many keys and
+  // more is seen, a call is slower than in splits, and so this is for up to four times as many tiles only.
+  const bool narrow = a.window && ((long long)a.window + a.sinks + 32 * waves / a.group) / tile + 3 <= (waves == 1 ? kTeamTiles * teams : 8) &&
+                      a.key_tiles <= 4 * (waves == 1 ? kTeamTiles * teams : 8);
+  if (waves == 1 && narrow) a.teams = teams;
   if (a.teams > 1) {
   } else if (waves > 1 && c.schedule) {
     // No splits: pieces and parts even out documents of different lengths, and one document alone, or equal
@@ -213,7 +219,7 @@ int plan(const musc_masked_attention& c, Args& a, int& waves) {
     // pieces cost a little, and short tiles fill up behind long ones.
     a.in_pieces = !a.in_parts && !c.q_order && whole < 4LL * a.slots;
     if (a.in_pieces) a.jobs = (int)schedule_pieces(a.row_tiles);
-  } else if (whole < (waves == 1 ? 1024 : 256)) {
+  } else if (whole < (waves == 1 ? 1024 : 256) && !narrow) {
     // few rows: their keys in splits of at least one tile (4 where four waves share the tiles)
     // (a window's first look over all tiles pays for fewer workgroups: 8 x 4096 of 32768 keys, 32 heads on 8 of
     // 128, bf16, 2048 waves 45 us with the join, 1024 36, 512 37)

@@ -120,15 +120,21 @@ def _batch_stride(name: str, x: torch.Tensor, leading, batch: int, tokens: int, 
 _EVERY = Tokens()
 
 
-def _heads(x, per):
-    """x, copied where its rows do not start on 16 bytes (per elements), and its strides."""
-    b, t, h, _ = x.shape
+def _heads(x, b, t, h, per):
+    """x, copied where its rows do not start on 16 bytes (per elements), its address and strides (a dimension of
+    one element has none)."""
+    at = x.data_ptr()
     sb, st, sh, last = x.stride()
-    sb, st, sh = sb if b > 1 else 0, st if t > 1 else 0, sh if h > 1 else 0
-    if last == 1 and not x.data_ptr() % 16 and not (sb | st | sh) % per:
-        return x, (sb, st, sh)
+    if b < 2:
+        sb = 0
+    if t < 2:
+        st = 0
+    if h < 2:
+        sh = 0
+    if last == 1 and not at % 16 and not (sb | st | sh) % per:
+        return x, (at, sb, st, sh)
     x = x.clone(memory_format=torch.contiguous_format)  # also where it is contiguous and starts off 16 bytes
-    return x, rt.token_strides(x)
+    return x, (x.data_ptr(), *rt.token_strides(x))
 
 
 def _prefix_heads(x, name, hk, d, dtype, index, per):
@@ -159,22 +165,25 @@ def _attend(q, k, v, scale, keys, queries, cap, slopes, out, window=None, prefix
     else:
         rt.require_no_gradient(q, k, v, slopes, out, *(prefix or ()))
     dtype, index = q.dtype, q.get_device()
-    if dtype not in _STORAGE:
+    storage = _STORAGE.get(dtype)
+    if storage is None:
         raise ValueError('q must be float32, float16 or bfloat16')
     b, tq, h, d = q.shape
-    kb, tk, hk, kd = k.shape
-    if kb != b or kd != d or k.dtype != dtype or v.dtype != dtype or k.get_device() != index or v.get_device() != index:
+    k_shape = k.shape
+    kb, tk, hk, kd = k_shape
+    if (kb != b or kd != d or k.dtype is not dtype or v.dtype is not dtype or k.get_device() != index
+            or v.get_device() != index):
         raise ValueError('k and v must match q in batch, head width, dtype and device')
-    if v.shape != k.shape:
+    if v.shape != k_shape:
         raise ValueError('v must match k in shape')
     if hk < 1 or h % hk:
         raise ValueError('heads of q must be a multiple of the heads of k')
-    per = 16 // q.element_size()
+    per = 4 if storage == rt.DTYPE_F32 else 8
     if d < per or d > 128 or d % per:
         raise ValueError(f'head width {d}: multiples of {per} up to 128 are supported for {dtype}')
-    q, qs = _heads(q, per)
-    k, ks = _heads(k, per)
-    v, vs = _heads(v, per)
+    q, q_args = _heads(q, b, tq, h, per)
+    k, k_args = _heads(k, b, tk, hk, per)
+    v, v_args = _heads(v, b, tk, hk, per)
     keys = _EVERY if keys is None else keys
     queries = keys if queries is None else queries
     kdocs, qdocs, kord, qord = keys.documents, queries.documents, keys.order, queries.order
@@ -239,7 +248,7 @@ def _attend(q, k, v, scale, keys, queries, cap, slopes, out, window=None, prefix
         first, block = keys._schedule_of[h // hk]
         schedule, schedule_sb = keys._schedule.data_ptr() + first, block if k_sb else 0
     call = rt.PACK_MASKED_ATTENTION.pack(
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), *qs, *ks, *vs, *os_, _STORAGE[dtype], b, tq, tk, h, hk, d,
+        q_args[0], k_args[0], v_args[0], o.data_ptr(), *q_args[1:], *k_args[1:], *v_args[1:], *os_, storage, b, tq, tk, h, hk, d,
         scale, cap, qd_ptr, qo_ptr, kd_ptr, ko_ptr, q_sb, k_sb, sum_ptr, sum_sb, qp_ptr, kp_ptr, qp_sb, kp_sb, slope_ptr,
         axes, schedule, schedule_sb)
     # the entry point of the call, and what it takes beside it

@@ -14,7 +14,8 @@ import torch
 
 from . import _runtime as rt
 
-_F32 = torch.float32
+_F32, _CONTIGUOUS = torch.float32, torch.contiguous_format
+_NO_WEIGHT = (None, 0, rt.DTYPE_F32, None)
 _STORAGE = {torch.float32: rt.DTYPE_F32, torch.float16: rt.DTYPE_F16, torch.bfloat16: rt.DTYPE_BF16}
 
 
@@ -50,16 +51,9 @@ class RotaryAxes:
         self.frequency, self.axis = both[:pairs], both[pairs:].view(torch.int32)[:pairs]
 
 
-def _head_rows(x, name, axes):
-    """(x with a contiguous last dimension, its batch, tokens and heads, their strides as rt.token_strides has them)."""
+def _refuse_heads(x, name, axes):
     rt.require_device_tensor(x, name)
-    if x.dim() != 4 or x.shape[3] != axes.head_dim or x.dtype not in _STORAGE:
-        raise ValueError(f'{name} must be a (B, T, heads, {axes.head_dim}) float32, float16 or bfloat16 tensor')
-    if x.stride(3) != 1:
-        x = x.contiguous()
-    b, t, h, _ = x.shape
-    sb, st, sh, _ = x.stride()
-    return x, b, t, h, (sb if b > 1 else 0, st if t > 1 else 0, sh if h > 1 else 0)
+    raise ValueError(f'{name} must be a (B, T, heads, {axes.head_dim}) float32, float16 or bfloat16 tensor')
 
 
 def _head_weight(weight, name, h, d, dtype, index):
@@ -71,37 +65,54 @@ def _head_weight(weight, name, h, d, dtype, index):
         raise ValueError(f"{name} must be ({d},) or ({h}, {d}) on its input's device, in its dtype or float32")
     at = weight.data_ptr()
     if at % 16 or not weight.is_contiguous():
-        weight = weight.clone(memory_format=torch.contiguous_format)     # read as 16-byte vectors
+        weight = weight.clone(memory_format=_CONTIGUOUS)     # read as 16-byte vectors
         at = weight.data_ptr()
     return at, d if dims == 2 else 0, _STORAGE[w_dtype], weight
 
 
-def _turned(out, x, name, t, h, d):
-    """(tensor to write, its strides as rt.token_strides has them)."""
-    if out is None:
-        return torch.empty_like(x, memory_format=torch.contiguous_format), (t * h * d, h * d, d)
-    out = rt.output_like(out, x, name)
-    return out, rt.token_strides(out)
-
-
 def _turn(q, k, positions, axes, inverse, out, norm):
-    q2, b, t, h, q_strides = _head_rows(q, 'q', axes)
+    d = axes.head_dim
+    rt.require_device_tensor(q, 'q')
+    if q.dim() != 4:
+        _refuse_heads(q, 'q', axes)
+    b, t, h, width = q.shape
+    dtype, index = q.dtype, q.get_device()
+    storage = _STORAGE.get(dtype)
+    if width != d or storage is None:
+        _refuse_heads(q, 'q', axes)
     if rt.elsewhere(q):
         with torch.cuda.device(q.device):
             return _turn(q, k, positions, axes, inverse, out, norm)
     if out is None:
+        q_out = k_out = None
         rt.require_no_gradient(q, k, positions)
     else:
-        rt.require_no_gradient(q, k, positions, *(out if isinstance(out, (tuple, list)) else (out,)))
-    index, dtype, d = q.get_device(), q.dtype, axes.head_dim
-    k2, ko, k_heads, k_args = None, None, 0, (0, 0, 0, 0, 0, 0, 0, 0)
-    if k is not None:
-        k2, kb, kt, hk, k_strides = _head_rows(k, 'k', axes)
-        if kb != b or kt != t or k2.dtype is not dtype or k2.get_device() != index:
-            raise ValueError('k must match q in batch, tokens, dtype and device')
-        if out is not None and len(out) != 2:
+        q_out, k_out = (out, None) if k is None else out if len(out) == 2 else (None, None)
+        if k is not None and len(out) != 2:
             raise ValueError('out must be (q_out, k_out)')
-    rt.require_device_tensor(positions, 'positions')
+        rt.require_no_gradient(q, k, positions, q_out, k_out)
+    sb, st, sh, last = q.stride()
+    if last != 1:
+        q = q.contiguous()
+        sb, st, sh, _ = q.stride()
+    # a dimension of one element has no stride
+    q_args = (q.data_ptr(), sb if b > 1 else 0, st if t > 1 else 0, sh if h > 1 else 0)
+    k_heads, k_args = 0, (0, 0, 0, 0, 0, 0, 0, 0)
+    if k is not None:
+        if not isinstance(k, torch.Tensor) or not k.is_cuda or k.dim() != 4:
+            _refuse_heads(k, 'k', axes)
+        kb, kt, k_heads, width = k.shape
+        if width != d:
+            _refuse_heads(k, 'k', axes)
+        if kb != b or kt != t or k.dtype is not dtype or k.get_device() != index:
+            raise ValueError('k must match q in batch, tokens, dtype and device')
+        sb, st, sh, last = k.stride()
+        if last != 1:
+            k = k.contiguous()
+            sb, st, sh, _ = k.stride()
+        k_args = (k.data_ptr(), sb if b > 1 else 0, st if t > 1 else 0, sh if k_heads > 1 else 0)
+    if not isinstance(positions, torch.Tensor) or not positions.is_cuda:
+        rt.require_device_tensor(positions, 'positions')
     n, p_dtype, p_shape = axes.axes, positions.dtype, positions.shape
     shared = len(p_shape) == 2
     if ((p_dtype is not _F32 and p_dtype is not torch.int32) or positions.get_device() != index
@@ -111,32 +122,40 @@ def _turn(q, k, positions, axes, inverse, out, norm):
     if frequency.get_device() != index:
         raise ValueError("axes must be on q's device")
     positions = positions.contiguous()
-    qw = kw = (None, 0, 0, None)
     if norm is not None:
         q_weight, k_weight, eps = norm
+        qw = kw = _NO_WEIGHT
         if q_weight is not None:
             qw = _head_weight(q_weight, 'q_weight', h, d, dtype, index)
         if k_weight is not None and k is not None:
-            kw = _head_weight(k_weight, 'k_weight', hk, d, dtype, index)
+            kw = _head_weight(k_weight, 'k_weight', k_heads, d, dtype, index)
         rt.require_no_gradient(qw[3], kw[3])
-    if k2 is not None:
-        ko, ko_strides = _turned(out[1] if out is not None else None, k2, 'k_out', t, hk, d)
-        if hk:
-            k_heads = hk
-            k_args = (k2.data_ptr(), *k_strides, ko.data_ptr(), *ko_strides)
-        out = out[0] if out is not None else None
-    qo, qo_strides = _turned(out, q2, 'q_out', t, h, d)
+    if k is not None:
+        if k_out is None:
+            ko = torch.empty_like(k, memory_format=_CONTIGUOUS)
+            k_args += (ko.data_ptr(), t * k_heads * d, k_heads * d, d)
+        else:
+            ko = rt.output_like(k_out, k, 'k_out')
+            k_args += (ko.data_ptr(), *rt.token_strides(ko))
+    if q_out is None:
+        qo = torch.empty_like(q, memory_format=_CONTIGUOUS)
+        q_args += (qo.data_ptr(), t * h * d, h * d, d)
+    else:
+        qo = rt.output_like(q_out, q, 'q_out')
+        q_args += (qo.data_ptr(), *rt.token_strides(qo))
     if b and t and h:
+        if not k_heads:
+            k_args = (0, 0, 0, 0, 0, 0, 0, 0)
         call = rt.PACK_ROTARY.pack(
-            q2.data_ptr(), *q_strides, qo.data_ptr(), *qo_strides, *k_args, positions.data_ptr(), 0 if shared else t * n,
-            frequency.data_ptr(), axes.axis.data_ptr(), h, k_heads, _STORAGE[dtype], b, t, d, p_dtype is torch.int32, n,
-            axes.pairs, axes.adjacent, inverse)
+            *q_args, *k_args, positions.data_ptr(), 0 if shared else t * n, frequency.data_ptr(), axes.axis.data_ptr(), h, k_heads,
+            storage, b, t, d, p_dtype is not _F32, n, axes.pairs, axes.adjacent, inverse)
         if norm is None:
             rt.check(rt.library().musc_rotary(call, rt.current_stream(index)), 'musc_rotary')
         else:
-            rt.check(rt.library().musc_norm_rotary(call, *qw[:3], *kw[:3], eps, rt.current_stream(index)), 'musc_norm_rotary')
+            rt.check(rt.library().musc_norm_rotary(call, qw[0], qw[1], qw[2], kw[0], kw[1], kw[2], eps, rt.current_stream(index)),
+                     'musc_norm_rotary')
     elif k_heads:
-        _turn(k2, None, positions, axes, inverse, ko, None if norm is None else (norm[1], None, norm[2]))
+        _turn(k, None, positions, axes, inverse, ko, None if norm is None else (norm[1], None, norm[2]))
     return qo if k is None else (qo, ko)
 
 

@@ -104,7 +104,11 @@ def test_prefix_workspace(lib):  # noqa: F811
     prefix = ctypes.byref(prefix_of())
     full = ctypes.byref(attention_call(batch=64, q_len=1024))
     assert lib.musc_prefix_attention_workspace_bytes(full, prefix, ctypes.byref(need)) == OK and need.value == 0
-    for change in (dict(q_len=1), dict(q_len=1, k_len=0, k=0, v=0), dict(q_len=40, batch=9)):
+    # few rows over few keys are joined by their workgroup; over many, and stacked ones, by a kernel
+    assert lib.musc_prefix_attention_workspace_bytes(ctypes.byref(attention_call(q_len=1)), prefix, ctypes.byref(need)) == OK
+    assert need.value == 0
+    prefix = ctypes.byref(prefix_of(len=1 << 15))
+    for change in (dict(q_len=1), dict(q_len=1, k_len=0, k=0, v=0), dict(q_len=40, batch=9), dict(q_len=1, batch=1)):
         call = ctypes.byref(attention_call(**change))
         assert lib.musc_prefix_attention_workspace_bytes(call, prefix, ctypes.byref(need)) == OK and need.value > 0
         for workspace, size in ((None, need.value), (P, need.value - 1), (ctypes.c_void_p(4100), need.value)):
