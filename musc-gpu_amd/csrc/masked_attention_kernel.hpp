@@ -224,9 +224,10 @@ __device__ __forceinline__ void attention_of_block(const Args& a, const uint32_t
   // see (bit 63: all from the 63rd on), found by all waves before any of them has its accumulators; and of
   // the splits only as many as there are such tiles (four of them for four waves) have work.
   const auto window_from = [&](int order) { return __builtin_elementwise_sub_sat(order, a.window - 1); };
-  auto may_see_tile = [&](const int4 k, const Range& r) __attribute__((always_inline)) {
-    return k.y >= 0 && k.x <= r.dmax && k.y >= r.dmin && k.z <= r.omax &&
-           (!windowed || k.w >= window_from(r.omin) || (k.w >= 0 && k.z < a.sinks));
+  auto may_see_tile = [&](const int4 k, const Range& r) __attribute__((always_inline)) {  // without branches
+    bool may = (k.y >= 0) & (k.x <= r.dmax) & (k.y >= r.dmin) & (k.z <= r.omax);
+    if (windowed) may &= (k.w >= window_from(r.omin)) | ((k.w >= 0) & (k.z < a.sinks));
+    return may;
   };
   unsigned long long chunks = ~0ull;
   constexpr int kLeast = kDtype == MUSC_DTYPE_F32 ? 2 : 4;  // tiles of a split
@@ -382,7 +383,7 @@ __device__ __forceinline__ void attention_of_block(const Args& a, const uint32_t
 
   // one staged tile; whole: every row sees every key.  careful: in a mixed tile, products
   // of keys that a row does not see are left out one by one (their V may be infinite or NaN)
-  auto attend = [&](int buf, int tile, bool whole, auto careful_c, auto read) __attribute__((always_inline)) {
+  auto attend = [&](int buf, int tile, bool whole, bool one, auto careful_c, auto read) __attribute__((always_inline)) {
     constexpr bool careful = decltype(careful_c)::value;
     // Byte places of this lane's operands: row lq (K) or the row and chunk of its V operand, in
     // chunk order from the permutation's exclusive or, which all further chunks keep.  Formed
@@ -514,6 +515,30 @@ __device__ __forceinline__ void attention_of_block(const Args& a, const uint32_t
       const uint32_t qsinks = windowed && order >= 0 && a.sinks > 0 ? (uint32_t)min(order, a.sinks - 1) + 1 : 0;
       const bool shared = prefixed && tile < p_tiles;
       const int rem = shared ? a.p.len - tile * kTile : k_len - (tile - p_tiles) * kTile;
+      if constexpr (windowed || prefixed) {
+        // orders, documents where the tile has more than one, and the end of the keys, one after the other
+        auto only = [&](auto seen_if) __attribute__((always_inline)) {
+#pragma unroll
+          for (int u = 0; u < kSub; ++u)
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const bool see = seen_if(32 * u + 8 * g + 4 * lh, i);
+                s[u][4 * g + i] = see ? s[u][4 * g + i] : -INFINITY;
+                if (careful && !see) seen &= ~(1u << (16 * u + 4 * g + i));
+              }
+        };
+        if (!shared) {
+          only([&](int key, int i) __attribute__((always_inline)) {
+            const int ko = ords_s[buf][key + i];
+            return windowed ? ((uint32_t)ko - (uint32_t)qfirst <= qspan) | ((uint32_t)ko < qsinks) : ko <= order;
+          });
+          if (!one)
+            only([&](int key, int i) __attribute__((always_inline)) { return docs_s[buf][key + i] == qdoc; });
+        }
+        if (rem < kTile) only([&](int key, int i) __attribute__((always_inline)) { return key + i < rem; });
+      } else
 #pragma unroll
       for (int u = 0; u < kSub; ++u)
 #pragma unroll
@@ -523,10 +548,7 @@ __device__ __forceinline__ void attention_of_block(const Args& a, const uint32_t
           const int4v ko = *reinterpret_cast<const int4v*>(&ords_s[buf][key]);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const bool in = windowed ? (uint32_t)ko[i] - (uint32_t)qfirst <= qspan || (uint32_t)ko[i] < qsinks : ko[i] <= qord;
-            bool see = kd[i] == qdoc && in;
-            if (prefixed) see = see || shared;
-            see = see && key + i < rem;
+            const bool see = kd[i] == qdoc && ko[i] <= qord && key + i < rem;
             s[u][4 * g + i] = see ? s[u][4 * g + i] : -INFINITY;
             if (careful && !see) seen &= ~(1u << (16 * u + 4 * g + i));
           }
@@ -663,12 +685,12 @@ __device__ __forceinline__ void attention_of_block(const Args& a, const uint32_t
 
   // the tiles that some row of the workgroup may see
   int chunk = 0, tiles_seen = 0;
-  unsigned long long todo = 0, any_word = 0, whole_word = 0;
+  unsigned long long todo = 0, any_word = 0, whole_word = 0, one_word = 0;
   auto sort_tiles = [&](const int4 k) __attribute__((always_inline)) {
     const int t = chunk * 64 + lane;
     const bool here = t >= lo && t < hi;
     const bool shared = prefixed && t < p_tiles;
-    auto may_see = [&](const Range& r) { return here && (shared ? r.dmax >= 0 : may_see_tile(k, r)); };
+    auto may_see = [&](const Range& r) { return here & (prefixed ? (shared & (r.dmax >= 0)) | (!shared & may_see_tile(k, r)) : may_see_tile(k, r)); };
     todo = __ballot(may_see(all_rows));
     if ((in_parts || kTeams > 1 || windowed) && parts > 1) {  // every parts-th of them
       const int number = tiles_seen + __popcll(todo & ((1ull << lane) - 1));
@@ -676,26 +698,28 @@ __device__ __forceinline__ void attention_of_block(const Args& a, const uint32_t
       todo = __ballot(((todo >> lane) & 1) && number % parts == part);
     }
     any_word = __ballot(may_see(mine));
-    const bool in_window = !windowed || k.z >= window_from(mine.omax) || (k.z >= 0 && k.w < a.sinks);
-    const bool whole = k.x == k.y && mine.dmin == mine.dmax && k.x == mine.dmin && k.w <= mine.omin && in_window &&
-                       (t + 1 - p_tiles) * kTile <= k_len;
-    whole_word = __ballot(here && (shared ? (t + 1) * kTile <= a.p.len : whole));
+    const bool one = (k.x == k.y) & (mine.dmin == mine.dmax) & (k.x == mine.dmin);
+    bool whole = one & ((t + 1 - p_tiles) * kTile <= k_len) & (k.w <= mine.omin);
+    if (windowed) whole &= (k.z >= window_from(mine.omax)) | ((k.z >= 0) & (k.w < a.sinks));
+    if (prefixed) whole = shared ? (t + 1) * kTile <= a.p.len : whole;
+    whole_word = __ballot(here & whole);
+    if (windowed || prefixed) one_word = __ballot(one);
   };
   struct Next {
     int tile;
-    bool any, whole;
+    bool any, whole, one;  // seen by some row of the wave; by all; by orders and the keys' end alone
   };
   auto next_tile = [&]() __attribute__((always_inline)) -> Next {
     while (todo == 0) {
       ++chunk;
       if (windowed)
         while (chunk * 64 < hi && !((chunks >> min(chunk, 63)) & 1)) ++chunk;
-      if (chunk * 64 >= hi) return Next{-1, false, false};
+      if (chunk * 64 >= hi) return Next{-1, false, false, false};
       sort_tiles(summary_of(chunk * 64 + lane));
     }
     const int bit = __builtin_ctzll(todo);
     todo &= todo - 1;
-    return Next{chunk * 64 + bit, (bool)((any_word >> bit) & 1), (bool)((whole_word >> bit) & 1)};
+    return Next{chunk * 64 + bit, (bool)((any_word >> bit) & 1), (bool)((whole_word >> bit) & 1), (bool)((one_word >> bit) & 1)};
   };
 
   auto walk = [&](auto careful_c) __attribute__((always_inline)) {
@@ -728,7 +752,7 @@ __device__ __forceinline__ void attention_of_block(const Args& a, const uint32_t
           asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
           if (after.tile >= 0) load_tile(after.tile, buf);
         };
-        if (now.any) attend(buf, now.tile, now.whole, careful_c, read);
+        if (now.any) attend(buf, now.tile, now.whole, now.one, careful_c, read);
         if (decltype(careful_c)::value || !now.any) read();
         buf ^= 1;
         now = then, then = after;
@@ -741,7 +765,7 @@ __device__ __forceinline__ void attention_of_block(const Args& a, const uint32_t
       if constexpr (kTeams > 1) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       else __syncthreads();  // everyone's is, and everyone is done with the other buffer
       if (then.tile >= 0) load_tile(then.tile, buf ^ 1);
-      if (now.any) attend(buf, now.tile, now.whole, careful_c, [] {});
+      if (now.any) attend(buf, now.tile, now.whole, now.one, careful_c, [] {});
       buf ^= 1;
       now = then;
     }
