@@ -127,10 +127,12 @@ struct Type<MUSC_DTYPE_BF16> {
 // product of two is hi hi + hi lo + lo hi, off by 3 2^-22 of itself at most, at 3/16 of the fp32 instructions'
 // time.  n takes the largest of a row of Q, of a tile of K and of 32 channels of V over the tiles so far to
 // 2^13 .. 2^14, so what is below 2^-17 of that is off by 2^-39 of the largest instead.  Probabilities are
-// taken 2^7 times as large, as in fp16.  Tiles that hold infinities or NaN go by fp32 instructions.
+// taken 2^7 times as large, as in fp16.  By fp32 instructions go tiles that hold infinities or NaN, whose keys
+// are 2^15 apart by their largest entries, or whose V is 2^15 below what was before it, and V of more documents
+// than one.  Keys that no row of the wave sees count in none of that, whatever they hold.
 struct Split {
   typedef _Float16 Vec __attribute__((ext_vector_type(8)));
-  static constexpr int kTop = 14, kLeast = -100, kInfinity = 0x7f800000;
+  static constexpr int kTop = 14, kLeast = -100, kApart = 15, kInfinity = 0x7f800000;
   static constexpr float kShift = 7.f;
   static __device__ __forceinline__ floatx16 mfma(Vec a, Vec b, floatx16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);

@@ -416,10 +416,18 @@ __device__ __forceinline__ void attention_of_block(const Args& a, const uint32_t
       for (int m = 0; m < kQ; ++m)
 #pragma unroll
         for (int j = 0; j < 4; ++j) most = __builtin_elementwise_maximum(most, fabsf(kf[0][m][j]));
-      const int bits = wave_max_int(__float_as_int(most));
+      // this lane's key, by its largest entry; one that no row of the wave sees does not count
+      bool counts = true;
+      if (!whole && !(prefixed && tile < p_tiles)) {
+        const int kd = docs_s[buf][lq], ko = ords_s[buf][lq];
+        counts = (kd >= mine.dmin) & (kd <= mine.dmax) & (ko <= mine.omax);
+        if (windowed) counts &= (ko >= window_from(mine.omin)) | ((uint32_t)ko < (uint32_t)a.sinks);
+      }
+      const int size = counts ? __float_as_int(halves_max(most)) : 0;
+      const int largest = wave_max_int(size), smallest = wave_min_int(size > 0 ? size : 0x7fffffff);
       int k_exp = Split::kTop;
-      if (!careful && q_whole && bits < Split::kInfinity) {
-        k_exp = Split::exponent(bits);
+      if (!careful && q_whole && largest < Split::kInfinity && (largest >> 23) - (smallest >> 23) <= Split::kApart) {
+        k_exp = Split::exponent(largest);
         const float by = Split::power(Split::kTop - k_exp);
 #pragma unroll
         for (int m = 0; m < kQ / 2; ++m) {
@@ -626,6 +634,15 @@ __device__ __forceinline__ void attention_of_block(const Args& a, const uint32_t
           o[x] = Ty::mfma(__builtin_bit_cast(TVec, careful ? read_v(mm, x) : vf[careful ? 0 : mm][careful ? 0 : x]), p[mm], o[x]);
     } else if constexpr (kSplit) {
       Split::Vec ph[2], pl[2];
+      uint32_t used = 0xffffu;  // keys (elements) that some row sees
+      if (!careful && !whole) {
+        used = 0;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const unsigned long long rows = __ballot((s[0][e] != 0.f) & live);
+          used |= (uint32_t)((lh ? (uint32_t)(rows >> 32) : (uint32_t)rows) != 0) << e;
+        }
+      }
 #pragma unroll
       for (int g = 0; g < 2; ++g)
 #pragma unroll
@@ -638,11 +655,11 @@ __device__ __forceinline__ void attention_of_block(const Args& a, const uint32_t
         for (int e = 0; e < 16; ++e) {
           f[e] = *reinterpret_cast<const float*>(
               all + (v_at ^ (x << 7) ^ ((e & 3) << 6) ^ (((e >> 2) & 1) << 5)) + (8 * (e >> 2) + (e & 3)) * kPitch);
+          if (!careful && !whole) f[e] = (used >> e) & 1 ? f[e] : 0.f;
           most = __builtin_elementwise_maximum(most, fabsf(f[e]));
         }
-        const int bits = wave_max_int(__float_as_int(most));
-        if (!careful && bits < Split::kInfinity) {
-          const int here = Split::exponent(bits);
+        const int bits = wave_max_int(__float_as_int(most)), here = Split::exponent(bits);
+        if (!careful && (whole || one) && bits < Split::kInfinity && (bits == 0 || here >= v_exp[x] - Split::kApart)) {
           if (here > v_exp[x]) {
 #pragma unroll
             for (int v = 0; v < 16; ++v) o[x][v] = __builtin_ldexpf(o[x][v], v_exp[x] - here);
@@ -703,7 +720,7 @@ __device__ __forceinline__ void attention_of_block(const Args& a, const uint32_t
     if (windowed) whole &= (k.z >= window_from(mine.omax)) | ((k.z >= 0) & (k.w < a.sinks));
     if (prefixed) whole = shared ? (t + 1) * kTile <= a.p.len : whole;
     whole_word = __ballot(here & whole);
-    if (windowed || prefixed) one_word = __ballot(one);
+    if (windowed || prefixed) one_word = __ballot(one | shared);
   };
   struct Next {
     int tile;

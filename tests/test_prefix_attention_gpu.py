@@ -133,6 +133,38 @@ def test_what_unseen_keys_hold_does_not_matter(device, tq, dtype):
     assert torch.isnan(got[..., 0, 5]).all() and torch.isfinite(got[..., 1, :]).all() and torch.isfinite(got[..., 0, :5]).all()
 
 
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize('b,tq,p', [(3, 1, 45), (40, 1, 900), (3, 90, 45)])
+def test_huge_numbers_in_unseen_keys(device, b, tq, p, dtype):
+    tk = 150
+    at, new = torch.arange(tk), torch.full((b, tq), 60)
+    qd = torch.zeros((b, tq), dtype=torch.int64)
+    qd[:, tq // 2 + 1:] = -1
+    q, k, v = heads(device, dtype, b, tq, tk, 2, 2, 64)
+    pk, pv = shared(device, dtype, p, 2, 64)
+    k[:, 61:] *= 1e30
+    v[:, 61:] *= 1e30
+    keys, queries = Tokens(i32(at * 0, device), i32(at, device)), Tokens(i32(qd, device), i32(new, device), queries_only=True)
+    got = prefix_attention(q, k, v, pk, pv, 0.3, keys=keys, queries=queries)
+    k, v = k.cpu(), v.cpu()
+    k[:, 61:] = v[:, 61:] = 0
+    check_prefix(got, q.cpu(), k, v, pk.cpu(), pv.cpu(), 0.3, see_own(qd, at * 0, new, at), qd >= 0)
+
+
+@pytest.mark.parametrize('tq', [1, 60])
+def test_documents_without_own_keys(device, tq):
+    b, p = 3, 70
+    qd = torch.zeros((b, tq), dtype=torch.int64)
+    qd[1] = -1
+    q, k, v = heads(device, torch.float16, b, tq, 4, 2, 2, 64)
+    pk, pv = shared(device, torch.float16, p, 2, 64)
+    none = torch.empty((b, 0), dtype=torch.int32, device=device)
+    side, queries = Tokens(none, none.clone()), Tokens(i32(qd, device), i32(qd * 0, device), queries_only=True)
+    got = prefix_attention(q, k[:, :0], v[:, :0], pk, pv, 0.3, keys=side, queries=queries)
+    check_prefix(got, q, k[:, :0], v[:, :0], pk, pv, 0.3, torch.ones((b, tq, 0), dtype=torch.bool), qd >= 0)
+    assert (got[1] == 0).all()
+
+
 @pytest.mark.parametrize('dtype', DTYPES)
 @pytest.mark.parametrize('t', [3, 150])
 def test_layouts(device, t, dtype):

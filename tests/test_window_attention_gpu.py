@@ -149,6 +149,80 @@ def test_what_unseen_keys_hold_does_not_matter(device, tq, dtype):
         assert torch.isnan(got[:, sees]).all()
 
 
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize('tq', [1, 90])
+@pytest.mark.parametrize('huge', [1e10, 1e30, 3e38])
+def test_huge_numbers_in_unseen_keys(device, huge, tq, dtype):
+    # what memory that was never written may hold, beside keys that are seen: behind the queries, before the
+    # window, in padding, and padded queries that would see them
+    tk = 300
+    at, new = torch.arange(tk), torch.arange(200, 200 + tq)
+    kd = torch.where(at < 290, 0, -1)
+    qd = torch.zeros(tq, dtype=torch.int64)
+    qd[tq // 2 + 1:] = -1
+    q, k, v = heads(device, dtype, 2, tq, tk, 2, 2, 64)
+    keys = Tokens(i32(kd, device), i32(at, device))
+    queries = Tokens(i32(qd, device), i32(new, device), queries_only=True)
+    seen = see(qd, kd, new, at, 40, 3)
+    unseen = ~seen[0].any(0)
+    k[:, unseen.to(device)] *= huge
+    v[:, unseen.to(device)] *= huge
+    got = masked_attention(q, k, v, 0.3, keys=keys, queries=queries, window=40, sinks=3)
+    check(got, q, torch.where(unseen[None, :, None, None], 0, k.cpu()), torch.where(unseen[None, :, None, None], 0, v.cpu()), 0.3,
+          seen=seen)
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize('d', [64, 96])
+def test_documents_and_keys_of_different_sizes(device, d, dtype):
+    sizes, scales = [40, 70, 20, 100, 5, 65], torch.tensor([1.0, 1e12, 1e-12, 1e5, 1e-3, 1e20])
+    docs = torch.repeat_interleave(torch.arange(6), torch.tensor(sizes))
+    at = torch.cat([torch.arange(n) for n in sizes])
+    q, k, v = heads(device, torch.float32, 1, 300, 300, 2, 1, d)
+    of = scales[docs][None, :, None, None].to(device)
+    q, k, v = (q / of).to(dtype), (k * of).to(dtype), (v * of).to(dtype)
+    side = Tokens(i32(docs, device), i32(at, device))
+    got = masked_attention(q, k, v, 0.2, keys=side, window=33, sinks=2)
+    check(got, q, k, v, 0.2, seen=see(docs, docs, at, at, 33, 2))
+    # one document whose values grow and shrink by 2^60 over its length
+    at = torch.arange(300)
+    grow = (2.0 ** (30 - (at - 150).abs() / 5).floor()).to(device)[None, :, None, None]
+    q, k, v = heads(device, torch.float32, 1, 300, 300, 2, 1, d)
+    k, v, q = (k * grow ** 0.1).to(dtype), (v * grow).to(dtype), q.to(dtype)
+    side = Tokens(i32(at * 0, device), i32(at, device))
+    got = masked_attention(q, k, v, 0.2, keys=side, window=20)
+    check(got, q, k, v, 0.2, seen=see(at * 0, at * 0, at, at, 20, 0))
+
+
+@pytest.mark.parametrize('tq', [1, 100])
+@pytest.mark.parametrize('size', [1e-30, 1e-12, 1e15])
+def test_fp32_sizes(device, size, tq):
+    at = torch.arange(150)
+    q, k, v = heads(device, torch.float32, 1, tq, 150, 2, 2, 64)
+    q, k, v = q / size, k * size, v * size
+    keys = Tokens(i32(at * 0, device), i32(at, device))
+    queries = Tokens(i32(at[:tq] * 0, device), i32(at[-tq:], device), queries_only=True)
+    got = masked_attention(q, k, v, 0.2, keys=keys, queries=queries, window=60, sinks=1)
+    check(got, q, k, v, 0.2, seen=see(at[:tq] * 0, at * 0, at[-tq:], at, 60, 1))
+
+
+def test_fp32_infinities_that_are_seen(device):
+    t = 120
+    q, k, v = heads(device, torch.float32, 1, t, t, 1, 1, 64)
+    at = torch.arange(t)
+    side = Tokens(i32(at * 0, device), i32(at, device))
+    v[0, 30, 0, 5], v[0, 70, 0, 6] = float('inf'), float('nan')
+    got = masked_attention(q, k, v, 0.1, keys=side, window=20)
+    assert (got[0, 30:50, 0, 5] == float('inf')).all() and torch.isnan(got[0, 70:90, 0, 6]).all()
+    got[0, 30:50, 0, 5] = got[0, 70:90, 0, 6] = 0
+    assert torch.isfinite(got).all()
+    k[0, 100, 0, 3] = float('nan')
+    q[0, 10, 0, 0] = float('inf')
+    got = masked_attention(q, k, v, 0.1, keys=side, window=20)
+    assert torch.isnan(got[0, 100:]).all() and torch.isnan(got[0, 10]).all()
+    assert torch.isfinite(got[0, 11:30]).all() and torch.isfinite(got[0, :10]).all()
+
+
 @pytest.mark.parametrize('dtype', DTYPES)
 def test_a_window_over_everything_is_masked_attention(device, dtype):
     t = 400
