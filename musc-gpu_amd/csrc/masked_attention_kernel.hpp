@@ -66,6 +66,10 @@ __device__ __forceinline__ void attention_of_block(const Args& a, const uint32_t
   // fp32 as three fp16 products, see Split in masked_attention.hpp
   constexpr bool kSplit = !k16 && (windowed || prefixed);
   constexpr float kShift = kSplit ? Split::kShift : Ty::kShift;
+  // few 16-bit rows of windows and prefixes: probabilities as two numbers each.  Their second product is in the
+  // shadow of the loads, and with rounded ones a few rows may be twice as far from float64 as their own rounding
+  // leaves them; over many rows it is 1.2 to 1.3 times.
+  constexpr bool kTwoTerms = k16 && (windowed || prefixed) && kWaves == 1;
   __shared__ __attribute__((aligned(1024))) char staged[2 * kTeams][2 * kPart];
   __shared__ __attribute__((aligned(16))) int docs_s[2 * kTeams][64], ords_s[2 * kTeams][64];
   __shared__ float pos_s[2 * kTeams][64 * kMaxAxes];
@@ -584,8 +588,18 @@ __device__ __forceinline__ void attention_of_block(const Args& a, const uint32_t
     for (int u = 0; u < kSub; ++u)
 #pragma unroll
       for (int v = 0; v < 16; ++v) s[u][v] = __builtin_amdgcn_exp2f(fmaf(s[u][v], to_log2, base));
-    TVec p[2 * kSub];
-    if constexpr (k16) {
+    TVec p[2 * kSub], rest[kTwoTerms ? 2 * kSub : 1];
+    if constexpr (kTwoTerms) {
+#pragma unroll
+      for (int mm = 0; mm < 2 * kSub; ++mm)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float f = s[mm >> 1][8 * (mm & 1) + j];
+          p[mm][j] = (T)f;
+          rest[mm][j] = (T)(f - (float)p[mm][j]);
+          l_run += f;
+        }
+    } else if constexpr (k16) {
 #pragma unroll
       for (int mm = 0; mm < 2 * kSub; ++mm)
 #pragma unroll
@@ -610,7 +624,7 @@ __device__ __forceinline__ void attention_of_block(const Args& a, const uint32_t
         for (int u = 0; u < kSub; ++u)
 #pragma unroll
           for (int v = 0; v < 16; ++v)
-            if (u == u0 && v == v0) pr = (float)(T)s[u][v];
+            if (u == u0 && v == v0) pr = kTwoTerms ? s[u][v] : (float)(T)s[u][v];
         pr = __shfl(pr, from, kWave);
         const bool see = (__shfl(seen, from, kWave) >> (16 * u0 + v0)) & 1;
 #pragma unroll
@@ -630,8 +644,11 @@ __device__ __forceinline__ void attention_of_block(const Args& a, const uint32_t
 #pragma unroll
       for (int mm = 0; mm < 2 * kSub; ++mm)
 #pragma unroll
-        for (int x = 0; x < kO; ++x)
-          o[x] = Ty::mfma(__builtin_bit_cast(TVec, careful ? read_v(mm, x) : vf[careful ? 0 : mm][careful ? 0 : x]), p[mm], o[x]);
+        for (int x = 0; x < kO; ++x) {
+          const TVec values = __builtin_bit_cast(TVec, careful ? read_v(mm, x) : vf[careful ? 0 : mm][careful ? 0 : x]);
+          if constexpr (kTwoTerms) o[x] = Ty::mfma(values, rest[mm], o[x]);
+          o[x] = Ty::mfma(values, p[mm], o[x]);
+        }
     } else if constexpr (kSplit) {
       Split::Vec ph[2], pl[2];
       uint32_t used = 0xffffu;  // keys (elements) that some row sees
