@@ -40,6 +40,30 @@
 // large copy.  fp32: its matrix instructions, 127 to 133 TFLOP/s (8192 tokens, 8 heads of 64, 96 and 128) of the
 // 153 of a product of 8192^3; the four-wave kernels of heads past 96 spill 46 to 75 registers.  One document of
 // few row tiles leaves CUs idle: a schedule takes the place of splits of the keys, see plan().
+//
+// Two further forms, kernels of their own (masked_attention_window_*.hip, masked_attention_prefix_*.hip):
+//
+//   window      seen(i, j) and (order(j) > order(i) - window or 0 <= order(j) < sinks)
+//   prefix      every key of a prefix that the batch shares, and of an entry's own keys seen(i, j)
+//
+// A window's waves first look over the summaries of all tiles, in parallel, and then go to those 64s of
+// tiles that hold some they see; splits share out the tiles that are seen.  A mixed tile's scores are tested
+// by orders, by documents where it has several, and by the end of the keys, each only where it tells: 64 keys
+// 1.5 us where a whole tile takes 0.9 (all tests on each score 2.2).  8192 tokens, window of 1024, 32 heads on 8 of
+// 128, bf16: 187 us, of it 8.4 for each tile of the 19 that 2048 workgroups in four rounds go over, the rest
+// what each round pays to read its Q, find its tiles and write its output.  8 single tokens, 4096 of 32768
+// keys: 31 us = 4.3 TB/s, and 4 for the join.  24 frames of 256 tokens, 16 heads of 64, bias over three
+// axes, fp16: 78 us, the bias as above.
+//
+// A prefix's tiles come before an entry's own in one walk.  Where the entries have few rows each, the rows of
+// all of them walk over the prefix together (it is read once, in full row tiles) and, in the same launch, each
+// entry's over its own keys; a join follows.  16 x 1370 tokens after 5480, 16 heads of 64, fp16: 760 to 810 us =
+// 0.76 to 0.81 PFLOP/s, as for one document of 8192.  32 single tokens after 16384 keys and over up to 700
+// of their own, 32 heads on 8 of 128, bf16: 35 us = 3.6 TB/s, and 6 for the join.
+//
+// Both keep the probabilities of few 16-bit rows in two numbers each, and fp32 as Split has it: a tile of 32
+// keys of heads of 96 takes 1150 cycles of matrix instructions (6144 of fp32 ones) and about 2500 of vector
+// ones.  3 x 1500 tokens, window of 250, 8 heads on 4 of 80, cap: 54 us, by fp32 instructions 78.
 #pragma once
 
 #include <hip/hip_bf16.h>

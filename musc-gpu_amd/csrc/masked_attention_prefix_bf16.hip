@@ -1,5 +1,4 @@
-// Masked attention after a shared prefix on bf16 storage (its matrix instructions, __builtin_amdgcn_mfma_*, are in
-// masked_attention_kernel.hpp).
+// Masked attention after a shared prefix on bf16 storage; the kernels are in masked_attention_kernel.hpp.
 #include "masked_attention_kernel.hpp"
 
 void musc::mattn::launch_prefix_bf16(const Args& a, const Args* more, int waves, hipStream_t stream) {

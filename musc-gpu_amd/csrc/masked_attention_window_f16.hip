@@ -1,5 +1,4 @@
-// Masked attention with a window and sinks on fp16 storage (its matrix instructions, __builtin_amdgcn_mfma_*, are in
-// masked_attention_kernel.hpp).
+// Masked attention with a window and sinks on fp16 storage; the kernels are in masked_attention_kernel.hpp.
 #include "masked_attention_kernel.hpp"
 
 void musc::mattn::launch_window_f16(const Args& a, int waves, hipStream_t stream) {

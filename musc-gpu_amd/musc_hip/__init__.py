@@ -12,7 +12,9 @@ include/musc_hip.h); nothing here computes on the CPU.
   pipeline.score_pool                           tokens -> maps + image scores, fused
   _layers_hip.rms_norm, rms_norm_quantized      root-mean-square norm of packed encoders, 8-bit output
   _rotary_hip.RotaryAxes, rotary                rotary positions over several axes
-  _masked_attention_hip.Tokens, masked_attention  packed images, padded rows, prefixes, caches
+  _rotary_hip.norm_rotary                       the same after a norm of every head of q and k
+  _masked_attention_hip.Tokens, masked_attention  packed images, padded rows, prefixes, caches, windows with sinks
+  _masked_attention_hip.prefix_attention        a batch that shares a prefix (reference images, a common text)
 """
 from ._backend import configure_backend, select_backend  # noqa: F401
 

@@ -2,8 +2,10 @@
 
 The fused block attention of _attention_hip sees every token of one image; here a query sees
 the keys of its own document (an image of a packed batch, the live part of a padded one) whose
-order is not past its own (a prefix, a causal text, the frames of a clip), and the scores may
-be capped by a tanh and lowered with the distance of two tokens.  The reference's blocks pass
+order is not past its own (a prefix, a causal text, the frames of a clip), of those the last
+ones and the first few if asked (a window with sinks), and the scores may be capped by a tanh and
+lowered with the distance of two tokens; prefix_attention is for batches whose entries share
+their first keys.  The reference's blocks pass
 masks to torch's math path (models/backbone/open_clip/transformer.py:232-234); nothing here
 writes the logits or a mask to memory.
 """
