@@ -220,11 +220,12 @@ int plan(const musc_masked_attention& c, Args& a, int& waves) {
     a.in_pieces = !a.in_parts && !c.q_order && whole < 4LL * a.slots;
     if (a.in_pieces) a.jobs = (int)schedule_pieces(a.row_tiles);
   } else if (whole < (waves == 1 ? 1024 : 256) && !narrow) {
-    // few rows: their keys in splits of at least one tile (4 where four waves share the tiles)
+    // few rows: their keys in splits of at least one tile (4 where four waves share the tiles; fp32 windows, whose
+    // tiles take long, 2)
     // (a window's first look over all tiles pays for fewer workgroups: 8 x 4096 of 32768 keys, 32 heads on 8 of
     // 128, bf16, 2048 waves 45 us with the join, 1024 36, 512 37)
     long long splits = ((waves == 1 ? (a.window ? 1024 : 2048) : 512) + whole - 1) / whole;
-    const int least = waves == 1 ? 1 : 4;
+    const int least = waves == 1 ? 1 : a.window && c.dtype == MUSC_DTYPE_F32 ? 2 : 4;
     if (splits > a.key_tiles / least) splits = a.key_tiles / least;
     if (splits > kMaxSplits) splits = kMaxSplits;
     a.splits = splits < 1 ? 1 : (int)splits;

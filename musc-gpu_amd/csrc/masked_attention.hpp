@@ -152,8 +152,8 @@ struct Type<MUSC_DTYPE_BF16> {
 // time.  n takes the largest of a row of Q, of a tile of K and of 32 channels of V over the tiles so far to
 // 2^13 .. 2^14, so what is below 2^-17 of that is off by 2^-39 of the largest instead.  Probabilities are
 // taken 2^7 times as large, as in fp16.  By fp32 instructions go tiles that hold infinities or NaN, whose keys
-// are 2^15 apart by their largest entries, or whose V is 2^15 below what was before it, and V of more documents
-// than one.  Keys that no row of the wave sees count in none of that, whatever they hold.
+// are 2^15 apart by their largest entries, or whose V is 2^15 below what was before it, or of several
+// documents as far apart.  Keys that no row of the wave sees count in none of that, whatever they hold.
 struct Split {
   typedef _Float16 Vec __attribute__((ext_vector_type(8)));
   static constexpr int kTop = 14, kLeast = -100, kApart = 15, kInfinity = 0x7f800000;
@@ -254,6 +254,20 @@ __device__ __forceinline__ int wave_min_int(int v) {
   return __builtin_amdgcn_readlane(v, 63);
 }
 __device__ __forceinline__ int wave_max_int(int v) { return ~wave_min_int(~v); }
+// All bits of the 32 lanes of each half, on every lane of it, in the same way.
+template <int kMove, int kRows>
+__device__ __forceinline__ uint32_t or_with(uint32_t v) {
+  return v | (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, kMove, kRows, 0xf, false);
+}
+__device__ __forceinline__ uint32_t halves_or(uint32_t v) {
+  v = or_with<0x111, 0xf>(v);
+  v = or_with<0x112, 0xf>(v);
+  v = or_with<0x114, 0xf>(v);
+  v = or_with<0x118, 0xf>(v);
+  v = or_with<0x142, 0xa>(v);
+  const uint32_t lower = __builtin_amdgcn_readlane((int)v, 31), upper = __builtin_amdgcn_readlane((int)v, 63);
+  return threadIdx.x & 32 ? upper : lower;
+}
 
 // The documents and orders of a set of rows: what a tile is compared with.
 struct Range {

@@ -651,14 +651,28 @@ __device__ __forceinline__ void attention_of_block(const Args& a, const uint32_t
         }
     } else if constexpr (kSplit) {
       Split::Vec ph[2], pl[2];
-      uint32_t used = 0xffffu;  // keys (elements) that some row sees
+      uint32_t used = 0xffffu;  // of this half's keys, those (by element) that some row sees
       if (!careful && !whole) {
         used = 0;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const unsigned long long rows = __ballot((s[0][e] != 0.f) & live);
-          used |= (uint32_t)((lh ? (uint32_t)(rows >> 32) : (uint32_t)rows) != 0) << e;
+        for (int e = 0; e < 16; ++e) used |= min(__float_as_uint(s[0][e]), 1u) << e;
+        used = halves_or(live ? used : 0);
+      }
+      // Several documents may have V of very different sizes, each of which its own rows see: whether the tile's
+      // used keys (lane lq has key lq) are near one another by their largest entries.
+      bool near = whole || one;
+      if (!careful && !near) {
+        float most = 0.f;
+#pragma unroll
+        for (int m = 0; m < kQ; ++m) {
+          const TVec row = *reinterpret_cast<const TVec*>(all + ((k_at + kPart) ^ (m << 5)));
+#pragma unroll
+          for (int j = 0; j < 4; ++j) most = __builtin_elementwise_maximum(most, fabsf(row[j]));
         }
+        const uint32_t used_there = (uint32_t)__shfl((int)used, 32 * ((lq >> 2) & 1), kWave);
+        const int size = (used_there >> ((lq >> 3) * 4 + (lq & 3))) & 1 ? __float_as_int(halves_max(most)) : 0;
+        const int largest = wave_max_int(size), smallest = wave_min_int(size > 0 ? size : 0x7fffffff);
+        near = largest < Split::kInfinity && (largest >> 23) - (smallest >> 23) <= Split::kApart;
       }
 #pragma unroll
       for (int g = 0; g < 2; ++g)
@@ -672,11 +686,11 @@ __device__ __forceinline__ void attention_of_block(const Args& a, const uint32_t
         for (int e = 0; e < 16; ++e) {
           f[e] = *reinterpret_cast<const float*>(
               all + (v_at ^ (x << 7) ^ ((e & 3) << 6) ^ (((e >> 2) & 1) << 5)) + (8 * (e >> 2) + (e & 3)) * kPitch);
-          if (!careful && !whole) f[e] = (used >> e) & 1 ? f[e] : 0.f;
+          if (!careful && !whole) f[e] = __int_as_float(__float_as_int(f[e]) & __builtin_amdgcn_sbfe((int)used, e, 1));
           most = __builtin_elementwise_maximum(most, fabsf(f[e]));
         }
         const int bits = wave_max_int(__float_as_int(most)), here = Split::exponent(bits);
-        if (!careful && (whole || one) && bits < Split::kInfinity && (bits == 0 || here >= v_exp[x] - Split::kApart)) {
+        if (!careful && near && bits < Split::kInfinity && (bits == 0 || here >= v_exp[x] - Split::kApart)) {
           if (here > v_exp[x]) {
 #pragma unroll
             for (int v = 0; v < 16; ++v) o[x][v] = __builtin_ldexpf(o[x][v], v_exp[x] - here);
