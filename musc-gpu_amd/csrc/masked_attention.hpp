@@ -163,6 +163,10 @@ struct Split {
   }
   // e with |x| < 2^e, from the bits of |x|; the smallest share kLeast
   static __device__ __forceinline__ int exponent(int bits) { return max((bits >> 23) - 126, kLeast); }
+  // whether some lane's size (bits of a largest entry; 0 does not count) is 2^kApart below the largest
+  static __device__ __forceinline__ bool apart(int size, int largest) {
+    return __any((size > 0) & ((largest >> 23) - (size >> 23) > kApart));
+  }
   static __device__ __forceinline__ float power(int e) { return __int_as_float((e + 127) << 23); }
   typedef _Float16 Two __attribute__((ext_vector_type(2)));
   // two of each: hi is opaque, or the compiler forms it a second time for lo

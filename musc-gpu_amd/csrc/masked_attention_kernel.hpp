@@ -428,9 +428,9 @@ __device__ __forceinline__ void attention_of_block(const Args& a, const uint32_t
         if (windowed) counts &= (ko >= window_from(mine.omin)) | ((uint32_t)ko < (uint32_t)a.sinks);
       }
       const int size = counts ? __float_as_int(halves_max(most)) : 0;
-      const int largest = wave_max_int(size), smallest = wave_min_int(size > 0 ? size : 0x7fffffff);
+      const int largest = wave_max_int(size);
       int k_exp = Split::kTop;
-      if (!careful && q_whole && largest < Split::kInfinity && (largest >> 23) - (smallest >> 23) <= Split::kApart) {
+      if (!careful && q_whole && largest < Split::kInfinity && !Split::apart(size, largest)) {
         k_exp = Split::exponent(largest);
         const float by = Split::power(Split::kTop - k_exp);
 #pragma unroll
@@ -671,8 +671,8 @@ __device__ __forceinline__ void attention_of_block(const Args& a, const uint32_t
         }
         const uint32_t used_there = (uint32_t)__shfl((int)used, 32 * ((lq >> 2) & 1), kWave);
         const int size = (used_there >> ((lq >> 3) * 4 + (lq & 3))) & 1 ? __float_as_int(halves_max(most)) : 0;
-        const int largest = wave_max_int(size), smallest = wave_min_int(size > 0 ? size : 0x7fffffff);
-        near = largest < Split::kInfinity && (largest >> 23) - (smallest >> 23) <= Split::kApart;
+        const int largest = wave_max_int(size);
+        near = largest < Split::kInfinity && !Split::apart(size, largest);
       }
 #pragma unroll
       for (int g = 0; g < 2; ++g)
