@@ -63,7 +63,7 @@
 //
 // Both keep the probabilities of few 16-bit rows in two numbers each, and fp32 as Split has it: a tile of 32
 // keys of heads of 96 takes 1150 cycles of matrix instructions (6144 of fp32 ones) and about 2500 of vector
-// ones.  3 x 1500 tokens, window of 250, 8 heads on 4 of 80, cap: 54 us, by fp32 instructions 78.
+// ones.  3 x 1500 tokens, window of 250, 8 heads on 4 of 80, cap: 57 us, by fp32 instructions 78.
 #pragma once
 
 #include <hip/hip_bf16.h>

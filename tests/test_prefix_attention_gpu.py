@@ -238,3 +238,17 @@ def test_refusals(device):
     empty = prefix_attention(q[:, :0], k, v, pk, pv, 1.0)
     assert empty.shape == (2, 0, 4, 64)
     assert (prefix_attention(q, k[:, :0], v[:, :0], pk[:0], pv[:0], 1.0) == 0).all()
+
+
+@pytest.mark.parametrize('dtype', [torch.float16, torch.float32])
+@pytest.mark.parametrize('b,tq', [(2, 1), (3, 200)])
+def test_prefixes_past_32_bit_offsets(device, b, tq, dtype):
+    """Heads of a wide prefix whose last tokens lie more than 2^32 bytes after the first."""
+    p, apart, d = 2100, (1 << 20) + 512, 64
+    wide = torch.empty((p, apart * (2 if dtype == torch.float16 else 1)), dtype=dtype, device=device)
+    q, k, v = heads(device, dtype, b, tq, 9, 2, 1, d)
+    pk, pv = shared(device, dtype, p, 1, d)
+    wide[:, 512:576], wide[:, -128:-64] = pk[:, 0], pv[:, 0]
+    assert (p - 64) * wide.stride(0) * wide.element_size() > 1 << 32
+    got = prefix_attention(q, k, v, wide[:, None, 512:576], wide[:, None, -128:-64], 0.3)
+    check_prefix(got, q, k, v, pk, pv, 0.3)

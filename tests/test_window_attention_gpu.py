@@ -269,3 +269,22 @@ def test_refusals(device):
             masked_attention(q, k, v, 1.0, keys=keys, window=4)
     with pytest.raises(ValueError, match='backward'):
         masked_attention(q.requires_grad_(), k, v, 1.0, keys=side, window=4)
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize('tq', [1, 40, 300])
+def test_caches_past_32_bit_offsets(device, tq, dtype):
+    """Heads of a wide cache, a token every 8 Ki numbers: the last keys lie more than 2^32 bytes after the first."""
+    tk, h, d = (1 << 18 if dtype == torch.bfloat16 else 1 << 17) + 1037, 2, 64
+    cache = torch.empty((1, tk, 1 << 13), dtype=dtype, device=device)
+    q, k, v = heads(device, dtype, 1, tq, tk, h, 1, d)
+    cache[..., 128:192], cache[..., 4096:4160] = k[:, :, 0], v[:, :, 0]
+    at = torch.arange(tk)
+    keys = Tokens(i32(torch.zeros(tk), device), i32(at, device))
+    queries = Tokens(i32(torch.zeros(tq), device), i32(at[-tq:], device), queries_only=True)
+    assert (tk - 300) * (1 << 13) * cache.element_size() > 1 << 32
+    got = masked_attention(q, cache[:, :, None, 128:192], cache[:, :, None, 4096:4160], 0.3, keys=keys, queries=queries,
+                           window=700, sinks=3)
+    some = torch.cat([at[:32], at[-1100:]])
+    seen = see(torch.zeros(tq), torch.zeros(len(some)), at[-tq:], some, 700, 3)
+    check(got, q, k[:, some], v[:, some], 0.3, seen=seen)
