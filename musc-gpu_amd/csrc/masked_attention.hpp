@@ -154,9 +154,11 @@ struct Type<MUSC_DTYPE_BF16> {
 // taken 2^7 times as large, as in fp16.  By fp32 instructions go tiles that hold infinities or NaN, whose keys
 // are 2^15 apart by their largest entries, or whose V is 2^15 below what was before it, or of several
 // documents as far apart.  Keys that no row of the wave sees count in none of that, whatever they hold.
+// Entries of V in tiles that go by fp32 instructions are taken below 2^(kMost + kTop): with probabilities up to
+// 2^15 their sums over 2^31 keys stay finite, beside an entry that is not.
 struct Split {
   typedef _Float16 Vec __attribute__((ext_vector_type(8)));
-  static constexpr int kTop = 14, kLeast = -100, kApart = 15, kInfinity = 0x7f800000;
+  static constexpr int kTop = 14, kLeast = -100, kMost = 64, kApart = 15, kInfinity = 0x7f800000;
   static constexpr float kShift = 7.f;
   static __device__ __forceinline__ floatx16 mfma(Vec a, Vec b, floatx16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);

@@ -651,6 +651,11 @@ __device__ __forceinline__ void attention_of_block(const Args& a, const uint32_t
         }
     } else if constexpr (kSplit) {
       Split::Vec ph[2], pl[2];
+      auto scale_to = [&](int x, int to) __attribute__((always_inline)) {
+#pragma unroll
+        for (int v = 0; v < 16; ++v) o[x][v] = __builtin_ldexpf(o[x][v], v_exp[x] - to);
+        v_exp[x] = to;
+      };
       uint32_t used = 0xffffu;  // of this half's keys, those (by element) that some row sees
       if (!careful && !whole) {
         used = 0;
@@ -691,11 +696,7 @@ __device__ __forceinline__ void attention_of_block(const Args& a, const uint32_t
         }
         const int bits = wave_max_int(__float_as_int(most)), here = Split::exponent(bits);
         if (!careful && near && bits < Split::kInfinity && (bits == 0 || here >= v_exp[x] - Split::kApart)) {
-          if (here > v_exp[x]) {
-#pragma unroll
-            for (int v = 0; v < 16; ++v) o[x][v] = __builtin_ldexpf(o[x][v], v_exp[x] - here);
-            v_exp[x] = here;
-          }
+          if (here > v_exp[x]) scale_to(x, here);
           const float by = Split::power(Split::kTop - v_exp[x]);
 #pragma unroll
           for (int g = 0; g < 2; ++g) {
@@ -708,6 +709,13 @@ __device__ __forceinline__ void attention_of_block(const Args& a, const uint32_t
             __builtin_amdgcn_sched_barrier(0);
           }
         } else {
+          if constexpr (!careful) {  // a scale in which the sums of the finite ones stay finite
+            float finite = 0.f;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) finite = fmaxf(finite, fabsf(f[e]) < INFINITY ? fabsf(f[e]) : 0.f);
+            const int least = Split::exponent(wave_max_int(__float_as_int(finite))) - Split::kMost;
+            if (least > v_exp[x]) scale_to(x, least);
+          }
           const float by = Split::power(Split::kTop - v_exp[x]);
 #pragma unroll
           for (int e = 0; e < 16; ++e)
