@@ -437,9 +437,10 @@ int musc_masked_attention_fwd(const musc_masked_attention* call, void* workspace
  * window >= 1, sinks >= 0, with orders on both sides.  Tiles that
  * no row of a workgroup sees are not read.  call->schedule is not used.
  * fp32, here and after a prefix: products are three fp16 ones of operands held in 22 bits (Q by row, K by 32 keys, V
- * by 32 channels), so a logit is off by 3 2^-22 of its sum of |q_c k_c| scale and an output by as much of its
- * V where these are within 2^17 of their largest; 32 keys whose largest entries are 2^15 apart, V that falls by
- * as much along the keys, infinities and NaN are computed with fp32 products.  What unseen keys hold has no effect. */
+ * by 32 keys and 32 channels), so a logit is off by 3 2^-22 of its sum of |q_c k_c| scale and an output by as much of its
+ * V where these are within 2^17 of the largest they are held with, and by 2^-39 of that largest for smaller ones.
+ * 32 keys whose largest entries are 2^15 apart in K or, in 32 channels, 2^6 in V, infinities and NaN are computed with
+ * fp32 products, so what keys hold that a query does not see costs it no more than these roundings. */
 int musc_window_attention_workspace_bytes(const musc_masked_attention* call, int window, int sinks, size_t* out);
 int musc_window_attention_fwd(const musc_masked_attention* call, int window, int sinks, void* workspace,
                               size_t workspace_bytes, hipStream_t stream);

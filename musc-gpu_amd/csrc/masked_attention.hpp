@@ -149,16 +149,23 @@ struct Type<MUSC_DTYPE_BF16> {
 
 // fp32 operands as two fp16 numbers each, x 2^n = hi + lo to 2^-22 of x, for windows and after prefixes: a
 // product of two is hi hi + hi lo + lo hi, off by 3 2^-22 of itself at most, at 3/16 of the fp32 instructions'
-// time.  n takes the largest of a row of Q, of a tile of K and of 32 channels of V over the tiles so far to
+// time.  n takes the largest of a row of Q, of a tile of K and of 32 channels of a tile's V to
 // 2^13 .. 2^14, so what is below 2^-17 of that is off by 2^-39 of the largest instead.  Probabilities are
-// taken 2^7 times as large, as in fp16.  By fp32 instructions go tiles that hold infinities or NaN, whose keys
-// are 2^15 apart by their largest entries, or whose V is 2^15 below what was before it, or of several
-// documents as far apart.  Keys that no row of the wave sees count in none of that, whatever they hold.
-// Entries of V in tiles that go by fp32 instructions are taken below 2^(kMost + kTop): with probabilities up to
-// 2^15 their sums over 2^31 keys stay finite, beside an entry that is not.
+// taken 2^7 times as large, as in fp16: those below 2^-10 of a row's largest are off by 2^-32 of that.
+//
+// What one row sees must not cost another its digits, so the keys of a tile have to be of one size.  By fp32
+// instructions go tiles that hold infinities or NaN; whose keys are 2^kApart apart by K's largest entries; and
+// blocks of V (32 keys, 32 channels) with an entry below 2^-kEntries of the scale, if also some key's largest entry
+// there is below 2^-kKeys of it (of standard normal V one block in 20 is asked so, and none of 4000 fails).  The scale
+// of a block stays while its largest entry is within 2^kFall of it; else o is taken to the block's own.
+// Keys that no row of the wave sees count in none of that, whatever they hold.
+//
+// V's scale is 2^kMost at most and 2^-kMost of the largest entry so far at least: with probabilities up to 2^15 the
+// sums over 2^31 keys stay finite, and entries from 2^-70 on stay normal numbers beside larger ones.
 struct Split {
   typedef _Float16 Vec __attribute__((ext_vector_type(8)));
-  static constexpr int kTop = 14, kLeast = -100, kMost = 64, kApart = 15, kInfinity = 0x7f800000;
+  static constexpr int kTop = 14, kLeast = -100, kMost = 64, kInfinity = 0x7f800000;
+  static constexpr int kApart = 15, kEntries = 17, kKeys = 6, kFall = 2;
   static constexpr float kShift = 7.f;
   static __device__ __forceinline__ floatx16 mfma(Vec a, Vec b, floatx16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);

@@ -380,7 +380,7 @@ __device__ __forceinline__ void attention_of_block(const Args& a, const uint32_t
   };
 
   floatx16 o[kO];
-  int v_exp[kSplit ? kO : 1];  // split: o is in 2^(v_exp - 14)
+  int v_exp[kSplit ? kO : 1], v_top[kSplit ? kO : 1];  // split: o is in 2^(v_exp - 14); the largest entry so far
   float m_run, l_run;  // running maximum (raw) and sum of this half's keys
   float base;          // exponent of a score: raw * to_log2 + base
   bool mixed_seen;
@@ -663,22 +663,20 @@ __device__ __forceinline__ void attention_of_block(const Args& a, const uint32_t
         for (int e = 0; e < 16; ++e) used |= min(__float_as_uint(s[0][e]), 1u) << e;
         used = halves_or(live ? used : 0);
       }
-      // Several documents may have V of very different sizes, each of which its own rows see: whether the tile's
-      // used keys (lane lq has key lq) are near one another by their largest entries.
-      bool near = whole || one;
-      if (!careful && !near) {
+      // The smallest of the used keys (lane lq has key lq) by their largest entries of block x; zeros do not count.
+      auto smallest_key = [&](int x) __attribute__((always_inline)) {
         float most = 0.f;
 #pragma unroll
-        for (int m = 0; m < kQ; ++m) {
+        for (int m = 4 * x; m < 4 * x + 4; ++m) {
           const TVec row = *reinterpret_cast<const TVec*>(all + ((k_at + kPart) ^ (m << 5)));
 #pragma unroll
           for (int j = 0; j < 4; ++j) most = __builtin_elementwise_maximum(most, fabsf(row[j]));
         }
+        most = halves_max(most);
         const uint32_t used_there = (uint32_t)__shfl((int)used, 32 * ((lq >> 2) & 1), kWave);
-        const int size = (used_there >> ((lq >> 3) * 4 + (lq & 3))) & 1 ? __float_as_int(halves_max(most)) : 0;
-        const int largest = wave_max_int(size);
-        near = largest < Split::kInfinity && !Split::apart(size, largest);
-      }
+        const bool counts = ((used_there >> ((lq >> 3) * 4 + (lq & 3))) & 1) & (most != 0.f);
+        return __int_as_float(wave_min_int(counts ? __float_as_int(most) : Split::kInfinity));
+      };
 #pragma unroll
       for (int g = 0; g < 2; ++g)
 #pragma unroll
@@ -686,18 +684,30 @@ __device__ __forceinline__ void attention_of_block(const Args& a, const uint32_t
 #pragma unroll
       for (int x = 0; x < kO; ++x) {
         float f[16];  // element e: key 8 (e / 4) + 4 lh + e % 4, channel 32 x + lq
-        float most = 0.f;
+        float most = 0.f, least = INFINITY;
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           f[e] = *reinterpret_cast<const float*>(
               all + (v_at ^ (x << 7) ^ ((e & 3) << 6) ^ (((e >> 2) & 1) << 5)) + (8 * (e >> 2) + (e & 3)) * kPitch);
-          if (!careful && !whole) f[e] = __int_as_float(__float_as_int(f[e]) & __builtin_amdgcn_sbfe((int)used, e, 1));
+          if (!careful) {
+            const int bits = __float_as_int(f[e]), mask = __builtin_amdgcn_sbfe((int)used, e, 1);
+            least = __builtin_elementwise_minimum(least, fabsf(__int_as_float((bits & mask) | (Split::kInfinity & ~mask))));
+            f[e] = __int_as_float(bits & mask);
+          }
           most = __builtin_elementwise_maximum(most, fabsf(f[e]));
         }
+        // The block's scale: as it was, or, where its largest entry has left that, its own; and whether it fits
+        // all entries, or all keys by their largest.
         const int bits = wave_max_int(__float_as_int(most)), here = Split::exponent(bits);
-        if (!careful && near && bits < Split::kInfinity && (bits == 0 || here >= v_exp[x] - Split::kApart)) {
-          if (here > v_exp[x]) scale_to(x, here);
-          const float by = Split::power(Split::kTop - v_exp[x]);
+        const bool kept = bits == 0 || (here <= v_exp[x] && here >= v_exp[x] - Split::kFall);
+        const int to = kept ? v_exp[x] : max(here, v_top[x] - Split::kMost);
+        bool fits = !careful && bits < Split::kInfinity && to <= Split::kMost;
+        if (fits && __any((32 * x + lq < d) & (least < Split::power(to - Split::kEntries))))
+          fits = smallest_key(x) >= Split::power(to - Split::kKeys);
+        if (fits) {
+          if (to != v_exp[x]) scale_to(x, to);
+          v_top[x] = max(v_top[x], to);
+          const float by = Split::power(Split::kTop - to);
 #pragma unroll
           for (int g = 0; g < 2; ++g) {
             Split::Vec vh, vl;
@@ -713,8 +723,8 @@ __device__ __forceinline__ void attention_of_block(const Args& a, const uint32_t
             float finite = 0.f;
 #pragma unroll
             for (int e = 0; e < 16; ++e) finite = fmaxf(finite, fabsf(f[e]) < INFINITY ? fabsf(f[e]) : 0.f);
-            const int least = Split::exponent(wave_max_int(__float_as_int(finite))) - Split::kMost;
-            if (least > v_exp[x]) scale_to(x, least);
+            v_top[x] = max(v_top[x], Split::exponent(wave_max_int(__float_as_int(finite))));
+            if (v_exp[x] < v_top[x] - Split::kMost) scale_to(x, v_top[x] - Split::kMost);
           }
           const float by = Split::power(Split::kTop - v_exp[x]);
 #pragma unroll
@@ -786,7 +796,7 @@ __device__ __forceinline__ void attention_of_block(const Args& a, const uint32_t
     m_run = -INFINITY, l_run = 0.f, base = kShift, mixed_seen = false;
     if constexpr (kSplit) {
 #pragma unroll
-      for (int x = 0; x < kO; ++x) v_exp[x] = decltype(careful_c)::value ? Split::kTop : Split::kLeast;
+      for (int x = 0; x < kO; ++x) v_exp[x] = decltype(careful_c)::value ? Split::kTop : Split::kLeast, v_top[x] = Split::kLeast;
     }
     chunk = lo / 64, tiles_seen = 0;
     sort_tiles(decltype(careful_c)::value ? summary_of(lo / 64 * 64 + lane) : first_summary);
