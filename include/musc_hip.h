@@ -437,10 +437,10 @@ int musc_masked_attention_fwd(const musc_masked_attention* call, void* workspace
  * window >= 1, sinks >= 0, with orders on both sides.  Tiles that
  * no row of a workgroup sees are not read.  call->schedule is not used.
  * fp32, here and after a prefix: products are three fp16 ones of operands held in 22 bits (Q by row, K by 32 keys, V
- * by 32 keys and 32 channels), so a logit is off by 3 2^-22 of its sum of |q_c k_c| scale and an output by as much of its
- * V where these are within 2^17 of the largest they are held with, and by 2^-39 of that largest for smaller ones.
- * 32 keys whose largest entries are 2^15 apart in K or, in 32 channels, 2^6 in V, infinities and NaN are computed with
- * fp32 products, so what keys hold that a query does not see costs it no more than these roundings. */
+ * by 32 keys and 32 channels).  A logit is off by 3 2^-22 of its sum of |q_c k_c| scale and 2^-23; an output by 3 2^-22 of
+ * its V where this is within 2^17 of its block's largest, and by 2^-39 of that largest for smaller entries.  Q and K whose
+ * largest product times scale may reach 2^8, V whose keys differ by more than 2^6 by their largest of 32 channels,
+ * infinities and NaN are computed with fp32 products, so keys cost a query that does not see them no more than that. */
 int musc_window_attention_workspace_bytes(const musc_masked_attention* call, int window, int sinks, size_t* out);
 int musc_window_attention_fwd(const musc_masked_attention* call, int window, int sinks, void* workspace,
                               size_t workspace_bytes, hipStream_t stream);

@@ -153,11 +153,14 @@ struct Type<MUSC_DTYPE_BF16> {
 // 2^13 .. 2^14, so what is below 2^-17 of that is off by 2^-39 of the largest instead.  Probabilities are
 // taken 2^7 times as large, as in fp16: those below 2^-10 of a row's largest are off by 2^-32 of that.
 //
-// What one row sees must not cost another its digits, so the keys of a tile have to be of one size.  By fp32
-// instructions go tiles that hold infinities or NaN; whose keys are 2^kApart apart by K's largest entries; and
-// blocks of V (32 keys, 32 channels) with an entry below 2^-kEntries of the scale, if also some key's largest entry
-// there is below 2^-kKeys of it (of standard normal V one block in 20 is asked so, and none of 4000 fails).  The scale
-// of a block stays while its largest entry is within 2^kFall of it; else o is taken to the block's own.
+// Q and K go by fp32 instructions, and Q as it is in memory, in tiles that hold infinities or NaN, or where the largest
+// of a row of Q, of the tile's K and the scale are 2^kProduct and more together: below that the 2^-39 come to
+// 2 D 2^(kProduct - 39) <= 2^-23 in a logit of any key, whatever the sizes of the others.
+//
+// Nor may V of a key that one row sees cost another its digits, so blocks of V (32 keys, 32 channels) are split if no
+// entry is below 2^-kEntries of the scale, or else no key's largest entry there is below 2^-kKeys of it (of standard
+// normal V one block in 20 is asked so, and none of 4000 fails).  The scale of a block stays while its largest entry is
+// within 2^kFall of it; else o is taken to the block's own.
 // Keys that no row of the wave sees count in none of that, whatever they hold.
 //
 // V's scale is 2^kMost at most and 2^-kMost of the largest entry so far at least: with probabilities up to 2^15 the
@@ -165,17 +168,13 @@ struct Type<MUSC_DTYPE_BF16> {
 struct Split {
   typedef _Float16 Vec __attribute__((ext_vector_type(8)));
   static constexpr int kTop = 14, kLeast = -100, kMost = 64, kInfinity = 0x7f800000;
-  static constexpr int kApart = 15, kEntries = 17, kKeys = 6, kFall = 2;
+  static constexpr int kProduct = 8, kNever = 1000, kEntries = 17, kKeys = 6, kFall = 2;
   static constexpr float kShift = 7.f;
   static __device__ __forceinline__ floatx16 mfma(Vec a, Vec b, floatx16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
   }
   // e with |x| < 2^e, from the bits of |x|; the smallest share kLeast
   static __device__ __forceinline__ int exponent(int bits) { return max((bits >> 23) - 126, kLeast); }
-  // whether some lane's size (bits of a largest entry; 0 does not count) is 2^kApart below the largest
-  static __device__ __forceinline__ bool apart(int size, int largest) {
-    return __any((size > 0) & ((largest >> 23) - (size >> 23) > kApart));
-  }
   static __device__ __forceinline__ float power(int e) { return __int_as_float((e + 127) << 23); }
   typedef _Float16 Two __attribute__((ext_vector_type(2)));
   // two of each: hi is opaque, or the compiler forms it a second time for lo

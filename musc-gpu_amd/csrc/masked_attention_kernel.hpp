@@ -284,10 +284,9 @@ __device__ __forceinline__ void attention_of_block(const Args& a, const uint32_t
     if (negate) qf[m] = -qf[m];
     if (c.scale == 0.f) qf[m] = TVec{};
   }
-  // split: this row's Q in 2^(q_exp - 14), and whether some row of the wave holds what cannot be split
+  // split: this row's Q in 2^(q_exp - 14), and the K (k_exp) up to which the wave's rows bear splitting
   Split::Vec qh[kSplit ? kQ / 2 : 1], ql[kSplit ? kQ / 2 : 1];
-  int q_exp = 0;
-  bool q_whole = true;
+  int q_exp = 0, k_most = 0;
   if constexpr (kSplit) {
     float most = 0.f;
 #pragma unroll
@@ -295,17 +294,12 @@ __device__ __forceinline__ void attention_of_block(const Args& a, const uint32_t
 #pragma unroll
       for (int j = 0; j < 4; ++j) most = __builtin_elementwise_maximum(most, fabsf(qf[m][j]));
     most = halves_max(most);
-    q_whole = __all(most < INFINITY);
     q_exp = Split::exponent(__float_as_int(most));
+    k_most = Split::kProduct - Split::exponent(__float_as_int(fabsf(scale))) -
+             wave_max_int(!live ? Split::kLeast : most < INFINITY ? q_exp : Split::kNever);
     const float by = Split::power(Split::kTop - q_exp);
 #pragma unroll
     for (int m = 0; m < kQ; m += 2) Split::split(qf[m], qf[m + 1], by, qh[m / 2], ql[m / 2]);
-    if (!q_whole) {  // then only their sum is used: infinities stay what they are
-#pragma unroll
-      for (int m = 0; m < kQ / 2; ++m)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) ql[m][j] = fabsf((float)qh[m][j]) < INFINITY ? ql[m][j] : (_Float16)0.f;
-    }
   }
   // the B operand of the distances: 1 and -position; slopes in raw units
 #pragma unroll
@@ -420,40 +414,43 @@ __device__ __forceinline__ void attention_of_block(const Args& a, const uint32_t
       for (int m = 0; m < kQ; ++m)
 #pragma unroll
         for (int j = 0; j < 4; ++j) most = __builtin_elementwise_maximum(most, fabsf(kf[0][m][j]));
-      // this lane's key, by its largest entry; one that no row of the wave sees does not count
+      // this lane's key's largest entry; one that no row of the wave sees does not count
       bool counts = true;
       if (!whole && !(prefixed && tile < p_tiles)) {
         const int kd = docs_s[buf][lq], ko = ords_s[buf][lq];
         counts = (kd >= mine.dmin) & (kd <= mine.dmax) & (ko <= mine.omax);
         if (windowed) counts &= (ko >= window_from(mine.omin)) | ((uint32_t)ko < (uint32_t)a.sinks);
       }
-      const int size = counts ? __float_as_int(halves_max(most)) : 0;
-      const int largest = wave_max_int(size);
-      int k_exp = Split::kTop;
-      if (!careful && q_whole && largest < Split::kInfinity && !Split::apart(size, largest)) {
-        k_exp = Split::exponent(largest);
-        const float by = Split::power(Split::kTop - k_exp);
+      const int largest = wave_max_int(counts ? __float_as_int(most) : 0), k_exp = Split::exponent(largest);
+      int by = 0;  // exponent of the products
+      if (!careful && largest < Split::kInfinity && k_exp <= k_most) {
+        const float k_by = Split::power(Split::kTop - k_exp);
+        by = k_exp + q_exp - 2 * Split::kTop;
 #pragma unroll
         for (int m = 0; m < kQ / 2; ++m) {
           Split::Vec kh, kl;
-          Split::split(kf[0][2 * m], kf[0][2 * m + 1], by, kh, kl);
+          Split::split(kf[0][2 * m], kf[0][2 * m + 1], k_by, kh, kl);
           s[0] = Split::mfma(kl, qh[m], s[0]);
           s[0] = Split::mfma(kh, ql[m], s[0]);
           s[0] = Split::mfma(kh, qh[m], s[0]);
           __builtin_amdgcn_sched_barrier(0);  // one pair's registers at a time
         }
       } else {
+        // Q as it is, read again: its parts have 22 bits only
+        int from = token;
+        asm volatile("" : "+v"(from));  // its address is formed here, not kept beside the parts
+        const T* again = static_cast<const T*>(c.q) + qb * c.q_sb + (long long)from * c.q_st + head * c.q_sh;
 #pragma unroll
-        for (int m = 0; m < kQ / 2; ++m) {
-          Split::Vec h = qh[m], l = ql[m];
-          asm volatile("" : "+v"(h), "+v"(l));  // Q's sums are formed here, not kept beside its parts
+        for (int m = 0; m < kQ; ++m) {
+          const int at = (2 * m + lh) * kPer;
+          TVec q = TVec{};
+          if (at < d && c.scale != 0.f) q = *reinterpret_cast<const TVec*>(again + at);
+          if (negate) q = -q;
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            s[0] = __builtin_amdgcn_mfma_f32_32x32x2f32(kf[0][2 * m + j / 4][j % 4], (float)h[j] + (float)l[j], s[0], 0, 0, 0);
+          for (int j = 0; j < 4; ++j) s[0] = __builtin_amdgcn_mfma_f32_32x32x2f32(kf[0][m][j], q[j], s[0], 0, 0, 0);
           __builtin_amdgcn_sched_barrier(0);
         }
       }
-      const int by = k_exp + q_exp - 2 * Split::kTop;
 #pragma unroll
       for (int v = 0; v < 16; ++v) s[0][v] = __builtin_ldexpf(s[0][v], by);
     } else {
