@@ -293,6 +293,7 @@ int plan_prefix(const musc_masked_attention& c, const musc_attention_prefix& p, 
   // 700 of their own, 32 heads on 8 of 128, bf16: 36 us and 7 for the join; 512 of each 40 and 11; apart 25, 22
   // and 11.
   a.partial = 1;
+  a.two_numbers = rows <= 32;
   waves = all <= 32 ? 1 : 4;
   more = a;
   more.stacked = 0;

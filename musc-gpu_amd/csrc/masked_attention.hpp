@@ -61,7 +61,8 @@
 // 0.76 to 0.81 PFLOP/s, as for one document of 8192.  32 single tokens after 16384 keys and over up to 700
 // of their own, 32 heads on 8 of 128, bf16: 35 us = 3.6 TB/s, and 6 for the join.
 //
-// Both keep the probabilities of few 16-bit rows in two numbers each, and fp32 as Split has it: a tile of 32
+// Both keep the probabilities of up to 32 16-bit rows of an entry in two numbers each (32 requests as above: 45 us all
+// told with one number, 46 with two), and fp32 as Split has it: a tile of 32
 // keys of heads of 96 takes 1150 cycles of matrix instructions (6144 of fp32 ones) and about 2500 of vector
 // ones.  3 x 1500 tokens, window of 250, 8 heads on 4 of 80, cap: 57 us, by fp32 instructions 78.
 #pragma once
@@ -189,7 +190,8 @@ struct Split {
     split(a[0], a[1], by, 0, hi, lo), split(a[2], a[3], by, 2, hi, lo);
     split(b[0], b[1], by, 4, hi, lo), split(b[2], b[3], by, 6, hi, lo);
   }
-  // By its series up to 0.3 (the next term is 2^-24 of it), and 1 - 2 / (1 + e^2x): off by 2^-20 of itself.
+  // By its series up to 0.3 (the next term is 2^-24 of it), and 1 - 2 / (1 + e^2x): off by 2^-21 of itself, as
+  // the other fp32 kernels' caps are (measured: 2^-21.8, tanhf 2^-22.6; tanhf takes 63 us where this takes 61).
   static __device__ __forceinline__ float tanh(float x) {
     const float y = x * x;
     float p = fmaf(y, 62.f / 2835.f, -17.f / 315.f);
@@ -229,6 +231,7 @@ struct Args {
   // the rows of all are stacked), and whether the rows' parts are joined even if there is one
   musc_attention_prefix p;
   int p_tiles, batches, stacked, partial;
+  int two_numbers;    // 16-bit types: four waves keep probabilities as two numbers
   int more_splits;    // for the join: parts over the own keys
   float *more_ml, *more_o;
   long long units;

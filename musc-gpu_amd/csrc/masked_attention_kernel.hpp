@@ -47,8 +47,10 @@ __device__ __forceinline__ int4v resource(const void* base, long long bytes) {
 // kSmallCap; kernels of their own, as tanhf beside the other form costs registers (parts of fp16 heads of 64:
 // 76 spilled instead of 17): 8192 tokens, 16 heads of 64, fp16, 730 us past kSmallCap, 450 up to it.
 // kWindowed: keys behind the window and past the sinks are not seen either.  kPrefixed: the first a.p_tiles
-// tiles are of a prefix that the batch shares; a.stacked: all rows of the batch over those tiles.
-constexpr int kCapped = 1, kBiased = 2, kInParts = 4, kEither = 8, kLargeCap = 16, kWindowed = 32, kPrefixed = 64;
+// tiles are of a prefix that the batch shares; a.stacked: all rows of the batch over those tiles.  kTwoNumbers (16-bit
+// types, four waves): probabilities as two numbers, as single waves have them.
+constexpr int kCapped = 1, kBiased = 2, kInParts = 4, kEither = 8, kLargeCap = 16, kWindowed = 32, kPrefixed = 64,
+              kTwoNumbers = 128;
 template <int kDtype, int kD, int kWaves, int kTeams, int kMode>
 __device__ __forceinline__ void attention_of_block(const Args& a, const uint32_t block, const uint32_t blocks) {
   using Ty = Type<kDtype>;
@@ -68,8 +70,9 @@ __device__ __forceinline__ void attention_of_block(const Args& a, const uint32_t
   constexpr float kShift = kSplit ? Split::kShift : Ty::kShift;
   // few 16-bit rows of windows and prefixes: probabilities as two numbers each.  Their second product is in the
   // shadow of the loads, and with rounded ones a few rows may be twice as far from float64 as their own rounding
-  // leaves them; over many rows it is 1.2 to 1.3 times.
-  constexpr bool kTwoTerms = k16 && (windowed || prefixed) && kWaves == 1;
+  // leaves them; over many rows it is 1.2 to 1.3 times.  Few rows of each of many entries likewise, so that an
+  // entry's output does not hang on how many others share its call.
+  constexpr bool kTwoTerms = k16 && (windowed || prefixed) && (kWaves == 1 || (kMode & kTwoNumbers) != 0);
   __shared__ __attribute__((aligned(1024))) char staged[2 * kTeams][2 * kPart];
   __shared__ __attribute__((aligned(16))) int docs_s[2 * kTeams][64], ords_s[2 * kTeams][64];
   __shared__ float pos_s[2 * kTeams][64 * kMaxAxes];
@@ -1184,6 +1187,14 @@ void launch_few(const Args& a, const Args* more, hipStream_t stream) {
   if (a.teams > 1) launch_one<kDtype, kD, 1, kTeams, kMode>(a, more, stream);
   else launch_one<kDtype, kD, 1, 1, kMode>(a, more, stream);
 }
+// Four waves.
+template <int kDtype, int kD, int kMode>
+void launch_many(const Args& a, const Args* more, hipStream_t stream) {
+  if constexpr (kDtype != MUSC_DTYPE_F32 && (kMode & kPrefixed) != 0) {
+    if (a.two_numbers) return launch_one<kDtype, kD, 4, 1, kMode | kTwoNumbers>(a, more, stream);
+  }
+  launch_one<kDtype, kD, 4, 1, kMode>(a, more, stream);
+}
 template <int kDtype, int kD, int kExtra>
 void launch_extra(const Args& a, const Args* more, int waves, hipStream_t stream) {
   const bool plain = !(a.c.cap > 0.f) && !a.c.axes;
@@ -1191,7 +1202,7 @@ void launch_extra(const Args& a, const Args* more, int waves, hipStream_t stream
   if constexpr (kDtype != MUSC_DTYPE_F32) {
     if (a.c.cap > kSmallCap) {
       if (waves == 1) launch_few<kDtype, kWide, kEither | kLargeCap | kExtra>(a, more, stream);
-      else launch_one<kDtype, kWide, 4, 1, kEither | kLargeCap | kExtra>(a, more, stream);
+      else launch_many<kDtype, kWide, kEither | kLargeCap | kExtra>(a, more, stream);
       return;
     }
   }
@@ -1199,9 +1210,9 @@ void launch_extra(const Args& a, const Args* more, int waves, hipStream_t stream
     if (plain) launch_few<kDtype, kWide, kExtra>(a, more, stream);
     else launch_few<kDtype, kWide, kEither | kExtra>(a, more, stream);
   } else if (plain) {
-    launch_one<kDtype, kD, 4, 1, kExtra>(a, more, stream);
+    launch_many<kDtype, kD, kExtra>(a, more, stream);
   } else {
-    launch_one<kDtype, kD, 4, 1, kEither | kExtra>(a, more, stream);
+    launch_many<kDtype, kD, kEither | kExtra>(a, more, stream);
   }
 }
 template <int kDtype, int kExtra>
