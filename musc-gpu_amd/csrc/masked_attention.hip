@@ -283,8 +283,17 @@ int plan_prefix(const musc_masked_attention& c, const musc_attention_prefix& p, 
     more = a, waves = 1;
     return shape(a, rows, c.batch, waves, true, true, teams, 0);
   }
-  const long long apart = c.batch * ((rows + kRowTile - 1) / kRowTile), together = (all + kRowTile - 1) / kRowTile;
-  a.stacked = c.batch > 1 && 2 * apart >= 3 * together && all * c.kv_heads < (1 << 24);
+  // Together over the prefix or each entry's rows by themselves.  Together there are fewer row tiles to take
+  // over it (counted in thirds, as a tile of a single wave is about one), and each row writes its output twice more
+  // and reads it, in fp32, for the join: worth it from so many keys of the prefix on, by storage, as a saved tile's
+  // keys outweigh a row (bf16, 1024 entries of 40 rows, 16 heads of 64: 1024 keys 566 us apart and 663 together,
+  // 4096 1755 and 1215; 512 of 4 rows, 8 heads of 128: 256 92 and 97, 512 130 and 105; fp32, 256 entries of 40 rows:
+  // 128 189 and 215, 256 282 and 245).  Row tiles that all begin at once anyway save nothing (16 entries of 70
+  // rows, 16 heads: 4096 keys 62 us apart, 85 together).  Parts that would take more than 1 GiB are not asked for.
+  const auto thirds = [](long long n) { return n <= 32 ? 1.0 : 3.0 * ((n + kRowTile - 1) / kRowTile); };
+  const double saved = c.batch * thirds(rows) - thirds(all), least = c.dtype == MUSC_DTYPE_F32 ? 12 : 72;
+  const bool rounds = rows <= 32 || heads * ((rows + kRowTile - 1) / kRowTile) > 512;
+  a.stacked = c.batch > 1 && rounds && saved * p.len >= least * all && (double)all * c.kv_heads * c.d <= (1 << 27);
   if (!a.stacked) {
     more = a, waves = rows <= 32 ? 1 : 4;
     return shape(a, rows, c.batch, waves, true, true, 1, waves == 1 ? 1024 : 512);

@@ -307,7 +307,8 @@ def prefix_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, prefix_k
     every query sees the whole prefix and, of k and v, what keys and queries let it see; (B, Tq, heads, D).
 
     prefix_k, prefix_v: (P, kv_heads, D), once for the batch; views are read in place as k and v are.
-    Single tokens and other short calls pass over the prefix together, so it is read once for all of them.
+    Entries of few tokens pass over a prefix that is long enough together, so it is read once for all of them (parts
+    of their outputs take up to 1 GiB meanwhile).
     Queries without a document (negative ids, padding) get zeros.  k and v may have no tokens, and the
     prefix none.  slopes need prefix_positions, float32 (P, axes), too.  The rest as for masked_attention.  No derivative."""
     rt.require_device_tensor(prefix_k, 'prefix_k')
