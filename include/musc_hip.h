@@ -448,7 +448,7 @@ int musc_window_attention_fwd(const musc_masked_attention* call, int window, int
 /* The same after a prefix that the whole batch shares: every query that has a document (all of them
  * in a call without documents) sees each of its len keys, and of the call's own keys those above.
  * Where the entries have few rows each and the prefix is long, the rows of all of them pass over it together; the
- * workspace for their parts is 1 GiB at most, .
+ * workspace for their parts is about 1 GiB at most.
  * k and v have heads of the call's d channels at token * st + head * sh, by the rules of the call's K and V;
  * positions: float32 (len, axes) rows, needed with call->axes.  len >= 1; call->k_len may be 0 (no own
  * keys; what is given of them is then not looked at).  call->schedule is not used. */

@@ -84,3 +84,26 @@ def test_errors_are_the_roundings_of_the_output(device, b, tq, d, dtype):
     out = reference(q, joined(pk, k), joined(pv, v), 0.1)[0]
     rms = lambda x: (x - out).pow(2).mean().sqrt().item()  # noqa: E731
     assert rms(got.double().cpu()) <= 1.1 * rms(out.to(dtype).double())
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('cap', [0.0, 300.0])
+def test_stacked_entries_beside_unseen_values(device, cap, dtype):
+    # NaN and infinities behind the prefix in its last tile, in caches that were never written, and in padding
+    b, h, hk, tk, p, d = 40, 8, 2, 90, 2301, 128
+    q, k, v = heads(device, dtype, b, 1, tk, h, hk, d)
+    room_k, room_v = shared(device, dtype, p + 30, hk, d)
+    room_k[p:], room_v[p:] = float('nan'), float('inf')
+    at, last = torch.arange(tk), (torch.arange(b)[:, None] * 7) % tk
+    qd = torch.where(torch.arange(b)[:, None] % 9 == 8, -1, 0)
+    unseen = (at[None] > last)[..., None, None].to(device)
+    full_k, full_v = k.masked_fill(unseen, float('inf')), v.masked_fill(unseen, float('nan'))
+    q[qd[:, 0].to(device) < 0] = float('nan')
+    keys = Tokens(i32(at * 0, device), i32(at, device))
+    queries = Tokens(i32(qd, device), i32(last, device), queries_only=True)
+    got = prefix_attention(q, full_k, full_v, room_k[:p], room_v[:p], 0.1, keys=keys, queries=queries, cap=cap)
+    live = qd[:, 0] >= 0
+    own = see_own(qd, at * 0, last, at)
+    seen = torch.cat([torch.ones((b, 1, p), dtype=torch.bool), own], 2)[live]
+    check(got[live], q[live], joined(room_k[:p], k)[live], joined(room_v[:p], v)[live], 0.1, seen=seen, cap=cap)
+    assert (got[~live] == 0).all()
