@@ -436,9 +436,12 @@ int musc_masked_attention_fwd(const musc_masked_attention* call, void* workspace
  *   order(j) > order(i) - window (its own place and the window - 1 before it) or 0 <= order(j) < sinks.
  * window >= 1, sinks >= 0, with orders on both sides.  Tiles that
  * no row of a workgroup sees are not read.  call->schedule is not used.
+ * 16-bit types, here and after a prefix: probabilities are rounded to the type (half a step each) in calls of more than 32
+ * rows (query tokens and heads of a group) an entry, and kept as two such numbers in smaller ones.
  * fp32, here and after a prefix: products are three fp16 ones of operands held in 22 bits (Q by row, K by 32 keys, V
  * by 32 keys and 32 channels).  A logit is off by 3 2^-22 of its sum of |q_c k_c| scale and 2^-23; an output by 3 2^-22 of
- * its V where this is within 2^17 of its block's largest, and by 2^-39 of that largest for smaller entries.  Q and K whose
+ * its V where this is within 2^17 of its block's largest, and by 2^-39 of that largest for smaller entries; probabilities
+ * below 2^-10 of a row's largest are off by 2^-32 of that.  Q and K whose
  * largest product times scale may reach 2^8, V whose keys differ by more than 2^6 by their largest of 32 channels,
  * infinities and NaN are computed with fp32 products, so keys cost a query that does not see them no more than that. */
 int musc_window_attention_workspace_bytes(const musc_masked_attention* call, int window, int sinks, size_t* out);

@@ -299,8 +299,8 @@ int plan_prefix(const musc_masked_attention& c, const musc_attention_prefix& p, 
     return shape(a, rows, c.batch, waves, true, true, 1, waves == 1 ? 1024 : 512);
   }
   // As many workgroups for each of the two as there are CUs: 32 single tokens after 16384 keys and over up to
-  // 700 of their own, 32 heads on 8 of 128, bf16: 36 us and 7 for the join; 512 of each 40 and 11; apart 25, 22
-  // and 11.
+  // 700 of their own, 32 heads on 8 of 128, bf16: 36 us and 7 for the join (38 with probabilities of two numbers); 512 of each 40 and 11; apart 25,
+  // 22 and 11.
   a.partial = 1;
   a.two_numbers = rows <= 32;
   waves = all <= 32 ? 1 : 4;

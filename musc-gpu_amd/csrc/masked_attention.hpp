@@ -59,12 +59,12 @@
 // all of them walk over the prefix together (it is read once, in full row tiles) and, in the same launch, each
 // entry's over its own keys; a join follows.  16 x 1370 tokens after 5480, 16 heads of 64, fp16: 760 to 810 us =
 // 0.76 to 0.81 PFLOP/s, as for one document of 8192.  32 single tokens after 16384 keys and over up to 700
-// of their own, 32 heads on 8 of 128, bf16: 35 us = 3.6 TB/s, and 6 for the join.
+// of their own, 32 heads on 8 of 128, bf16: 38 us = 3.3 TB/s, and 6 for the join.
 //
 // Both keep the probabilities of up to 32 16-bit rows of an entry in two numbers each (32 requests as above: 45 us all
 // told with one number, 46 with two), and fp32 as Split has it: a tile of 32
-// keys of heads of 96 takes 1150 cycles of matrix instructions (6144 of fp32 ones) and about 2500 of vector
-// ones.  3 x 1500 tokens, window of 250, 8 heads on 4 of 80, cap: 57 us, by fp32 instructions 78.
+// keys of heads of 96 takes 1150 cycles of matrix instructions (6144 of fp32 ones) and about 2700 of vector
+// ones.  3 x 1500 tokens, window of 250, 8 heads on 4 of 80, cap: 60 us, by fp32 instructions 78.
 #pragma once
 
 #include <hip/hip_bf16.h>

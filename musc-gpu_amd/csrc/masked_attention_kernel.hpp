@@ -70,7 +70,7 @@ __device__ __forceinline__ void attention_of_block(const Args& a, const uint32_t
   constexpr float kShift = kSplit ? Split::kShift : Ty::kShift;
   // few 16-bit rows of windows and prefixes: probabilities as two numbers each.  Their second product is in the
   // shadow of the loads, and with rounded ones a few rows may be twice as far from float64 as their own rounding
-  // leaves them; over many rows it is 1.2 to 1.3 times.  Few rows of each of many entries likewise, so that an
+  // leaves them; over many rows it is 1.2 to 1.3 times (and two numbers 10 to 39 % of the time).  Few rows of each of many entries likewise, so that an
   // entry's output does not hang on how many others share its call.
   constexpr bool kTwoTerms = k16 && (windowed || prefixed) && (kWaves == 1 || (kMode & kTwoNumbers) != 0);
   __shared__ __attribute__((aligned(1024))) char staged[2 * kTeams][2 * kPart];
