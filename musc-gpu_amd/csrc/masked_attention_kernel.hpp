@@ -849,11 +849,12 @@ __device__ __forceinline__ void attention_of_block(const Args& a, const uint32_t
   if (kTeams > 1 ? __any(bad) : __syncthreads_or(bad)) walk(std::integral_constant<bool, true>{});
 
   l_run = halves_sum(l_run);
-  if constexpr (kSplit) {
+  if constexpr (kSplit) {  // without the probabilities' factor: V up to the type's end, as the other fp32 kernels bear
+    l_run = __builtin_ldexpf(l_run, -(int)kShift);
 #pragma unroll
     for (int x = 0; x < kO; ++x)
 #pragma unroll
-      for (int v = 0; v < 16; ++v) o[x][v] = __builtin_ldexpf(o[x][v], v_exp[x] - Split::kTop);
+      for (int v = 0; v < 16; ++v) o[x][v] = __builtin_ldexpf(o[x][v], v_exp[x] - Split::kTop - (int)kShift);
   }
   if constexpr (kTeams > 1) {
     // each team's (maximum, sum) and output in its own place, then all of them in order

@@ -87,3 +87,24 @@ def test_the_largest_numbers_after_small_ones(device, largest, d):
     side = Tokens(i32(docs, device), i32(at, device))
     got = masked_attention(q, k, v, 0.05, keys=side, window=50)
     check(got, q, k, v, 0.05, seen=see(docs, docs, at, at, 50, 0))
+
+
+@pytest.mark.parametrize('tq', [1, 20, 200])
+@pytest.mark.parametrize('d', [64, 128])
+def test_values_near_the_end_of_the_type(device, d, tq):
+    # four keys of up to 2^125 each: their sum is a number
+    t = 230
+    q, k, v = heads(device, torch.float32, 1, tq, t, 2, 1, d)
+    v = v.clamp(-1, 1) * 2.0 ** 125
+    at, new = torch.arange(t), torch.arange(t)[-tq:]
+    got = masked_attention(q, k, v, 1e-3, keys=Tokens(i32(at * 0, device), i32(at, device)), window=4,
+                           queries=Tokens(i32(new * 0, device), i32(new, device), queries_only=True))
+    check(got, q, k, v, 1e-3, seen=see(new * 0, at * 0, new, at, 4, 0))
+
+
+@pytest.mark.parametrize('b,tq', SHAPES)
+def test_values_near_the_end_of_the_type_after_a_prefix(device, b, tq):
+    q, k, v = heads(device, torch.float32, b, tq, 2, 2, 1, 64)
+    pk, pv = shared(device, torch.float32, 3000, 1, 64)
+    v, pv = v.clamp(-1, 1) * 2.0 ** 114, pv.clamp(-1, 1) * 2.0 ** 114       # the sum over 3002 keys below 2^126
+    check(prefix_attention(q, k, v, pk, pv, 1e-3), q, joined(pk, k), joined(pv, v), 1e-3)
